@@ -33,6 +33,7 @@ typedef struct ihipStream_t* tt_stream_t; /* layout-compatible with hipStream_t 
 enum tt_status { TT_OK = 0, TT_ERR_INVALID = -1, TT_ERR_WORKSPACE = -2, TT_ERR_UNSUPPORTED = -3 };
 enum tt_index_dtype { TT_IDS_I32 = 0, TT_IDS_I64 = 1 };
 enum tt_compute_dtype { TT_F32 = 0, TT_BF16 = 1, TT_BF16_SPLIT = 2 };
+enum tt_elem_dtype { TT_E_F32 = 0, TT_E_BF16 = 1, TT_E_F16 = 2 }; /* element types of the operators below */
 enum tt_scatter_mode {
   TT_SCATTER_SORTED = 0, /* deterministic: stable radix sort + segmented row reduce; writes every row */
   TT_SCATTER_ATOMIC = 1  /* global_atomic_add_f32 into caller-zeroed grad; order-dependent */
@@ -189,6 +190,21 @@ int tt_bag_col_reduce_ex(const int32_t* seg_all, const int32_t* vals_all, int64_
                          const float* gs_all, int64_t V, int El, float* grad, float* slab, float* exp_avg,
                          float* exp_avg_sq, const void* adam_args, void* ws, size_t ws_bytes, tt_stream_t stream);
 
+/* ---- token lookup with a scale (LookupEmbedding.forward's (B, L, E) rows, twotower/embeddings.py:40) ----
+ * tt_lookup_fwd: out[t, :] = scale * table[ids[t], :] for n tokens, formed in fp32 and rounded once; an
+ *   id outside [0, V) yields a zero row.  table: V rows of E elements, row stride ld_table; out: n x E.
+ *   Types (tt_elem_dtype): out = table's, or bf16 / fp16 rows of an fp32 table.
+ * tt_lookup_bwd: grad[r, :] = scale * sum of dout[t, :] over the tokens with ids[t] = r (none for r =
+ *   padding_idx, -1: no padding id), every one of the V rows written.  Sums are fp32 in a fixed order
+ *   (bitwise reproducible), rounded once to grad's type; dout has out's type, grad the table's.
+ *   ws: tt_lookup_bwd_ws_size bytes (0 for short calls). */
+int tt_lookup_fwd(const void* table, int table_dtype, int64_t V, int E, int64_t ld_table, const void* ids,
+                  int ids_dtype, int64_t n, float scale, void* out, int out_dtype, tt_stream_t stream);
+size_t tt_lookup_bwd_ws_size(int64_t n, int64_t V, int E);
+int tt_lookup_bwd(const void* dout, int dout_dtype, const void* ids, int ids_dtype, int64_t n, int64_t V, int E,
+                  int64_t padding_idx, float scale, void* grad, int grad_dtype, void* ws, size_t ws_bytes,
+                  tt_stream_t stream);
+
 /* ---- dense AdamW (torch.optim.AdamW, twotower/train.py:359, .step() :139) ---------
  * p *= 1 - lr*wd;  m = lerp(m, g, 1-b1);  v = b2*v + (1-b2)*g*g;
  * p -= lr/(1-b1^step) * m / (sqrt(v)/sqrt(1-b2^step) + eps).   step is 1-based.
@@ -244,6 +260,25 @@ typedef struct {
 int tt_adamw_multi_ex(const tt_adamw_tensor* tensors, const tt_adamw_grad_parts* parts, int count,
                       const tt_adam_slot* next, int nnext, double lr, double beta1, double beta2, double eps,
                       double weight_decay, unsigned* ticket, tt_stream_t stream);
+
+/* ---- global gradient norm over many tensors, and clipping (torch.nn.utils.clip_grad_norm_ between
+ * loss.backward() and optimizer.step(), twotower/train.py:138-139) ----
+ * norm = (sum g^2)^(1/2) over every element of every tensor, or max |g| (inf_norm != 0), in 64 bits,
+ * rounded once to *norm; scale != 0: dst = src * min(1, max_norm / (norm + 1e-6)), formed in fp32 and
+ * rounded once.  dst may be src (then an unclipped call writes nothing) or another tensor of src's type
+ * or fp32; tensors must not overlap otherwise.  Any count: TT_CLIP_MAX_TENSORS per launch, passed
+ * by value.  ws: tt_clip_ws_size(count) bytes, 8-byte aligned. */
+#define TT_CLIP_MAX_TENSORS 128
+typedef struct {
+  const void* src;
+  void* dst;
+  int64_t n;
+  int src_dtype; /* tt_elem_dtype */
+  int dst_dtype;
+} tt_clip_tensor;
+size_t tt_clip_ws_size(int count);
+int tt_clip_grads(const tt_clip_tensor* tensors, int count, int inf_norm, double max_norm, int scale,
+                  float* norm, void* ws, size_t ws_bytes, tt_stream_t stream);
 
 /* ---- mean of n floats (the loss reductions' F.cross_entropy / .mean(), losses.py:44,85,116):
  * one workgroup, fixed-order sums (bitwise reproducible); the in-batch forward forms it itself
@@ -304,6 +339,24 @@ int tt_multi_neg_bwd(const float* q, const float* p, const float* negs, int64_t 
  * for bit to tt_multi_neg_bwd followed by tt_l2norm_bwd on those rows. */
 int tt_multi_neg_bwd_l2(const float* qpn, int64_t B, int N, const float* norms, float inv_tau,
                         const float* grad_loss, float* dx, tt_stream_t stream);
+
+/* ---- paired preference loss (losses.preference_loss, beside the pairwise losses of twotower/losses.py) ----
+ * Pair (i, k): h = q_i . (p_i - n_ik) * inv_tau - ref[i K + k] (ref NULL: 0).  kind 0, sigmoid: (1 - s)
+ * softplus(-beta h) + s softplus(beta h) with s = smoothing; kind 1, squared: (h - 1 / (2 beta))^2.
+ * mask (B x K bytes, NULL: all valid): a pair with mask 0 is not read.  q, p: B rows of H elements (row
+ * strides ldq, ldp); n: row (i, k) at i ldn_b + k ldn_k; elements of one tt_elem_dtype.
+ * fwd writes coef[i K + k] = dl/dh (0 where masked; NULL to skip), margins[i K + k] = h (0 where masked;
+ * NULL to skip), *loss = the mean over the valid pairs (0 if none) and *inv_pairs = 1 / max(pairs, 1) (loss
+ * NULL: neither).  ws: 8 B bytes.  bwd reads coef, inv_pairs and the upstream scalar grad_loss
+ * (device) and writes dq (B x H), dp (B x H), dn (B x K x H), zero rows for masked pairs. */
+int tt_preference_fwd(const void* q, int64_t ldq, const void* p, int64_t ldp, const void* n, int64_t ldn_b,
+                      int64_t ldn_k, int dtype, int64_t B, int K, int H, const float* ref, const uint8_t* mask,
+                      int kind, float beta, float inv_tau, float smoothing, float* coef, float* margins, float* loss,
+                      float* inv_pairs, void* ws, size_t ws_bytes, tt_stream_t stream);
+int tt_preference_bwd(const void* q, int64_t ldq, const void* p, int64_t ldp, const void* n, int64_t ldn_b,
+                      int64_t ldn_k, int dtype, int64_t B, int K, int H, const uint8_t* mask, float inv_tau,
+                      const float* coef, const float* inv_pairs, const float* grad_loss, void* dq, void* dp, void* dn,
+                      tt_stream_t stream);
 
 /* ---- in-batch sampled softmax (in_batch_sampled_softmax_loss, twotower/losses.py:88-118)
  * S = q d^T (B x M, never materialised), logits = S * inv_tau, label of row i is column
@@ -432,6 +485,31 @@ int tt_topk_rows(const float* scores, int64_t nrows, int64_t ncols, int k, float
 size_t tt_topk_rows_ws_size(int64_t nrows, int64_t ncols, int k);
 int tt_topk_rows_ex(const float* scores, int64_t nrows, int64_t ncols, int k, void* ws, size_t ws_bytes,
                     float* out_vals, int64_t* out_idx, tt_stream_t stream);
+
+/* ---- 4-bit rows with group scales: the document index of the search at 4.5 bits a value ----
+ * Row j, column k: (code - 8) * scale[j, k / group], codes 0..15, bf16 scales, group in {32, 64, 128},
+ * H <= TT_INT4_MAX_H.  codes and scales are laid out for the scoring kernel (opaque: tiles of 16 rows),
+ * tt_int4_codes_bytes / tt_int4_scales_bytes long, 16-byte aligned.
+ * tt_int4_quantize: x (n rows of H elements, row stride ld, a tt_elem_dtype) -> scale = max |group| / 7
+ *   rounded to bf16, code = 8 + the nearest integer of x / scale (ties to even) in -7..7; a group
+ *   with a non-finite value gets a NaN scale.
+ * tt_int4_pack: c (n x H int8, -8..7, others clamped) and sc (n x ceil(H / group) bf16) -> the layout.
+ * tt_int4_unpack: the layout -> out (n x H fp32), the values the codes stand for.
+ * tt_int4_scores: scores[i n + j] = sum_k q[i, k] value[j, k] for nq fp32 / bf16 / fp16 queries (row
+ *   stride ldq): products of the codes with q (as three fp16 terms, 33 bits) on the matrix cores,
+ *   accumulated in fp32 per 32 columns, scaled and added in fp32.  A query with a non-finite
+ *   value scores NaN. */
+#define TT_INT4_MAX_H 4096
+size_t tt_int4_codes_bytes(int64_t n, int H);
+size_t tt_int4_scales_bytes(int64_t n, int H, int group);
+int tt_int4_quantize(const void* x, int dtype, int64_t n, int H, int64_t ld, int group, void* codes, void* scales,
+                     tt_stream_t stream);
+int tt_int4_pack(const int8_t* c, const void* sc, int64_t n, int H, int group, void* codes, void* scales,
+                 tt_stream_t stream);
+int tt_int4_unpack(const void* codes, const void* scales, int64_t n, int H, int group, float* out,
+                   tt_stream_t stream);
+int tt_int4_scores(const void* q, int dtype, int64_t nq, int64_t ldq, const void* codes, const void* scales, int64_t n,
+                   int H, int group, float* scores, tt_stream_t stream);
 
 /* ---- device-resident batch feeder (TripletDataset.__getitem__ + DataLoader collate,
  * twotower/dataset.py:262-285, twotower/train.py:411-417): dst[r, :L] = src[idx[r], :L] for int32

@@ -1,0 +1,854 @@
+"""GPU: the token lookup, preference loss, gradient clipping and 4-bit index operators against plain 64-bit
+implementations, at the sizes, types, strides and masks where they can go wrong.
+
+Tolerances count roundings: u = 2^-24 is half a step of fp32, HALF[t] half a step of the stored type.  A sum of m
+fp32 terms is off by at most m u times the sum of their magnitudes; a stored value by HALF[t] of itself
+(or half the smallest subnormal)."""
+import math
+
+import pytest
+import torch
+
+import twotower_amd as tt
+from twotower_amd import _lib, losses, ops, optim
+
+from test_operators_cpu import pair_terms
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+U = 2.0 ** -24
+HALF = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}
+TINY = {F32: 2.0 ** -149, BF16: 2.0 ** -133, F16: 2.0 ** -24}  # smallest subnormals
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def check(got, want, bound, what=""):
+    """|got - want| <= bound elementwise, finite and non-finite places alike."""
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape
+    bad = ~((got - want).abs() <= bound)
+    same = (got == want) | (got.isnan() & want.isnan())
+    bad &= ~same
+    if bad.any():
+        i = bad.flatten().nonzero()[0].item()
+        b = bound if not isinstance(bound, torch.Tensor) else bound.expand_as(want).flatten()[i].item()
+        raise AssertionError(f"{what}: {bad.sum().item()} of {bad.numel()} off; first at {i}: got "
+                             f"{got.flatten()[i].item()!r}, want {want.flatten()[i].item()!r}, bound {b}")
+
+
+def stored(want, t):
+    """How far a value of type t may be from `want` by its one rounding."""
+    return want.abs() * HALF[t] + TINY[t]
+
+
+# ---------------------------------------------------------------------------------------------
+# token lookup
+def lookup_case(V, E, shape, dtype, ids_dtype, out_dtype, pad, hot, seed):
+    g = gen(seed)
+    w = torch.randn(V, E, generator=g, device=DEV).to(dtype)
+    ids = torch.randint(0, V, shape, generator=g, device=DEV)
+    if hot:  # most tokens name one row
+        ids = torch.where(torch.rand(shape, generator=g, device=DEV) < hot, torch.full_like(ids, V // 2), ids)
+    if pad is not None:
+        ids = torch.where(torch.rand(shape, generator=g, device=DEV) < 0.4, torch.full_like(ids, pad % V), ids)
+    dout = torch.randn(*shape, E, generator=g, device=DEV).to(out_dtype or dtype)
+    return w, ids.to(ids_dtype), dout
+
+
+def check_lookup(w, ids, dout, scale, pad, out_dtype, out, grad):
+    V, E = w.shape
+    flat = ids.reshape(-1).long()
+    inside = (flat >= 0) & (flat < V)
+    rows = w.double()[flat.clamp(0, V - 1)] * scale
+    rows[~inside] = 0
+    rows = rows.view(*ids.shape, E)
+    t = out_dtype or w.dtype
+    check(out, rows, 2 * U * rows.abs() + stored(rows, t), "rows")  # the factor and the product, then the type
+    keep = inside & (flat != (pad % V if pad is not None else -1))
+    d = dout.double().reshape(-1, E)[keep] * scale
+    want = torch.zeros(V, E, dtype=torch.float64, device=DEV).index_add_(0, flat[keep], d)
+    mass = torch.zeros(V, E, dtype=torch.float64, device=DEV).index_add_(0, flat[keep], d.abs())
+    count = torch.zeros(V, dtype=torch.float64, device=DEV).index_add_(0, flat[keep], torch.ones_like(d[:, 0]))
+    check(grad, want, (count + 3).unsqueeze(1) * U * mass + stored(want, w.dtype), "gradient")
+    assert not grad[count == 0].any()
+
+
+LOOKUPS = [
+    # V, E, ids shape, type, id type, out type, padding id, share of one hot row
+    (34, 64, (64, 64), F32, torch.int64, None, 0, 0.0),          # 4096 tokens: the longest call without a sort
+    (34, 64, (4097,), F32, torch.int64, None, 0, 0.0),           # one more
+    (50_000, 128, (1, 64), BF16, torch.int32, None, 0, 0.0),
+    (1, 1, (1,), F32, torch.int64, None, None, 0.0),
+    (1, 5, (7000,), F16, torch.int32, None, None, 0.0),          # one row, every token its own
+    (7, 1, (3, 5), BF16, torch.int64, None, -1, 0.0),            # padding id from the end
+    (301, 100, (37, 29), F16, torch.int32, None, None, 0.0),
+    (301, 100, (61, 83), F16, torch.int64, BF16, 3, 0.0),        # (refused: see below)
+    (301, 100, (61, 83), F32, torch.int64, BF16, 3, 0.0),
+    (301, 36, (61, 83), F32, torch.int32, F16, None, 0.0),
+    (1000, 256, (4000,), F32, torch.int64, None, None, 0.9),     # a hot row shared by a workgroup
+    (1000, 256, (60_000,), F32, torch.int64, None, None, 0.9),   # a hot row in pieces
+    (129, 513, (5000,), F32, torch.int32, None, 1, 0.3),         # wider than a wave's accesses, odd
+    (129, 1030, (300,), BF16, torch.int32, None, 1, 0.3),
+    (70_000, 8, (20_000,), BF16, torch.int64, None, 0, 0.1),
+    (2048, 512, (9000,), F16, torch.int64, None, 0, 0.5),
+]
+
+
+@pytest.mark.parametrize("V, E, shape, dtype, ids_dtype, out_dtype, pad, hot", LOOKUPS)
+def test_lookup_against_plain(V, E, shape, dtype, ids_dtype, out_dtype, pad, hot):
+    w, ids, dout = lookup_case(V, E, shape, dtype, ids_dtype, out_dtype, pad, hot, 1)
+    w.requires_grad_(True)
+    if out_dtype is not None and dtype != F32:
+        with pytest.raises(TypeError, match="out_dtype"):
+            ops.embedding_lookup(w, ids, out_dtype=out_dtype)
+        return
+    scale = math.sqrt(E)
+    out = ops.embedding_lookup(w, ids, scale=scale, padding_idx=pad, out_dtype=out_dtype)
+    (grad,) = torch.autograd.grad(out, w, dout)
+    assert out.dtype == (out_dtype or dtype) and grad.dtype == dtype
+    check_lookup(w.detach(), ids, dout, scale, pad, out_dtype, out.detach(), grad)
+    again = ops.embedding_lookup(w, ids, scale=scale, padding_idx=pad, out_dtype=out_dtype)
+    assert torch.equal(torch.autograd.grad(again, w, dout)[0], grad)  # a fixed order: the same bits
+    with torch.no_grad():
+        assert torch.equal(ops.embedding_lookup(w, ids, scale=scale, out_dtype=out_dtype), out)
+
+
+@pytest.mark.parametrize("n", [0, 600, 5000])
+def test_lookup_ids_outside_the_table(n):
+    V, E = 40, 24
+    w, ids, dout = lookup_case(V, E, (n,), F32, torch.int64, None, None, 0.0, 2)
+    ids[::3] = torch.tensor([-1, V, 2 ** 40, -2 ** 40], device=DEV).repeat(n)[:ids[::3].numel()]
+    w.requires_grad_(True)
+    out = ops.embedding_lookup(w, ids, scale=0.5)
+    (grad,) = torch.autograd.grad(out, w, dout)
+    check_lookup(w.detach(), ids, dout, 0.5, None, None, out.detach(), grad)
+
+
+@pytest.mark.parametrize("n", [900, 9000])
+def test_lookup_strides_and_alignment(n):
+    g = gen(3)
+    wide = torch.randn(500, 3 + 64 + 5, generator=g, device=DEV)
+    ids = torch.randint(0, 500, (n // 30, 30), generator=g, device=DEV).t()  # not contiguous
+    dout = torch.randn(30, n // 30, 64, generator=g, device=DEV).transpose(0, 1).contiguous().transpose(0, 1)
+    for first in (0, 1, 2, 3):  # the rows start off a 16-byte boundary, their stride is wider than E
+        w = wide[:, first:first + 64].detach().requires_grad_(True)
+        out = ops.embedding_lookup(w, ids, scale=3.0, padding_idx=7)
+        (grad,) = torch.autograd.grad(out, w, dout)
+        check_lookup(w.detach(), ids, dout, 3.0, 7, None, out.detach(), grad)
+
+
+@pytest.mark.parametrize("n", [900, 9000])
+def test_lookup_non_finite_rows_stay_in_their_places(n):
+    w, ids, dout = lookup_case(50, 16, (n,), F32, torch.int64, None, 0, 0.0, 4)
+    w[0] = math.nan  # the padding row
+    w[1] = math.inf
+    dout[ids == 0] = math.nan  # gradients at padding tokens
+    w.requires_grad_(True)
+    out = ops.embedding_lookup(w, ids, scale=2.0, padding_idx=0)
+    (grad,) = torch.autograd.grad(out, w, dout)
+    assert torch.equal(out.isnan().all(-1), ids == 0) and torch.equal(out.isinf().all(-1), ids == 1)
+    assert grad.isfinite().all() and not grad[0].any()
+
+
+def test_lookup_backward_through_a_loss_matches_differences():
+    w, ids, _ = lookup_case(9, 6, (4, 5), F32, torch.int64, None, 0, 0.0, 5)
+    ids[0, :2] = 3  # the same id twice
+    w.requires_grad_(True)
+    (grad,) = torch.autograd.grad((ops.embedding_lookup(w, ids, scale=1.5, padding_idx=0) ** 2).sum(), w)
+
+    def f(x):  # the loss in 64 bits
+        return ((x[ids] * 1.5) ** 2).sum()
+
+    x, step = w.detach().double(), 1e-4
+    for r in range(1, 9):
+        for e in range(6):
+            lo, hi = x.clone(), x.clone()
+            lo[r, e] -= step
+            hi[r, e] += step
+            want = (f(hi) - f(lo)).item() / (2 * step)  # (exact for a square, up to 2^-53 f / step < 1e-10)
+            assert abs(grad[r, e].item() - want) <= 30 * U * abs(want) + 1e-9
+
+
+@pytest.mark.parametrize("n", [700, 30_000])
+def test_lookup_captured_and_replayed(n):
+    V, E = 400, 64
+    w, ids, dout = lookup_case(V, E, (n,), F32, torch.int64, None, 0, 0.2, 6)
+    w.requires_grad_(True)
+
+    def step():
+        out = ops.embedding_lookup(w, ids, scale=2.0, padding_idx=0)
+        return out.detach(), torch.autograd.grad(out, w, dout)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in range(4):
+        ids.copy_(torch.randint(0, V, (n,), generator=gen(60 + k), device=DEV))
+        dout.copy_(torch.randn(n, E, generator=gen(70 + k), device=DEV))
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
+
+
+def test_lookup_on_another_stream():
+    w, ids, dout = lookup_case(3000, 64, (20_000,), F32, torch.int64, None, 0, 0.1, 7)
+    w.requires_grad_(True)
+    want = torch.autograd.grad(ops.embedding_lookup(w, ids), w, dout)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = torch.autograd.grad(ops.embedding_lookup(w, ids), w, dout)[0]
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_lookup_offsets_beyond_32_bits():
+    V, E, n = 1000, 512, 4_300_000  # 2.2e9 output elements
+    w = torch.randn(V, E, generator=gen(8), device=DEV).to(BF16).requires_grad_(True)
+    ids = torch.randint(0, V, (n,), generator=gen(9), device=DEV, dtype=torch.int32)
+    out = ops.embedding_lookup(w, ids)
+    assert torch.equal(out[-3:], w[ids[-3:].long()])
+    ids.clamp_(0, V - 2)
+    ids[-2:] = V - 1
+    dout = torch.zeros_like(out)
+    dout[-2:] = 1.0
+    (grad,) = torch.autograd.grad(ops.embedding_lookup(w, ids), w, dout)
+    assert (grad[-1] == 2.0).all() and not grad[:-1].any()
+
+
+def test_lookup_embedding_module_uses_the_kernels():
+    emb = tt.embeddings.build("lookup", vocab_size=50, embedding_dim=16, scale=4.0).to(DEV)
+    ids = torch.randint(0, 50, (3, 7), generator=gen(10), device=DEV)
+    with _lib.record_calls() as calls:
+        out = emb(ids)
+        out.sum().backward()
+    assert {"tt_lookup_fwd", "tt_lookup_bwd"} <= calls
+    assert torch.equal(out, emb.embedding(ids) * 4.0)  # a power of two: no rounding
+    count = torch.zeros(50, device=DEV).index_add_(0, ids.flatten(), torch.ones(21, device=DEV))
+    count[0] = 0  # the padding row
+    assert torch.equal(emb.embedding.weight.grad, (4.0 * count).unsqueeze(1).expand(50, 16))
+
+
+# ---------------------------------------------------------------------------------------------
+# preference loss
+def pref_case(B, H, K, dtype, ref, mask, seed):
+    g = gen(seed)
+
+    def rows(*shape):
+        return torch.nn.functional.normalize(torch.randn(*shape, H, generator=g, device=DEV), dim=-1).to(dtype)
+
+    q, p, n = rows(B), rows(B), rows(B, K)
+    r = torch.randn(B, K, generator=g, device=DEV) + 1.0 if ref else None
+    m = torch.rand(B, K, generator=g, device=DEV) >= mask if mask else None
+    return q, p, n, r, m
+
+
+def check_pref(q, p, n, r, m, got, beta=0.5, temperature=0.1, smooth=0.0, kind="sigmoid", upstream=1.0):
+    """got = (loss, dq, dp, dn) against the formulas in 64 bits, within the roundings of an fp32 evaluation."""
+    B, K, H = n.shape
+    on = torch.ones(B, K, dtype=torch.bool, device=DEV) if m is None else m
+    any_on = on.any(1)
+    # absent rows count as zeros: nothing of them may reach a result
+    Q = torch.where(any_on.unsqueeze(1), q.double(), 0.0)
+    P = torch.where(any_on.unsqueeze(1), p.double(), 0.0)
+    N = torch.where(on.unsqueeze(2), n.double(), 0.0)
+    D = (P.unsqueeze(1) - N) * on.unsqueeze(2)
+    h = (Q.unsqueeze(1) * D).sum(2) / temperature - (0 if r is None else r.double())
+    l, dl = pair_terms(h, beta, smooth, kind)
+    l, dl = l * on, dl * on
+    pairs = max(1, int(on.sum()))
+    # h: difference, H products and sums, 1 / temperature and its product, the subtraction of ref
+    eh = ((H + 5) * U * (Q.unsqueeze(1) * D).abs().sum(2) / temperature + 2 * U * (h.abs() + (0 if r is None else r.double().abs()))) * on
+    if kind == "sigmoid":  # |l'| <= beta; l'' <= beta^2 / 4; exp and log1p within 4 steps, sigma and the sums a few more
+        el = beta * eh + 16 * U * (l + on * math.log(2))
+        ed = beta ** 2 / 4 * eh + 16 * U * beta * on
+        ed = ed + beta * 4 * U * (beta * h).abs() * torch.exp(-(beta * h).abs())  # the rounding of beta h
+    else:
+        el = 2 * (h - 0.5 / beta).abs() * (eh + 4 * U * (h.abs() + 0.5 / beta)) + (eh + 4 * U * (h.abs() + 0.5 / beta)) ** 2 + 2 * U * l
+        ed = 2 * (eh + 4 * U * (h.abs() + 0.5 / beta)) * on
+    loss, dq, dp, dn = got
+    check(loss, upstream ** 0 * l.sum() / pairs, el.sum() / pairs + (K + 4) * U * l.sum() / pairs, "loss")
+    G = upstream / (pairs * temperature)
+    wq = G * (dl.unsqueeze(2) * D).sum(1)
+    bq = abs(G) * ((ed + (K + 6) * U * dl.abs()).unsqueeze(2) * D.abs()).sum(1)
+    wp = G * dl.sum(1, keepdim=True) * Q
+    bp = abs(G) * (ed + (K + 6) * U * dl.abs()).sum(1, keepdim=True) * Q.abs()
+    wn = -G * dl.unsqueeze(2) * Q.unsqueeze(1)
+    bn = abs(G) * (ed + 6 * U * dl.abs()).unsqueeze(2) * Q.unsqueeze(1).abs()
+    for a, w, b, t, nm in ((dq, wq, bq, q, "dq"), (dp, wp, bp, p, "dp"), (dn, wn, bn, n, "dn")):
+        check(a, w, b + stored(w.abs() + b, t.dtype), nm)
+
+
+PREFS = [
+    # B, H, K, type, ref, masked share, beta, temperature, smoothing, kind
+    (64, 128, 1, F32, False, 0.0, 1.0, 0.1, 0.0, "sigmoid"),
+    (8192, 256, 1, F32, True, 0.0, 0.5, 0.1, 0.1, "sigmoid"),
+    (1000, 256, 4, BF16, True, 0.3, 0.5, 0.1, 0.0, "squared"),
+    (1, 1, 1, F32, False, 0.0, 0.1, 0.1, 0.0, "sigmoid"),
+    (3, 7, 5, F16, True, 0.5, 1.0, 0.05, 0.0, "sigmoid"),
+    (257, 100, 2, BF16, False, 0.0, 0.1, 1.0, 0.3, "sigmoid"),
+    (33, 1030, 9, F32, True, 0.8, 0.5, 0.1, 0.0, "squared"),
+    (129, 2048, 1, BF16, False, 0.0, 1.0, 0.05, 0.0, "sigmoid"),
+    (5000, 20, 3, F16, True, 0.9, 1.0, 0.1, 0.0, "squared"),
+]
+
+
+@pytest.mark.parametrize("B, H, K, dtype, ref, mask, beta, temperature, smooth, kind", PREFS)
+def test_preference_against_plain(B, H, K, dtype, ref, mask, beta, temperature, smooth, kind):
+    q, p, n, r, m = pref_case(B, H, K, dtype, ref, mask, 20)
+    for t in (q, p, n):
+        t.requires_grad_(True)
+    kw = dict(beta=beta, temperature=temperature, label_smoothing=smooth, loss_type=kind)
+    loss = losses.preference_loss(q, p, n, ref_margin=r, mask=m, **kw)
+    assert loss.dtype == F32 and loss.dim() == 0
+    grads = torch.autograd.grad(loss, (q, p, n))
+    check_pref(q.detach(), p.detach(), n.detach(), r, m, (loss.detach(), *grads), beta, temperature, smooth, kind)
+    again = losses.preference_loss(q, p, n, ref_margin=r, mask=m, **kw)
+    assert torch.equal(again, loss)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(again, (q, p, n)), grads))
+
+
+def test_preference_masked_pairs_are_not_read():
+    q, p, n, r, _ = pref_case(40, 64, 3, F32, True, 0.0, 21)
+    m = torch.ones(40, 3, dtype=torch.bool, device=DEV)
+    m[::4, 1] = False
+    m[5] = False  # a query with no pair left
+    n[~m] = math.nan
+    r[~m] = math.inf
+    q[5], p[5] = math.nan, math.inf
+    for t in (q, p, n):
+        t.requires_grad_(True)
+    loss = losses.preference_loss(q, p, n, ref_margin=r, mask=m, beta=0.5)
+    grads = torch.autograd.grad(loss, (q, p, n))
+    assert not grads[0][5].any() and not grads[1][5].any() and not grads[2][~m].any()
+    check_pref(q.detach(), p.detach(), n.detach(), torch.where(m, r, 0.0), m, (loss.detach(), *grads))
+
+
+@pytest.mark.parametrize("B", [0, 1, 700, 30_000])
+def test_preference_with_no_pair(B):
+    q, p, n, _, _ = pref_case(B, 16, 2, F32, False, 0.0, 22)
+    m = torch.zeros(B, 2, dtype=torch.bool, device=DEV)
+    for t in (q, p, n):
+        t.requires_grad_(True)
+    loss = losses.preference_loss(q, p, n, mask=m)
+    assert loss.item() == 0.0
+    assert all(not g.any() and g.shape == t.shape for g, t in zip(torch.autograd.grad(loss, (q, p, n)), (q, p, n)))
+
+
+def test_preference_extreme_margins():
+    q = torch.ones(4, 1, device=DEV, requires_grad=True)
+    p = torch.tensor([[1e4], [-1e4], [100.0], [-100.0]], device=DEV, requires_grad=True)
+    n = torch.zeros(4, 1, device=DEV, requires_grad=True)
+    loss = losses.preference_loss(q, p, n, beta=1.0, temperature=1.0)
+    dq, dp, dn = torch.autograd.grad(loss, (q, p, n))
+    # softplus(-h): 0, 1e4, e^-100 (below 2^-126), 100; its derivative -sigma(-h): 0, -1, ~0, -1
+    assert abs(loss.item() - 10100 / 4) <= 4 * U * 10100
+    want = torch.tensor([[0.0], [-0.25], [0.0], [-0.25]], dtype=torch.float64, device=DEV)
+    check(dp, want, 1e-40 + U, "dp")
+    check(dn, -want, 1e-40 + U, "dn")
+    assert dq.isfinite().all()
+    (g,) = torch.autograd.grad(losses.preference_loss(q, p, n, beta=1.0, temperature=1.0) * 3.0, p)
+    check(g, 3 * want, 4 * U, "upstream")
+
+
+def test_preference_strides():
+    g = gen(23)
+    wide = torch.randn(50, 5 + 96, generator=g, device=DEV)
+    negs = torch.randn(3, 50, 100, generator=g, device=DEV)  # (K, B, H + 4)
+    q, p = wide[:, 5:37], wide[:, 64:96]
+    n = negs.permute(1, 0, 2)[:, :, 2:34]
+    odd = torch.randn(50, 32, 2, generator=g, device=DEV)[..., 0]  # elements two apart
+    for a, b, c in ((q, p, n), (odd, p, n), (q, odd, negs.permute(1, 0, 2)[:, :, :32])):
+        a, b, c = (t.detach().requires_grad_(True) for t in (a, b, c))
+        loss = losses.preference_loss(a, b, c, beta=0.5, temperature=5.0)
+        grads = torch.autograd.grad(loss, (a, b, c))
+        check_pref(a.detach(), b.detach(), c.detach(), None, None, (loss.detach(), *grads), temperature=5.0)
+
+
+@pytest.mark.parametrize("K", [1, 3])
+def test_preference_on_the_fused_tower_output(K):
+    B, H = 60, 64
+    base = torch.randn((2 + K) * B, H, generator=gen(24), device=DEV, requires_grad=True)
+    y = base * 0.3
+    q, p, n = torch.split(y, [B, B, K * B])
+    n3 = n if K == 1 else n.view(B, K, H)
+    loss = losses.preference_loss(q, p, n3, beta=0.5)
+    assert "Packed" in type(loss.grad_fn).__name__
+    (got,) = torch.autograd.grad(loss, base)
+    a, b, c = (t.detach().clone().requires_grad_(True) for t in (q, p, n3))
+    want = torch.autograd.grad(losses.preference_loss(a, b, c, beta=0.5), (a, b, c))
+    assert torch.equal(got, torch.cat([t.reshape(-1, H) for t in want]) * 0.3)
+
+
+def test_preference_margin_is_the_reference_term():
+    q, p, n, _, _ = pref_case(77, 48, 2, BF16, False, 0.0, 25)
+    r = losses.preference_margin(q.requires_grad_(True), p, n, temperature=0.1)
+    assert not r.requires_grad and r.shape == (77, 2)
+    loss = losses.preference_loss(q, p, n, ref_margin=r, beta=0.5, temperature=0.1)
+    assert abs(loss.item() - math.log(2)) <= 8 * U  # the model is its own reference: every margin is 0
+    one = losses.preference_loss(q, p, n[:, 0], ref_margin=r[:, 0], beta=0.5)
+    assert abs(one.item() - math.log(2)) <= 8 * U
+
+
+@pytest.mark.parametrize("B", [30, 3000])
+def test_preference_captured_and_replayed(B):
+    q, p, n, r, m = pref_case(B, 64, 2, F32, True, 0.3, 26)
+    for t in (q, p, n):
+        t.requires_grad_(True)
+
+    def step():
+        loss = losses.preference_loss(q, p, n, ref_margin=r, mask=m, beta=0.5)
+        return (loss.detach(), *torch.autograd.grad(loss, (q, p, n)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in range(3):
+        new = pref_case(B, 64, 2, F32, True, 0.3 if k < 2 else 1.1, 27 + k)
+        with torch.no_grad():
+            for old, t in zip((q, p, n, r, m), new):
+                old.copy_(t)
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+
+
+# ---------------------------------------------------------------------------------------------
+# gradient norm and clipping
+def clip_case(sizes, types, seed, scale=1.0):
+    g = gen(seed)
+    return [(torch.randn(s, generator=g, device=DEV) * scale).to(t) for s, t in zip(sizes, types)]
+
+
+def check_clip(grads, outs, norm, max_norm, kind):
+    every = torch.cat([x.double().flatten() for x in grads]) if grads else torch.zeros(1, device=DEV).double()
+    want = every.abs().max() if kind == math.inf else every.square().sum().sqrt()
+    check(norm, want, 1.001 * U * want, "norm")  # 64-bit sums of n terms: n 2^-53, then one fp32 rounding
+    coef = (max_norm / (want + 1e-6)).clamp(max=1.0)
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        w = g.double() * coef  # the factor's rounding, the product's, the type's
+        check(o, w, 2.001 * U * w.abs() + stored(w, o.dtype), f"tensor {i}")
+
+
+CLIPS = [
+    ([65536, 256, 65536, 256], [F32] * 4, 1.0, 2.0),
+    ([1], [F32], 0.5, 2.0),
+    ([16384, 16385, 16383, 7], [BF16] * 4, 1.0, 2.0),
+    ([5, 0, 70001, 3], [F16, F32, BF16, F32], 1.0, 2.0),
+    ([5, 0, 70001, 3], [F16, F32, BF16, F32], 0.3, math.inf),
+    ([100_003], [F32], 1e6, 2.0),   # not clipped
+    ([1000] * 128, [F32] * 128, 1.0, 2.0),
+    ([97] * 129 + [30_000] * 150, [F32, BF16, F16] * 93, 1.0, 2.0),  # several launches
+]
+
+
+@pytest.mark.parametrize("sizes, types, max_norm, kind", CLIPS)
+def test_clip_against_plain(sizes, types, max_norm, kind):
+    grads = clip_case(sizes, types, 30)
+    before = [g.clone() for g in grads]
+    norm = ops.clip_grad_norm(grads, None, norm_type=kind)  # the norm alone changes nothing
+    assert all(torch.equal(a, b) for a, b in zip(grads, before))
+    outs = list(torch.split(torch.full((sum(sizes),), 7.0, device=DEV), sizes))  # fp32 views at odd offsets
+    norm2 = ops.clip_grad_norm(grads, max_norm, norm_type=kind, out=outs)
+    assert torch.equal(norm, norm2) and all(torch.equal(a, b) for a, b in zip(grads, before))
+    check_clip(before, outs, norm, max_norm, kind)
+    norm3 = ops.clip_grad_norm(grads, max_norm, norm_type=kind)  # in place
+    assert torch.equal(norm, norm3)
+    check_clip(before, grads, norm, max_norm, kind)
+    if max_norm > norm.item():
+        assert all(torch.equal(a, b) for a, b in zip(grads, before))
+    assert all(torch.equal(o.to(g.dtype), g) for o, g in zip(outs, grads))
+
+
+def test_clip_layouts():
+    g = gen(31)
+    a = torch.randn(300, 40, generator=g, device=DEV).t()          # dense, another order
+    b = torch.randn(64, 50, generator=g, device=DEV)[:, 3:20]      # gaps between the rows
+    c = torch.randn(1001, generator=g, device=DEV)[1:]             # off a 16-byte boundary
+    gap = b._base.clone()
+    before = [t.clone() for t in (a, b, c)]
+    o = [torch.empty(40, 300, device=DEV), torch.empty(64, 17, device=DEV), torch.empty(2000, device=DEV)[::2]]
+    norm = ops.clip_grad_norm([a, b, c], 1.0, out=o)
+    check_clip(before, o, norm, 1.0, 2.0)
+    ops.clip_grad_norm([a, b, c], 1.0)
+    check_clip(before, [a, b, c], norm, 1.0, 2.0)
+    gap[:, 3:20] = b
+    assert torch.equal(gap, b._base)  # the memory between the rows is untouched
+
+
+@pytest.mark.parametrize("v, dtype", [(1e30, F32), (1e-30, F32), (3e38, F32), (6e4, F16), (1e-40, F32)])
+def test_clip_does_not_overflow_before_the_norm(v, dtype):
+    t = torch.full((10_000,), v, dtype=dtype, device=DEV)
+    before = t.clone()
+    norm = ops.clip_grad_norm([t], 1.0)
+    want = before[0].double() * 100
+    if want > torch.finfo(F32).max:  # the norm itself does not fit 32 bits: reported inf, the gradients clipped by it
+        assert norm.isinf()
+    else:
+        check(norm, want, 1.001 * U * want + TINY[F32], "norm")
+    check_w = before.double() * min(1.0, 1.0 / (want.item() + 1e-6))
+    check(t, check_w, 2.001 * U * check_w + stored(check_w, dtype), "clipped")
+
+
+@pytest.mark.parametrize("kind", [2.0, math.inf])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_clip_non_finite_norms_spread_as_in_torch(kind, bad):
+    t = torch.ones(30_000, device=DEV)
+    t[12_345] = bad
+    p = torch.nn.Parameter(torch.zeros_like(t))
+    p.grad = t.clone()
+    want = torch.nn.utils.clip_grad_norm_([p], 1.0, kind)
+    norm = ops.clip_grad_norm([t], 1.0, kind)
+    assert torch.equal(norm.isnan(), want.isnan()) and torch.equal(norm.isinf(), want.isinf())
+    check(t, p.grad, 0.0, "clipped")
+    with pytest.raises(RuntimeError, match="non-finite"):
+        q = torch.nn.Parameter(torch.zeros_like(t))
+        q.grad = torch.full_like(t, bad)
+        optim.clip_grad_norm_([q], 1.0, kind, error_if_nonfinite=True)
+    assert torch.equal(q.grad.isfinite(), torch.zeros_like(t, dtype=torch.bool))  # raised before anything changed
+
+
+def test_clip_of_empty_tensors():
+    norm = ops.clip_grad_norm([torch.empty(0, device=DEV), torch.empty(3, 0, device=DEV)], 1.0)
+    assert norm.item() == 0.0 and norm.device.type == "cuda"
+
+
+def test_clip_grad_norm_of_parameters():
+    ps = [torch.nn.Parameter(torch.zeros(s, device=DEV)) for s in ((30, 40), (7,), (1,))]
+    for p in ps[:2]:
+        p.grad = torch.randn(p.shape, generator=gen(32), device=DEV)
+    before = [p.grad.clone() for p in ps[:2]]
+    norm = optim.clip_grad_norm_((p for p in [*ps, ps[0]]), 1.0)  # one without a gradient, one twice
+    check_clip(before, [p.grad for p in ps[:2]], norm, 1.0, 2.0)
+
+
+def test_clip_offsets_beyond_32_bits():
+    n = 2 ** 31 + 5
+    t = torch.zeros(n, dtype=BF16, device=DEV)
+    t[-3:] = 2.0
+    t[0] = 2.0
+    norm = ops.clip_grad_norm([t], 2.0)
+    assert norm.item() == 4.0
+    assert (t[-3:] == 1.0).all() and t[0] == 1.0 and not t[1:-3].any()
+
+
+def test_clip_captured_and_replayed():
+    sizes, types = [70_000, 33, 5000] * 50, [F32, BF16, F32] * 50  # two launches' lists
+    grads = clip_case(sizes, types, 33)
+    outs = [torch.empty(s, device=DEV) for s in sizes]
+    ops.clip_grad_norm(grads, 1.0, out=outs)
+    graphs, norms = [], []
+    for _ in range(2):  # two graphs over the same tensors: each has its own workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            norms.append(ops.clip_grad_norm(grads, 1.0, out=outs))
+        graphs.append(graph)
+    for k in range(3):
+        for g, new in zip(grads, clip_case(sizes, types, 34 + k, scale=10.0 ** (k - 1))):
+            g.copy_(new)
+        want = [torch.empty_like(o) for o in outs]
+        wn = ops.clip_grad_norm(grads, 1.0, out=want)
+        for graph, norm in zip(graphs, norms):
+            for o in outs:
+                o.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(norm, wn) and all(torch.equal(a, b) for a, b in zip(outs, want)), k
+
+
+# ---------------------------------------------------------------------------------------------
+# 4-bit rows
+def exact_quantize(x, group):
+    """Codes and scales by the definition in 64 bits: bf16(max / 7) and x / scale, each rounded to nearest even."""
+    n, H = x.shape
+    ng = -(-H // group)
+    pad = torch.nn.functional.pad(x.double(), (0, ng * group - H)).view(n, ng, group)
+    s = pad.abs().amax(2) / 7
+    e = torch.floor(torch.log2(s.clamp(min=2.0 ** -126)))
+    step = torch.exp2(e - 7)
+    s = torch.round(s / step) * step  # (torch.round: ties to even)
+    c = torch.where(s.unsqueeze(2) > 0, torch.round(pad / s.unsqueeze(2)), 0.0).clamp(-7, 7)
+    return (c * s.unsqueeze(2)).view(n, -1)[:, :H], s
+
+
+INT4 = [(1, 1, 32), (5, 31, 32), (16, 32, 64), (17, 33, 32), (40, 100, 64), (1000, 128, 128), (333, 256, 32),
+        (50, 300, 128), (19, 4096, 64)]
+
+
+@pytest.mark.parametrize("n, H, group", INT4)
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_int4_quantize_is_the_definition(n, H, group, dtype):
+    x = torch.randn(n, H, generator=gen(40), device=DEV)
+    x[0] = (torch.arange(H, device=DEV) % 15 - 7) * 0.5  # quotients that are integers and halves
+    if n > 2:
+        x[1] = 0.0
+        x[2] *= 1e-3
+    x = x.to(dtype)
+    rows = ops.Int4Rows.quantize(x, group)
+    want, _ = exact_quantize(x, group)
+    assert torch.equal(rows.dequantize().double(), want)
+    # a row's group is off by at most half a step of its scale (and its clamp: the scale's own rounding, 7 2^-8)
+    assert ((want - x.double()).abs() <= 0.5001 * x.double().abs().amax(1, keepdim=True) / 7 * (1 + 2 ** -7)
+            + 7 * 2.0 ** -8 * x.double().abs().amax(1, keepdim=True) / 7).all()
+
+
+def test_int4_quantize_ties_and_extremes():
+    x = torch.zeros(8, 32, device=DEV)
+    x[0] = torch.linspace(-7, 7, 32, device=DEV)
+    x[1, :4] = torch.tensor([7.0, 0.5, 1.5, -2.5], device=DEV)  # scale 1: ties to even
+    x[2] = 1e38
+    x[3] = 1e-37
+    x[4, 3] = math.nan
+    x[5, 3] = math.inf
+    x[6, 0] = 7 * (1 + 2.0 ** -8)  # the quotient is a bf16 tie, exactly
+    x[7, 0] = 1e-42  # a scale below every bf16 number
+    got = ops.Int4Rows.quantize(x, 32).dequantize()
+    assert got[1, :4].tolist() == [7.0, 0.0, 2.0, -2.0]
+    want, _ = exact_quantize(x[[0, 2, 3, 6]], 32)
+    assert torch.equal(got[[0, 2, 3, 6]].double(), want)
+    assert got[4].isnan().all() and got[5].isnan().all()
+    assert got[7].abs().max() <= 1e-42
+
+
+def check_scores(got, q, values, scale_mass, nblk):
+    """values (n, H) 64 bit.  Per 32 columns three chains of 32 exact products added in fp32 (the adders may
+    truncate: a whole step each), the three joined; then one product and one sum per block; q itself
+    to 2^-27 of its largest element."""
+    q = q.double()
+    want = q @ values.t()
+    mass = q.abs() @ values.abs().t()
+    bound = (2 * (3 * 32 + 3) + nblk + 4) * U * mass
+    bound = bound + 2.0 ** -27 * q.abs().amax(1, keepdim=True) * values.abs().sum(1)
+    check(got, want, bound + TINY[F32], "scores")
+
+
+@pytest.mark.parametrize("n, H, group", INT4)
+@pytest.mark.parametrize("nq, dtype", [(1, F32), (4, BF16), (5, F16), (16, F32), (33, F32), (64, BF16), (70, F32)])
+def test_int4_scores_against_plain(n, H, group, nq, dtype):
+    g = gen(41)
+    codes = torch.randint(-8, 8, (n, H), generator=g, device=DEV, dtype=torch.int8)
+    scales = (torch.rand(n, -(-H // group), generator=g, device=DEV) + 0.1).to(BF16)
+    rows = ops.Int4Rows.from_codes(codes, scales, group)
+    values = codes.double() * scales.double().repeat_interleave(group, 1)[:, :H]
+    assert torch.equal(rows.dequantize().double(), values)
+    q = torch.randn(nq, H, generator=g, device=DEV).to(dtype)
+    got = ops.int4_scores(q, rows)
+    assert got.shape == (nq, n) and got.dtype == F32
+    check_scores(got, q, values, scales, -(-H // 32))
+    assert torch.equal(ops.int4_scores(q, rows), got)
+
+
+def test_int4_scores_strides_and_shapes():
+    g = gen(42)
+    x = torch.randn(100, 64, generator=g, device=DEV)
+    rows = ops.Int4Rows.quantize(torch.nn.functional.pad(x, (3, 5))[:, 3:67], 32)  # rows 72 apart, off alignment
+    assert torch.equal(rows.dequantize(), ops.Int4Rows.quantize(x, 32).dequantize())
+    wide = torch.randn(6, 75, generator=g, device=DEV)
+    q = wide[:, 5:69]
+    want = ops.int4_scores(q.contiguous(), rows)
+    assert torch.equal(ops.int4_scores(q, rows), want)
+    assert torch.equal(ops.int4_scores(q.t().contiguous().t(), rows), want)
+    assert torch.equal(ops.int4_scores(q[2], rows), ops.int4_scores(q[2:3], rows))
+    assert torch.equal(ops.int4_scores(q[:1].expand(5, 64), rows)[4], ops.int4_scores(q[:1].repeat(5, 1), rows)[4])
+    assert ops.int4_scores(q[:0], rows).shape == (0, 100)
+    empty = ops.Int4Rows.quantize(x[:0], 32)
+    assert ops.int4_scores(q, empty).shape == (6, 0) and empty.dequantize().shape == (0, 64)
+
+
+def test_int4_scores_query_scales_and_non_finite():
+    g = gen(43)
+    codes = torch.randint(-8, 8, (50, 96), generator=g, device=DEV, dtype=torch.int8)
+    scales = (torch.rand(50, 3, generator=g, device=DEV) + 0.1).to(BF16)
+    scales[7, 1] = math.nan
+    scales[9, 1] = math.inf
+    rows = ops.Int4Rows.from_codes(codes, scales, 32)
+    fine = torch.ones(50, dtype=torch.bool, device=DEV)
+    fine[[7, 9]] = False
+    values = codes.double() * scales.double().repeat_interleave(32, 1)
+    for nq in (4, 12, 40):
+        q = torch.randn(nq, 96, generator=g, device=DEV)
+        q[0] *= 1e-30
+        q[1] *= 1e30
+        q[2, 5] = math.nan
+        q[3] = 0.0
+        got = ops.int4_scores(q, rows)
+        ok = torch.ones(nq, dtype=torch.bool, device=DEV)
+        ok[2] = False
+        check_scores(got[ok][:, fine], q[ok], values[fine], scales, 3)
+        assert got[2].isnan().all() and got[:, 7].isnan().all()
+        assert not got[4:, 9].isfinite().any()
+        assert not got[3, fine].any()
+
+
+def test_int4_scores_offsets_beyond_32_bits():
+    n, H = 34_000_000, 256  # 4.35 GB of codes
+    codes = torch.zeros(n, H, dtype=torch.int8, device=DEV)
+    codes[-5:] = torch.arange(-5, 0, device=DEV, dtype=torch.int8).unsqueeze(1)
+    rows = ops.Int4Rows.from_codes(codes, torch.ones(n, H // 128, dtype=BF16, device=DEV), 128)
+    del codes
+    got = ops.int4_scores(torch.ones(1, H, device=DEV), rows)
+    assert got[0, -5:].tolist() == [-5.0 * H, -4.0 * H, -3.0 * H, -2.0 * H, -1.0 * H]
+    assert not got[0, :-5].any()
+
+
+def test_int4_scores_captured_and_on_another_stream():
+    rows = ops.Int4Rows.quantize(torch.randn(1000, 128, generator=gen(44), device=DEV), 64)
+    q = torch.randn(3, 128, generator=gen(45), device=DEV)
+    ops.int4_scores(q, rows)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.int4_scores(q, rows)
+    for k in range(3):
+        q.copy_(torch.randn(3, 128, generator=gen(46 + k), device=DEV))
+        want = ops.int4_scores(q, rows)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = ops.int4_scores(q, rows)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, want)
+
+
+# ---------------------------------------------------------------------------------------------
+# the operators together: a fine-tuning step and the index that serves its tower
+class TokenTower(torch.nn.Module):
+    """A foreign tower that pools its token rows itself (softmax-weighted by a learned direction)."""
+
+    def __init__(self, embedding, hidden_dim):
+        super().__init__()
+        self.embedding = embedding
+        self.gate = torch.nn.Parameter(torch.randn(embedding.embedding_dim) * 0.1)
+        self.out = torch.nn.Linear(embedding.embedding_dim, hidden_dim)
+
+    def forward(self, ids):
+        rows = self.embedding(ids)
+        a = (rows * self.gate).sum(-1).masked_fill(ids == 0, -1e9).softmax(-1)
+        return torch.nn.functional.normalize(self.out((a.unsqueeze(-1) * rows).sum(1)), dim=-1)
+
+
+def token_model(seed):
+    torch.manual_seed(seed)
+    emb = tt.embeddings.build("lookup", vocab_size=300, embedding_dim=64, scale=8.0)
+    with torch.no_grad():
+        emb.embedding.weight.mul_(0.125)
+    return tt.TwoTower(TokenTower(emb, 128), tied_weights=True)
+
+
+def triplets(B, L, seed):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(1, 300, (3, B, L), generator=g)
+    ids[:, :, L // 2:] *= (torch.rand(3, B, L - L // 2, generator=g) > 0.4)
+    return ids
+
+
+@pytest.mark.parametrize("B", [16, 400])  # 960 and 24,000 tokens a step: both forms of the lookup's gradient
+def test_fine_tuning_step_against_64_bits(B):
+    model, ref64 = token_model(50), token_model(50).double()
+    frozen = token_model(51).to(DEV)
+    model.to(DEV)
+    ids = triplets(B, 20, 52)
+    gpu = ids.to(DEV)
+    with torch.no_grad():
+        ref = losses.preference_margin(*(frozen.encode_query(t) for t in gpu))
+    loss_fn = losses.build("preference", beta=0.5, ref_margin=ref)
+    opt = optim.AdamW(model.parameters(), lr=1e-3, capturable=True)
+    step = tt.TrainStep(model, loss_fn, opt, max_grad_norm=0.05)
+    with _lib.record_calls() as calls:
+        loss = step(*gpu)
+    assert {"tt_lookup_fwd", "tt_lookup_bwd", "tt_preference_fwd", "tt_preference_bwd", "tt_clip_grads"} <= calls
+    # the same step in 64 bits on the CPU
+    q, p, n = (ref64.query_tower(t) for t in ids)
+    h = (q * (p - n)).sum(-1) / 0.1 - ref.cpu().double()[:, 0]
+    want = torch.nn.functional.softplus(-0.5 * h).mean()
+    want.backward()
+    params = [x for x in ref64.parameters()]
+    norm = torch.nn.utils.clip_grad_norm_(params, 0.05)
+    # fp32 towers: some 1e-6 relative in the margins (|h| up to 20), less in their means
+    assert abs(loss.item() - want.item()) < 1e-5 * max(1.0, want.item())
+    assert abs(step.grad_norm.item() - norm.item()) < 1e-4 * norm.item()
+    for a, b in zip(model.parameters(), params):
+        assert (a.grad.cpu().double() - b.grad).norm() <= 1e-4 * b.grad.norm()
+    total = torch.cat([x.grad.flatten() for x in model.parameters()]).double().norm().item()
+    assert abs(total - min(0.05, norm.item())) < 1e-5
+
+
+def test_captured_fine_tuning_equals_eager():
+    batches = [triplets(32, 20, 60 + k).to(DEV) for k in range(6)]
+    runs = []
+    for graph in (False, True):
+        model = token_model(53).to(DEV)
+        opt = optim.AdamW(model.parameters(), lr=1e-2, capturable=True)
+        step = tt.TrainStep(model, losses.build("preference", beta=0.5), opt, graph=graph, max_grad_norm=0.1)
+        runs.append(([step(*b).item() for b in batches], [x.detach().clone() for x in model.parameters()]))
+    # one arithmetic, but library GEMMs may pick another form under capture
+    assert all(abs(a - b) < 1e-4 for a, b in zip(runs[0][0], runs[1][0]))
+    for a, b in zip(runs[0][1], runs[1][1]):
+        assert (a - b).norm() <= 1e-3 * b.norm()
+
+
+def test_clipping_beside_the_hand_written_tower_head():
+    """The mean-pool tower's head may form its weight gradients on a side stream: the norm needs them all."""
+    def build():
+        torch.manual_seed(54)
+        emb = tt.embeddings.build("lookup", vocab_size=500, embedding_dim=256)
+        return tt.build_two_tower("mean", emb, hidden_dim=256, tied_weights=True).to(DEV)
+
+    ids = triplets(64, 12, 55).to(DEV)
+    ref = build()
+    loss = losses.build("preference", beta=0.5)(*ref(*ids))
+    loss.backward()
+    want = torch.nn.utils.clip_grad_norm_(ref.parameters(), 0.01)
+    model = build()
+    opt = optim.AdamW(model.parameters(), capturable=True)
+    step = tt.TrainStep(model, losses.build("preference", beta=0.5), opt, max_grad_norm=0.01)
+    step(*ids)
+    assert abs(step.grad_norm.item() - want.item()) <= 1e-5 * want.item()
+    for a, b in zip(model.parameters(), ref.parameters()):
+        assert (a.grad - b.grad).norm() <= 1e-5 * b.grad.norm()
+
+
+@pytest.mark.parametrize("group", [32, 64])
+def test_search_with_a_4_bit_index(group, tmp_path):
+    model = token_model(56).to(DEV)
+    docs = triplets(500, 20, 57)[0].to(DEV)
+    plain = tt.search.TwoTowerSearch(model)
+    plain.index_document_ids(docs)
+    s = tt.search.TwoTowerSearch(model, index_dtype="int4", index_group=group)
+    s.index_document_ids(docs)
+    assert s.document_embeddings is None and s.index.n == 500
+    queries = docs[:9]
+    scores, idx = s.search_ids(queries, top_k=5)
+    # the top of the scores against the index's own values, in 64 bits
+    q = torch.nn.functional.normalize(plain.encode_queries(queries).double(), dim=-1)
+    want = q @ s.index.dequantize().double().t()
+    top = want.topk(5, dim=1).values
+    assert (scores.double() - top).abs().max() <= 400 * U * 10
+    assert torch.equal(idx[:, 0], torch.arange(9, device=DEV))  # a document is its own nearest
+    # 4 bits: a unit row's values are off by at most half a step of max / 7 each
+    full, _ = plain.search_ids(queries, top_k=5)
+    assert (scores - full).abs().max() < 0.2
+    s.save_index(str(tmp_path / "index.pt"))
+    r = tt.search.TwoTowerSearch(model)
+    r.load_index(str(tmp_path / "index.pt"))
+    again, idx2 = r.search_ids(queries, top_k=5)
+    assert torch.equal(again, scores) and torch.equal(idx2, idx)

@@ -1,0 +1,250 @@
+"""CPU: argument checks of the token lookup, preference loss, gradient clipping and 4-bit index operators, at the
+Python entry points and at the C ABI (every refused call returns before a launch), and the loss
+formulas' derivatives against differences."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import twotower_amd as tt
+from twotower_amd import _lib, losses, ops, optim
+
+P = 4096  # a pointer-shaped value; refused calls never read it
+
+
+# ---------------------------------------------------------------------------------------------
+# Python entry points
+@pytest.mark.parametrize("kw, err, msg", [
+    (dict(weight=torch.zeros(4)), ValueError, "weight must be"),
+    (dict(weight=torch.zeros(0, 4)), ValueError, "weight must be"),
+    (dict(weight=torch.zeros(4, 4, dtype=torch.float64)), TypeError, "weight must be float32"),
+    (dict(ids=torch.zeros(2, dtype=torch.int16)), TypeError, "token ids must be"),
+    (dict(weight=torch.zeros(4, 8).t()), ValueError, "rows must be contiguous"),
+    (dict(weight=torch.zeros(1, 4).expand(5, 4)), ValueError, "must not overlap"),
+    (dict(out_dtype=torch.float64), TypeError, "out_dtype"),
+    (dict(weight=torch.zeros(4, 4, dtype=torch.bfloat16), out_dtype=torch.float32), TypeError, "out_dtype"),
+    (dict(padding_idx=4), ValueError, "padding_idx"),
+    (dict(padding_idx=-5), ValueError, "padding_idx"),
+    (dict(), RuntimeError, "no CPU fallback"),
+])
+def test_lookup_refusals(kw, err, msg):
+    args = dict(weight=torch.zeros(4, 4), ids=torch.zeros(2, 3, dtype=torch.int64))
+    args.update(kw)
+    with pytest.raises(err, match=msg):
+        ops.embedding_lookup(**args)
+
+
+def test_lookup_of_a_column_sharded_table_is_refused(monkeypatch):
+    w = torch.nn.Parameter(torch.zeros(4, 4))
+    w._tt_column = type("Col", (), {"stale": True})()
+    monkeypatch.setattr(_lib, "same_device", lambda *a: None)
+    with pytest.raises(RuntimeError, match="column-sharded"):
+        ops.embedding_lookup(w, torch.zeros(2, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("kw, err, msg", [
+    (dict(p=torch.zeros(3, 5)), ValueError, "q and p must both be"),
+    (dict(q=torch.zeros(3, 4, 1)), ValueError, "q and p must both be"),
+    (dict(n=torch.zeros(2, 4)), ValueError, "n must be"),
+    (dict(n=torch.zeros(3, 0, 4)), ValueError, "n must be"),
+    (dict(n=torch.zeros(3, 2, 5)), ValueError, "n must be"),
+    (dict(p=torch.zeros(3, 4, dtype=torch.bfloat16)), TypeError, "one type"),
+    (dict(ref_margin=torch.zeros(3)), ValueError, "ref_margin must be"),
+    (dict(ref_margin=torch.zeros(3, 2, dtype=torch.int64)), TypeError, "ref_margin must be"),
+    (dict(mask=torch.ones(3, 1, dtype=torch.bool)), ValueError, "mask must be"),
+    (dict(mask=torch.ones(3, 2)), TypeError, "mask must be bool"),
+    (dict(beta=0.0), ValueError, "beta and temperature"),
+    (dict(temperature=-1.0), ValueError, "beta and temperature"),
+    (dict(temperature=math.nan), ValueError, "beta and temperature"),
+    (dict(label_smoothing=1.0), ValueError, "label_smoothing"),
+    (dict(label_smoothing=0.1, loss_type="squared"), ValueError, "label_smoothing"),
+    (dict(loss_type="hinge"), ValueError, "loss_type"),
+    (dict(), RuntimeError, "no CPU fallback"),
+])
+def test_preference_refusals(kw, err, msg):
+    args = dict(q=torch.zeros(3, 4), p=torch.zeros(3, 4), n=torch.zeros(3, 2, 4))
+    args.update(kw)
+    with pytest.raises(err, match=msg):
+        losses.preference_loss(args.pop("q"), args.pop("p"), args.pop("n"), **args)
+
+
+def test_preference_is_built_by_name():
+    f = losses.build("preference", beta=0.5)
+    assert f.func is losses.preference_loss and f.keywords == {"beta": 0.5}
+    assert tt.preference_loss is losses.preference_loss
+
+
+@pytest.mark.parametrize("grads, kw, err, msg", [
+    ([torch.ones(3)], dict(max_norm=-1.0), ValueError, "max_norm"),
+    ([torch.ones(3)], dict(max_norm=math.nan), ValueError, "max_norm"),
+    ([torch.ones(3)], dict(norm_type=1.0), ValueError, "norm_type"),
+    ([torch.ones(3)], dict(out=[]), ValueError, "out tensors"),
+    ([torch.ones(3)], dict(out=[torch.ones(4)]), ValueError, "out 0 has shape"),
+    ([torch.ones(3)], dict(out=[torch.ones(3, dtype=torch.bfloat16)]), TypeError, "gradient 0"),
+    ([torch.ones(3)], dict(max_norm=None, out=[torch.ones(3)]), ValueError, "out needs a max_norm"),
+    ([torch.ones(3, dtype=torch.float64)], {}, TypeError, "gradient 0"),
+    ([torch.ones(3, 3).to_sparse()], {}, RuntimeError, "sparse"),
+    ([torch.ones(1, 3).expand(4, 3)], {}, ValueError, "share memory"),
+    ([torch.ones(3)], {}, RuntimeError, "no CPU fallback"),
+])
+def test_clip_refusals(grads, kw, err, msg):
+    args = dict(max_norm=1.0)
+    args.update(kw)
+    with pytest.raises(err, match=msg):
+        ops.clip_grad_norm(grads, **args)
+
+
+def test_clip_refuses_the_same_memory_twice():
+    t = torch.ones(8)
+    with pytest.raises(ValueError, match="written twice"):
+        ops.clip_grad_norm([t, t.view(2, 4)], 1.0)
+
+
+def test_clip_of_nothing_and_of_a_fused_table():
+    assert ops.clip_grad_norm([], 1.0).item() == 0.0
+    assert optim.clip_grad_norm_([torch.nn.Parameter(torch.ones(2))], 1.0).item() == 0.0
+    w = torch.nn.Parameter(torch.ones(2, 2))
+    w._tt_deferred = ops.DeferredTableGrad()
+    w._tt_deferred.parts.append(("part",))
+    with pytest.raises(RuntimeError, match="factored form"):
+        optim.clip_grad_norm_([w], 1.0)
+
+
+def test_train_step_refuses_clipping_a_fused_table():
+    emb = tt.embeddings.build("lookup", vocab_size=20, embedding_dim=8)
+    model = tt.build_two_tower("mean", emb, hidden_dim=16, tied_weights=True)
+    opt = optim.AdamW(model.parameters(), fused_tables=True, tables=[emb])
+    loss = losses.build("preference")
+    with pytest.raises(ValueError, match="dense gradients"):
+        tt.TrainStep(model, loss, opt, max_grad_norm=1.0)
+    opt.release_tables()
+    tt.TrainStep(model, loss, opt, max_grad_norm=1.0)
+    with pytest.raises(ValueError, match="must not be negative"):
+        tt.TrainStep(model, loss, opt, max_grad_norm=-1.0)
+
+
+def test_a_table_differentiated_both_ways_is_refused():
+    d = ops.DeferredTableGrad()
+    d.added_dense()
+    assert not d.pending()  # a dense gradient alone is stepped as usual ...
+    d.parts.append(("part",))
+    assert d.pending()  # ... and says nothing about the next step
+    d.added_dense()
+    with pytest.raises(RuntimeError, match="pooled lookups only"):
+        d.pending()
+    assert not d.parts and not d.pending()
+
+
+@pytest.mark.parametrize("make, err, msg", [
+    (lambda: ops.Int4Rows.quantize(torch.zeros(4)), ValueError, "x must be"),
+    (lambda: ops.Int4Rows.quantize(torch.zeros(4, 8), group=48), ValueError, "group must be"),
+    (lambda: ops.Int4Rows.quantize(torch.zeros(4, 4097)), ValueError, "rows of 1 to 4096"),
+    (lambda: ops.Int4Rows.quantize(torch.zeros(4, 8, dtype=torch.int32)), TypeError, "x must be float32"),
+    (lambda: ops.Int4Rows.quantize(torch.zeros(4, 8)), RuntimeError, "no CPU fallback"),
+    (lambda: ops.Int4Rows.from_codes(torch.zeros(4, 40), torch.zeros(4, 2).bfloat16()), ValueError, "int8"),
+    (lambda: ops.Int4Rows.from_codes(torch.zeros(4, 40, dtype=torch.int8), torch.zeros(4, 1).bfloat16()), ValueError,
+     r"scales must be \(4, 2\)"),
+    (lambda: ops.Int4Rows.from_codes(torch.zeros(4, 40, dtype=torch.int8), torch.zeros(4, 2)), ValueError, "bfloat16"),
+    (lambda: ops.Int4Rows(torch.zeros(7, dtype=torch.uint8), torch.zeros(7, dtype=torch.uint8), 4, 40, 32), ValueError,
+     "codes must be 512"),
+])
+def test_int4_refusals(make, err, msg):
+    with pytest.raises(err, match=msg):
+        make()
+
+
+def test_search_refuses_an_unknown_index_type():
+    with pytest.raises(ValueError, match="index_dtype"):
+        tt.search.TwoTowerSearch(torch.nn.Identity(), device="cpu", index_dtype="int8")
+
+
+def test_lookup_embedding_on_the_cpu_is_the_plain_gather():
+    emb = tt.embeddings.build("lookup", vocab_size=9, embedding_dim=6, scale=2.0)
+    ids = torch.tensor([[1, 0, 8]])
+    assert torch.equal(emb(ids), emb.embedding(ids) * 2.0)
+    assert list(emb.state_dict()) == ["embedding.weight"]
+
+
+# ---------------------------------------------------------------------------------------------
+# C ABI
+_CLIP = (_lib.ClipTensor * 1)(_lib.ClipTensor(P, P, 3, 0, 0))
+
+
+@pytest.mark.parametrize("name, args, msg", [
+    ("tt_lookup_fwd", (P, 0, 0, 4, 4, P, 0, 1, 1.0, P, 0, None), "V=0 out of range"),
+    ("tt_lookup_fwd", (P, 0, 5, 0, 4, P, 0, 1, 1.0, P, 0, None), "E=0"),
+    ("tt_lookup_fwd", (P, 0, 5, 4, 3, P, 0, 1, 1.0, P, 0, None), "ld_table=3"),
+    ("tt_lookup_fwd", (P, 0, 5, 4, 4, None, 0, 1, 1.0, P, 0, None), "ids is NULL"),
+    ("tt_lookup_fwd", (P, 0, 5, 4, 4, P, 2, 1, 1.0, P, 0, None), "ids_dtype=2"),
+    ("tt_lookup_fwd", (P, 1, 5, 4, 4, P, 0, 1, 1.0, P, 0, None), "rows of type 0"),
+    ("tt_lookup_fwd", (P, 0, 5, 4, 4, P, 0, 2 ** 31, 1.0, P, 0, None), "out of range"),
+    ("tt_lookup_fwd", (None, 0, 5, 4, 4, P, 0, 1, 1.0, P, 0, None), "null pointer"),
+    ("tt_lookup_bwd", (None, 0, P, 0, 1, 5, 4, -1, 1.0, P, 0, None, 0, None), "null pointer"),
+    ("tt_lookup_bwd", (P, 0, P, 0, 5000, 5, 4, -1, 1.0, P, 0, None, 0, None), "workspace too small"),
+    ("tt_preference_fwd", (P, 4, P, 4, P, 4, 4, 3, 2, 1, 4, None, None, 0, 1.0, 1.0, 0.0, P, None, P, P, P, 16, None),
+     "element type 3"),
+    ("tt_preference_fwd", (P, 4, P, 4, P, 4, 4, 0, 2, 0, 4, None, None, 0, 1.0, 1.0, 0.0, P, None, P, P, P, 16, None),
+     "bad shape"),
+    ("tt_preference_fwd", (P, 4, P, 4, P, 4, 4, 0, 2, 1, 4, None, None, 2, 1.0, 1.0, 0.0, P, None, P, P, P, 16, None),
+     "loss kind 2"),
+    ("tt_preference_fwd", (P, 4, P, 4, P, 4, 4, 0, 2, 1, 4, None, None, 0, 0.0, 1.0, 0.0, P, None, P, P, P, 16, None),
+     "must be positive"),
+    ("tt_preference_fwd", (P, 4, P, 4, P, 4, 4, 0, 2, 1, 4, None, None, 0, 1.0, 1.0, 0.0, P, None, P, P, P, 15, None),
+     "workspace too small"),
+    ("tt_preference_fwd", (P, 4, P, 4, P, 4, 4, 0, 2, 1, 4, None, None, 0, 1.0, 1.0, 0.0, P, None, P, None, P, 16, None),
+     "null pointer"),
+    ("tt_preference_bwd", (P, 4, P, 4, P, 4, 4, 0, 2, 1, 4, None, 1.0, P, P, None, P, P, P, None), "null pointer"),
+    ("tt_clip_grads", (None, 1, 0, 1.0, 1, P, P, 1 << 20, None), "null pointer"),
+    ("tt_clip_grads", (_CLIP, 1, 0, -1.0, 1, P, P, 1 << 20, None), "max_norm"),
+    ("tt_clip_grads", (_CLIP, 1, 0, 1.0, 1, P, P, 8, None), "workspace too small"),
+    ("tt_clip_grads", ((_lib.ClipTensor * 1)(_lib.ClipTensor(P, None, 3, 0, 0)), 1, 0, 1.0, 1, P, P, 1 << 20, None),
+     "tensor 0 is NULL"),
+    ("tt_clip_grads", ((_lib.ClipTensor * 1)(_lib.ClipTensor(P, P, 3, 0, 1)), 1, 0, 1.0, 1, P, P, 1 << 20, None),
+     "of type 0 into type 1"),
+    ("tt_clip_grads", ((_lib.ClipTensor * 1)(_lib.ClipTensor(P, P, -1, 0, 0)), 1, 0, 1.0, 1, P, P, 1 << 20, None),
+     "-1 elements"),
+    ("tt_int4_quantize", (P, 0, 4, 4097, 4097, 32, P, P, None), "H=4097"),
+    ("tt_int4_quantize", (P, 0, 4, 64, 63, 32, P, P, None), "ld=63"),
+    ("tt_int4_quantize", (P, 0, 4, 64, 64, 16, P, P, None), "group=16"),
+    ("tt_int4_quantize", (P, 0, 4, 64, 64, 32, P + 4, P, None), "16-byte aligned"),
+    ("tt_int4_pack", (None, P, 4, 64, 32, P, P, None), "null pointer"),
+    ("tt_int4_unpack", (P, P, 4, 64, 32, None, None), "null pointer"),
+    ("tt_int4_scores", (P, 0, 1, 63, P, P, 4, 64, 32, P, None), "ldq=63"),
+    ("tt_int4_scores", (P, 7, 1, 64, P, P, 4, 64, 32, P, None), "query type 7"),
+    ("tt_int4_scores", (P, 0, 1, 64, None, P, 4, 64, 32, P, None), "null pointer"),
+])
+def test_c_abi_refusals(name, args, msg):
+    rc = getattr(_lib.lib(), name)(*args)
+    assert rc == -1
+    assert msg in _lib.last_error(), _lib.last_error()
+
+
+def test_c_abi_sizes():
+    lib = _lib.lib()
+    assert lib.tt_lookup_bwd_ws_size(100, 50, 8) == 0  # short calls take no workspace
+    assert lib.tt_lookup_bwd_ws_size(100_000, 50, 8) > 0
+    assert lib.tt_int4_codes_bytes(17, 33) == 2 * 2 * 256  # two tiles of 16 rows, two 32-column blocks
+    assert lib.tt_int4_scales_bytes(17, 33, 32) == 2 * 1 * 16 * 4 * 2
+    assert lib.tt_clip_ws_size(1) == lib.tt_clip_ws_size(1000) == 2048 * 8
+    assert ctypes.sizeof(_lib.ClipTensor) == 32
+
+
+# ---------------------------------------------------------------------------------------------
+# the formulas the kernels' gradients are tested with, against central differences in 64 bits
+def pair_terms(h, beta, smooth, kind):
+    """(loss, d loss / d h) of margins in 64 bits (numerically stable, from the definition)."""
+    if kind == "sigmoid":
+        sp = torch.nn.functional.softplus
+        x = beta * h
+        return (1 - smooth) * sp(-x) + smooth * sp(x), beta * (smooth - torch.sigmoid(-x))
+    return (h - 0.5 / beta) ** 2, 2 * (h - 0.5 / beta)
+
+
+@pytest.mark.parametrize("kind, smooth", [("sigmoid", 0.0), ("sigmoid", 0.1), ("squared", 0.0)])
+def test_pair_derivative_against_differences(kind, smooth):
+    h = torch.linspace(-6, 6, 41, dtype=torch.float64)
+    step = 1e-5  # a central difference is off by step^2 l''' / 6 + 2^-53 |l| / step < 1e-9
+    lo, hi = (pair_terms(h + d, 0.7, smooth, kind)[0] for d in (-step, step))
+    _, dl = pair_terms(h, 0.7, smooth, kind)
+    assert (((hi - lo) / (2 * step)) - dl).abs().max() < 1e-8

@@ -18,13 +18,13 @@ from .embeddings import BaseEmbedding, LookupEmbedding
 from .encoders import (AveragePoolingTower, BaseTower, MeanPoolingTower, TOWER_REGISTRY, TwoTower, build_tower,
                        build_two_tower)
 from .losses import (LOSS_REGISTRY, contrastive_triplet_loss, in_batch_sampled_softmax_loss,
-                     multiple_negatives_loss)
+                     multiple_negatives_loss, preference_loss, preference_margin)
 from .train_step import TrainStep
 
 __all__ = [
     "BaseEmbedding", "LookupEmbedding", "BaseTower", "MeanPoolingTower", "AveragePoolingTower", "TwoTower",
     "TOWER_REGISTRY", "LOSS_REGISTRY", "build_tower", "build_two_tower", "contrastive_triplet_loss",
-    "multiple_negatives_loss", "in_batch_sampled_softmax_loss", "TrainStep", "install", "data", "distributed",
+    "multiple_negatives_loss", "in_batch_sampled_softmax_loss", "preference_loss", "preference_margin", "TrainStep", "install", "data", "distributed",
     "embeddings", "encoders", "losses", "ops", "optim", "checkpoint", "search",
 ]
 
@@ -49,7 +49,7 @@ def install(package: str = "twotower") -> None:
     enc.TOWER_REGISTRY["avg_pool"] = AveragePoolingTower
     enc.TwoTower = TwoTower
     enc.build_two_tower = build_two_tower
-    for name, fn in LOSS_REGISTRY.items():
+    for name, fn in {**losses.EXTRA_LOSSES, **LOSS_REGISTRY}.items():
         los.LOSS_REGISTRY[name] = fn
     train_mod = sys.modules.get(f"{package}.train")
     if train_mod is not None:

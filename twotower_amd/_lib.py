@@ -18,6 +18,8 @@ LIB_PATH = os.environ.get("TT_LIB") or os.path.join(os.path.dirname(os.path.absp
 HEADER_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "twotower_amd.h")
 
 TT_IDS_I32, TT_IDS_I64 = 0, 1
+ELEM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum tt_elem_dtype
+TT_CLIP_MAX_TENSORS, TT_INT4_MAX_H = 128, 4096
 TT_INBATCH_TAIL_ROWS, TT_INBATCH_MAX_PARTS = 64, 512  # twotower_amd.h
 TT_F32, TT_BF16, TT_BF16_SPLIT = 0, 1, 2
 TT_SCATTER_SORTED, TT_SCATTER_ATOMIC = 0, 1
@@ -47,6 +49,11 @@ class AdamwTensor(ctypes.Structure):
 class AdamwGradParts(ctypes.Structure):
     """tt_adamw_grad_parts"""
     _fields_ = [("part", _vp), ("stride", _c_i64), ("slabs", _c_int)]
+
+
+class ClipTensor(ctypes.Structure):
+    """tt_clip_tensor"""
+    _fields_ = [("src", _vp), ("dst", _vp), ("n", _c_i64), ("src_dtype", _c_int), ("dst_dtype", _c_int)]
 
 
 # name -> (restype, argtypes); must mirror include/twotower_amd.h
@@ -88,6 +95,22 @@ _SIGNATURES = {
     "tt_adamw_multi_ex": (_c_int, [ctypes.POINTER(AdamwTensor), ctypes.POINTER(AdamwGradParts), _c_int,
                                    ctypes.POINTER(AdamSlot), _c_int, _c_f64, _c_f64, _c_f64, _c_f64, _c_f64, _vp,
                                    _vp]),
+    "tt_lookup_fwd": (_c_int, [_vp, _c_int, _c_i64, _c_int, _c_i64, _vp, _c_int, _c_i64, _c_f32, _vp, _c_int, _vp]),
+    "tt_lookup_bwd_ws_size": (_c_sz, [_c_i64, _c_i64, _c_int]),
+    "tt_lookup_bwd": (_c_int, [_vp, _c_int, _vp, _c_int, _c_i64, _c_i64, _c_int, _c_i64, _c_f32, _vp, _c_int, _vp,
+                               _c_sz, _vp]),
+    "tt_preference_fwd": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_int, _vp,
+                                   _vp, _c_int, _c_f32, _c_f32, _c_f32, _vp, _vp, _vp, _vp, _vp, _c_sz, _vp]),
+    "tt_preference_bwd": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_int, _vp,
+                                   _c_f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "tt_clip_ws_size": (_c_sz, [_c_int]),
+    "tt_clip_grads": (_c_int, [_vp, _c_int, _c_int, _c_f64, _c_int, _vp, _vp, _c_sz, _vp]),
+    "tt_int4_codes_bytes": (_c_sz, [_c_i64, _c_int]),
+    "tt_int4_scales_bytes": (_c_sz, [_c_i64, _c_int, _c_int]),
+    "tt_int4_quantize": (_c_int, [_vp, _c_int, _c_i64, _c_int, _c_i64, _c_int, _vp, _vp, _vp]),
+    "tt_int4_pack": (_c_int, [_vp, _vp, _c_i64, _c_int, _c_int, _vp, _vp, _vp]),
+    "tt_int4_unpack": (_c_int, [_vp, _vp, _c_i64, _c_int, _c_int, _vp, _vp]),
+    "tt_int4_scores": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_int, _c_int, _vp, _vp]),
     "tt_cosine_scores": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_int, _vp, _vp]),
     "tt_topk_rows": (_c_int, [_vp, _c_i64, _c_i64, _c_int, _vp, _vp, _vp]),
     "tt_topk_rows_ws_size": (_c_sz, [_c_i64, _c_i64, _c_int]),
@@ -422,6 +445,28 @@ def require_gpu(*tensors: torch.Tensor) -> None:
         if t is not None and not t.is_cuda:
             raise RuntimeError("twotower_amd: the HIP kernels need GPU tensors (no CPU fallback); "
                                f"got a tensor on {t.device}")
+
+
+def same_device(*tensors: torch.Tensor) -> None:
+    """Every tensor on the first one's GPU: a kernel gets raw pointers, so a mixed call would fault."""
+    require_gpu(*tensors)
+    dev = tensors[0].device
+    for t in tensors[1:]:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"twotower_amd: tensors on different devices ({dev} and {t.device})")
+
+
+def on_device(t: torch.Tensor):
+    """Makes t's GPU the current one around a launch (its stream belongs to it); nothing to do, and
+    nothing done, where it is."""
+    return _nullctx() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def elem_dtype_code(t: torch.Tensor, name: str) -> int:
+    code = ELEM_DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
 
 
 def ids_dtype_code(ids: torch.Tensor) -> int:

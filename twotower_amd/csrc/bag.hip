@@ -312,6 +312,7 @@ struct SortSrc {  // pass 0: ids (keys == nullptr); later passes: the previous p
   const int32_t* vals;
   double inv_L;  // 1 / L: the entry -> (sequence, position) split without a 64-bit division
   const int32_t* nvalid;  // passes after the first: the first pass's output length (device)
+  int64_t first;  // the lowest id that is a token: 1 for the bags (id 0 is their mask), 0 for token lookups
   // entries this pass reads: every id slot in the first pass (masked ones are dropped there),
   // the first pass's valid entries after it
   __device__ __forceinline__ int64_t count(int64_t n) const { return keys ? (int64_t)*nvalid : n; }
@@ -331,7 +332,7 @@ struct SortSrc {  // pass 0: ids (keys == nullptr); later passes: the previous p
     seq += (seq + 1) * L <= i ? 1 : 0;
     const int64_t t = i - seq * L;
     const int64_t id = (int64_t)ids[seq * ld + t];
-    const bool valid = id > 0 && id < V && id != padding_idx;
+    const bool valid = id >= first && id < V && id != padding_idx;
     key = valid ? (uint32_t)id : (uint32_t)V;
     val = (int32_t)seq;
   }
@@ -1242,7 +1243,7 @@ struct BwdWs {
 // sum over long rows of ceil(len / piece_len) <= sum (len / kPieceT + 1) < 2 n / kPieceT
 int64_t max_pieces_for(int64_t n) { return 2 * ((n + kPieceT - 1) / kPieceT) + 1; }
 
-BwdWs carve(void* base, int64_t nseq, int L, int64_t V, int E, size_t sort_bytes) {
+BwdWs carve(void* base, int64_t nseq, int L, int64_t V, int E, size_t sort_bytes, bool with_gs = true) {
   BwdWs w{};
   const size_t n = (size_t)nseq * L;
   size_t off = 0;
@@ -1253,7 +1254,7 @@ BwdWs carve(void* base, int64_t nseq, int L, int64_t V, int E, size_t sort_bytes
   };
   char* b = static_cast<char*>(base);
   const size_t o_ki = take(n * 4), o_ko = take(n * 4), o_vi = take(n * 4), o_vo = take(n * 4);
-  const size_t o_gs = take((size_t)nseq * E * 4);
+  const size_t o_gs = take(with_gs ? (size_t)nseq * E * 4 : 0);
   const size_t o_ss = take((size_t)(V + 1) * 4);
   const size_t o_tmp = take(sort_bytes);
   const int64_t mp = max_pieces_for((int64_t)n);
@@ -1403,7 +1404,7 @@ int launch_piece_sum(const BwdWs& w, int64_t V, int E, hipStream_t s) {
 // pieces of long rows (bag_plan_starts_kernel, bag_plan_pieces_kernel).
 template <typename IdT>
 int plan_front(const IdT* ids, int64_t nseq, int L, int64_t ld, int64_t V, int64_t padding_idx, const BwdWs& w,
-               hipStream_t s, int part = -1) {
+               hipStream_t s, int part = -1, int64_t first = 1) {
   // part -1: the whole plan; 0: every sort pass but the last; 1: the last pass, the segment starts
   // and the pieces (tt_bag_plan_part: the two halves on one stream compute what one call does)
   const int64_t n = nseq * L;
@@ -1425,7 +1426,7 @@ int plan_front(const IdT* ids, int64_t nseq, int L, int64_t ld, int64_t V, int64
   int32_t* cnt = static_cast<int32_t*>(w.sort_tmp);
   int32_t* total = cnt + (size_t)nd * sh.ntiles;
   int32_t* nvalid = total + nd;  // written by the first pass's scatter
-  SortSrc<IdT> src{ids, L, ld, V, padding_idx, nullptr, nullptr, L > 0 ? 1.0 / (double)L : 0.0, nvalid};
+  SortSrc<IdT> src{ids, L, ld, V, padding_idx, nullptr, nullptr, L > 0 ? 1.0 / (double)L : 0.0, nvalid, first};
   const int p_begin = part == 1 ? sh.P - 1 : 0, p_end = part == 0 ? sh.P - 1 : sh.P;
   if (p_begin > 0) {  // the previous pass's output (pass p writes _out when P - 1 - p is even)
     const bool prev_out = ((sh.P - 1 - (p_begin - 1)) & 1) == 0;
@@ -1512,6 +1513,27 @@ int check_common(int64_t V, int E, const void* ids, int ids_dtype, int64_t nseq,
 }
 
 }  // namespace
+
+// The same sort for token lookups (lookup.hip): every id in [0, V) is a token, a sequence is one token,
+// so the sorted values are token indices, and there are no scaled rows to keep.
+static BwdWs token_plan_carve(void* ws, int64_t n, int64_t V, int E) {
+  void* base = ws ? reinterpret_cast<void*>(align_up(reinterpret_cast<size_t>(ws), 256)) : nullptr;
+  return carve(base, n, 1, V, E, sort_tmp_bytes(n, V), false);
+}
+
+size_t token_plan_bytes(int64_t n, int64_t V, int E) { return token_plan_carve(nullptr, n, V, E).total + 256; }
+
+int token_plan_build(const void* ids, int ids_dtype, int64_t n, int64_t V, int E, int64_t padding_idx, void* ws,
+                     size_t ws_bytes, TokenPlan* plan, hipStream_t s) {
+  const BwdWs w = token_plan_carve(ws, n, V, E);
+  TT_REQUIRE(n > 0 && ws != nullptr && w.total + 256 <= ws_bytes, "workspace too small: need %zu have %zu",
+             w.total + 256, ws_bytes);
+  *plan = TokenPlan{w.seg_start, w.vals_out, w.nch, w.piece_off, w.piece_beg, w.piece_end, w.partial, w.max_pieces};
+  return ids_dtype == TT_IDS_I32
+             ? plan_front(static_cast<const int32_t*>(ids), n, 1, 1, V, padding_idx, w, s, -1, 0)
+             : plan_front(static_cast<const int64_t*>(ids), n, 1, 1, V, padding_idx, w, s, -1, 0);
+}
+
 }  // namespace tt
 
 using namespace tt;

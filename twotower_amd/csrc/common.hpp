@@ -130,6 +130,61 @@ __device__ __forceinline__ void adam_update(float& p, float g, float& m, float& 
 }
 
 
+// Element types of the token lookup, preference, clipping and 4-bit index kernels (enum tt_elem_dtype).  Each computes
+// in fp32 and rounds a stored element once (nearest even).  VEC consecutive elements move as one access
+// of at most 16 bytes (two for 8 floats), whose alignment the caller checks (vec_for).
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Elems {
+  T v[VEC];
+};
+template <int VEC, typename T>
+__device__ __forceinline__ void load_elems(const T* p, float (&x)[VEC]) {
+  const Elems<T, VEC> e = *reinterpret_cast<const Elems<T, VEC>*>(p);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) x[i] = (float)e.v[i];
+}
+template <int VEC, typename T>
+__device__ __forceinline__ void store_elems(T* p, const float (&x)[VEC]) {
+  Elems<T, VEC> e;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) e.v[i] = (T)x[i];
+  *reinterpret_cast<Elems<T, VEC>*>(p) = e;
+}
+inline int elem_bytes(int dtype) { return dtype == TT_E_F32 ? 4 : 2; }
+inline bool elem_ok(int dtype) { return dtype == TT_E_F32 || dtype == TT_E_BF16 || dtype == TT_E_F16; }
+// The widest VEC in {8, 4, 2, 1} that divides every count in n[] and keeps each pointer's access aligned
+// (pointer i holds elements of bytes[i] bytes; rows start at multiples of the counts).
+inline int vec_for(const int64_t* n, int nn, const void* const* p, const int* bytes, int np) {
+  for (int v = 8; v > 1; v >>= 1) {
+    bool ok = true;
+    for (int i = 0; i < nn; ++i) ok = ok && n[i] % v == 0;
+    for (int i = 0; i < np; ++i) {
+      const size_t a = (size_t)(bytes[i] * v < 16 ? bytes[i] * v : 16);
+      ok = ok && reinterpret_cast<size_t>(p[i]) % a == 0;
+    }
+    if (ok) return v;
+  }
+  return 1;
+}
+
+// The sort plan of a token lookup's gradient (built in bag.hip by the bags' counting sort, read by
+// lookup.hip): row r's tokens are vals[seg_start[r] .. seg_start[r + 1]), in token order; a row of more than
+// kPieceT tokens has nch[r] pieces from slot piece_off[r] (piece k sums tokens piece_beg[k] .. piece_end[k]
+// of vals into partial[k]); piece_off[V] is the number of pieces.
+struct TokenPlan {
+  const int32_t* seg_start;
+  const int32_t* vals;
+  const int32_t* nch;
+  const int32_t* piece_off;
+  const int32_t* piece_beg;
+  const int32_t* piece_end;
+  float* partial;
+  int64_t max_pieces;
+};
+size_t token_plan_bytes(int64_t n, int64_t V, int E);
+int token_plan_build(const void* ids, int ids_dtype, int64_t n, int64_t V, int E, int64_t padding_idx, void* ws,
+                     size_t ws_bytes, TokenPlan* plan, hipStream_t s);
+
 // The tower head's weight planes (tt_head_split*, head.hip): each fp32 weight is cut into three
 // bf16 terms, x = a0 + a1 + a2 exactly.  Job j of SplitJobs writes the three planes of an n x k
 // matrix (W is n x k, or k x n when transposed) at planes_base + off[j]; element i = n * k + k'.

@@ -1,0 +1,293 @@
+// The global norm of many gradient tensors, and clipping by it.
+//
+//   norm = (sum over all tensors of g^2)^(1/2)   or   max |g|
+//   dst  = src * min(1, max_norm / (norm + 1e-6))
+//
+// Bound by bytes: every gradient is read once for the norm and once more to be scaled (from the
+// Infinity Cache where the tensors fit), and written once.  Tensors are cut into chunks; a
+// launch takes up to TT_CLIP_MAX_TENSORS of them by value, so nothing is staged through memory and
+// a captured call keeps its own list.  Squares are added in 64 bits: the norm neither overflows
+// nor underflows before its own rounding to 32 bits, and the vector units have room for it beside
+// the loads.  All sums run in a fixed order (no atomics).
+#include "common.hpp"
+
+namespace tt {
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kChunk = 16384;       // elements per chunk
+constexpr int kMaxParts = 2048;     // partial norms of all launches together
+constexpr int kNormBlocks = 1024;   // workgroups (= partials) of one norm launch
+constexpr int kScaleBlocks = 2048;
+
+struct ClipList {
+  const void* src[TT_CLIP_MAX_TENSORS];
+  void* dst[TT_CLIP_MAX_TENSORS];
+  int64_t n[TT_CLIP_MAX_TENSORS];
+  int32_t first[TT_CLIP_MAX_TENSORS + 1];  // first chunk of each tensor
+  uint8_t type[TT_CLIP_MAX_TENSORS];       // src type | dst type << 2
+  int count;
+};
+
+__device__ __forceinline__ int tensor_of(const ClipList& l, int chunk) {
+  int lo = 0, hi = l.count - 1;  // the last tensor with first[] <= chunk
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (l.first[mid] <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ bool aligned16(const void* p) { return ((size_t)p & 15) == 0; }
+
+template <bool INF>
+__device__ __forceinline__ void norm_add(double& a, float g) {
+  if constexpr (INF) {
+    const double m = (double)fabsf(g);
+    a = (m > a || m != m) ? m : a;  // a NaN stays
+  } else {
+    a = __builtin_fma((double)g, (double)g, a);
+  }
+}
+template <bool INF>
+__device__ __forceinline__ double norm_join(double a, double b) {
+  if constexpr (INF) return (b > a || b != b) ? b : a;
+  else return a + b;
+}
+
+// this thread's part of a chunk: 16-byte accesses where the tensor is aligned, four in flight
+template <typename T, bool INF>
+__device__ __forceinline__ double norm_chunk(const T* __restrict__ p, int n) {
+  constexpr int VEC = 16 / sizeof(T), U = 4;
+  double acc[U] = {};
+  if (aligned16(p)) {
+    const int nv = n / VEC;
+    for (int i = threadIdx.x; i < nv; i += U * kBlock) {
+      float x[U][VEC];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[u][j] = 0.f;
+        if (i + u * kBlock < nv) load_elems<VEC>(p + (size_t)(i + u * kBlock) * VEC, x[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) norm_add<INF>(acc[u], x[u][j]);
+    }
+    for (int i = nv * VEC + threadIdx.x; i < n; i += kBlock) norm_add<INF>(acc[0], (float)p[i]);
+  } else {
+    for (int i = threadIdx.x; i < n; i += 4 * U * kBlock) {
+      float x[4 * U];
+#pragma unroll
+      for (int u = 0; u < 4 * U; ++u) x[u] = i + u * kBlock < n ? (float)p[i + u * kBlock] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 4 * U; ++u) norm_add<INF>(acc[u % U], x[u]);
+    }
+  }
+  return norm_join<INF>(norm_join<INF>(acc[0], acc[1]), norm_join<INF>(acc[2], acc[3]));
+}
+
+template <bool INF>
+__device__ __forceinline__ double block_join(double a) {
+  __shared__ double ws[kBlock / kWave];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) a = norm_join<INF>(a, __shfl_xor(a, o));
+  if (lane_id() == 0) ws[threadIdx.x >> 6] = a;
+  __syncthreads();
+  double r = ws[0];
+#pragma unroll
+  for (int k = 1; k < kBlock / kWave; ++k) r = norm_join<INF>(r, ws[k]);
+  __syncthreads();
+  return r;
+}
+
+template <bool INF>
+__global__ __launch_bounds__(kBlock) void clip_norm_kernel(ClipList l, double* __restrict__ parts) {
+  double acc = 0.0;
+  const int chunks = l.first[l.count];
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const int t = tensor_of(l, c);
+    const int64_t at = (int64_t)(c - l.first[t]) * kChunk;
+    const int64_t left = l.n[t] - at;
+    const int n = (int)(left < kChunk ? left : kChunk);
+    const int ty = l.type[t] & 3;
+    double a;
+    if (ty == TT_E_F32) a = norm_chunk<float, INF>(static_cast<const float*>(l.src[t]) + at, n);
+    else if (ty == TT_E_BF16) a = norm_chunk<__bf16, INF>(static_cast<const __bf16*>(l.src[t]) + at, n);
+    else a = norm_chunk<_Float16, INF>(static_cast<const _Float16*>(l.src[t]) + at, n);
+    acc = norm_join<INF>(acc, a);
+  }
+  acc = block_join<INF>(acc);
+  if (threadIdx.x == 0) parts[blockIdx.x] = acc;
+}
+
+template <bool INF>
+__device__ __forceinline__ double joined_norm(const double* __restrict__ parts, int np) {
+  double a = 0.0;
+  for (int i = threadIdx.x; i < np; i += kBlock) a = norm_join<INF>(a, parts[i]);
+  a = block_join<INF>(a);
+  return INF ? a : __builtin_sqrt(a);
+}
+
+// The factor as a * b: b = 1 but for factors so small (gradients near 1e38) that fp32 would hold them as
+// subnormals of few bits; then b = 2^-64 takes the power and a keeps the 24 bits.
+struct Coef {
+  float a, b;
+  __device__ __forceinline__ float operator()(float x) const { return (x * a) * b; }
+};
+__device__ __forceinline__ Coef clip_coef(double norm, double max_norm) {
+  const double c = max_norm / (norm + 1e-6);
+  if (c > 0.0 && c < 0x1p-100) return Coef{(float)(c * 0x1p64), 0x1p-64f};
+  return Coef{c < 1.0 || c != c ? (float)c : 1.f, 1.f};
+}
+
+template <bool INF>
+__global__ __launch_bounds__(kBlock) void clip_finish_kernel(const double* __restrict__ parts, int np,
+                                                             float* __restrict__ norm) {
+  const double v = joined_norm<INF>(parts, np);
+  if (threadIdx.x == 0) *norm = (float)v;
+}
+
+template <typename TS, typename TD>
+__device__ __forceinline__ void scale_chunk(const TS* src, TD* dst, int n, Coef coef) {
+  constexpr int VEC = 16 / sizeof(TS), U = 4;  // (src may be dst: every element is read by the thread that writes it)
+  if (aligned16(src) && aligned16(dst)) {
+    const int nv = n / VEC;
+    for (int i = threadIdx.x; i < nv; i += U * kBlock) {
+      float x[U][VEC];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * kBlock < nv) load_elems<VEC>(src + (size_t)(i + u * kBlock) * VEC, x[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * kBlock < nv) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) x[u][j] = coef(x[u][j]);
+          store_elems<VEC>(dst + (size_t)(i + u * kBlock) * VEC, x[u]);
+        }
+    }
+    for (int i = nv * VEC + threadIdx.x; i < n; i += kBlock) dst[i] = (TD)coef((float)src[i]);
+  } else {
+    for (int i = threadIdx.x; i < n; i += 4 * U * kBlock) {
+      float x[4 * U];
+#pragma unroll
+      for (int u = 0; u < 4 * U; ++u) x[u] = i + u * kBlock < n ? (float)src[i + u * kBlock] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 4 * U; ++u)
+        if (i + u * kBlock < n) dst[i + u * kBlock] = (TD)coef(x[u]);
+    }
+  }
+}
+
+// Chunks in descending order: the norm pass read the last ones last, so they are still cached.
+template <bool INF>
+__global__ __launch_bounds__(kBlock) void clip_scale_kernel(ClipList l, const double* __restrict__ parts, int np,
+                                                            double max_norm, float* __restrict__ norm) {
+  const double v = joined_norm<INF>(parts, np);
+  const Coef coef = clip_coef(v, max_norm);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
+  const int chunks = l.first[l.count];
+  for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
+    const int t = tensor_of(l, c);
+    const int64_t at = (int64_t)(c - l.first[t]) * kChunk;
+    const int64_t left = l.n[t] - at;
+    const int n = (int)(left < kChunk ? left : kChunk);
+    const int ty = l.type[t];
+    if (coef.a == 1.f && coef.b == 1.f && l.src[t] == l.dst[t]) continue;  // in place and not clipped: nothing changes
+#define TT_SC(TS, TD) scale_chunk<TS, TD>(static_cast<const TS*>(l.src[t]) + at, static_cast<TD*>(l.dst[t]) + at, n, coef)
+    if (ty == (TT_E_F32 | TT_E_F32 << 2)) TT_SC(float, float);
+    else if (ty == (TT_E_BF16 | TT_E_BF16 << 2)) TT_SC(__bf16, __bf16);
+    else if (ty == (TT_E_F16 | TT_E_F16 << 2)) TT_SC(_Float16, _Float16);
+    else if (ty == (TT_E_BF16 | TT_E_F32 << 2)) TT_SC(__bf16, float);
+    else TT_SC(_Float16, float);
+#undef TT_SC
+  }
+}
+
+// tensors [at, at + TT_CLIP_MAX_TENSORS) of the call as one launch's list
+void fill_list(ClipList& l, const tt_clip_tensor* t, int at, int count) {
+  const int m = count - at < TT_CLIP_MAX_TENSORS ? count - at : TT_CLIP_MAX_TENSORS;
+  int64_t chunk = 0;
+  for (int i = 0; i < m; ++i) {
+    l.src[i] = t[at + i].src;
+    l.dst[i] = t[at + i].dst;
+    l.n[i] = t[at + i].n;
+    l.type[i] = (uint8_t)(t[at + i].src_dtype | t[at + i].dst_dtype << 2);
+    l.first[i] = (int32_t)chunk;
+    chunk += (t[at + i].n + kChunk - 1) / kChunk;
+  }
+  l.first[m] = (int32_t)chunk;
+  l.count = m;
+}
+
+template <bool INF>
+int run_clip(const tt_clip_tensor* t, int count, bool scale, double max_norm, float* norm, double* parts,
+             hipStream_t s) {
+  const int launches = (count + TT_CLIP_MAX_TENSORS - 1) / TT_CLIP_MAX_TENSORS;
+  int cap = launches > 0 ? kMaxParts / launches : 1;
+  cap = cap < 1 ? 1 : cap > kNormBlocks ? kNormBlocks : cap;
+  static_assert(sizeof(ClipList) <= 3840, "kernel arguments");
+  ClipList l;
+  int np = 0;
+  for (int at = 0; at < count; at += TT_CLIP_MAX_TENSORS) {
+    fill_list(l, t, at, count);
+    const int chunks = l.first[l.count];
+    if (chunks == 0) continue;
+    const int g = chunks < cap ? chunks : cap;
+    clip_norm_kernel<INF><<<dim3(g), dim3(kBlock), 0, s>>>(l, parts + np);
+    TT_LAUNCH_CHECK("clip_norm");
+    np += g;
+  }
+  bool wrote = false;
+  if (scale)
+    for (int at = 0; at < count; at += TT_CLIP_MAX_TENSORS) {
+      if (launches > 1) fill_list(l, t, at, count);
+      const int chunks = l.first[l.count];
+      if (chunks == 0) continue;
+      const int g = chunks < kScaleBlocks ? chunks : kScaleBlocks;
+      clip_scale_kernel<INF><<<dim3(g), dim3(kBlock), 0, s>>>(l, parts, np, max_norm, wrote ? nullptr : norm);
+      TT_LAUNCH_CHECK("clip_scale");
+      wrote = true;
+    }
+  if (!wrote) {
+    clip_finish_kernel<INF><<<dim3(1), dim3(kBlock), 0, s>>>(parts, np, norm);
+    TT_LAUNCH_CHECK("clip_finish");
+  }
+  return TT_OK;
+}
+
+}  // namespace
+}  // namespace tt
+
+using namespace tt;
+
+extern "C" size_t tt_clip_ws_size(int count) {
+  const int64_t launches = ((int64_t)(count > 0 ? count : 1) + TT_CLIP_MAX_TENSORS - 1) / TT_CLIP_MAX_TENSORS;
+  return sizeof(double) * (size_t)(launches > kMaxParts ? launches : kMaxParts);
+}
+
+extern "C" int tt_clip_grads(const tt_clip_tensor* tensors, int count, int inf_norm, double max_norm, int scale,
+                             float* norm, void* ws, size_t ws_bytes, tt_stream_t stream) {
+  TT_REQUIRE(count >= 0 && (tensors || count == 0) && norm, "clip: null pointer or count=%d", count);
+  TT_REQUIRE(!scale || max_norm >= 0.0, "clip: max_norm must not be negative");
+  TT_REQUIRE(ws && ws_bytes >= tt_clip_ws_size(count) && reinterpret_cast<size_t>(ws) % 8 == 0,
+             "workspace too small: need %zu have %zu", tt_clip_ws_size(count), ws_bytes);
+  for (int i = 0; i < count; ++i) {
+    const tt_clip_tensor& t = tensors[i];
+    TT_REQUIRE(t.n >= 0 && t.n < (int64_t(1) << 37), "clip: tensor %d has %lld elements", i, (long long)t.n);
+    TT_REQUIRE(t.n == 0 || (t.src && (!scale || t.dst)), "clip: tensor %d is NULL", i);
+    TT_REQUIRE(elem_ok(t.src_dtype) && (!scale || t.dst_dtype == t.src_dtype || t.dst_dtype == TT_E_F32),
+               "clip: tensor %d of type %d into type %d", i, t.src_dtype, t.dst_dtype);
+  }
+  for (int at = 0; at < count; at += TT_CLIP_MAX_TENSORS) {  // a launch's chunks are counted in 32 bits
+    int64_t chunks = 0;
+    for (int i = at; i < count && i < at + TT_CLIP_MAX_TENSORS; ++i) chunks += (tensors[i].n + kChunk - 1) / kChunk;
+    TT_REQUIRE(chunks < (int64_t(1) << 31) - kScaleBlocks, "clip: too many elements");
+  }
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  double* parts = static_cast<double*>(ws);
+  return inf_norm ? run_clip<true>(tensors, count, scale != 0, max_norm, norm, parts, s)
+                  : run_clip<false>(tensors, count, scale != 0, max_norm, norm, parts, s);
+}

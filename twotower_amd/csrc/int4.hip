@@ -1,0 +1,455 @@
+// 4-bit rows with group scales, and their products with a few fp32 vectors: the document index of the
+// search at 4.5 bits a value (group 32) instead of 32.
+//
+//   score[i, j] = sum_g s_jg sum_{k in g} (c_jk - 8) q_ik
+//
+// One or a few queries are bound by the index bytes (n (H / 2 + 2 H / group)); 256 codes a row leave no
+// time to widen each code to a float in vector instructions, so the inner sums run on the
+// matrix cores: codes are small integers, exact in fp16, and q is cut into three fp16 terms
+// (33 bits of it), so v_mfma_f32_16x16x32_f16 forms the sum of 32 exact products in fp32; the group's
+// scale multiplies that sum.  32 columns are the instruction's K and the smallest group.
+//
+// Layout (written once per index): tiles of 16 rows; a tile is a run of quads of 128 columns, a quad
+// of 64 lanes x 16 bytes in the order the kernel loads it: lane (row j = l % 16, h = l / 16), dword d
+// holds row j's columns 128 quad + 32 d + 8 h .. + 7.  A wave's load is 1 KB of consecutive bytes and
+// dword d is the B operand of column block d without any exchange.  A short last quad has as many
+// dwords a lane as column blocks.  Nibble s of a dword is column 2 s, nibble s + 4 column 2 s + 1, so
+// (u >> 4 s) & 0x000f000f is an fp16 pair in operand order.  Scales: per tile and quad, 16 rows x 128 / group.
+#include "common.hpp"
+
+namespace tt {
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kWavesPerBlock = kBlock / kWave;
+constexpr int kRows = 16;   // documents per tile
+constexpr int kBlk = 32;    // columns per matrix instruction
+constexpr int kQuad = 128;  // columns per lane load
+constexpr int kTPW = 2;     // tiles a wave scores together (they share the query operands' LDS reads)
+constexpr uint32_t kZeroCodes = 0x88888888u;
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+inline int blocks_of(int H) { return (H + kBlk - 1) / kBlk; }
+inline int quads_of(int H) { return (H + kQuad - 1) / kQuad; }
+inline int64_t tiles_of(int64_t n) { return (n + kRows - 1) / kRows; }
+
+__device__ __forceinline__ float bf16_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+
+// where row `row`'s dwords of column block b are: dword h at [h * 16 * dpl], dpl = dwords per lane of its quad
+__device__ __forceinline__ int64_t code_word(int64_t row, int b, int nblk, int& dpl) {
+  const int quad = b >> 2, d = b & 3;
+  dpl = nblk - 4 * quad < 4 ? nblk - 4 * quad : 4;
+  return (row / kRows) * nblk * 64 + quad * 256 + (row % kRows) * dpl + d;
+}
+__device__ __forceinline__ int64_t scale_at(int64_t row, int b, int nquad, int group) {
+  const int spq = kQuad / group, quad = b >> 2;
+  return (((row / kRows) * nquad + quad) * kRows + row % kRows) * spq + (b & 3) * kBlk / group;
+}
+
+// 8 codes (0..15) of columns 8 h .. 8 h + 7 -> their dword
+__device__ __forceinline__ uint32_t pack8(const int* c) {
+  uint32_t u = 0;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) u |= (uint32_t)c[2 * s] << (4 * s) | (uint32_t)c[2 * s + 1] << (4 * s + 16);
+  return u;
+}
+
+__device__ __forceinline__ void write_codes(uint32_t* codes, int64_t row, int b, int nblk, const int* c) {
+  int dpl;
+  const int64_t at = code_word(row, b, nblk, dpl);
+#pragma unroll
+  for (int h = 0; h < 4; ++h) codes[at + (int64_t)h * kRows * dpl] = pack8(c + 8 * h);
+}
+
+// max / 7 rounded to bf16, to nearest even of the exact quotient: the fp32 quotient is on the right side
+// of every bf16 midpoint unless it equals one, and 7 x a midpoint (9 bits) is exact in fp32.
+__device__ __forceinline__ uint16_t group_scale(float mx) {
+  const uint32_t u = __float_as_uint(mx / 7.f);
+  uint32_t r = u >> 16;
+  const uint32_t low = u & 0xffffu;
+  bool up = low > 0x8000u;
+  if (low == 0x8000u) {
+    const float d = __builtin_fmaf(-7.f, __uint_as_float(u), mx);  // sign of the exact difference
+    up = d > 0.f || (d == 0.f && (r & 1));
+  }
+  return (uint16_t)(r + (up ? 1 : 0));
+}
+
+// the integer nearest to x / s (ties to even), |x / s| <= 7.5: x - r s is exact in fp32 for the small
+// integers r next to the quotient, so the comparison with s / 2 decides the rounding exactly.
+__device__ __forceinline__ int group_code(float x, float s) {
+  float r = rintf(x / s);
+  const float d = __builtin_fmaf(-r, s, x);
+  const float twice = 2.f * d;
+  const bool odd = ((int)r) & 1;
+  if (twice > s || (twice == s && odd)) r += 1.f;
+  else if (twice < -s || (twice == -s && odd)) r -= 1.f;
+  return (int)fminf(fmaxf(r, -7.f), 7.f);
+}
+
+// One thread per (row, column block); the lanes of a group join their maxima.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void int4_quantize_kernel(const T* __restrict__ x, int64_t n, int H, int64_t ld,
+                                                               int group, int nblk, int nquad,
+                                                               uint32_t* __restrict__ codes,
+                                                               uint16_t* __restrict__ scales) {
+  const int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  const int64_t row = id / (4 * nquad);
+  const int b = (int)(id - row * (4 * nquad));
+  if (row >= (n + kRows - 1) / kRows * kRows) return;  // (whole groups of lanes leave together)
+  float v[kBlk];
+  float mx = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kBlk; ++i) {
+    const int k = b * kBlk + i;
+    v[i] = row < n && k < H ? (float)x[row * ld + k] : 0.f;
+    bad = bad || !(fabsf(v[i]) <= 3.402823466e38f);
+    mx = fmaxf(mx, fabsf(v[i]));
+  }
+  for (int o = 1; o < group / kBlk; o <<= 1) {
+    mx = fmaxf(mx, __shfl_xor(mx, o));
+    bad = __shfl_xor((int)bad, o) || bad;
+  }
+  uint16_t sb = group_scale(mx);
+  if (bad) sb = 0x7fc0u;
+  if ((b & (group / kBlk - 1)) == 0) scales[scale_at(row, b, nquad, group)] = sb;
+  if (b >= nblk) return;
+  const float s = bf16_value(sb);
+  int c[kBlk];
+#pragma unroll
+  for (int i = 0; i < kBlk; ++i) c[i] = 8 + ((bad || s == 0.f) ? 0 : group_code(v[i], s));
+  write_codes(codes, row, b, nblk, c);
+}
+
+__global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restrict__ src,
+                                                           const uint16_t* __restrict__ sc, int64_t n, int H,
+                                                           int group, int nblk, int nquad,
+                                                           uint32_t* __restrict__ codes,
+                                                           uint16_t* __restrict__ scales) {
+  const int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  const int64_t row = id / (4 * nquad);
+  const int b = (int)(id - row * (4 * nquad));
+  if (row >= (n + kRows - 1) / kRows * kRows) return;
+  const int ng = (H + group - 1) / group, g = b * kBlk / group;
+  if ((b & (group / kBlk - 1)) == 0)
+    scales[scale_at(row, b, nquad, group)] = row < n && g < ng ? sc[row * ng + g] : (uint16_t)0;
+  if (b >= nblk) return;
+  int c[kBlk];
+#pragma unroll
+  for (int i = 0; i < kBlk; ++i) {
+    const int k = b * kBlk + i;
+    const int v = row < n && k < H ? (int)src[row * H + k] : 0;
+    c[i] = 8 + (v < -8 ? -8 : v > 7 ? 7 : v);
+  }
+  write_codes(codes, row, b, nblk, c);
+}
+
+__global__ __launch_bounds__(kBlock) void int4_unpack_kernel(const uint32_t* __restrict__ codes,
+                                                             const uint16_t* __restrict__ scales, int64_t n, int H,
+                                                             int group, int nblk, int nquad, float* __restrict__ out) {
+  const int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  const int64_t row = id / nblk;
+  const int b = (int)(id - row * nblk);
+  if (row >= n) return;
+  const float s = bf16_value(scales[scale_at(row, b, nquad, group)]);
+  int dpl;
+  const int64_t at = code_word(row, b, nblk, dpl);
+  for (int h = 0; h < 4; ++h) {
+    const uint32_t u = codes[at + (int64_t)h * kRows * dpl];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = b * kBlk + 8 * h + i;
+      const int c = (int)(u >> (4 * (i >> 1) + 16 * (i & 1))) & 15;
+      if (k < H) out[row * H + k] = (float)(c - 8) * s;
+    }
+  }
+}
+
+// ---- scores.  Query rows are the A operand (16 rows), documents the B operand, so a lane of the
+// result holds one document (column l % 16) and the four A rows 4 h .. 4 h + 3 of its quarter h = l / 16.
+//   NQT = 0: up to 4 queries; A rows 4 i, 4 i + 1, 4 i + 2 are query i's three terms, so one instruction
+//            does all of them and the lane adds its own rows;
+//   NQT > 0: 16 queries per A operand, NQT operands; three instructions chain the terms.
+template <int NQT>
+struct QueryTiles {
+  static constexpr int kOps = NQT == 0 ? 1 : 3 * NQT;   // A operands per column block
+  static constexpr int kQ = NQT == 0 ? 4 : 16 * NQT;    // queries per pass
+  static constexpr int kAcc = NQT == 0 ? 1 : 4 * NQT;   // results per lane and document tile
+};
+
+__device__ __forceinline__ f16x8 widen(uint32_t u) {
+  // nibble pairs under the exponent of 1024 are the fp16 numbers 1024 + c; minus 1032: c - 8, exact
+  union { f16x8 v; f16x2 p[4]; uint32_t w[4]; } r;
+  const f16x2 bias = {(_Float16)(-1032.f), (_Float16)(-1032.f)};
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    r.w[s] = ((u >> (4 * s)) & 0x000f000fu) | 0x64006400u;
+    r.p[s] += bias;
+  }
+  return r.v;
+}
+
+// 2^3 <= max |q| 2^e < 2^4: the fp16 terms then reach 2^-27 of the largest element or 33 bits below the element
+__device__ __forceinline__ int query_exponent(float mx) {
+  return mx > 0.f && mx <= 3.402823466e38f ? 3 - ilogbf(mx) : 0;
+}
+
+template <typename T, int NQT, int SPQ>
+__global__ __launch_bounds__(kBlock) void int4_scores_kernel(const T* __restrict__ q, int nq, int64_t ldq,
+                                                             const uint32_t* __restrict__ codes,
+                                                             const uint16_t* __restrict__ scales, int64_t n, int H,
+                                                             int nblk, int nquad, float* __restrict__ scores,
+                                                             int64_t ld_scores) {
+  using Q = QueryTiles<NQT>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  f16x8* A = reinterpret_cast<f16x8*>(smem);  // [4 nquad][kOps][64]
+  __shared__ int qe[Q::kQ];
+  const int lane = lane_id(), w = threadIdx.x >> 6, j = lane & 15, h = lane >> 4;
+  for (int i = w; i < Q::kQ; i += kWavesPerBlock) {
+    float mx = 0.f;
+    if (i < nq)
+      for (int k = lane; k < H; k += kWave) mx = fmaxf(mx, fabsf((float)q[i * ldq + k]));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    if (lane == 0) qe[i] = query_exponent(mx);
+  }
+  __syncthreads();
+  for (int it = threadIdx.x; it < 4 * nquad * Q::kOps * kWave; it += kBlock) {
+    const int l = it & 63, a = (it >> 6) % Q::kOps, b = (it >> 6) / Q::kOps;
+    const int m = l & 15, k0 = b * kBlk + 8 * (l >> 4);
+    const int i = NQT == 0 ? m >> 2 : (a / 3) * 16 + m;   // query
+    const int term = NQT == 0 ? m & 3 : a % 3;
+    f16x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int k = k0 + e;
+      const float x = i < nq && k < H && term < 3 ? ldexpf((float)q[i * ldq + k], qe[i]) : 0.f;
+      const _Float16 t0 = (_Float16)x;
+      const float r1 = x - (float)t0;
+      const _Float16 t1 = (_Float16)r1;
+      const _Float16 t2 = (_Float16)(r1 - (float)t1);
+      v[e] = term == 0 ? t0 : term == 1 ? t1 : t2;
+    }
+    A[it] = v;
+  }
+  __syncthreads();
+
+  const int64_t ntile = (n + kRows - 1) / kRows;
+  const int64_t step = (int64_t)gridDim.x * kWavesPerBlock * kTPW;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t t0 = ((int64_t)blockIdx.x * kWavesPerBlock + w) * kTPW; t0 < ntile; t0 += step) {
+    float acc[kTPW][Q::kAcc] = {};
+    for (int b = 0; b < nquad; ++b) {
+      const int dpl = nblk - 4 * b < 4 ? nblk - 4 * b : 4;
+      uint32_t c[kTPW][4];
+      float s[kTPW][SPQ];
+#pragma unroll
+      for (int u = 0; u < kTPW; ++u) {
+        const int64_t t = t0 + u < ntile ? t0 + u : ntile - 1;  // (a clamped tile is never stored)
+        const uint32_t* p = codes + t * nblk * 64 + b * 256 + lane * dpl;
+        if (dpl == 4) {
+          const tt_u32x4 x = *reinterpret_cast<const tt_u32x4*>(p);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) c[u][d] = x[d];
+        } else {
+#pragma unroll
+          for (int d = 0; d < 4; ++d) c[u][d] = d < dpl ? p[d] : kZeroCodes;
+        }
+        const Elems<uint16_t, SPQ> x =
+            *reinterpret_cast<const Elems<uint16_t, SPQ>*>(scales + ((t * nquad + b) * kRows + j) * SPQ);
+#pragma unroll
+        for (int g = 0; g < SPQ; ++g) s[u][g] = bf16_value(x.v[g]);
+      }
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        if (d >= dpl) break;
+        f16x8 B[kTPW];
+#pragma unroll
+        for (int u = 0; u < kTPW; ++u) B[u] = widen(c[u][d]);
+        const f16x8* Ab = A + (size_t)(4 * b + d) * Q::kOps * kWave + lane;
+        if constexpr (NQT == 0) {
+          const f16x8 a = Ab[0];
+#pragma unroll
+          for (int u = 0; u < kTPW; ++u) {
+            const f32x4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, B[u], zero, 0, 0, 0);
+            acc[u][0] = __builtin_fmaf(s[u][d * SPQ / 4], (r[2] + r[1]) + r[0], acc[u][0]);
+          }
+        } else {
+#pragma unroll
+          for (int qt = 0; qt < NQT; ++qt) {
+            const f16x8 a0 = Ab[(3 * qt) * kWave], a1 = Ab[(3 * qt + 1) * kWave], a2 = Ab[(3 * qt + 2) * kWave];
+#pragma unroll
+            for (int u = 0; u < kTPW; ++u) {
+              f32x4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(a2, B[u], zero, 0, 0, 0);
+              r = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, B[u], r, 0, 0, 0);
+              r = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, B[u], r, 0, 0, 0);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                acc[u][4 * qt + e] = __builtin_fmaf(s[u][d * SPQ / 4], r[e], acc[u][4 * qt + e]);
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kTPW; ++u) {
+      const int64_t doc = (t0 + u) * kRows + j;
+      if (doc >= n) continue;
+#pragma unroll
+      for (int r = 0; r < Q::kAcc; ++r) {
+        const int i = NQT == 0 ? h : 16 * (r >> 2) + 4 * h + (r & 3);
+        if (i < nq) scores[i * ld_scores + doc] = ldexpf(acc[u][r], -qe[i]);
+      }
+    }
+  }
+}
+
+constexpr size_t kMaxLds = 96 * 1024;  // query operands per workgroup
+
+template <typename T, int NQT, int SPQ>
+int launch_scores(const T* q, int nq, int64_t ldq, const uint32_t* codes, const uint16_t* scales, int64_t n, int H,
+                  float* scores, int64_t ld_scores, hipStream_t s) {
+  const int nquad = quads_of(H);
+  const size_t lds = (size_t)4 * nquad * QueryTiles<NQT>::kOps * kWave * 16;
+  const int64_t groups = (tiles_of(n) + kTPW * kWavesPerBlock - 1) / (kTPW * kWavesPerBlock);
+  const int per_cu = lds > 64 * 1024 ? 1 : lds > 32 * 1024 ? 2 : lds > 16 * 1024 ? 4 : 8;
+  const int64_t most = 256 * per_cu;
+  auto kernel = int4_scores_kernel<T, NQT, SPQ>;
+  if (lds > 64 * 1024)
+    TT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)lds), "int4_scores LDS");
+  kernel<<<dim3((unsigned)(groups < most ? groups : most)), dim3(kBlock), lds, s>>>(
+      q, nq, ldq, codes, scales, n, H, blocks_of(H), nquad, scores, ld_scores);
+  TT_LAUNCH_CHECK("int4_scores");
+  return TT_OK;
+}
+
+template <typename T, int SPQ>
+int scores_passes(const T* q, int64_t nq, int64_t ldq, const uint32_t* codes, const uint16_t* scales, int64_t n, int H,
+                  float* scores, hipStream_t s) {
+  const size_t lds16 = (size_t)4 * quads_of(H) * 3 * kWave * 16;  // one 16-query operand set
+  for (int64_t i = 0; i < nq;) {
+    const int64_t left = nq - i;
+    const T* qi = q + i * ldq;
+    float* si = scores + i * n;
+    int rc, m;
+    if (left <= 4 || lds16 > kMaxLds) {
+      m = (int)(left < 4 ? left : 4);
+      rc = launch_scores<T, 0, SPQ>(qi, m, ldq, codes, scales, n, H, si, n, s);
+    } else if (left <= 16 || 2 * lds16 > kMaxLds) {
+      m = (int)(left < 16 ? left : 16);
+      rc = launch_scores<T, 1, SPQ>(qi, m, ldq, codes, scales, n, H, si, n, s);
+    } else if (left <= 32 || 4 * lds16 > kMaxLds) {
+      m = (int)(left < 32 ? left : 32);
+      rc = launch_scores<T, 2, SPQ>(qi, m, ldq, codes, scales, n, H, si, n, s);
+    } else {
+      m = (int)(left < 64 ? left : 64);
+      rc = launch_scores<T, 4, SPQ>(qi, m, ldq, codes, scales, n, H, si, n, s);
+    }
+    if (rc) return rc;
+    i += m;
+  }
+  return TT_OK;
+}
+
+template <typename T>
+int scores_groups(const void* q, int64_t nq, int64_t ldq, const void* codes, const void* scales, int64_t n, int H,
+                  int group, float* out, hipStream_t s) {
+  const T* tq = static_cast<const T*>(q);
+  const uint32_t* c = static_cast<const uint32_t*>(codes);
+  const uint16_t* sc = static_cast<const uint16_t*>(scales);
+  if (group == 32) return scores_passes<T, 4>(tq, nq, ldq, c, sc, n, H, out, s);
+  if (group == 64) return scores_passes<T, 2>(tq, nq, ldq, c, sc, n, H, out, s);
+  return scores_passes<T, 1>(tq, nq, ldq, c, sc, n, H, out, s);
+}
+
+int check_int4(int64_t n, int H, int group, const void* codes, const void* scales) {
+  TT_REQUIRE(n >= 0 && n < (int64_t(1) << 40) / TT_INT4_MAX_H, "int4: n=%lld rows out of range", (long long)n);
+  TT_REQUIRE(H >= 1 && H <= TT_INT4_MAX_H, "int4: H=%d must be in [1, %d]", H, TT_INT4_MAX_H);
+  TT_REQUIRE(group == 32 || group == 64 || group == 128, "int4: group=%d must be 32, 64 or 128", group);
+  TT_REQUIRE(n == 0 || (codes && scales), "null pointer");
+  TT_REQUIRE(reinterpret_cast<size_t>(codes) % 16 == 0 && reinterpret_cast<size_t>(scales) % 16 == 0,
+             "int4: codes and scales must be 16-byte aligned");
+  return TT_OK;
+}
+
+// threads of the layout kernels: one per (row of a whole tile, column block of a whole quad)
+inline int64_t layout_blocks(int64_t n, int H) {
+  return (tiles_of(n) * kRows * 4 * quads_of(H) + kBlock - 1) / kBlock;
+}
+
+}  // namespace
+}  // namespace tt
+
+using namespace tt;
+
+extern "C" size_t tt_int4_codes_bytes(int64_t n, int H) {
+  return n < 0 || H < 1 ? 0 : (size_t)tiles_of(n) * blocks_of(H) * 256;
+}
+
+extern "C" size_t tt_int4_scales_bytes(int64_t n, int H, int group) {
+  return n < 0 || H < 1 || group < 1 ? 0 : (size_t)tiles_of(n) * quads_of(H) * kRows * (kQuad / group) * 2;
+}
+
+extern "C" int tt_int4_quantize(const void* x, int dtype, int64_t n, int H, int64_t ld, int group, void* codes,
+                                void* scales, tt_stream_t stream) {
+  if (int rc = check_int4(n, H, group, codes, scales)) return rc;
+  TT_REQUIRE(elem_ok(dtype) && ld >= H && (x || n == 0), "int4: element type %d, ld=%lld", dtype, (long long)ld);
+  if (n == 0) return TT_OK;
+  TT_REQUIRE(layout_blocks(n, H) < (int64_t(1) << 31), "int4: too many values");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)layout_blocks(n, H)), block(kBlock);
+#define TT_QZ(T)                                                                                              \
+  int4_quantize_kernel<T><<<grid, block, 0, s>>>(static_cast<const T*>(x), n, H, ld, group, blocks_of(H),     \
+                                                 quads_of(H), static_cast<uint32_t*>(codes),                  \
+                                                 static_cast<uint16_t*>(scales))
+  if (dtype == TT_E_F32) TT_QZ(float);
+  else if (dtype == TT_E_BF16) TT_QZ(__bf16);
+  else TT_QZ(_Float16);
+#undef TT_QZ
+  TT_LAUNCH_CHECK("int4_quantize");
+  return TT_OK;
+}
+
+extern "C" int tt_int4_pack(const int8_t* c, const void* sc, int64_t n, int H, int group, void* codes, void* scales,
+                            tt_stream_t stream) {
+  if (int rc = check_int4(n, H, group, codes, scales)) return rc;
+  TT_REQUIRE(n == 0 || (c && sc), "null pointer");
+  if (n == 0) return TT_OK;
+  TT_REQUIRE(layout_blocks(n, H) < (int64_t(1) << 31), "int4: too many values");
+  int4_pack_kernel<<<dim3((unsigned)layout_blocks(n, H)), dim3(kBlock), 0, reinterpret_cast<hipStream_t>(stream)>>>(
+      c, static_cast<const uint16_t*>(sc), n, H, group, blocks_of(H), quads_of(H), static_cast<uint32_t*>(codes),
+      static_cast<uint16_t*>(scales));
+  TT_LAUNCH_CHECK("int4_pack");
+  return TT_OK;
+}
+
+extern "C" int tt_int4_unpack(const void* codes, const void* scales, int64_t n, int H, int group, float* out,
+                              tt_stream_t stream) {
+  if (int rc = check_int4(n, H, group, codes, scales)) return rc;
+  TT_REQUIRE(n == 0 || out, "null pointer");
+  if (n == 0) return TT_OK;
+  const int64_t blocks = (n * blocks_of(H) + kBlock - 1) / kBlock;
+  TT_REQUIRE(blocks < (int64_t(1) << 31), "int4: too many values");
+  int4_unpack_kernel<<<dim3((unsigned)blocks), dim3(kBlock), 0, reinterpret_cast<hipStream_t>(stream)>>>(
+      static_cast<const uint32_t*>(codes), static_cast<const uint16_t*>(scales), n, H, group, blocks_of(H),
+      quads_of(H), out);
+  TT_LAUNCH_CHECK("int4_unpack");
+  return TT_OK;
+}
+
+extern "C" int tt_int4_scores(const void* q, int dtype, int64_t nq, int64_t ldq, const void* codes, const void* scales,
+                              int64_t n, int H, int group, float* scores, tt_stream_t stream) {
+  if (int rc = check_int4(n, H, group, codes, scales)) return rc;
+  TT_REQUIRE(nq >= 0 && elem_ok(dtype) && ldq >= H, "int4: nq=%lld, query type %d, ldq=%lld", (long long)nq, dtype,
+             (long long)ldq);
+  if (nq == 0 || n == 0) return TT_OK;
+  TT_REQUIRE(q && scores, "null pointer");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == TT_E_F32) return scores_groups<float>(q, nq, ldq, codes, scales, n, H, group, scores, s);
+  if (dtype == TT_E_BF16) return scores_groups<__bf16>(q, nq, ldq, codes, scales, n, H, group, scores, s);
+  return scores_groups<_Float16>(q, nq, ldq, codes, scales, n, H, group, scores, s);
+}

@@ -1,0 +1,363 @@
+// Token lookup with a scale, and its gradient by sorted tokens.
+//
+//   out[t, :]  = s W[id_t, :]                                  (ids outside [0, V): a zero row)
+//   dW[r, :]   = s sum_{t : id_t = r, r != padding_idx} dout[t, :]     (every row written)
+//
+// Both move bytes and add: the forward reads each token's row (repeated rows from L2) and writes
+// n E elements, the backward reads n E elements once and writes V E.  The backward needs each
+// row's tokens together: a long call sorts them (the bags' stable counting sort, token_plan_build), a short one
+// lets every workgroup pick the tokens of its own rows from the ids.
+#include "common.hpp"
+
+namespace tt {
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kWavesPerBlock = kBlock / kWave;
+
+__device__ __forceinline__ int64_t id_at(const void* ids, bool wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(ids)[i] : (int64_t)static_cast<const int32_t*>(ids)[i];
+}
+
+// log2 of the lanes that hold one row: the smallest power of two covering its E / VEC accesses.
+inline int row_lanes_log2(int E, int vec) {
+  int l = 0;
+  while (l < 6 && (vec << l) < E) ++l;
+  return l;
+}
+
+// ---- forward: a group of 2^lg lanes per token, U tokens in flight per group.
+template <typename TW, typename TO, int VEC, int U>
+__global__ __launch_bounds__(kBlock) void lookup_fwd_kernel(const TW* __restrict__ table, int64_t V, int E, int64_t ld,
+                                                            const void* __restrict__ ids, bool wide, int64_t n,
+                                                            float scale, TO* __restrict__ out, int lg) {
+  const int lane = lane_id(), groups = kWave >> lg, sub = lane >> lg, c = lane & ((1 << lg) - 1);
+  const int64_t wave = (int64_t)blockIdx.x * kWavesPerBlock + (threadIdx.x >> 6);
+  const int64_t t0 = wave * groups * U + sub;
+  int64_t id[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t t = t0 + (int64_t)u * groups;
+    id[u] = t < n ? id_at(ids, wide, t) : -1;
+  }
+  for (int e = c * VEC; e < E; e += VEC << lg) {
+    float x[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[u][i] = 0.f;
+      if (id[u] >= 0 && id[u] < V) load_elems<VEC>(table + id[u] * ld + e, x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t t = t0 + (int64_t)u * groups;
+      if (t < n) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[u][i] = (id[u] >= 0 && id[u] < V) ? scale * x[u][i] : 0.f;
+        store_elems<VEC>(out + t * E + e, x[u]);
+      }
+    }
+  }
+}
+
+// ---- gradient of a short call (n <= kDirectN): one launch, no workspace.  A workgroup owns R
+// consecutive rows; it reads all ids, keeps its own tokens in LDS in token order, and a wave per
+// row adds that row's tokens.  A row with more than kCoop tokens is shared by the workgroup's waves,
+// each adding the tokens of its part of the list, folded in wave order.
+constexpr int kDirectN = 4096;
+constexpr int kDirectThreads = 512;
+constexpr int kDirectWaves = kDirectThreads / kWave;
+constexpr int kDirectRows = 64;
+constexpr int kCoop = 64;
+
+// acc += the rows of dout named by list[beg, end) whose local row is r, in list order
+template <typename TO, int VEC>
+__device__ __forceinline__ void direct_add(const TO* __restrict__ dout, int E, int e, bool on,
+                                           const uint32_t* list, int beg, int end, int r, float (&acc)[VEC]) {
+  constexpr int U = 8;
+  const int lane = lane_id();
+  for (int b = beg; b < end; b += kWave) {
+    const uint32_t v = b + lane < end ? list[b + lane] : 0xffffffffu;
+    uint64_t m = __ballot((int)(v & 255u) == r);
+    while (m) {
+      int64_t tok[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        tok[u] = m ? (int64_t)(__builtin_amdgcn_readlane((int)v, __builtin_ctzll(m)) >> 8) : -1;
+        m &= m - 1;  // (0 stays 0)
+      }
+      float x[U][VEC];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[u][i] = 0.f;
+        if (on && tok[u] >= 0) load_elems<VEC>(dout + tok[u] * E + e, x[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (tok[u] >= 0) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) acc[i] += x[u][i];
+        }
+    }
+  }
+}
+
+template <typename TO, typename TW, int VEC>
+__global__ __launch_bounds__(kDirectThreads) void lookup_grad_direct_kernel(
+    const TO* __restrict__ dout, const void* __restrict__ ids, bool wide, int n, int64_t V, int E, int R, int64_t pad,
+    float scale, TW* __restrict__ grad) {
+  __shared__ uint32_t list[kDirectN];  // token << 8 | local row
+  __shared__ int cnt[kDirectRows];
+  __shared__ int wcnt[kDirectWaves];
+  __shared__ float part[kDirectWaves][kWave * VEC];
+  const int lane = lane_id(), w = threadIdx.x >> 6;
+  const int64_t r0 = (int64_t)blockIdx.x * R;
+  const int rows = (int)(V - r0 < R ? V - r0 : R);
+  if (threadIdx.x < kDirectRows) cnt[threadIdx.x] = 0;
+  int m = 0;  // tokens kept so far (the same in every thread)
+  __syncthreads();
+  for (int base = 0; base < n; base += kDirectThreads) {
+    const int i = base + threadIdx.x;
+    const int64_t id = i < n ? id_at(ids, wide, i) : -1;
+    const bool mine = id >= r0 && id < r0 + rows && id != pad;
+    const uint64_t b = __ballot(mine);
+    if (lane == 0) wcnt[w] = __popcll(b);
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int k = 0; k < kDirectWaves; ++k) {
+      before += k < w ? wcnt[k] : 0;
+      all += wcnt[k];
+    }
+    if (mine) {
+      const int local = (int)(id - r0);
+      list[m + before + __popcll(b & ((uint64_t(1) << lane) - 1))] = (uint32_t)i << 8 | (uint32_t)local;
+      atomicAdd(&cnt[local], 1);
+    }
+    m += all;
+    __syncthreads();
+  }
+  for (int r = w; r < rows; r += kDirectWaves) {
+    const int c = cnt[r];
+    if (c > kCoop) continue;
+    for (int e0 = 0; e0 < E; e0 += kWave * VEC) {
+      const int e = e0 + lane * VEC;
+      float acc[VEC] = {};
+      if (c) direct_add<TO, VEC>(dout, E, e, e < E, list, 0, m, r, acc);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] *= scale;
+      if (e < E) store_elems<VEC>(grad + (r0 + r) * E + e, acc);
+    }
+  }
+  const int share = (m + kDirectWaves - 1) / kDirectWaves;
+  for (int r = 0; r < rows; ++r) {
+    if (cnt[r] <= kCoop) continue;
+    for (int e0 = 0; e0 < E; e0 += kWave * VEC) {
+      const int e = e0 + lane * VEC;
+      float acc[VEC] = {};
+      direct_add<TO, VEC>(dout, E, e, e < E, list, min(w * share, m), min((w + 1) * share, m), r, acc);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) part[w][lane * VEC + i] = acc[i];
+      __syncthreads();
+      if (w == 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          float a = part[0][lane * VEC + i];
+#pragma unroll
+          for (int k = 1; k < kDirectWaves; ++k) a += part[k][lane * VEC + i];
+          acc[i] = a * scale;
+        }
+        if (e < E) store_elems<VEC>(grad + (r0 + r) * E + e, acc);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ---- gradient of a long call, from the sort plan.  A group of 2^lg lanes adds the entries
+// [beg, end): U running sums (entry k to sum k % U), folded in order.
+template <typename T, int VEC, int U, bool INDIRECT>
+__device__ __forceinline__ void sorted_add(const T* __restrict__ src, const int32_t* __restrict__ vals, int E, int e,
+                                           int beg, int end, float (&acc)[VEC]) {
+  float part[U][VEC];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) part[u][i] = 0.f;
+  for (int k = beg; k < end; k += U) {
+    int64_t row[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) row[u] = k + u < end ? (INDIRECT ? (int64_t)vals[k + u] : (int64_t)(k + u)) : -1;
+    float x[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[u][i] = 0.f;
+      if (row[u] >= 0) load_elems<VEC>(src + row[u] * E + e, x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) part[u][i] += x[u][i];
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    acc[i] = part[0][i];
+#pragma unroll
+    for (int u = 1; u < U; ++u) acc[i] += part[u][i];
+  }
+}
+
+template <typename TO, int VEC>
+__global__ __launch_bounds__(kBlock) void lookup_piece_sum_kernel(TokenPlan p, const TO* __restrict__ dout, int64_t V,
+                                                                  int E, int lg) {
+  const int lane = lane_id(), groups = kWave >> lg, sub = lane >> lg, c = lane & ((1 << lg) - 1);
+  const int64_t np = p.piece_off[V];
+  const int64_t step = (int64_t)gridDim.x * kWavesPerBlock * groups;
+  for (int64_t k = ((int64_t)blockIdx.x * kWavesPerBlock + (threadIdx.x >> 6)) * groups + sub; k < np; k += step) {
+    const int beg = p.piece_beg[k], end = p.piece_end[k];
+    for (int e = c * VEC; e < E; e += VEC << lg) {
+      float acc[VEC];
+      sorted_add<TO, VEC, 8, true>(dout, p.vals, E, e, beg, end, acc);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) p.partial[k * E + e + i] = acc[i];
+    }
+  }
+}
+
+template <typename TO, typename TW, int VEC>
+__global__ __launch_bounds__(kBlock) void lookup_row_sum_kernel(TokenPlan p, const TO* __restrict__ dout, int64_t V,
+                                                                int E, float scale, TW* __restrict__ grad, int lg) {
+  const int lane = lane_id(), groups = kWave >> lg, sub = lane >> lg, c = lane & ((1 << lg) - 1);
+  const int64_t r = ((int64_t)blockIdx.x * kWavesPerBlock + (threadIdx.x >> 6)) * groups + sub;
+  if (r >= V) return;
+  const int np = p.nch[r], beg = p.seg_start[r], end = p.seg_start[r + 1];
+  for (int e = c * VEC; e < E; e += VEC << lg) {
+    float acc[VEC];
+    if (np > 0) {
+      const int k = p.piece_off[r];
+      sorted_add<float, VEC, 4, false>(p.partial, nullptr, E, e, k, k + np, acc);
+    } else {
+      sorted_add<TO, VEC, 4, true>(dout, p.vals, E, e, beg, end, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] *= scale;
+    store_elems<VEC>(grad + r * E + e, acc);
+  }
+}
+
+template <typename TW, typename TO>
+int launch_fwd(const void* table, int64_t V, int E, int64_t ld, const void* ids, bool wide, int64_t n, float scale,
+               void* out, hipStream_t s) {
+  const int64_t counts[] = {E, ld};
+  const void* ptrs[] = {table, out};
+  const int bytes[] = {(int)sizeof(TW), (int)sizeof(TO)};
+  int vec = vec_for(counts, 2, ptrs, bytes, 2);
+  if (sizeof(TW) == 4 && sizeof(TO) == 4 && vec > 4) vec = 4;
+  const int lg = row_lanes_log2(E, vec);
+  constexpr int U = 4;
+  const int64_t per_block = (int64_t)kWavesPerBlock * (kWave >> lg) * U;
+  const dim3 grid((unsigned)((n + per_block - 1) / per_block)), block(kBlock);
+  const TW* t = static_cast<const TW*>(table);
+  TO* o = static_cast<TO*>(out);
+#define TT_LF(VV) \
+  case VV: lookup_fwd_kernel<TW, TO, VV, U><<<grid, block, 0, s>>>(t, V, E, ld, ids, wide, n, scale, o, lg); break;
+  switch (vec) { TT_LF(8) TT_LF(4) TT_LF(2) default: TT_LF(1) }
+#undef TT_LF
+  TT_LAUNCH_CHECK("lookup_fwd");
+  return TT_OK;
+}
+
+template <typename TW, typename TO>
+int launch_bwd(const void* dout, const void* ids, int ids_dtype, int64_t n, int64_t V, int E, int64_t pad, float scale,
+               void* grad, void* ws, size_t ws_bytes, hipStream_t s) {
+  const int64_t counts[] = {E};
+  const void* ptrs[] = {n > 0 ? dout : grad, grad};
+  const int bytes[] = {(int)sizeof(TO), (int)sizeof(TW)};
+  int vec = vec_for(counts, 1, ptrs, bytes, 2);
+  if (sizeof(TW) == 4 && sizeof(TO) == 4 && vec > 4) vec = 4;
+  const TO* d = static_cast<const TO*>(dout);
+  TW* g = static_cast<TW*>(grad);
+  if (n <= kDirectN) {
+    int64_t R = V / 1024;
+    R = R < 1 ? 1 : R > kDirectRows ? kDirectRows : R;
+    const dim3 grid((unsigned)((V + R - 1) / R)), block(kDirectThreads);
+#define TT_LD(VV) \
+  case VV: lookup_grad_direct_kernel<TO, TW, VV><<<grid, block, 0, s>>>(d, ids, ids_dtype == TT_IDS_I64, (int)n, V, E, (int)R, pad, scale, g); break;
+    switch (vec) { TT_LD(8) TT_LD(4) TT_LD(2) default: TT_LD(1) }
+#undef TT_LD
+    TT_LAUNCH_CHECK("lookup_grad_direct");
+    return TT_OK;
+  }
+  TokenPlan p;
+  if (int rc = token_plan_build(ids, ids_dtype, n, V, E, pad, ws, ws_bytes, &p, s)) return rc;
+  const int lg = row_lanes_log2(E, vec), groups = kWave >> lg;
+  const int64_t pb = (p.max_pieces + kWavesPerBlock * groups - 1) / (kWavesPerBlock * groups);
+  const dim3 pgrid((unsigned)(pb < 2048 ? pb : 2048)), block(kBlock);
+  const dim3 rgrid((unsigned)((V + kWavesPerBlock * groups - 1) / (kWavesPerBlock * groups)));
+#define TT_LS(VV)                                                                                   \
+  case VV:                                                                                          \
+    lookup_piece_sum_kernel<TO, VV><<<pgrid, block, 0, s>>>(p, d, V, E, lg);                         \
+    TT_LAUNCH_CHECK("lookup_piece_sum");                                                            \
+    lookup_row_sum_kernel<TO, TW, VV><<<rgrid, block, 0, s>>>(p, d, V, E, scale, g, lg);             \
+    break;
+  switch (vec) { TT_LS(8) TT_LS(4) TT_LS(2) default: TT_LS(1) }
+#undef TT_LS
+  TT_LAUNCH_CHECK("lookup_row_sum");
+  return TT_OK;
+}
+
+int check_lookup(int64_t n, int64_t V, int E, const void* ids, int ids_dtype, int table_dtype, int out_dtype) {
+  TT_REQUIRE(V > 0 && V < (int64_t(1) << 31) - 1, "V=%lld out of range", (long long)V);
+  TT_REQUIRE(E > 0, "E=%d must be positive", E);
+  TT_REQUIRE(n >= 0 && n < (int64_t(1) << 31), "n=%lld tokens out of range", (long long)n);
+  TT_REQUIRE(ids_dtype == TT_IDS_I32 || ids_dtype == TT_IDS_I64, "ids_dtype=%d", ids_dtype);
+  TT_REQUIRE(ids != nullptr || n == 0, "ids is NULL");
+  TT_REQUIRE(elem_ok(table_dtype) && elem_ok(out_dtype) && (out_dtype == table_dtype || table_dtype == TT_E_F32),
+             "lookup: rows of type %d from a table of type %d", out_dtype, table_dtype);
+  return TT_OK;
+}
+
+}  // namespace
+}  // namespace tt
+
+using namespace tt;
+
+// (table, row) types: equal, or fp32 -> 16 bit
+#define TT_LOOKUP_TYPES(TABLE, ROW, CALL)                                                     \
+  do {                                                                                       \
+    if ((TABLE) == TT_E_BF16) return CALL(__bf16, __bf16);                                   \
+    if ((TABLE) == TT_E_F16) return CALL(_Float16, _Float16);                                \
+    if ((ROW) == TT_E_BF16) return CALL(float, __bf16);                                      \
+    if ((ROW) == TT_E_F16) return CALL(float, _Float16);                                     \
+    return CALL(float, float);                                                               \
+  } while (0)
+
+extern "C" int tt_lookup_fwd(const void* table, int table_dtype, int64_t V, int E, int64_t ld_table, const void* ids,
+                             int ids_dtype, int64_t n, float scale, void* out, int out_dtype, tt_stream_t stream) {
+  if (int rc = check_lookup(n, V, E, ids, ids_dtype, table_dtype, out_dtype)) return rc;
+  TT_REQUIRE(ld_table >= E, "ld_table=%lld < E=%d", (long long)ld_table, E);
+  if (n == 0) return TT_OK;
+  TT_REQUIRE(table && out, "null pointer");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+#define TT_CALL(TW, TO) (launch_fwd<TW, TO>(table, V, E, ld_table, ids, ids_dtype == TT_IDS_I64, n, scale, out, s))
+  TT_LOOKUP_TYPES(table_dtype, out_dtype, TT_CALL);
+#undef TT_CALL
+}
+
+extern "C" size_t tt_lookup_bwd_ws_size(int64_t n, int64_t V, int E) {
+  return n <= kDirectN || V <= 0 || E <= 0 ? 0 : token_plan_bytes(n, V, E);
+}
+
+extern "C" int tt_lookup_bwd(const void* dout, int dout_dtype, const void* ids, int ids_dtype, int64_t n, int64_t V,
+                             int E, int64_t padding_idx, float scale, void* grad, int grad_dtype, void* ws,
+                             size_t ws_bytes, tt_stream_t stream) {
+  if (int rc = check_lookup(n, V, E, ids, ids_dtype, grad_dtype, dout_dtype)) return rc;
+  TT_REQUIRE(grad && (dout || n == 0), "null pointer");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+#define TT_CALL(TW, TO) \
+  (launch_bwd<TW, TO>(dout, ids, ids_dtype, n, V, E, padding_idx, scale, grad, ws, ws_bytes, s))
+  TT_LOOKUP_TYPES(grad_dtype, dout_dtype, TT_CALL);
+#undef TT_CALL
+}

@@ -32,12 +32,21 @@ class BaseEmbedding(nn.Module, ABC):
         logger.info(f"Embedding parameters: {self.vocab_size * self.embedding_dim:,}")
 
 
+def _plain_embedding(m: nn.Module) -> bool:
+    """An nn.Embedding whose forward is nothing but the row gather of a type the HIP lookup has."""
+    return (type(m) is nn.Embedding and m.max_norm is None and not m.scale_grad_by_freq and not m.sparse
+            and m.weight.dtype in _lib.ELEM_DTYPES and not m._forward_hooks and not m._forward_pre_hooks)
+
+
 class LookupEmbedding(BaseEmbedding):
     """Trainable lookup table (twotower/embeddings.py:24-40) with a fused pooled lookup."""
 
     def __init__(self, vocab_size: int, embedding_dim: int, padding_idx: int = 0,
-                 scatter_mode: str = "sorted"):
+                 scatter_mode: str = "sorted", scale: float = 1.0):
+        """scale: factor of the token rows that forward() returns (e.g. embedding_dim ** 0.5); the pooled
+        lookup is the reference's and takes none."""
         super().__init__(vocab_size, embedding_dim, padding_idx)
+        self.scale = float(scale)
         self.embedding = nn.Embedding(vocab_size, embedding_dim, padding_idx=padding_idx)
         if scatter_mode not in ("sorted", "atomic"):
             raise ValueError(f"scatter_mode must be 'sorted' or 'atomic', got {scatter_mode!r}")
@@ -49,9 +58,14 @@ class LookupEmbedding(BaseEmbedding):
         return self.embedding.weight
 
     def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
-        """(B, L) ids -> (B, L, E) rows: the reference's unfused contract, kept for foreign
-        towers.  The towers of this package never call it (they use pool_mean)."""
-        return self.embedding(input_ids)
+        """(B, L) ids -> (B, L, E) rows times ``scale``: the reference's unfused contract, for foreign
+        towers.  The towers of this package never call it (they use pool_mean).  On the GPU one HIP
+        gather forward and, for the dense table gradient, a sum over sorted tokens (ops.embedding_lookup)."""
+        inner = self.embedding
+        if input_ids.is_cuda and inner.weight.is_cuda and _plain_embedding(inner):
+            return ops.embedding_lookup(inner.weight, input_ids, self.scale, inner.padding_idx)
+        rows = inner(input_ids)
+        return rows if self.scale == 1.0 else rows * self.scale
 
     def pool_mean(self, input_ids: torch.Tensor) -> torch.Tensor:
         """(B, L) ids -> (B, E): sum_{ids>0} W[ids] / (count + 1e-9) on the HIP bag kernel

@@ -63,6 +63,40 @@ def multiple_negatives_loss(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg_
     return ops.MultiNegLoss.apply(q_emb, d_pos_emb, d_neg_embs, 1.0 / float(temperature))
 
 
+def preference_loss(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg_embs: torch.Tensor,
+                    ref_margin: torch.Tensor | None = None, mask: torch.Tensor | None = None, beta: float = 0.1,
+                    temperature: float = 0.1, label_smoothing: float = 0.0,
+                    loss_type: str = "sigmoid") -> torch.Tensor:
+    """Paired preference loss (log ratios) of (query, preferred, rejected) embeddings.
+
+    Under the in-batch softmax (logits q . d / temperature) the log ratio of two documents of a query
+    is (q . p - q . n) / temperature.  Pair (i, k) has the margin
+    h = q_i . (p_i - n_ik) / temperature - ref_margin_ik, with ``ref_margin`` the same log ratio under a frozen
+    reference model (preference_margin; None: 0), and the loss is the mean over the pairs of
+      "sigmoid":  (1 - label_smoothing) softplus(-beta h) + label_smoothing softplus(beta h)
+      "squared":  (h - 1 / (2 beta))^2.
+
+    q_emb, d_pos_emb (B, H); d_neg_embs (B, H) or (B, K, H); one of float32 / bfloat16 / float16, computed in
+    fp32, gradients rounded once.  ref_margin: (B, K) floats ((B,) for K = 1), a constant.  mask: (B, K)
+    bool, False for a missing pair, whose row is not read (it may hold anything), counts nothing and gets
+    a zero gradient; with no pair left the loss is 0."""
+    packed = None
+    if d_neg_embs.dim() in (2, 3) and q_emb.dim() == 2 and d_neg_embs.is_contiguous():
+        B, K = q_emb.shape[0], 1 if d_neg_embs.dim() == 2 else d_neg_embs.shape[1]
+        if B and K and d_pos_emb.shape == q_emb.shape and d_neg_embs.numel() == B * K * q_emb.shape[1]:
+            packed = _packed(q_emb, d_pos_emb, d_neg_embs.view(B * K, -1))
+    return ops.preference_loss(q_emb, d_pos_emb, d_neg_embs, ref_margin=ref_margin, mask=mask, beta=beta,
+                               temperature=temperature, label_smoothing=label_smoothing, loss_type=loss_type,
+                               packed=packed)
+
+
+def preference_margin(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg_embs: torch.Tensor,
+                      temperature: float = 0.1) -> torch.Tensor:
+    """(B, K) float32 log ratios q_i . (p_i - n_ik) / temperature, without gradients: a frozen model's give the
+    ``ref_margin`` of preference_loss, the trained model's its reward margins."""
+    return ops.preference_margin(q_emb, d_pos_emb, d_neg_embs, temperature)
+
+
 def _candidates(p: torch.Tensor, n: torch.Tensor) -> torch.Tensor:
     """cat([p, n]) without a copy when p and n are consecutive row blocks of one tensor
     (TwoTower's fused output): a narrow() of their common base, so autograd stays exact."""
@@ -138,11 +172,16 @@ LOSS_REGISTRY = {
     "multiple_negatives": multiple_negatives_loss,
     "in_batch": in_batch_sampled_softmax_loss,
 }
+# losses of this package beside the reference's names (build() and install() offer both)
+EXTRA_LOSSES = {
+    "preference": preference_loss,
+}
 
 
 def build(name: str, **kwargs) -> Callable:
     """Loss by name with bound kwargs (losses.py:129-150)."""
-    if name not in LOSS_REGISTRY:
-        raise ValueError(f"Unknown loss function: {name}. Available options: {list(LOSS_REGISTRY.keys())}")
-    fn = LOSS_REGISTRY[name]
+    known = {**EXTRA_LOSSES, **LOSS_REGISTRY}
+    if name not in known:
+        raise ValueError(f"Unknown loss function: {name}. Available options: {[*LOSS_REGISTRY, *EXTRA_LOSSES]}")
+    fn = known[name]
     return partial(fn, **kwargs) if kwargs else fn

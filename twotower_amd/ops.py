@@ -249,7 +249,7 @@ class DeferredTableGrad:
     parts (optim.BackwardTableUpdate: the fused update inside loss.backward(), for a loop that
     keeps torch.optim.AdamW)."""
 
-    __slots__ = ("parts", "padding_idx", "gather_group", "on_backward", "queued")
+    __slots__ = ("parts", "padding_idx", "gather_group", "on_backward", "queued", "dense")
 
     def __init__(self, padding_idx: int | None = 0, gather_group=None, on_backward=None):
         self.parts: list[tuple] = []
@@ -257,6 +257,22 @@ class DeferredTableGrad:
         self.gather_group = gather_group
         self.on_backward = on_backward
         self.queued = False
+        self.dense = False  # an embedding_lookup of the table left a dense .grad this step
+
+    def pending(self) -> bool:
+        """Whether this step left parts for the fused update.  It takes no dense gradient beside them: a
+        step that differentiated the table both ways is refused, not updated with one of the two."""
+        dense, self.dense = self.dense, False
+        if self.parts and dense:
+            self.parts.clear()
+            raise RuntimeError("the fused table update takes pooled lookups only, and this step also differentiated "
+                               "an embedding_lookup of the table: build the optimizer with fused_tables=False")
+        return bool(self.parts)
+
+    def added_dense(self) -> None:
+        """An embedding_lookup backward gave the table a dense gradient."""
+        self.dense = True
+        self.added()
 
     def added(self) -> None:
         """A backward node appended its part: queue on_backward for the end of this backward pass
@@ -510,6 +526,87 @@ def bag_mean_pool(weight: torch.Tensor, ids: torch.Tensor, padding_idx: int | No
         # materialize()) reads the full local weight instead: rank-local evaluation and search.
         return BagMeanPoolColumn.apply(weight, ids, padding_idx, col, want_plan)
     return BagMeanPool.apply(weight, ids, padding_idx, scatter_mode, want_plan)
+
+
+# --------------------------------------------------------------------------------------------
+# Token lookup with a scale   (twotower/embeddings.py:40, the (B, L, E) rows a tower may pool itself)
+def _lookup_fwd(weight, ids, scale, out_dtype):
+    V, E = weight.shape
+    out = torch.empty(*ids.shape, E, dtype=out_dtype, device=weight.device)
+    if out.numel():
+        with _lib.on_device(weight):
+            call("tt_lookup_fwd", ptr(weight), _lib.ELEM_DTYPES[weight.dtype], V, E, weight.stride(0), ptr(ids),
+                 _lib.ids_dtype_code(ids), ids.numel(), scale, ptr(out), _lib.ELEM_DTYPES[out_dtype],
+                 stream_of(weight))
+    return out
+
+
+class EmbeddingLookup(torch.autograd.Function):
+    """out = scale * weight[ids], gradient by sorted tokens (see embedding_lookup)."""
+
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding_idx, out_dtype):
+        ctx.save_for_backward(ids)
+        ctx.meta = (weight.shape, weight.dtype, scale, padding_idx)
+        ctx.weight_ref = weight
+        return _lookup_fwd(weight, ids, scale, out_dtype)
+
+    @staticmethod
+    def backward(ctx, dout):
+        (ids,) = ctx.saved_tensors
+        (V, E), dtype, scale, pad = ctx.meta
+        deferred = getattr(ctx.weight_ref, "_tt_deferred", None)
+        if deferred is not None:
+            deferred.added_dense()
+        dout = dout.contiguous()
+        n = ids.numel()
+        grad = torch.empty(V, E, dtype=dtype, device=dout.device)
+        nbytes = _lib.lib().tt_lookup_bwd_ws_size(n, V, E)
+        # per call, not shared: two captured graphs (or streams) may run their backwards at once
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dout.device) if nbytes else None
+        with _lib.on_device(dout):
+            call("tt_lookup_bwd", ptr(dout), _lib.ELEM_DTYPES[dout.dtype], ptr(ids), _lib.ids_dtype_code(ids), n, V, E,
+                 pad, scale, ptr(grad), _lib.ELEM_DTYPES[dtype], ptr(ws), nbytes, stream_of(dout))
+        return grad, None, None, None, None
+
+
+def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None,
+                     out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """scale * weight[ids]: the rows (ids.shape + (E,)) of a (V, E) float32 / bfloat16 / float16 table for
+    int32 / int64 ids of any shape, formed in fp32 and rounded once to ``out_dtype`` (the table's type, or
+    bfloat16 / float16 rows of a float32 table).  An id outside [0, V) yields a zero row and no
+    gradient (torch.nn.functional.embedding aborts the process on the GPU).
+
+    The gradient is dense: every row of the table, scale times the sum of its tokens' gradients in
+    fp32 in a fixed order (bitwise reproducible), rounded once to the table's type; the row of
+    ``padding_idx`` (negative: from the end, as in torch) gets zeros."""
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"weight must be a non-empty (V, E) table, got shape {tuple(weight.shape)}")
+    _lib.elem_dtype_code(weight, "weight")
+    _lib.ids_dtype_code(ids)
+    V, E = weight.shape
+    if (weight.stride(1) != 1 and E > 1) or (weight.stride(0) < E and V > 1):
+        raise ValueError(f"weight rows must be contiguous and must not overlap, got strides {weight.stride()}")
+    out_dtype = weight.dtype if out_dtype is None else out_dtype
+    if out_dtype != weight.dtype and not (weight.dtype == _FLOAT and out_dtype in _lib.ELEM_DTYPES):
+        raise TypeError(f"out_dtype {out_dtype} from a {weight.dtype} table is not supported")
+    if ids.numel() >= 2 ** 31:
+        raise ValueError(f"at most 2^31 - 1 ids per call, got {ids.numel()}")
+    scale = float(scale)
+    pad = -1
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError(f"padding_idx {padding_idx} outside a table of {V} rows")
+        pad = padding_idx % V
+    _lib.same_device(weight, ids)
+    col = getattr(weight, "_tt_column", None)
+    if col is not None and (col.stale or (torch.is_grad_enabled() and weight.requires_grad)):
+        raise RuntimeError("embedding_lookup reads the whole table: this one is column-sharded; materialize() it and "
+                           "call under no_grad, or use bag_mean_pool")
+    ids = ids.contiguous()
+    if weight.requires_grad and torch.is_grad_enabled():
+        return EmbeddingLookup.apply(weight, ids, scale, pad, out_dtype)
+    return _lookup_fwd(weight, ids, scale, out_dtype)
 
 
 # --------------------------------------------------------------------------------------------
@@ -1059,6 +1156,150 @@ class MultiNegLossPacked(torch.autograd.Function):
 
 
 # --------------------------------------------------------------------------------------------
+# preference_loss: paired log ratios of tower outputs
+PREFERENCE_KINDS = {"sigmoid": 0, "squared": 1}
+
+
+def _pref_rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _pref_args(q, p, n):
+    """(q, p, n with a pair axis, element type) of a checked call."""
+    if q.dim() != 2 or p.shape != q.shape:
+        raise ValueError(f"q and p must both be (B, H), got {tuple(q.shape)} and {tuple(p.shape)}")
+    if n.dim() == 2:
+        n = n.unsqueeze(1)
+    if n.dim() != 3 or n.shape[0] != q.shape[0] or n.shape[2] != q.shape[1] or n.shape[1] < 1:
+        raise ValueError(f"n must be (B, H) or (B, K, H) with K >= 1 beside q {tuple(q.shape)}, got {tuple(n.shape)}")
+    if q.shape[1] < 1:
+        raise ValueError("H must be at least 1")
+    dt = _lib.elem_dtype_code(q, "q")
+    if p.dtype != q.dtype or n.dtype != q.dtype:
+        raise TypeError(f"q, p and n must have one type, got {q.dtype}, {p.dtype}, {n.dtype}")
+    return _pref_rows(q, "q"), _pref_rows(p, "p"), _pref_rows(n, "n"), dt
+
+
+def _pref_pairs(t, name, dtype, B, K, device):
+    """A contiguous (B, K) side input (ref_margin, mask); (B,) is taken where K = 1."""
+    if t is None:
+        return None
+    if t.shape != (B, K) and not (K == 1 and t.shape == (B,)):
+        raise ValueError(f"{name} must be ({B}, {K}), got {tuple(t.shape)}")
+    if t.device != device:
+        raise RuntimeError(f"twotower_amd: {name} is on {t.device}, the embeddings on {device}")
+    if dtype == torch.bool:
+        if t.dtype != torch.bool:
+            raise TypeError(f"{name} must be bool, got {t.dtype}")
+    elif not t.dtype.is_floating_point:
+        raise TypeError(f"{name} must be a floating-point tensor, got {t.dtype}")
+    return t.detach().to(dtype).contiguous()
+
+
+def _pref_fwd(q, p, n, dt, ref, mask, opts, margins=None, loss=None):
+    """Fills margins, or loss and returns the side buffer: dl/dh (B K), 1 / pairs, then 2 B words of scratch."""
+    (B, K, H), (kind, beta, inv_tau, smooth) = n.shape, opts
+    side, at = None, (None, None, None)
+    if loss is not None:
+        side = torch.empty(B * K + 1 + 2 * B, dtype=_FLOAT, device=q.device)
+        base = side.data_ptr()
+        at = (base, base + 4 * B * K, base + 4 * (B * K + 1))
+    with _lib.on_device(q):
+        call("tt_preference_fwd", ptr(q), q.stride(0), ptr(p), p.stride(0), ptr(n), n.stride(0), n.stride(1), dt, B, K,
+             H, ptr(ref), ptr(mask), kind, beta, inv_tau, smooth, at[0], ptr(margins), ptr(loss), at[1], at[2], 8 * B,
+             stream_of(q))
+    return side
+
+
+def _pref_bwd(q, p, n, dt, mask, opts, side, g, dq, dp, dn):
+    B, K, H = n.shape
+    g = g.to(_FLOAT).contiguous()
+    base = side.data_ptr()
+    with _lib.on_device(q):
+        call("tt_preference_bwd", ptr(q), q.stride(0), ptr(p), p.stride(0), ptr(n), n.stride(0), n.stride(1), dt, B, K,
+             H, ptr(mask), opts[2], base, base + 4 * B * K, ptr(g), ptr(dq), ptr(dp), ptr(dn), stream_of(q))
+
+
+class PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, p, n, dt, ref, mask, opts):
+        loss = torch.empty((), dtype=_FLOAT, device=q.device)
+        side = _pref_fwd(q, p, n, dt, ref, mask, opts, loss=loss)
+        ctx.save_for_backward(q, p, n, mask, side)
+        ctx.meta = (dt, opts)
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        q, p, n, mask, side = ctx.saved_tensors
+        dq, dp, dn = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, p, n))
+        _pref_bwd(q, p, n, ctx.meta[0], mask, ctx.meta[1], side, g, dq, dp, dn)
+        return dq, dp, dn, None, None, None, None
+
+
+class PreferenceLossPacked(torch.autograd.Function):
+    """The same loss on one ((2 + K) B, H) tensor [q; p; negatives] (TwoTower's fused output): the
+    three gradients are written into one tensor, so autograd runs no split backward."""
+
+    @staticmethod
+    def forward(ctx, qpn, B, K, dt, ref, mask, opts):
+        loss = torch.empty((), dtype=_FLOAT, device=qpn.device)
+        side = _pref_fwd(qpn[:B], qpn[B:2 * B], qpn[2 * B:].view(B, K, -1), dt, ref, mask, opts, loss=loss)
+        ctx.save_for_backward(qpn, mask, side)
+        ctx.meta = (B, K, dt, opts)
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        qpn, mask, side = ctx.saved_tensors
+        B, K, dt, opts = ctx.meta
+        grad = torch.empty_like(qpn)
+        _pref_bwd(qpn[:B], qpn[B:2 * B], qpn[2 * B:].view(B, K, -1), dt, mask, opts, side, g, grad[:B], grad[B:2 * B],
+                  grad[2 * B:])
+        return grad, None, None, None, None, None, None
+
+
+def _pref_opts(beta, temperature, label_smoothing, loss_type):
+    if loss_type not in PREFERENCE_KINDS:
+        raise ValueError(f"loss_type must be one of {sorted(PREFERENCE_KINDS)}, got {loss_type!r}")
+    beta, temperature, smooth = float(beta), float(temperature), float(label_smoothing)
+    if not (0.0 < beta < float("inf") and 0.0 < temperature < float("inf")):
+        raise ValueError(f"beta and temperature must be positive, got {beta} and {temperature}")
+    if not 0.0 <= smooth < 1.0:
+        raise ValueError(f"label_smoothing must be in [0, 1), got {smooth}")
+    if smooth and loss_type != "sigmoid":
+        raise ValueError("label_smoothing is a term of the sigmoid loss")
+    return PREFERENCE_KINDS[loss_type], beta, 1.0 / temperature, smooth
+
+
+def preference_loss(q: torch.Tensor, p: torch.Tensor, n: torch.Tensor, ref_margin: torch.Tensor | None = None,
+                    mask: torch.Tensor | None = None, beta: float = 0.1, temperature: float = 0.1,
+                    label_smoothing: float = 0.0, loss_type: str = "sigmoid",
+                    packed: torch.Tensor | None = None) -> torch.Tensor:
+    """losses.preference_loss on the HIP row kernels.  packed: the one tensor [q; p; n] that q, p and n are
+    the consecutive row blocks of, which then receives the gradient."""
+    opts = _pref_opts(beta, temperature, label_smoothing, loss_type)
+    q, p, n, dt = _pref_args(q, p, n)
+    B, K, _ = n.shape
+    ref = _pref_pairs(ref_margin, "ref_margin", _FLOAT, B, K, q.device)
+    mask = _pref_pairs(mask, "mask", torch.bool, B, K, q.device)
+    _lib.same_device(q, p, n)
+    if packed is not None:
+        return PreferenceLossPacked.apply(packed, B, K, dt, ref, mask, opts)
+    return PreferenceLoss.apply(q, p, n, dt, ref, mask, opts)
+
+
+def preference_margin(q: torch.Tensor, p: torch.Tensor, n: torch.Tensor, temperature: float = 0.1) -> torch.Tensor:
+    """losses.preference_margin: (B, K) float32 margins, no gradient."""
+    opts = _pref_opts(1.0, temperature, 0.0, "sigmoid")
+    q, p, n, dt = _pref_args(q.detach(), p.detach(), n.detach())
+    _lib.same_device(q, p, n)
+    margins = torch.empty(n.shape[:2], dtype=_FLOAT, device=q.device)
+    _pref_fwd(q, p, n, dt, None, None, opts, margins=margins)
+    return margins
+
+
+# --------------------------------------------------------------------------------------------
 # in_batch_sampled_softmax_loss   (twotower/losses.py:88-118), fused MFMA scorer
 _BWD_FORMS = {"recompute": _lib.TT_INBATCH_BWD_RECOMPUTE, "stored": _lib.TT_INBATCH_BWD_STORED}
 
@@ -1338,6 +1579,79 @@ def in_batch_softmax_loss(q: torch.Tensor, d: torch.Tensor, temperature: float =
 
 
 # --------------------------------------------------------------------------------------------
+# global gradient norm and clipping (between twotower/train.py:138 and :139)
+def _dense(t: torch.Tensor) -> bool:
+    """t's elements fill one block of memory, in any order (a norm and a product need no more)."""
+    return t.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(t)
+
+
+def clip_grad_norm(grads, max_norm: float | None, norm_type: float = 2.0, out=None) -> torch.Tensor:
+    """The global norm (norm_type 2 or inf) of all gradients as a 0-dim float32 tensor, and the gradients times
+    min(1, max_norm / (norm + 1e-6)), in place or into ``out`` (one tensor per gradient, of its type or
+    float32, so half-precision accumulators can be clipped into the fp32 gradients an optimizer steps
+    with).  max_norm None: the norm alone.  float32 / bfloat16 / float16 tensors, mixed at will; the norm is
+    formed in 64 bits in a fixed order, each product is rounded once; no host synchronisation.
+    A non-finite norm spreads as in torch.nn.utils.clip_grad_norm_ (inf: zeros and NaN, NaN: NaN)."""
+    grads = list(grads)
+    if norm_type not in (2, 2.0, float("inf")):
+        raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
+    scale = max_norm is not None
+    if scale and not float(max_norm) >= 0.0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    if not scale and out is not None:
+        raise ValueError("out needs a max_norm")
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads):
+        raise ValueError(f"{len(outs)} out tensors for {len(grads)} gradients")
+    if not grads:
+        return torch.zeros((), dtype=_FLOAT)
+    first = grads[0]
+    dev, codes = first.device, _lib.ELEM_DTYPES
+    items = (_lib.ClipTensor * len(grads))()
+    copies, seen = [], set()
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        if g.is_sparse:
+            raise RuntimeError("clip_grad_norm does not support sparse gradients")
+        gd, od = codes.get(g.dtype), codes.get(o.dtype)
+        if gd is None or (od != gd and od != 0):
+            raise TypeError(f"gradient {i} of {g.dtype} into {o.dtype}: float32, bfloat16 or float16, into its own type "
+                            "or float32")
+        if g.shape != o.shape:
+            raise ValueError(f"out {i} has shape {tuple(o.shape)}, the gradient {tuple(g.shape)}")
+        src = dst = g
+        if o is not g:
+            src = g if g.is_contiguous() else g.contiguous()
+            dst = o
+            if not o.is_contiguous():
+                dst = torch.empty(o.shape, dtype=o.dtype, device=dev)
+                copies.append((o, dst))
+        elif not _dense(g):
+            if scale and torch._debug_has_internal_overlap(g) == 1:
+                raise ValueError(f"gradient {i} has elements that share memory (an expanded tensor): clip a copy")
+            src = dst = g.contiguous()
+            if scale:
+                copies.append((g, dst))
+        if scale and g.numel():
+            if dst.data_ptr() in seen:
+                raise ValueError(f"gradient {i} is written twice: the same memory is listed more than once")
+            seen.add(dst.data_ptr())
+        items[i] = _lib.ClipTensor(src.data_ptr(), dst.data_ptr(), g.numel(), gd, od)
+        if src is not g:
+            copies.append((None, src))  # kept until the launches are queued
+    _lib.same_device(first, *grads, *(outs if outs is not grads else ()))
+    norm = torch.empty((), dtype=_FLOAT, device=dev)
+    nbytes = _lib.lib().tt_clip_ws_size(len(grads))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with _lib.on_device(first):
+        call("tt_clip_grads", items, len(grads), int(norm_type == float("inf")), float(max_norm) if scale else 0.0,
+             int(scale), ptr(norm), ptr(ws), nbytes, stream_of(first))
+    for o, t in copies:
+        if o is not None:
+            o.copy_(t)
+    return norm
+
+
+# --------------------------------------------------------------------------------------------
 # torch.optim.AdamW step (twotower/train.py:359, :139)
 def adamw_step(param: torch.Tensor, grad: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, *,
                lr: float, beta1: float, beta2: float, eps: float, weight_decay: float, step: int) -> None:
@@ -1489,3 +1803,113 @@ def topk_rows(scores: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor]
 
 def cosine_topk(q: torch.Tensor, docs: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor]:
     return topk_rows(cosine_scores(q, docs), k)
+
+
+# --------------------------------------------------------------------------------------------
+# 4-bit document index
+class Int4Rows:
+    """(n, H) rows held as 4-bit codes with a bfloat16 scale per ``group`` columns: row j, column k stands for
+    code[j, k] * scale[j, k // group], codes -8..7.  ``codes`` and ``scales`` are device buffers in the scoring
+    kernel's own layout (written once); build with ``quantize`` or ``from_codes``, read back with
+    ``dequantize``, score with ``int4_scores``."""
+
+    __slots__ = ("codes", "scales", "n", "H", "group")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n: int, H: int, group: int):
+        n, H = _int4_shape(n, H, group)
+        lib = _lib.lib()
+        want = (lib.tt_int4_codes_bytes(n, H), lib.tt_int4_scales_bytes(n, H, group))
+        for t, nm, b in ((codes, "codes", want[0]), (scales, "scales", want[1])):
+            if t.dtype != torch.uint8 or t.dim() != 1 or not t.is_contiguous() or t.numel() != b:
+                raise ValueError(f"{nm} must be {b} contiguous uint8 bytes for {n} rows of {H}, group {group}")
+            if t.numel() and t.data_ptr() % 16:
+                raise ValueError(f"{nm} must be 16-byte aligned")
+        _lib.same_device(codes, scales)
+        self.codes, self.scales, self.n, self.H, self.group = codes, scales, n, H, int(group)
+
+    @classmethod
+    def _empty(cls, n: int, H: int, group: int, device) -> "Int4Rows":
+        n, H = _int4_shape(n, H, group)
+        lib = _lib.lib()
+        return cls(torch.empty(lib.tt_int4_codes_bytes(n, H), dtype=torch.uint8, device=device),
+                   torch.empty(lib.tt_int4_scales_bytes(n, H, group), dtype=torch.uint8, device=device), n, H, group)
+
+    @classmethod
+    def quantize(cls, x: torch.Tensor, group: int = 32) -> "Int4Rows":
+        """Rows of x (n, H): scale = max |group| / 7 rounded to bfloat16, code = x / scale rounded to the nearest
+        integer (ties to even).  A group with a non-finite value reads back as NaN."""
+        if x.dim() != 2:
+            raise ValueError(f"x must be (n, H), got shape {tuple(x.shape)}")
+        dt = _lib.elem_dtype_code(x, "x")
+        _int4_shape(*x.shape, group)
+        require_gpu(x)
+        if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
+            x = x.contiguous()
+        r = cls._empty(x.shape[0], x.shape[1], group, x.device)
+        with _lib.on_device(x):
+            call("tt_int4_quantize", ptr(x), dt, r.n, r.H, max(x.stride(0), r.H), r.group, ptr(r.codes), ptr(r.scales),
+                 stream_of(x))
+        return r
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, group: int = 32) -> "Int4Rows":
+        """From (n, H) int8 codes (-8..7; values outside are clamped) and (n, ceil(H / group)) bfloat16 scales."""
+        if codes.dim() != 2 or codes.dtype != torch.int8:
+            raise ValueError(f"codes must be (n, H) int8, got {tuple(codes.shape)} {codes.dtype}")
+        n, H = _int4_shape(*codes.shape, group)
+        if scales.dtype != torch.bfloat16 or tuple(scales.shape) != (n, -(-H // group)):
+            raise ValueError(f"scales must be ({n}, {-(-H // group)}) bfloat16, got {tuple(scales.shape)} {scales.dtype}")
+        _lib.same_device(codes, scales)
+        codes, scales = codes.contiguous(), scales.contiguous()
+        r = cls._empty(n, H, group, codes.device)
+        with _lib.on_device(codes):
+            call("tt_int4_pack", ptr(codes), ptr(scales), n, H, r.group, ptr(r.codes), ptr(r.scales), stream_of(codes))
+        return r
+
+    def dequantize(self) -> torch.Tensor:
+        """The (n, H) float32 values the codes stand for."""
+        out = torch.empty(self.n, self.H, dtype=_FLOAT, device=self.codes.device)
+        with _lib.on_device(self.codes):
+            call("tt_int4_unpack", ptr(self.codes), ptr(self.scales), self.n, self.H, self.group, ptr(out),
+                 stream_of(self.codes))
+        return out
+
+    def to(self, device) -> "Int4Rows":
+        if torch.device(device).type != "cuda":
+            raise RuntimeError("twotower_amd: a 4-bit index lives on a GPU (state() copies it to the host)")
+        return Int4Rows(self.codes.to(device), self.scales.to(device), self.n, self.H, self.group)
+
+    def state(self) -> dict:
+        """A host copy for torch.save; from_state(state, device) restores it."""
+        return {"codes": self.codes.cpu(), "scales": self.scales.cpu(), "n": self.n, "H": self.H, "group": self.group}
+
+    @classmethod
+    def from_state(cls, state: dict, device) -> "Int4Rows":
+        return cls(state["codes"].to(device), state["scales"].to(device), state["n"], state["H"], state["group"])
+
+
+def _int4_shape(n, H, group) -> tuple[int, int]:
+    if group not in (32, 64, 128):
+        raise ValueError(f"group must be 32, 64 or 128, got {group}")
+    if not 1 <= H <= _lib.TT_INT4_MAX_H or n < 0:
+        raise ValueError(f"rows of 1 to {_lib.TT_INT4_MAX_H} values, got ({n}, {H})")
+    return int(n), int(H)
+
+
+def int4_scores(q: torch.Tensor, rows: Int4Rows) -> torch.Tensor:
+    """(nq, n) float32 products q_i . row_j of (nq, H) or (H,) float32 / bfloat16 / float16 queries with 4-bit
+    rows, in fp32 accuracy (the codes are exact, each query element keeps 33 bits or more than fp32 beside
+    the largest).  A query with a non-finite value scores NaN everywhere."""
+    if q.dim() == 1:
+        q = q.unsqueeze(0)
+    if q.dim() != 2 or q.shape[1] != rows.H:
+        raise ValueError(f"queries must be (nq, {rows.H}), got shape {tuple(q.shape)}")
+    dt = _lib.elem_dtype_code(q, "q")
+    _lib.same_device(q, rows.codes)
+    if q.stride(1) != 1 or q.stride(0) < rows.H:
+        q = q.contiguous()
+    out = torch.empty(q.shape[0], rows.n, dtype=_FLOAT, device=q.device)
+    with _lib.on_device(q):
+        call("tt_int4_scores", ptr(q), dt, q.shape[0], max(q.stride(0), rows.H), ptr(rows.codes), ptr(rows.scales),
+             rows.n, rows.H, rows.group, ptr(out), stream_of(q))
+    return out

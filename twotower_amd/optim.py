@@ -218,7 +218,7 @@ class AdamW(torch.optim.Optimizer):
         self._side_grads.join()
         for p in group["params"]:
             deferred = getattr(p, "_tt_deferred", None)
-            if deferred is not None and deferred.parts:
+            if deferred is not None and deferred.pending():
                 st = self._state(p, False)
                 st["step"] += 1
                 col = self._columns.get(id(p))
@@ -257,7 +257,7 @@ class AdamW(torch.optim.Optimizer):
         slots, dense, fused, shards, dense_ids, columns = [], [], [], [], [], []
         for p in group["params"]:
             deferred = getattr(p, "_tt_deferred", None)
-            if deferred is not None and deferred.parts:
+            if deferred is not None and deferred.pending():
                 st = self._state(p, True)
                 a = self._adam_args(p)
                 slots.append((st["step"], a))
@@ -423,6 +423,34 @@ class AdamW(torch.optim.Optimizer):
                 distributed.all_gather_rows(stor[clo:chi], sh.own(stor, c), sh.group)
 
 
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_ on the HIP kernels (ops.clip_grad_norm): scales every parameter's .grad in
+    place by min(1, max_norm / (norm + 1e-6)) and returns the global norm as a device tensor, without a
+    host synchronisation (error_if_nonfinite reads it and raises).  A parameter listed twice counts
+    once.  A table whose gradient a fused optimizer holds in factored form has no .grad to take part: such
+    a call is refused rather than clipped without it."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    params = list({id(p): p for p in parameters}.values())
+    if any(getattr(p, "_tt_deferred", None) is not None and p._tt_deferred.parts for p in params):
+        raise RuntimeError("clip_grad_norm_: a fused table's gradient is kept in factored form and has no norm here; "
+                           "build the optimizer with fused_tables=False to clip it")
+    for p in params:
+        if getattr(p, "_tt_side_grads", None) is not None:
+            p._tt_side_grads.join()  # gradients still being formed on a side stream
+    grads = [p.grad for p in params if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    norm = ops.clip_grad_norm([g.detach() for g in grads], None if error_if_nonfinite else max_norm, norm_type)
+    if error_if_nonfinite:
+        if not math.isfinite(norm.item()):
+            raise RuntimeError(f"the total norm of order {norm_type} for gradients from `parameters` is non-finite, "
+                               "so it cannot be clipped")
+        norm = ops.clip_grad_norm([g.detach() for g in grads], max_norm, norm_type)
+    return norm
+
+
 class BackwardTableUpdate:
     """The fused table update for a loop that keeps ``torch.optim.AdamW`` (the reference's
     ``train.py:359``, stepped at ``:139``): at the end of every ``loss.backward()`` the table's
@@ -472,7 +500,7 @@ class BackwardTableUpdate:
     def __call__(self) -> None:
         w = self.weight
         deferred = w._tt_deferred
-        if not deferred.parts:
+        if not deferred.pending():
             return
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("table_update 'backward' runs eagerly (host step counter); use TrainStep with "

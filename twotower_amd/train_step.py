@@ -20,11 +20,26 @@ import torch
 from . import ops
 from .distributed import GradSync, capture_blocker, is_active
 from .losses import scorer_prep_dtype
+from .optim import clip_grad_norm_
 
 
 class TrainStep:
     def __init__(self, model: torch.nn.Module, loss_fn, optimizer: torch.optim.Optimizer, group=None,
-                 graph: bool = False, eager_steps: int = 2):
+                 graph: bool = False, eager_steps: int = 2, max_grad_norm: float | None = None):
+        """max_grad_norm: clip the gradients to this global 2-norm between backward and the optimizer step
+        (optim.clip_grad_norm_; data parallel: the norm of the all-reduced gradients, the same on every
+        rank).  The whole gradient takes part, so it needs dense gradients: an optimizer with fused tables,
+        or updates made inside backward, are refused.  ``grad_norm`` is the last step's norm before clipping, on the
+        device."""
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        self.grad_norm: torch.Tensor | None = None
+        if self.max_grad_norm is not None:
+            if not self.max_grad_norm >= 0.0:
+                raise ValueError(f"max_grad_norm must not be negative, got {max_grad_norm}")
+            if any(getattr(p, "_tt_deferred", None) is not None for p in model.parameters()) or getattr(
+                    optimizer, "_tt_dense_update", None) is not None:
+                raise ValueError("max_grad_norm needs dense gradients that reach optimizer.step(): build the optimizer "
+                                 "with fused_tables=False and no update inside backward")
         self.model = model
         self.loss_fn = loss_fn
         self.optimizer = optimizer
@@ -34,7 +49,9 @@ class TrainStep:
         # (optim.AdamW): the all-reduce then overlaps the table update
         # (set on the optimizer only for the duration of this step's optimizer.step(): a plain loop
         # that calls GradSync.sync() itself must not see a second all-reduce)
-        self._sync_in_step = self.sync is not None and hasattr(optimizer, "_grad_sync")
+        # (with clipping the norm needs the reduced gradients first: synced before the step)
+        self._sync_in_step = (self.sync is not None and hasattr(optimizer, "_grad_sync")
+                              and self.max_grad_norm is None)
         # a single-device bf16 in-batch loss: the tied towers' head prepares its operands
         # (TT_SCORER_PREP=0: the loss's own prep pass, for comparison)
         # Opened only around this step's own forward (_scorer_prep_open): set on the model for
@@ -62,7 +79,8 @@ class TrainStep:
         side = getattr(self.optimizer, "_side_grads", None)
         if side is not None:
             side.join()
-            side.active = True
+            # clipping reads every gradient before the optimizer: nothing is left on a side stream
+            side.active = self.max_grad_norm is None
         try:
             defer = ops.deferred_loss_mean() if self._defer_mean else contextlib.nullcontext()
             with defer, self._scorer_prep_open():  # the loss is read after the backward below
@@ -80,6 +98,8 @@ class TrainStep:
                 loss.backward(seed)
             if self.sync is not None and not self._sync_in_step:
                 self.sync.sync()
+            if self.max_grad_norm is not None:
+                self.grad_norm = clip_grad_norm_(self.model.parameters(), self.max_grad_norm)
             if self._sync_in_step:  # the optimizer launches the all-reduce inside this step only
                 self.optimizer._grad_sync = self.sync
             self.optimizer.step()
@@ -178,6 +198,7 @@ class TrainStep:
                 deferred = getattr(p, "_tt_deferred", None)
                 if deferred is not None:
                     deferred.parts.clear()
+                    deferred.dense = False
         side = getattr(self.optimizer, "_side_grads", None)
         if side is not None:
             side.reset()

@@ -197,13 +197,20 @@ int tt_bag_col_reduce_ex(const int32_t* seg_all, const int32_t* vals_all, int64_
  * tt_lookup_bwd: grad[r, :] = scale * sum of dout[t, :] over the tokens with ids[t] = r (none for r =
  *   padding_idx, -1: no padding id), every one of the V rows written.  Sums are fp32 in a fixed order
  *   (bitwise reproducible), rounded once to grad's type; dout has out's type, grad the table's.
- *   ws: tt_lookup_bwd_ws_size bytes (0 for short calls). */
+ *   ws: tt_lookup_bwd_ws_size bytes, 16-byte aligned (0 for short calls).
+ * tt_lookup_plan: the half of the backward that needs the ids alone, their sort (tt_lookup_plan_size bytes;
+ *   0 for short calls, which need none), to be called before tt_lookup_bwd with the same ids, n, V and
+ *   padding_idx, on the same stream or one that it waits for (it may run beside the forward).  The plan is
+ *   only read by tt_lookup_bwd. */
 int tt_lookup_fwd(const void* table, int table_dtype, int64_t V, int E, int64_t ld_table, const void* ids,
                   int ids_dtype, int64_t n, float scale, void* out, int out_dtype, tt_stream_t stream);
-size_t tt_lookup_bwd_ws_size(int64_t n, int64_t V, int E);
+size_t tt_lookup_plan_size(int64_t n, int64_t V);
+int tt_lookup_plan(const void* ids, int ids_dtype, int64_t n, int64_t V, int64_t padding_idx, void* plan,
+                   size_t plan_bytes, tt_stream_t stream);
+size_t tt_lookup_bwd_ws_size(int64_t n, int E);
 int tt_lookup_bwd(const void* dout, int dout_dtype, const void* ids, int ids_dtype, int64_t n, int64_t V, int E,
-                  int64_t padding_idx, float scale, void* grad, int grad_dtype, void* ws, size_t ws_bytes,
-                  tt_stream_t stream);
+                  int64_t padding_idx, float scale, void* grad, int grad_dtype, const void* plan, size_t plan_bytes,
+                  void* ws, size_t ws_bytes, tt_stream_t stream);
 
 /* ---- dense AdamW (torch.optim.AdamW, twotower/train.py:359, .step() :139) ---------
  * p *= 1 - lr*wd;  m = lerp(m, g, 1-b1);  v = b2*v + (1-b2)*g*g;
@@ -266,19 +273,13 @@ int tt_adamw_multi_ex(const tt_adamw_tensor* tensors, const tt_adamw_grad_parts*
  * norm = (sum g^2)^(1/2) over every element of every tensor, or max |g| (inf_norm != 0), in 64 bits,
  * rounded once to *norm; scale != 0: dst = src * min(1, max_norm / (norm + 1e-6)), formed in fp32 and
  * rounded once.  dst may be src (then an unclipped call writes nothing) or another tensor of src's type
- * or fp32; tensors must not overlap otherwise.  Any count: TT_CLIP_MAX_TENSORS per launch, passed
- * by value.  ws: tt_clip_ws_size(count) bytes, 8-byte aligned. */
+ * or fp32; tensors must not overlap otherwise.  The five arrays (host memory) describe `count` tensors:
+ * pointers, elements, tt_elem_dtype codes.  Any count: TT_CLIP_MAX_TENSORS per launch, passed by value.  ws: tt_clip_ws_size(count) bytes, 8-byte aligned. */
 #define TT_CLIP_MAX_TENSORS 128
-typedef struct {
-  const void* src;
-  void* dst;
-  int64_t n;
-  int src_dtype; /* tt_elem_dtype */
-  int dst_dtype;
-} tt_clip_tensor;
 size_t tt_clip_ws_size(int count);
-int tt_clip_grads(const tt_clip_tensor* tensors, int count, int inf_norm, double max_norm, int scale,
-                  float* norm, void* ws, size_t ws_bytes, tt_stream_t stream);
+int tt_clip_grads(const void* const* src, void* const* dst, const int64_t* n, const uint8_t* src_dtype,
+                  const uint8_t* dst_dtype, int count, int inf_norm, double max_norm, int scale, float* norm, void* ws,
+                  size_t ws_bytes, tt_stream_t stream);
 
 /* ---- mean of n floats (the loss reductions' F.cross_entropy / .mean(), losses.py:44,85,116):
  * one workgroup, fixed-order sums (bitwise reproducible); the in-batch forward forms it itself

@@ -168,7 +168,11 @@ def test_lookup_embedding_on_the_cpu_is_the_plain_gather():
 
 # ---------------------------------------------------------------------------------------------
 # C ABI
-_CLIP = (_lib.ClipTensor * 1)(_lib.ClipTensor(P, P, 3, 0, 0))
+
+
+def _clip(src=P, dst=P, n=3, st=0, dt=0, max_norm=1.0, ws=1 << 20):
+    a = [(ctypes.c_int64 * 1)(v or 0) for v in (src, dst, n)]
+    return (*a, bytes([st]), bytes([dt]), 1, 0, max_norm, 1, P, P, ws, None)
 
 
 @pytest.mark.parametrize("name, args, msg", [
@@ -180,8 +184,11 @@ _CLIP = (_lib.ClipTensor * 1)(_lib.ClipTensor(P, P, 3, 0, 0))
     ("tt_lookup_fwd", (P, 1, 5, 4, 4, P, 0, 1, 1.0, P, 0, None), "rows of type 0"),
     ("tt_lookup_fwd", (P, 0, 5, 4, 4, P, 0, 2 ** 31, 1.0, P, 0, None), "out of range"),
     ("tt_lookup_fwd", (None, 0, 5, 4, 4, P, 0, 1, 1.0, P, 0, None), "null pointer"),
-    ("tt_lookup_bwd", (None, 0, P, 0, 1, 5, 4, -1, 1.0, P, 0, None, 0, None), "null pointer"),
-    ("tt_lookup_bwd", (P, 0, P, 0, 5000, 5, 4, -1, 1.0, P, 0, None, 0, None), "workspace too small"),
+    ("tt_lookup_bwd", (None, 0, P, 0, 1, 5, 4, -1, 1.0, P, 0, None, 0, None, 0, None), "null pointer"),
+    ("tt_lookup_bwd", (P, 0, P, 0, 5000, 5, 4, -1, 1.0, P, 0, None, 0, P, 1 << 30, None), "plan too small"),
+    ("tt_lookup_bwd", (P, 0, P, 0, 5000, 5, 4, -1, 1.0, P, 0, P, 1 << 30, P, 8, None), "workspace too small"),
+    ("tt_lookup_plan", (P, 0, 5000, 5, -1, P, 100, None), "workspace too small"),
+    ("tt_lookup_plan", (None, 0, 5000, 5, -1, P, 1 << 30, None), "ids is NULL"),
     ("tt_preference_fwd", (P, 4, P, 4, P, 4, 4, 3, 2, 1, 4, None, None, 0, 1.0, 1.0, 0.0, P, None, P, P, P, 16, None),
      "element type 3"),
     ("tt_preference_fwd", (P, 4, P, 4, P, 4, 4, 0, 2, 0, 4, None, None, 0, 1.0, 1.0, 0.0, P, None, P, P, P, 16, None),
@@ -195,15 +202,13 @@ _CLIP = (_lib.ClipTensor * 1)(_lib.ClipTensor(P, P, 3, 0, 0))
     ("tt_preference_fwd", (P, 4, P, 4, P, 4, 4, 0, 2, 1, 4, None, None, 0, 1.0, 1.0, 0.0, P, None, P, None, P, 16, None),
      "null pointer"),
     ("tt_preference_bwd", (P, 4, P, 4, P, 4, 4, 0, 2, 1, 4, None, 1.0, P, P, None, P, P, P, None), "null pointer"),
-    ("tt_clip_grads", (None, 1, 0, 1.0, 1, P, P, 1 << 20, None), "null pointer"),
-    ("tt_clip_grads", (_CLIP, 1, 0, -1.0, 1, P, P, 1 << 20, None), "max_norm"),
-    ("tt_clip_grads", (_CLIP, 1, 0, 1.0, 1, P, P, 8, None), "workspace too small"),
-    ("tt_clip_grads", ((_lib.ClipTensor * 1)(_lib.ClipTensor(P, None, 3, 0, 0)), 1, 0, 1.0, 1, P, P, 1 << 20, None),
-     "tensor 0 is NULL"),
-    ("tt_clip_grads", ((_lib.ClipTensor * 1)(_lib.ClipTensor(P, P, 3, 0, 1)), 1, 0, 1.0, 1, P, P, 1 << 20, None),
-     "of type 0 into type 1"),
-    ("tt_clip_grads", ((_lib.ClipTensor * 1)(_lib.ClipTensor(P, P, -1, 0, 0)), 1, 0, 1.0, 1, P, P, 1 << 20, None),
-     "-1 elements"),
+    ("tt_clip_grads", (None, None, None, None, None, 1, 0, 1.0, 1, P, P, 1 << 20, None), "null pointer"),
+    ("tt_clip_grads", _clip(max_norm=-1.0), "max_norm"),
+    ("tt_clip_grads", _clip(ws=8), "workspace too small"),
+    ("tt_clip_grads", _clip(dst=None), "tensor 0 is NULL"),
+    ("tt_clip_grads", _clip(dt=1), "of type 0 into type 1"),
+    ("tt_clip_grads", _clip(st=3, dt=3), "of type 3 into type 3"),
+    ("tt_clip_grads", _clip(n=-1), "-1 elements"),
     ("tt_int4_quantize", (P, 0, 4, 4097, 4097, 32, P, P, None), "H=4097"),
     ("tt_int4_quantize", (P, 0, 4, 64, 63, 32, P, P, None), "ld=63"),
     ("tt_int4_quantize", (P, 0, 4, 64, 64, 16, P, P, None), "group=16"),
@@ -222,12 +227,12 @@ def test_c_abi_refusals(name, args, msg):
 
 def test_c_abi_sizes():
     lib = _lib.lib()
-    assert lib.tt_lookup_bwd_ws_size(100, 50, 8) == 0  # short calls take no workspace
-    assert lib.tt_lookup_bwd_ws_size(100_000, 50, 8) > 0
+    assert lib.tt_lookup_bwd_ws_size(100, 8) == lib.tt_lookup_plan_size(100, 50) == 0  # short calls take none
+    assert lib.tt_lookup_bwd_ws_size(100_000, 8) == (2 * 3125 + 97) * 8 * 4  # heads, tails, super-tiles
+    assert lib.tt_lookup_plan_size(100_000, 50) > 4 * 4 * 100_000
     assert lib.tt_int4_codes_bytes(17, 33) == 2 * 2 * 256  # two tiles of 16 rows, two 32-column blocks
     assert lib.tt_int4_scales_bytes(17, 33, 32) == 2 * 1 * 16 * 4 * 2
     assert lib.tt_clip_ws_size(1) == lib.tt_clip_ws_size(1000) == 2048 * 8
-    assert ctypes.sizeof(_lib.ClipTensor) == 32
 
 
 # ---------------------------------------------------------------------------------------------

@@ -51,11 +51,6 @@ class AdamwGradParts(ctypes.Structure):
     _fields_ = [("part", _vp), ("stride", _c_i64), ("slabs", _c_int)]
 
 
-class ClipTensor(ctypes.Structure):
-    """tt_clip_tensor"""
-    _fields_ = [("src", _vp), ("dst", _vp), ("n", _c_i64), ("src_dtype", _c_int), ("dst_dtype", _c_int)]
-
-
 # name -> (restype, argtypes); must mirror include/twotower_amd.h
 _SIGNATURES = {
     "tt_version": (_c_int, []),
@@ -96,15 +91,18 @@ _SIGNATURES = {
                                    ctypes.POINTER(AdamSlot), _c_int, _c_f64, _c_f64, _c_f64, _c_f64, _c_f64, _vp,
                                    _vp]),
     "tt_lookup_fwd": (_c_int, [_vp, _c_int, _c_i64, _c_int, _c_i64, _vp, _c_int, _c_i64, _c_f32, _vp, _c_int, _vp]),
-    "tt_lookup_bwd_ws_size": (_c_sz, [_c_i64, _c_i64, _c_int]),
+    "tt_lookup_plan_size": (_c_sz, [_c_i64, _c_i64]),
+    "tt_lookup_plan": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_sz, _vp]),
+    "tt_lookup_bwd_ws_size": (_c_sz, [_c_i64, _c_int]),
     "tt_lookup_bwd": (_c_int, [_vp, _c_int, _vp, _c_int, _c_i64, _c_i64, _c_int, _c_i64, _c_f32, _vp, _c_int, _vp,
-                               _c_sz, _vp]),
+                               _c_sz, _vp, _c_sz, _vp]),
     "tt_preference_fwd": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_int, _vp,
                                    _vp, _c_int, _c_f32, _c_f32, _c_f32, _vp, _vp, _vp, _vp, _vp, _c_sz, _vp]),
     "tt_preference_bwd": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_int, _vp,
                                    _c_f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "tt_clip_ws_size": (_c_sz, [_c_int]),
-    "tt_clip_grads": (_c_int, [_vp, _c_int, _c_int, _c_f64, _c_int, _vp, _vp, _c_sz, _vp]),
+    "tt_clip_grads": (_c_int, [_vp, _vp, _vp, ctypes.c_char_p, ctypes.c_char_p, _c_int, _c_int, _c_f64, _c_int, _vp,
+                               _vp, _c_sz, _vp]),
     "tt_int4_codes_bytes": (_c_sz, [_c_i64, _c_int]),
     "tt_int4_scales_bytes": (_c_sz, [_c_i64, _c_int, _c_int]),
     "tt_int4_quantize": (_c_int, [_vp, _c_int, _c_i64, _c_int, _c_i64, _c_int, _vp, _vp, _vp]),
@@ -285,6 +283,9 @@ def _nullctx():
     return contextlib.nullcontext()
 
 
+_NULL = contextlib.nullcontext()  # (stateless: one serves every use)
+
+
 def join_side_grads(params) -> None:
     """Make the current stream wait for every side-stream gradient of ``params``."""
     seen = set()
@@ -459,7 +460,7 @@ def same_device(*tensors: torch.Tensor) -> None:
 def on_device(t: torch.Tensor):
     """Makes t's GPU the current one around a launch (its stream belongs to it); nothing to do, and
     nothing done, where it is."""
-    return _nullctx() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _NULL if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def elem_dtype_code(t: torch.Tensor, name: str) -> int:

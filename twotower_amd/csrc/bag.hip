@@ -1404,7 +1404,7 @@ int launch_piece_sum(const BwdWs& w, int64_t V, int E, hipStream_t s) {
 // pieces of long rows (bag_plan_starts_kernel, bag_plan_pieces_kernel).
 template <typename IdT>
 int plan_front(const IdT* ids, int64_t nseq, int L, int64_t ld, int64_t V, int64_t padding_idx, const BwdWs& w,
-               hipStream_t s, int part = -1, int64_t first = 1) {
+               hipStream_t s, int part = -1, int64_t first = 1, bool pieces = true) {
   // part -1: the whole plan; 0: every sort pass but the last; 1: the last pass, the segment starts
   // and the pieces (tt_bag_plan_part: the two halves on one stream compute what one call does)
   const int64_t n = nseq * L;
@@ -1465,6 +1465,7 @@ int plan_front(const IdT* ids, int64_t nseq, int L, int64_t ld, int64_t V, int64
   bag_plan_starts_kernel<<<dim3((unsigned)((nst + kBlock - 1) / kBlock)), block, 0, s>>>(w.keys_out, nvalid, V,
                                                                                        w.seg_start, w.piece_off + V);
   TT_LAUNCH_CHECK("bag_plan_starts");
+  if (!pieces) return TT_OK;
   bag_plan_pieces_kernel<<<dim3((unsigned)((V + 1 + kBlock - 1) / kBlock)), block, 0, s>>>(
       w.seg_start, V, w.nch, w.piece_off, w.piece_beg, w.piece_end);
   TT_LAUNCH_CHECK("bag_plan_pieces");
@@ -1515,23 +1516,29 @@ int check_common(int64_t V, int E, const void* ids, int ids_dtype, int64_t nseq,
 }  // namespace
 
 // The same sort for token lookups (lookup.hip): every id in [0, V) is a token, a sequence is one token,
-// so the sorted values are token indices, and there are no scaled rows to keep.
-static BwdWs token_plan_carve(void* ws, int64_t n, int64_t V, int E) {
+// so the sorted values are token indices; no scaled rows and no pieces to keep.
+static BwdWs token_plan_carve(void* ws, int64_t n, int64_t V) {
   void* base = ws ? reinterpret_cast<void*>(align_up(reinterpret_cast<size_t>(ws), 256)) : nullptr;
-  return carve(base, n, 1, V, E, sort_tmp_bytes(n, V), false);
+  return carve(base, n, 1, V, 0, sort_tmp_bytes(n, V), false);
 }
 
-size_t token_plan_bytes(int64_t n, int64_t V, int E) { return token_plan_carve(nullptr, n, V, E).total + 256; }
+size_t token_plan_bytes(int64_t n, int64_t V) { return token_plan_carve(nullptr, n, V).total + 256; }
 
-int token_plan_build(const void* ids, int ids_dtype, int64_t n, int64_t V, int E, int64_t padding_idx, void* ws,
-                     size_t ws_bytes, TokenPlan* plan, hipStream_t s) {
-  const BwdWs w = token_plan_carve(ws, n, V, E);
-  TT_REQUIRE(n > 0 && ws != nullptr && w.total + 256 <= ws_bytes, "workspace too small: need %zu have %zu",
-             w.total + 256, ws_bytes);
-  *plan = TokenPlan{w.seg_start, w.vals_out, w.nch, w.piece_off, w.piece_beg, w.piece_end, w.partial, w.max_pieces};
+TokenPlan token_plan_view(void* plan, int64_t n, int64_t V) {
+  const BwdWs w = token_plan_carve(plan, n, V);
+  const SortShape sh = sort_shape(n, V);
+  const int32_t* total = static_cast<const int32_t*>(w.sort_tmp) + ((size_t)1 << sh.D) * sh.ntiles;
+  return TokenPlan{w.seg_start, w.keys_out, w.vals_out, total + ((size_t)1 << sh.D)};
+}
+
+int token_plan_build(const void* ids, int ids_dtype, int64_t n, int64_t V, int64_t padding_idx, void* plan,
+                     size_t plan_bytes, hipStream_t s) {
+  const BwdWs w = token_plan_carve(plan, n, V);
+  TT_REQUIRE(n > 0 && plan != nullptr && w.total + 256 <= plan_bytes, "workspace too small: need %zu have %zu",
+             w.total + 256, plan_bytes);
   return ids_dtype == TT_IDS_I32
-             ? plan_front(static_cast<const int32_t*>(ids), n, 1, 1, V, padding_idx, w, s, -1, 0)
-             : plan_front(static_cast<const int64_t*>(ids), n, 1, 1, V, padding_idx, w, s, -1, 0);
+             ? plan_front(static_cast<const int32_t*>(ids), n, 1, 1, V, padding_idx, w, s, -1, 0, false)
+             : plan_front(static_cast<const int64_t*>(ids), n, 1, 1, V, padding_idx, w, s, -1, 0, false);
 }
 
 }  // namespace tt

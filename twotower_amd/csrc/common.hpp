@@ -150,6 +150,19 @@ __device__ __forceinline__ void store_elems(T* p, const float (&x)[VEC]) {
   for (int i = 0; i < VEC; ++i) e.v[i] = (T)x[i];
   *reinterpret_cast<Elems<T, VEC>*>(p) = e;
 }
+// the same past the caches: for rows that this launch does not read again
+template <int VEC, typename T>
+__device__ __forceinline__ void store_elems_nt(T* p, const float (&x)[VEC]) {
+  constexpr int kBytes = sizeof(T) * VEC;
+  Elems<T, VEC> e;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) e.v[i] = (T)x[i];
+  if constexpr (kBytes == 16) {
+    __builtin_nontemporal_store(__builtin_bit_cast(tt_u32x4, e), reinterpret_cast<tt_u32x4*>(p));
+  } else {
+    *reinterpret_cast<Elems<T, VEC>*>(p) = e;
+  }
+}
 inline int elem_bytes(int dtype) { return dtype == TT_E_F32 ? 4 : 2; }
 inline bool elem_ok(int dtype) { return dtype == TT_E_F32 || dtype == TT_E_BF16 || dtype == TT_E_F16; }
 // The widest VEC in {8, 4, 2, 1} that divides every count in n[] and keeps each pointer's access aligned
@@ -168,22 +181,18 @@ inline int vec_for(const int64_t* n, int nn, const void* const* p, const int* by
 }
 
 // The sort plan of a token lookup's gradient (built in bag.hip by the bags' counting sort, read by
-// lookup.hip): row r's tokens are vals[seg_start[r] .. seg_start[r + 1]), in token order; a row of more than
-// kPieceT tokens has nch[r] pieces from slot piece_off[r] (piece k sums tokens piece_beg[k] .. piece_end[k]
-// of vals into partial[k]); piece_off[V] is the number of pieces.
+// lookup.hip): the kept tokens' rows `keys` in ascending order, their token indices `vals` (a row's in token
+// order), row r's at [seg_start[r], seg_start[r + 1]); *count tokens were kept.
 struct TokenPlan {
   const int32_t* seg_start;
+  const uint32_t* keys;
   const int32_t* vals;
-  const int32_t* nch;
-  const int32_t* piece_off;
-  const int32_t* piece_beg;
-  const int32_t* piece_end;
-  float* partial;
-  int64_t max_pieces;
+  const int32_t* count;
 };
-size_t token_plan_bytes(int64_t n, int64_t V, int E);
-int token_plan_build(const void* ids, int ids_dtype, int64_t n, int64_t V, int E, int64_t padding_idx, void* ws,
-                     size_t ws_bytes, TokenPlan* plan, hipStream_t s);
+size_t token_plan_bytes(int64_t n, int64_t V);
+TokenPlan token_plan_view(void* plan, int64_t n, int64_t V);
+int token_plan_build(const void* ids, int ids_dtype, int64_t n, int64_t V, int64_t padding_idx, void* plan,
+                     size_t plan_bytes, hipStream_t s);
 
 // The tower head's weight planes (tt_head_split*, head.hip): each fp32 weight is cut into three
 // bf16 terms, x = a0 + a1 + a2 exactly.  Job j of SplitJobs writes the three planes of an n x k

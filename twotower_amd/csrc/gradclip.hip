@@ -206,33 +206,43 @@ __global__ __launch_bounds__(kBlock) void clip_scale_kernel(ClipList l, const do
   }
 }
 
+// the call's tensors, as the caller's host arrays
+struct ClipCall {
+  const void* const* src;
+  void* const* dst;
+  const int64_t* n;
+  const uint8_t* src_dtype;
+  const uint8_t* dst_dtype;
+  int count;
+};
+
 // tensors [at, at + TT_CLIP_MAX_TENSORS) of the call as one launch's list
-void fill_list(ClipList& l, const tt_clip_tensor* t, int at, int count) {
-  const int m = count - at < TT_CLIP_MAX_TENSORS ? count - at : TT_CLIP_MAX_TENSORS;
+void fill_list(ClipList& l, const ClipCall& t, int at) {
+  const int m = t.count - at < TT_CLIP_MAX_TENSORS ? t.count - at : TT_CLIP_MAX_TENSORS;
   int64_t chunk = 0;
   for (int i = 0; i < m; ++i) {
-    l.src[i] = t[at + i].src;
-    l.dst[i] = t[at + i].dst;
-    l.n[i] = t[at + i].n;
-    l.type[i] = (uint8_t)(t[at + i].src_dtype | t[at + i].dst_dtype << 2);
+    l.src[i] = t.src[at + i];
+    l.dst[i] = t.dst[at + i];
+    l.n[i] = t.n[at + i];
+    l.type[i] = (uint8_t)(t.src_dtype[at + i] | t.dst_dtype[at + i] << 2);
     l.first[i] = (int32_t)chunk;
-    chunk += (t[at + i].n + kChunk - 1) / kChunk;
+    chunk += (t.n[at + i] + kChunk - 1) / kChunk;
   }
   l.first[m] = (int32_t)chunk;
   l.count = m;
 }
 
 template <bool INF>
-int run_clip(const tt_clip_tensor* t, int count, bool scale, double max_norm, float* norm, double* parts,
+int run_clip(const ClipCall& t, bool scale, double max_norm, float* norm, double* parts,
              hipStream_t s) {
-  const int launches = (count + TT_CLIP_MAX_TENSORS - 1) / TT_CLIP_MAX_TENSORS;
+  const int count = t.count, launches = (count + TT_CLIP_MAX_TENSORS - 1) / TT_CLIP_MAX_TENSORS;
   int cap = launches > 0 ? kMaxParts / launches : 1;
   cap = cap < 1 ? 1 : cap > kNormBlocks ? kNormBlocks : cap;
   static_assert(sizeof(ClipList) <= 3840, "kernel arguments");
   ClipList l;
   int np = 0;
   for (int at = 0; at < count; at += TT_CLIP_MAX_TENSORS) {
-    fill_list(l, t, at, count);
+    fill_list(l, t, at);
     const int chunks = l.first[l.count];
     if (chunks == 0) continue;
     const int g = chunks < cap ? chunks : cap;
@@ -243,7 +253,7 @@ int run_clip(const tt_clip_tensor* t, int count, bool scale, double max_norm, fl
   bool wrote = false;
   if (scale)
     for (int at = 0; at < count; at += TT_CLIP_MAX_TENSORS) {
-      if (launches > 1) fill_list(l, t, at, count);
+      if (launches > 1) fill_list(l, t, at);
       const int chunks = l.first[l.count];
       if (chunks == 0) continue;
       const int g = chunks < kScaleBlocks ? chunks : kScaleBlocks;
@@ -268,26 +278,27 @@ extern "C" size_t tt_clip_ws_size(int count) {
   return sizeof(double) * (size_t)(launches > kMaxParts ? launches : kMaxParts);
 }
 
-extern "C" int tt_clip_grads(const tt_clip_tensor* tensors, int count, int inf_norm, double max_norm, int scale,
+extern "C" int tt_clip_grads(const void* const* src, void* const* dst, const int64_t* n, const uint8_t* src_dtype,
+                             const uint8_t* dst_dtype, int count, int inf_norm, double max_norm, int scale,
                              float* norm, void* ws, size_t ws_bytes, tt_stream_t stream) {
-  TT_REQUIRE(count >= 0 && (tensors || count == 0) && norm, "clip: null pointer or count=%d", count);
+  TT_REQUIRE(count >= 0 && ((src && dst && n && src_dtype && dst_dtype) || count == 0) && norm,
+             "clip: null pointer or count=%d", count);
   TT_REQUIRE(!scale || max_norm >= 0.0, "clip: max_norm must not be negative");
   TT_REQUIRE(ws && ws_bytes >= tt_clip_ws_size(count) && reinterpret_cast<size_t>(ws) % 8 == 0,
              "workspace too small: need %zu have %zu", tt_clip_ws_size(count), ws_bytes);
+  int64_t chunks = 0;  // of one launch, counted in 32 bits
   for (int i = 0; i < count; ++i) {
-    const tt_clip_tensor& t = tensors[i];
-    TT_REQUIRE(t.n >= 0 && t.n < (int64_t(1) << 37), "clip: tensor %d has %lld elements", i, (long long)t.n);
-    TT_REQUIRE(t.n == 0 || (t.src && (!scale || t.dst)), "clip: tensor %d is NULL", i);
-    TT_REQUIRE(elem_ok(t.src_dtype) && (!scale || t.dst_dtype == t.src_dtype || t.dst_dtype == TT_E_F32),
-               "clip: tensor %d of type %d into type %d", i, t.src_dtype, t.dst_dtype);
-  }
-  for (int at = 0; at < count; at += TT_CLIP_MAX_TENSORS) {  // a launch's chunks are counted in 32 bits
-    int64_t chunks = 0;
-    for (int i = at; i < count && i < at + TT_CLIP_MAX_TENSORS; ++i) chunks += (tensors[i].n + kChunk - 1) / kChunk;
+    TT_REQUIRE(n[i] >= 0 && n[i] < (int64_t(1) << 44), "clip: tensor %d has %lld elements", i, (long long)n[i]);
+    TT_REQUIRE(n[i] == 0 || (src[i] && (!scale || dst[i])), "clip: tensor %d is NULL", i);
+    TT_REQUIRE(elem_ok(src_dtype[i]) && elem_ok(dst_dtype[i]) &&
+                   (dst_dtype[i] == src_dtype[i] || dst_dtype[i] == TT_E_F32),
+               "clip: tensor %d of type %d into type %d", i, src_dtype[i], dst_dtype[i]);
+    chunks = (i % TT_CLIP_MAX_TENSORS ? chunks : 0) + (n[i] + kChunk - 1) / kChunk;
     TT_REQUIRE(chunks < (int64_t(1) << 31) - kScaleBlocks, "clip: too many elements");
   }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   double* parts = static_cast<double*>(ws);
-  return inf_norm ? run_clip<true>(tensors, count, scale != 0, max_norm, norm, parts, s)
-                  : run_clip<false>(tensors, count, scale != 0, max_norm, norm, parts, s);
+  const ClipCall t{src, dst, n, src_dtype, dst_dtype, count};
+  return inf_norm ? run_clip<true>(t, scale != 0, max_norm, norm, parts, s)
+                  : run_clip<false>(t, scale != 0, max_norm, norm, parts, s);
 }

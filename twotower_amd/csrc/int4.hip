@@ -21,7 +21,6 @@ namespace tt {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kWavesPerBlock = kBlock / kWave;
 constexpr int kRows = 16;   // documents per tile
 constexpr int kBlk = 32;    // columns per matrix instruction
 constexpr int kQuad = 128;  // columns per lane load
@@ -197,85 +196,143 @@ __device__ __forceinline__ int query_exponent(float mx) {
   return mx > 0.f && mx <= 3.402823466e38f ? 3 - ilogbf(mx) : 0;
 }
 
-template <typename T, int NQT, int SPQ>
-__global__ __launch_bounds__(kBlock) void int4_scores_kernel(const T* __restrict__ q, int nq, int64_t ldq,
-                                                             const uint32_t* __restrict__ codes,
-                                                             const uint16_t* __restrict__ scales, int64_t n, int H,
-                                                             int nblk, int nquad, float* __restrict__ scores,
-                                                             int64_t ld_scores) {
+// elements k0 .. k0 + 7 of query i, zeros past the queries and past H
+template <typename T>
+__device__ __forceinline__ void load_query(const T* __restrict__ q, int i, int nq, int64_t ldq, int H, int k0,
+                                           bool wide, float (&x)[8]) {
+  const T* p = q + i * ldq + k0;
+#pragma unroll
+  for (int g = 0; g < 8; g += 4) {
+    float y[4] = {0.f, 0.f, 0.f, 0.f};
+    if (i < nq && wide) {
+      if (k0 + g < H) load_elems<4>(p + g, y);
+    } else if (i < nq) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (k0 + g + e < H) y[e] = (float)p[g + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[g + e] = y[e];
+  }
+}
+
+// What a wave loads for one quad of its tiles.
+template <int SPQ>
+struct QuadLoad {
+  uint32_t c[kTPW][4];
+  Elems<uint16_t, SPQ> s[kTPW];
+};
+template <int SPQ>
+__device__ __forceinline__ void load_quad(QuadLoad<SPQ>& x, const uint32_t* __restrict__ codes,
+                                          const uint16_t* __restrict__ scales, int64_t t0, int64_t ntile, int b,
+                                          int nblk, int nquad, int lane) {
+  const int dpl = nblk - 4 * b < 4 ? nblk - 4 * b : 4;
+#pragma unroll
+  for (int u = 0; u < kTPW; ++u) {
+    const int64_t t = t0 + u < ntile ? t0 + u : ntile - 1;  // (a clamped tile is never stored)
+    const uint32_t* p = codes + t * nblk * 64 + b * 256 + lane * dpl;
+    if (dpl == 4) {
+      const tt_u32x4 v = *reinterpret_cast<const tt_u32x4*>(p);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) x.c[u][d] = v[d];
+    } else {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) x.c[u][d] = d < dpl ? p[d] : kZeroCodes;
+    }
+    x.s[u] = *reinterpret_cast<const Elems<uint16_t, SPQ>*>(scales + ((t * nquad + b) * kRows + (lane & 15)) * SPQ);
+  }
+}
+
+template <typename T, int NQT, int SPQ, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void int4_scores_kernel(const T* __restrict__ q, int nq, int64_t ldq,
+                                                            const uint32_t* __restrict__ codes,
+                                                            const uint16_t* __restrict__ scales, int64_t n, int H,
+                                                            int nblk, int nquad, bool wide,
+                                                            float* __restrict__ scores, int64_t ld_scores) {
   using Q = QueryTiles<NQT>;
+  constexpr int kWaves = BLOCK / kWave;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   f16x8* A = reinterpret_cast<f16x8*>(smem);  // [4 nquad][kOps][64]
   __shared__ int qe[Q::kQ];
   const int lane = lane_id(), w = threadIdx.x >> 6, j = lane & 15, h = lane >> 4;
-  for (int i = w; i < Q::kQ; i += kWavesPerBlock) {
-    float mx = 0.f;
-    if (i < nq)
-      for (int k = lane; k < H; k += kWave) mx = fmaxf(mx, fabsf((float)q[i * ldq + k]));
+  const int64_t ntile = (n + kRows - 1) / kRows;
+  const int64_t step = (int64_t)gridDim.x * kWaves * kTPW;
+  int64_t t0 = ((int64_t)blockIdx.x * kWaves + w) * kTPW;
+  QuadLoad<SPQ> cur;  // the first documents are on their way while the queries are laid out
+  if (t0 < ntile) load_quad<SPQ>(cur, codes, scales, t0, ntile, 0, nblk, nquad, lane);
+
+  // A thread takes 8 elements of one query (several runs of 8 where there are more): their maximum joins the
+  // query's (an integer maximum of the bits, whatever the order), then their terms go to the operands.
+  if (threadIdx.x < Q::kQ) qe[threadIdx.x] = 0;
+  __syncthreads();
+  const int items = nblk * Q::kQ * 4;
+  float x[8];
+  for (int it = threadIdx.x; it < items; it += BLOCK) {
+    const int i = (it >> 2) % Q::kQ, k0 = ((it >> 2) / Q::kQ) * kBlk + 8 * (it & 3);
+    load_query(q, i, nq, ldq, H, k0, wide, x);
+    uint32_t mx = 0;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-    if (lane == 0) qe[i] = query_exponent(mx);
+    for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(fabsf(x[e])));
+    if (mx) atomicMax(reinterpret_cast<uint32_t*>(&qe[i]), mx);
   }
   __syncthreads();
-  for (int it = threadIdx.x; it < 4 * nquad * Q::kOps * kWave; it += kBlock) {
-    const int l = it & 63, a = (it >> 6) % Q::kOps, b = (it >> 6) / Q::kOps;
-    const int m = l & 15, k0 = b * kBlk + 8 * (l >> 4);
-    const int i = NQT == 0 ? m >> 2 : (a / 3) * 16 + m;   // query
-    const int term = NQT == 0 ? m & 3 : a % 3;
-    f16x8 v;
+  int own_e = threadIdx.x < Q::kQ ? query_exponent(__int_as_float(qe[threadIdx.x])) : 0;
+  __syncthreads();
+  if (threadIdx.x < Q::kQ) qe[threadIdx.x] = own_e;
+  __syncthreads();
+  for (int it = threadIdx.x; it < items; it += BLOCK) {
+    const int hh = it & 3, i = (it >> 2) % Q::kQ, b = (it >> 2) / Q::kQ;
+    if (items > BLOCK) load_query(q, i, nq, ldq, H, b * kBlk + 8 * hh, wide, x);
+    f16x8 t0v, t1v, t2v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int k = k0 + e;
-      const float x = i < nq && k < H && term < 3 ? ldexpf((float)q[i * ldq + k], qe[i]) : 0.f;
-      const _Float16 t0 = (_Float16)x;
-      const float r1 = x - (float)t0;
-      const _Float16 t1 = (_Float16)r1;
-      const _Float16 t2 = (_Float16)(r1 - (float)t1);
-      v[e] = term == 0 ? t0 : term == 1 ? t1 : t2;
+      const float y = ldexpf(x[e], qe[i]);
+      t0v[e] = (_Float16)y;
+      const float r1 = y - (float)t0v[e];
+      t1v[e] = (_Float16)r1;
+      t2v[e] = (_Float16)(r1 - (float)t1v[e]);
     }
-    A[it] = v;
+    if constexpr (NQT == 0) {
+      f16x8* at = A + b * kWave + hh * 16 + 4 * i;
+      at[0] = t0v;
+      at[1] = t1v;
+      at[2] = t2v;
+      at[3] = f16x8{};
+    } else {
+      f16x8* at = A + ((size_t)b * Q::kOps + 3 * (i >> 4)) * kWave + hh * 16 + (i & 15);
+      at[0] = t0v;
+      at[kWave] = t1v;
+      at[2 * kWave] = t2v;
+    }
   }
   __syncthreads();
 
-  const int64_t ntile = (n + kRows - 1) / kRows;
-  const int64_t step = (int64_t)gridDim.x * kWavesPerBlock * kTPW;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t t0 = ((int64_t)blockIdx.x * kWavesPerBlock + w) * kTPW; t0 < ntile; t0 += step) {
+  for (; t0 < ntile; t0 += step) {
     float acc[kTPW][Q::kAcc] = {};
     for (int b = 0; b < nquad; ++b) {
       const int dpl = nblk - 4 * b < 4 ? nblk - 4 * b : 4;
-      uint32_t c[kTPW][4];
-      float s[kTPW][SPQ];
-#pragma unroll
-      for (int u = 0; u < kTPW; ++u) {
-        const int64_t t = t0 + u < ntile ? t0 + u : ntile - 1;  // (a clamped tile is never stored)
-        const uint32_t* p = codes + t * nblk * 64 + b * 256 + lane * dpl;
-        if (dpl == 4) {
-          const tt_u32x4 x = *reinterpret_cast<const tt_u32x4*>(p);
-#pragma unroll
-          for (int d = 0; d < 4; ++d) c[u][d] = x[d];
-        } else {
-#pragma unroll
-          for (int d = 0; d < 4; ++d) c[u][d] = d < dpl ? p[d] : kZeroCodes;
-        }
-        const Elems<uint16_t, SPQ> x =
-            *reinterpret_cast<const Elems<uint16_t, SPQ>*>(scales + ((t * nquad + b) * kRows + j) * SPQ);
-#pragma unroll
-        for (int g = 0; g < SPQ; ++g) s[u][g] = bf16_value(x.v[g]);
-      }
+      QuadLoad<SPQ> next;  // the quad after this one, loaded before this one is used
+      const bool last = b + 1 == nquad;
+      if (!last || t0 + step < ntile)
+        load_quad<SPQ>(next, codes, scales, last ? t0 + step : t0, ntile, last ? 0 : b + 1, nblk, nquad, lane);
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
         if (d >= dpl) break;
         f16x8 B[kTPW];
+        float s[kTPW];
 #pragma unroll
-        for (int u = 0; u < kTPW; ++u) B[u] = widen(c[u][d]);
+        for (int u = 0; u < kTPW; ++u) {
+          B[u] = widen(cur.c[u][d]);
+          s[u] = bf16_value(cur.s[u].v[d * SPQ / 4]);
+        }
         const f16x8* Ab = A + (size_t)(4 * b + d) * Q::kOps * kWave + lane;
         if constexpr (NQT == 0) {
           const f16x8 a = Ab[0];
 #pragma unroll
           for (int u = 0; u < kTPW; ++u) {
             const f32x4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, B[u], zero, 0, 0, 0);
-            acc[u][0] = __builtin_fmaf(s[u][d * SPQ / 4], (r[2] + r[1]) + r[0], acc[u][0]);
+            acc[u][0] = __builtin_fmaf(s[u], (r[2] + r[1]) + r[0], acc[u][0]);
           }
         } else {
 #pragma unroll
@@ -287,12 +344,12 @@ __global__ __launch_bounds__(kBlock) void int4_scores_kernel(const T* __restrict
               r = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, B[u], r, 0, 0, 0);
               r = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, B[u], r, 0, 0, 0);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                acc[u][4 * qt + e] = __builtin_fmaf(s[u][d * SPQ / 4], r[e], acc[u][4 * qt + e]);
+              for (int e = 0; e < 4; ++e) acc[u][4 * qt + e] = __builtin_fmaf(s[u], r[e], acc[u][4 * qt + e]);
             }
           }
         }
       }
+      cur = next;
     }
 #pragma unroll
     for (int u = 0; u < kTPW; ++u) {
@@ -309,22 +366,37 @@ __global__ __launch_bounds__(kBlock) void int4_scores_kernel(const T* __restrict
 
 constexpr size_t kMaxLds = 96 * 1024;  // query operands per workgroup
 
-template <typename T, int NQT, int SPQ>
-int launch_scores(const T* q, int nq, int64_t ldq, const uint32_t* codes, const uint16_t* scales, int64_t n, int H,
-                  float* scores, int64_t ld_scores, hipStream_t s) {
+template <typename T, int NQT, int SPQ, int BLOCK>
+int launch_scores_block(const T* q, int nq, int64_t ldq, const uint32_t* codes, const uint16_t* scales, int64_t n,
+                        int H, float* scores, int64_t ld_scores, hipStream_t s) {
   const int nquad = quads_of(H);
   const size_t lds = (size_t)4 * nquad * QueryTiles<NQT>::kOps * kWave * 16;
-  const int64_t groups = (tiles_of(n) + kTPW * kWavesPerBlock - 1) / (kTPW * kWavesPerBlock);
-  const int per_cu = lds > 64 * 1024 ? 1 : lds > 32 * 1024 ? 2 : lds > 16 * 1024 ? 4 : 8;
-  const int64_t most = 256 * per_cu;
-  auto kernel = int4_scores_kernel<T, NQT, SPQ>;
+  const int64_t per = (int64_t)kTPW * (BLOCK / kWave), groups = (tiles_of(n) + per - 1) / per;
+  // (for up to 4 queries every wave that fits; more leave the time to fewer, longer workgroups)
+  int64_t per_cu = (int64_t)(160 * 1024) / (int64_t)(lds + 1024);  // workgroups a CU's LDS and 32 waves hold
+  const int64_t waves = NQT == 0 ? 32 : 16;
+  if (per_cu > waves * kWave / BLOCK) per_cu = waves * kWave / BLOCK;
+  const int64_t most = 256 * (per_cu < 1 ? 1 : per_cu);
+  const int64_t rounds = (groups + most - 1) / most;  // every workgroup the same number of passes, nearly
+  const bool wide = H % 4 == 0 && ldq % 4 == 0 && reinterpret_cast<size_t>(q) % (4 * sizeof(T)) == 0;
+  auto kernel = int4_scores_kernel<T, NQT, SPQ, BLOCK>;
   if (lds > 64 * 1024)
     TT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                (int)lds), "int4_scores LDS");
-  kernel<<<dim3((unsigned)(groups < most ? groups : most)), dim3(kBlock), lds, s>>>(
-      q, nq, ldq, codes, scales, n, H, blocks_of(H), nquad, scores, ld_scores);
+  kernel<<<dim3((unsigned)((groups + rounds - 1) / rounds)), dim3(BLOCK), lds, s>>>(
+      q, nq, ldq, codes, scales, n, H, blocks_of(H), nquad, wide, scores, ld_scores);
   TT_LAUNCH_CHECK("int4_scores");
   return TT_OK;
+}
+
+// Small workgroups spread a short index over the CUs; with more tiles than that, larger ones share one set
+// of query operands in LDS between more waves.
+template <typename T, int NQT, int SPQ>
+int launch_scores(const T* q, int nq, int64_t ldq, const uint32_t* codes, const uint16_t* scales, int64_t n, int H,
+                  float* scores, int64_t ld_scores, hipStream_t s) {
+  if (NQT > 1 && tiles_of(n) > 256 * 4 * kTPW)
+    return launch_scores_block<T, NQT, SPQ, 512>(q, nq, ldq, codes, scales, n, H, scores, ld_scores, s);
+  return launch_scores_block<T, NQT, SPQ, 256>(q, nq, ldq, codes, scales, n, H, scores, ld_scores, s);
 }
 
 template <typename T, int SPQ>

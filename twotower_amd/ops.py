@@ -532,7 +532,7 @@ def bag_mean_pool(weight: torch.Tensor, ids: torch.Tensor, padding_idx: int | No
 # Token lookup with a scale   (twotower/embeddings.py:40, the (B, L, E) rows a tower may pool itself)
 def _lookup_fwd(weight, ids, scale, out_dtype):
     V, E = weight.shape
-    out = torch.empty(*ids.shape, E, dtype=out_dtype, device=weight.device)
+    out = weight.new_empty((*ids.shape, E), dtype=out_dtype)
     if out.numel():
         with _lib.on_device(weight):
             call("tt_lookup_fwd", ptr(weight), _lib.ELEM_DTYPES[weight.dtype], V, E, weight.stride(0), ptr(ids),
@@ -560,13 +560,21 @@ class EmbeddingLookup(torch.autograd.Function):
             deferred.added_dense()
         dout = dout.contiguous()
         n = ids.numel()
-        grad = torch.empty(V, E, dtype=dtype, device=dout.device)
-        nbytes = _lib.lib().tt_lookup_bwd_ws_size(n, V, E)
-        # per call, not shared: two captured graphs (or streams) may run their backwards at once
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dout.device) if nbytes else None
+        grad = dout.new_empty((V, E), dtype=dtype)
+        nbytes = _lib.lib().tt_lookup_bwd_ws_size(n, E)
+        size = _lib.lib().tt_lookup_plan_size(n, V)
         with _lib.on_device(dout):
+            plan = ws = None
+            if size:
+                # Sorted here, not beside the forward on a side stream: the gather fills the memory system and every
+                # CU, and the sort beside it ended no sooner (forward and backward back to back 352 against 344
+                # us at 8192 x 64 tokens).  Buffers per call, not shared: two captured graphs, or streams, may run
+                # their backwards at once.
+                plan = dout.new_empty((size,), dtype=torch.uint8)
+                call("tt_lookup_plan", ptr(ids), _lib.ids_dtype_code(ids), n, V, pad, ptr(plan), size, stream_of(dout))
+                ws = dout.new_empty((nbytes,), dtype=torch.uint8)
             call("tt_lookup_bwd", ptr(dout), _lib.ELEM_DTYPES[dout.dtype], ptr(ids), _lib.ids_dtype_code(ids), n, V, E,
-                 pad, scale, ptr(grad), _lib.ELEM_DTYPES[dtype], ptr(ws), nbytes, stream_of(dout))
+                 pad, scale, ptr(grad), _lib.ELEM_DTYPES[dtype], ptr(plan), size, ptr(ws), nbytes, stream_of(dout))
         return grad, None, None, None, None
 
 
@@ -1201,7 +1209,7 @@ def _pref_fwd(q, p, n, dt, ref, mask, opts, margins=None, loss=None):
     (B, K, H), (kind, beta, inv_tau, smooth) = n.shape, opts
     side, at = None, (None, None, None)
     if loss is not None:
-        side = torch.empty(B * K + 1 + 2 * B, dtype=_FLOAT, device=q.device)
+        side = q.new_empty((B * K + 1 + 2 * B,), dtype=_FLOAT)
         base = side.data_ptr()
         at = (base, base + 4 * B * K, base + 4 * (B * K + 1))
     with _lib.on_device(q):
@@ -1223,7 +1231,7 @@ def _pref_bwd(q, p, n, dt, mask, opts, side, g, dq, dp, dn):
 class PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, p, n, dt, ref, mask, opts):
-        loss = torch.empty((), dtype=_FLOAT, device=q.device)
+        loss = q.new_empty((), dtype=_FLOAT)
         side = _pref_fwd(q, p, n, dt, ref, mask, opts, loss=loss)
         ctx.save_for_backward(q, p, n, mask, side)
         ctx.meta = (dt, opts)
@@ -1232,7 +1240,8 @@ class PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         q, p, n, mask, side = ctx.saved_tensors
-        dq, dp, dn = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, p, n))
+        # (empty_like: torch.empty with a device argument takes four times as long on autograd's thread)
+        dq, dp, dn = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, p, n))
         _pref_bwd(q, p, n, ctx.meta[0], mask, ctx.meta[1], side, g, dq, dp, dn)
         return dq, dp, dn, None, None, None, None
 
@@ -1243,7 +1252,7 @@ class PreferenceLossPacked(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qpn, B, K, dt, ref, mask, opts):
-        loss = torch.empty((), dtype=_FLOAT, device=qpn.device)
+        loss = qpn.new_empty((), dtype=_FLOAT)
         side = _pref_fwd(qpn[:B], qpn[B:2 * B], qpn[2 * B:].view(B, K, -1), dt, ref, mask, opts, loss=loss)
         ctx.save_for_backward(qpn, mask, side)
         ctx.meta = (B, K, dt, opts)
@@ -1607,47 +1616,51 @@ def clip_grad_norm(grads, max_norm: float | None, norm_type: float = 2.0, out=No
         return torch.zeros((), dtype=_FLOAT)
     first = grads[0]
     dev, codes = first.device, _lib.ELEM_DTYPES
-    items = (_lib.ClipTensor * len(grads))()
-    copies, seen = [], set()
-    for i, (g, o) in enumerate(zip(grads, outs)):
-        if g.is_sparse:
-            raise RuntimeError("clip_grad_norm does not support sparse gradients")
-        gd, od = codes.get(g.dtype), codes.get(o.dtype)
-        if gd is None or (od != gd and od != 0):
-            raise TypeError(f"gradient {i} of {g.dtype} into {o.dtype}: float32, bfloat16 or float16, into its own type "
-                            "or float32")
-        if g.shape != o.shape:
-            raise ValueError(f"out {i} has shape {tuple(o.shape)}, the gradient {tuple(g.shape)}")
-        src = dst = g
-        if o is not g:
-            src = g if g.is_contiguous() else g.contiguous()
-            dst = o
-            if not o.is_contiguous():
-                dst = torch.empty(o.shape, dtype=o.dtype, device=dev)
-                copies.append((o, dst))
-        elif not _dense(g):
-            if scale and torch._debug_has_internal_overlap(g) == 1:
-                raise ValueError(f"gradient {i} has elements that share memory (an expanded tensor): clip a copy")
-            src = dst = g.contiguous()
-            if scale:
-                copies.append((g, dst))
-        if scale and g.numel():
-            if dst.data_ptr() in seen:
-                raise ValueError(f"gradient {i} is written twice: the same memory is listed more than once")
-            seen.add(dst.data_ptr())
-        items[i] = _lib.ClipTensor(src.data_ptr(), dst.data_ptr(), g.numel(), gd, od)
-        if src is not g:
-            copies.append((None, src))  # kept until the launches are queued
-    _lib.same_device(first, *grads, *(outs if outs is not grads else ()))
-    norm = torch.empty((), dtype=_FLOAT, device=dev)
-    nbytes = _lib.lib().tt_clip_ws_size(len(grads))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    types = [codes.get(g.dtype) for g in grads]
+    otypes = types if outs is grads else [codes.get(o.dtype) for o in outs]
+    if None in types or any(o != g and o != 0 for g, o in zip(types, otypes)):
+        i = next(i for i, (g, o) in enumerate(zip(types, otypes)) if g is None or (o != g and o != 0))
+        raise TypeError(f"gradient {i} of {grads[i].dtype} into {outs[i].dtype}: float32, bfloat16 or float16, into its own "
+                        "type or float32")
+    if any(g.is_sparse for g in grads):
+        raise RuntimeError("clip_grad_norm does not support sparse gradients")
+    copies = []
+    if outs is grads:
+        src = [g if g.is_contiguous() or _dense(g) else g.contiguous() for g in grads]
+        dst = src
+        if scale:
+            copies = [(g, t) for g, t in zip(grads, src) if t is not g]
+            for g, _ in copies:
+                if torch._debug_has_internal_overlap(g) == 1:
+                    raise ValueError(f"a gradient of shape {tuple(g.shape)} has elements that share memory (an expanded "
+                                     "tensor): clip a copy")
+    else:
+        if any(g.shape != o.shape for g, o in zip(grads, outs)):
+            i = next(i for i, (g, o) in enumerate(zip(grads, outs)) if g.shape != o.shape)
+            raise ValueError(f"out {i} has shape {tuple(outs[i].shape)}, the gradient {tuple(grads[i].shape)}")
+        src = [g if g.is_contiguous() else g.contiguous() for g in grads]
+        dst = [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in outs]
+        copies = [(o, t) for o, t in zip(outs, dst) if t is not o]
+    sizes = [g.numel() for g in grads]
+    src_at = [t.data_ptr() for t in src]
+    dst_at = src_at if dst is src else [t.data_ptr() for t in dst]
+    if scale and len(set(dst_at)) != len(dst_at):
+        written = [a for a, n in zip(dst_at, sizes) if n]
+        if len(set(written)) != len(written):
+            raise ValueError("a gradient is written twice: the same memory is listed more than once")
+    if first.get_device() < 0 or any(g.get_device() != first.get_device() for g in grads) or (
+            outs is not grads and any(o.get_device() != first.get_device() for o in outs)):
+        _lib.same_device(first, *grads, *outs)  # (says which)
+    n = len(grads)
+    norm = first.new_empty((), dtype=_FLOAT)
+    nbytes = _lib.lib().tt_clip_ws_size(n)
+    ws = first.new_empty((nbytes,), dtype=torch.uint8)
     with _lib.on_device(first):
-        call("tt_clip_grads", items, len(grads), int(norm_type == float("inf")), float(max_norm) if scale else 0.0,
+        call("tt_clip_grads", (ctypes.c_int64 * n)(*src_at), (ctypes.c_int64 * n)(*dst_at), (ctypes.c_int64 * n)(*sizes),
+             bytes(types), bytes(otypes), n, int(norm_type == float("inf")), float(max_norm) if scale else 0.0,
              int(scale), ptr(norm), ptr(ws), nbytes, stream_of(first))
     for o, t in copies:
-        if o is not None:
-            o.copy_(t)
+        o.copy_(t)
     return norm
 
 

@@ -41,6 +41,7 @@ _VMEM_PREFIX = ("global_", "buffer_", "scratch_", "tbuffer_")
 def compile_to_asm(src: str, out_dir: str, extra=()) -> str:
     out = os.path.join(out_dir, os.path.basename(src) + ".s")
     cmd = [HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
+           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
            "-I" + os.path.join(ROOT, "include"), *extra, "--cuda-device-only", "-S", src, "-o", out]
     subprocess.run(cmd, check=True, stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
     return out

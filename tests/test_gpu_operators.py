@@ -391,6 +391,21 @@ def test_preference_on_the_fused_tower_output(K):
     assert torch.equal(got, torch.cat([t.reshape(-1, H) for t in want]) * 0.3)
 
 
+def test_preference_on_views_that_are_their_own_leaves():
+    x = torch.randn(60, 32, generator=gen(28), device=DEV)
+    q, p, n = (t.requires_grad_(True) for t in x.split([20, 20, 20]))  # blocks of a tensor without a gradient
+    loss = losses.preference_loss(q, p, n, beta=0.5)
+    got = torch.autograd.grad(loss, (q, p, n))
+    a, b, c = (t.detach().clone().requires_grad_(True) for t in (q, p, n))
+    assert all(torch.equal(u, v) for u, v in zip(got, torch.autograd.grad(losses.preference_loss(a, b, c, beta=0.5), (a, b, c))))
+    y = x.clone().requires_grad_(True)
+    with torch.no_grad():
+        q = y[:20]  # no gradient is wanted through the queries
+    loss = losses.preference_loss(q, y[20:40], y[40:], beta=0.5)
+    (g,) = torch.autograd.grad(loss, y)
+    assert not g[:20].any() and torch.equal(g[20:40], got[1]) and torch.equal(g[40:], got[2])
+
+
 def test_preference_margin_is_the_reference_term():
     q, p, n, _, _ = pref_case(77, 48, 2, BF16, False, 0.0, 25)
     r = losses.preference_margin(q.requires_grad_(True), p, n, temperature=0.1)

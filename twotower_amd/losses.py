@@ -85,6 +85,11 @@ def preference_loss(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg_embs: to
         B, K = q_emb.shape[0], 1 if d_neg_embs.dim() == 2 else d_neg_embs.shape[1]
         if B and K and d_pos_emb.shape == q_emb.shape and d_neg_embs.numel() == B * K * q_emb.shape[1]:
             packed = _packed(q_emb, d_pos_emb, d_neg_embs.view(B * K, -1))
+            # (one gradient for the base stands for the three only where autograd would bring them there: not
+            # for leaves that are views of a plain tensor, nor for views taken under no_grad)
+            if packed is not None and not (packed.requires_grad == q_emb.requires_grad == d_pos_emb.requires_grad
+                                           == d_neg_embs.requires_grad):
+                packed = None
     return ops.preference_loss(q_emb, d_pos_emb, d_neg_embs, ref_margin=ref_margin, mask=mask, beta=beta,
                                temperature=temperature, label_smoothing=label_smoothing, loss_type=loss_type,
                                packed=packed)

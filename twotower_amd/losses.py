@@ -87,8 +87,8 @@ def preference_loss(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg_embs: to
             packed = _packed(q_emb, d_pos_emb, d_neg_embs.view(B * K, -1))
             # (one gradient for the base stands for the three only where autograd would bring them there: not
             # for leaves that are views of a plain tensor, nor for views taken under no_grad)
-            if packed is not None and not (packed.requires_grad == q_emb.requires_grad == d_pos_emb.requires_grad
-                                           == d_neg_embs.requires_grad):
+            if packed is not None and any(v.is_leaf == packed.requires_grad or v.requires_grad != packed.requires_grad
+                                          for v in (q_emb, d_pos_emb, d_neg_embs)):
                 packed = None
     return ops.preference_loss(q_emb, d_pos_emb, d_neg_embs, ref_margin=ref_margin, mask=mask, beta=beta,
                                temperature=temperature, label_smoothing=label_smoothing, loss_type=loss_type,

@@ -295,7 +295,8 @@ __global__ __launch_bounds__(kBlock) void lookup_super_sum_kernel(TokenPlan p, c
 
 // What the tiles left to do: the first `join_blocks` workgroups add up the rows that cross tiles (a group per
 // tile, for a row that leaves its first tile there; first, because the most frequent row is the longest
-// chain), the others write the rows without tokens (a group per row).
+// chain), the others write the rows without tokens.
+constexpr int kZeroRows = 32;
 template <typename TW, int VEC>
 __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, int64_t V, int E, float scale,
                                                                  TW* __restrict__ grad, int lg, unsigned join_blocks,
@@ -304,10 +305,17 @@ __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, in
                                                                  const float* __restrict__ sup) {
   const int c = threadIdx.x & ((1 << lg) - 1);
   if (blockIdx.x >= join_blocks) {
-    const int64_t r = ((int64_t)(blockIdx.x - join_blocks) * kBlock + threadIdx.x) >> lg;
-    if (r >= V || p.seg_start[r] != p.seg_start[r + 1]) return;
+    // a wave reads kZeroRows rows' bounds at once and stores the empty ones (a group of lanes per row at a
+    // time): the stores follow each other without a load between them
+    const int64_t r0 = ((int64_t)(blockIdx.x - join_blocks) * kWavesPerBlock + (threadIdx.x >> 6)) * kZeroRows;
+    const int lane = lane_id(), groups = kWave >> lg;
+    const int64_t mine = r0 + lane;
+    const bool none = lane < kZeroRows && mine < V && p.seg_start[mine] == p.seg_start[mine + 1];
+    const uint64_t empty = __ballot(none);
     const float zero[VEC] = {};
-    for (int e = c * VEC; e < E; e += VEC << lg) store_elems_nt<VEC>(grad + r * E + e, zero);
+    for (int i = lane >> lg; i < kZeroRows; i += groups)
+      if (empty >> i & 1)
+        for (int e = c * VEC; e < E; e += VEC << lg) store_elems_nt<VEC>(grad + (r0 + i) * E + e, zero);
     return;
   }
   const int64_t t0 = ((int64_t)blockIdx.x * kBlock + threadIdx.x) >> lg;
@@ -381,7 +389,8 @@ int launch_bwd(const void* dout, const void* ids, int ids_dtype, int64_t n, int6
   const int64_t tiles = (n + kTile - 1) / kTile, supers = tiles / kSuper, per = kBlock >> lg;
   float *head = ws, *tail = head + tiles * E, *sup = tail + tiles * E;
   auto grid = [&](int64_t groups) { return dim3((unsigned)((groups + per - 1) / per)); };
-  const dim3 block(kBlock), join(grid(V).x + grid(tiles).x);
+  const int64_t zero_rows = (int64_t)kWavesPerBlock * kZeroRows;
+  const dim3 block(kBlock), join((unsigned)(grid(tiles).x + (V + zero_rows - 1) / zero_rows));
 #define TT_LS(VV)                                                                                                  \
   case VV:                                                                                                         \
     lookup_tile_sum_kernel<TO, TW, VV><<<grid(tiles), block, 0, s>>>(p, d, E, scale, g, lg, head, tail);           \

@@ -5,9 +5,11 @@ Reference call sites each op replaces are cited per function (paths inside k0r1g
 """
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
 import functools
+import operator
 import os
 
 import torch
@@ -1589,6 +1591,10 @@ def in_batch_softmax_loss(q: torch.Tensor, d: torch.Tensor, temperature: float =
 
 # --------------------------------------------------------------------------------------------
 # global gradient norm and clipping (between twotower/train.py:138 and :139)
+_CLIP_TYPES = {(0, 0), (1, 1), (2, 2), (1, 0), (2, 0)}  # (gradient, out) type codes of tt_clip_grads
+_IS_SPARSE = operator.attrgetter("is_sparse")
+
+
 def _dense(t: torch.Tensor) -> bool:
     """t's elements fill one block of memory, in any order (a norm and a product need no more)."""
     return t.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(t)
@@ -1616,49 +1622,56 @@ def clip_grad_norm(grads, max_norm: float | None, norm_type: float = 2.0, out=No
         return torch.zeros((), dtype=_FLOAT)
     first = grads[0]
     dev, codes = first.device, _lib.ELEM_DTYPES
+    # (a long list's call is bound by this loop-free Python: about 0.7 us a tensor)
     types = [codes.get(g.dtype) for g in grads]
     otypes = types if outs is grads else [codes.get(o.dtype) for o in outs]
-    if None in types or any(o != g and o != 0 for g, o in zip(types, otypes)):
-        i = next(i for i, (g, o) in enumerate(zip(types, otypes)) if g is None or (o != g and o != 0))
+    if not _CLIP_TYPES.issuperset(zip(types, otypes)):
+        i = next(i for i, pair in enumerate(zip(types, otypes)) if pair not in _CLIP_TYPES)
         raise TypeError(f"gradient {i} of {grads[i].dtype} into {outs[i].dtype}: float32, bfloat16 or float16, into its own "
                         "type or float32")
-    if any(g.is_sparse for g in grads):
+    if any(map(_IS_SPARSE, grads)):
         raise RuntimeError("clip_grad_norm does not support sparse gradients")
     copies = []
+    src = dst = grads
     if outs is grads:
-        src = [g if g.is_contiguous() or _dense(g) else g.contiguous() for g in grads]
-        dst = src
-        if scale:
-            copies = [(g, t) for g, t in zip(grads, src) if t is not g]
-            for g, _ in copies:
-                if torch._debug_has_internal_overlap(g) == 1:
-                    raise ValueError(f"a gradient of shape {tuple(g.shape)} has elements that share memory (an expanded "
-                                     "tensor): clip a copy")
+        if not all(map(torch.Tensor.is_contiguous, grads)):
+            src = dst = [g if _dense(g) else g.contiguous() for g in grads]
+            if scale:
+                copies = [(g, t) for g, t in zip(grads, src) if t is not g]
+                for g, _ in copies:
+                    if torch._debug_has_internal_overlap(g) == 1:
+                        raise ValueError(f"a gradient of shape {tuple(g.shape)} has elements that share memory (an expanded "
+                                         "tensor): clip a copy")
     else:
-        if any(g.shape != o.shape for g, o in zip(grads, outs)):
+        if [g.shape for g in grads] != [o.shape for o in outs]:
             i = next(i for i, (g, o) in enumerate(zip(grads, outs)) if g.shape != o.shape)
             raise ValueError(f"out {i} has shape {tuple(outs[i].shape)}, the gradient {tuple(grads[i].shape)}")
-        src = [g if g.is_contiguous() else g.contiguous() for g in grads]
-        dst = [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in outs]
-        copies = [(o, t) for o, t in zip(outs, dst) if t is not o]
-    sizes = [g.numel() for g in grads]
-    src_at = [t.data_ptr() for t in src]
-    dst_at = src_at if dst is src else [t.data_ptr() for t in dst]
+        dst = outs
+        if not (all(map(torch.Tensor.is_contiguous, grads)) and all(map(torch.Tensor.is_contiguous, outs))):
+            src = [g.contiguous() for g in grads]
+            dst = [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in outs]
+            copies = [(o, t) for o, t in zip(outs, dst) if t is not o]
+    sizes = list(map(torch.Tensor.numel, grads))
+    src_at = list(map(torch.Tensor.data_ptr, src))
+    dst_at = src_at if dst is src else list(map(torch.Tensor.data_ptr, dst))
     if scale and len(set(dst_at)) != len(dst_at):
         written = [a for a, n in zip(dst_at, sizes) if n]
         if len(set(written)) != len(written):
             raise ValueError("a gradient is written twice: the same memory is listed more than once")
-    if first.get_device() < 0 or any(g.get_device() != first.get_device() for g in grads) or (
-            outs is not grads and any(o.get_device() != first.get_device() for o in outs)):
+    devices = set(map(torch.Tensor.get_device, grads))
+    if outs is not grads:
+        devices.update(map(torch.Tensor.get_device, outs))
+    if len(devices) > 1 or -1 in devices:
         _lib.same_device(first, *grads, *outs)  # (says which)
     n = len(grads)
     norm = first.new_empty((), dtype=_FLOAT)
     nbytes = _lib.lib().tt_clip_ws_size(n)
     ws = first.new_empty((nbytes,), dtype=torch.uint8)
+    lists = [array.array("q", v) for v in (src_at, dst_at, sizes)]
     with _lib.on_device(first):
-        call("tt_clip_grads", (ctypes.c_int64 * n)(*src_at), (ctypes.c_int64 * n)(*dst_at), (ctypes.c_int64 * n)(*sizes),
-             bytes(types), bytes(otypes), n, int(norm_type == float("inf")), float(max_norm) if scale else 0.0,
-             int(scale), ptr(norm), ptr(ws), nbytes, stream_of(first))
+        call("tt_clip_grads", *[v.buffer_info()[0] for v in lists], bytes(types), bytes(otypes), n,
+             int(norm_type == float("inf")), float(max_norm) if scale else 0.0, int(scale), ptr(norm), ptr(ws), nbytes,
+             stream_of(first))
     for o, t in copies:
         o.copy_(t)
     return norm

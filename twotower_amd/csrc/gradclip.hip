@@ -15,9 +15,9 @@ namespace tt {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kChunk = 16384;       // elements per chunk
+constexpr int kChunk = 8192;        // elements per chunk
 constexpr int kMaxParts = 2048;     // partial norms of all launches together
-constexpr int kNormBlocks = 1024;   // workgroups (= partials) of one norm launch
+constexpr int kNormBlocks = 2048;   // workgroups (= partials) of one norm launch
 constexpr int kScaleBlocks = 2048;
 
 struct ClipList {
@@ -165,7 +165,7 @@ __device__ __forceinline__ void scale_chunk(const TS* src, TD* dst, int n, Coef 
         if (i + u * kBlock < nv) {
 #pragma unroll
           for (int j = 0; j < VEC; ++j) x[u][j] = coef(x[u][j]);
-          store_elems<VEC>(dst + (size_t)(i + u * kBlock) * VEC, x[u]);
+          store_elems_nt<VEC>(dst + (size_t)(i + u * kBlock) * VEC, x[u]);
         }
     }
     for (int i = nv * VEC + threadIdx.x; i < n; i += kBlock) dst[i] = (TD)coef((float)src[i]);

@@ -227,6 +227,8 @@ def test_c_abi_refusals(name, args, msg):
 
 def test_c_abi_sizes():
     lib = _lib.lib()
+    for n, short in ((_lib.TT_LOOKUP_DIRECT_TOKENS, True), (_lib.TT_LOOKUP_DIRECT_TOKENS + 1, False)):
+        assert (lib.tt_lookup_plan_size(n, 50) == 0) is short and (lib.tt_lookup_bwd_ws_size(n, 8) == 0) is short
     assert lib.tt_lookup_bwd_ws_size(100, 8) == lib.tt_lookup_plan_size(100, 50) == 0  # short calls take none
     assert lib.tt_lookup_bwd_ws_size(100_000, 8) == (2 * 3125 + 97) * 8 * 4  # heads, tails, super-tiles
     assert lib.tt_lookup_plan_size(100_000, 50) > 4 * 4 * 100_000

@@ -19,7 +19,7 @@ HEADER_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__fil
 
 TT_IDS_I32, TT_IDS_I64 = 0, 1
 ELEM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum tt_elem_dtype
-TT_CLIP_MAX_TENSORS, TT_INT4_MAX_H = 128, 4096
+TT_LOOKUP_DIRECT_TOKENS, TT_INT4_MAX_H = 4096, 4096
 TT_INBATCH_TAIL_ROWS, TT_INBATCH_MAX_PARTS = 64, 512  # twotower_amd.h
 TT_F32, TT_BF16, TT_BF16_SPLIT = 0, 1, 2
 TT_SCATTER_SORTED, TT_SCATTER_ATOMIC = 0, 1
@@ -283,8 +283,6 @@ def _nullctx():
     return contextlib.nullcontext()
 
 
-_NULL = contextlib.nullcontext()  # (stateless: one serves every use)
-
 
 def join_side_grads(params) -> None:
     """Make the current stream wait for every side-stream gradient of ``params``."""
@@ -451,16 +449,23 @@ def require_gpu(*tensors: torch.Tensor) -> None:
 def same_device(*tensors: torch.Tensor) -> None:
     """Every tensor on the first one's GPU: a kernel gets raw pointers, so a mixed call would fault."""
     require_gpu(*tensors)
-    dev = tensors[0].device
+    dev = tensors[0].get_device()
     for t in tensors[1:]:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"twotower_amd: tensors on different devices ({dev} and {t.device})")
+        if t is not None and t.get_device() != dev:
+            raise RuntimeError(f"twotower_amd: tensors on different devices ({tensors[0].device} and {t.device})")
 
 
-def on_device(t: torch.Tensor):
-    """Makes t's GPU the current one around a launch (its stream belongs to it); nothing to do, and
-    nothing done, where it is."""
-    return _NULL if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+_GET_DEVICE = torch._C._cuda_getDevice
+
+
+def launch(t: torch.Tensor, name: str, *args) -> None:
+    """call(name, *args, stream) on t's GPU and its current stream, whichever GPU is current."""
+    i = t.get_device()
+    if i == _GET_DEVICE():
+        call(name, *args, _RAW_STREAM(i) if _RAW_STREAM is not None else stream_of(t))
+    else:
+        with torch.cuda.device(i):
+            call(name, *args, stream_of(t))
 
 
 def elem_dtype_code(t: torch.Tensor, name: str) -> int:

@@ -64,7 +64,7 @@ __global__ __launch_bounds__(kBlock) void lookup_fwd_kernel(const TW* __restrict
 // consecutive rows; it reads all ids, keeps its own tokens in LDS in token order, and a wave per
 // row adds that row's tokens.  A row with more than kCoop tokens is shared by the workgroup's waves,
 // each adding the tokens of its part of the list, folded in wave order.
-constexpr int kDirectN = 4096;
+constexpr int kDirectN = TT_LOOKUP_DIRECT_TOKENS;
 constexpr int kDirectThreads = 512;
 constexpr int kDirectWaves = kDirectThreads / kWave;
 constexpr int kDirectRows = 64;

@@ -15,7 +15,7 @@ import os
 import torch
 
 from . import _lib
-from ._lib import call, ptr, require_gpu, stream_of
+from ._lib import call, launch, ptr, require_gpu, stream_of
 
 _FLOAT = torch.float32
 
@@ -535,11 +535,10 @@ def bag_mean_pool(weight: torch.Tensor, ids: torch.Tensor, padding_idx: int | No
 def _lookup_fwd(weight, ids, scale, out_dtype):
     V, E = weight.shape
     out = weight.new_empty((*ids.shape, E), dtype=out_dtype)
-    if out.numel():
-        with _lib.on_device(weight):
-            call("tt_lookup_fwd", ptr(weight), _lib.ELEM_DTYPES[weight.dtype], V, E, weight.stride(0), ptr(ids),
-                 _lib.ids_dtype_code(ids), ids.numel(), scale, ptr(out), _lib.ELEM_DTYPES[out_dtype],
-                 stream_of(weight))
+    n = ids.numel()
+    if n:
+        launch(weight, "tt_lookup_fwd", weight.data_ptr(), _lib.ELEM_DTYPES[weight.dtype], V, E, weight.stride(0),
+               ids.data_ptr(), _lib.ids_dtype_code(ids), n, scale, out.data_ptr(), _lib.ELEM_DTYPES[out_dtype])
     return out
 
 
@@ -563,20 +562,19 @@ class EmbeddingLookup(torch.autograd.Function):
         dout = dout.contiguous()
         n = ids.numel()
         grad = dout.new_empty((V, E), dtype=dtype)
-        nbytes = _lib.lib().tt_lookup_bwd_ws_size(n, E)
-        size = _lib.lib().tt_lookup_plan_size(n, V)
-        with _lib.on_device(dout):
-            plan = ws = None
-            if size:
-                # Sorted here, not beside the forward on a side stream: the gather fills the memory system and every
-                # CU, and the sort beside it ended no sooner (forward and backward back to back 352 against 344
-                # us at 8192 x 64 tokens).  Buffers per call, not shared: two captured graphs, or streams, may run
-                # their backwards at once.
-                plan = dout.new_empty((size,), dtype=torch.uint8)
-                call("tt_lookup_plan", ptr(ids), _lib.ids_dtype_code(ids), n, V, pad, ptr(plan), size, stream_of(dout))
-                ws = dout.new_empty((nbytes,), dtype=torch.uint8)
-            call("tt_lookup_bwd", ptr(dout), _lib.ELEM_DTYPES[dout.dtype], ptr(ids), _lib.ids_dtype_code(ids), n, V, E,
-                 pad, scale, ptr(grad), _lib.ELEM_DTYPES[dtype], ptr(plan), size, ptr(ws), nbytes, stream_of(dout))
+        plan = ws = None
+        size = nbytes = 0
+        if n > _lib.TT_LOOKUP_DIRECT_TOKENS:
+            # Sorted here, not beside the forward on a side stream: the gather fills the memory system and every CU,
+            # and the sort beside it ended no sooner (forward and backward back to back 352 against 344 us at
+            # 8192 x 64 tokens).  Buffers per call, not shared: two captured graphs, or streams, may run their
+            # backwards at once.
+            size, nbytes = _lib.lib().tt_lookup_plan_size(n, V), _lib.lib().tt_lookup_bwd_ws_size(n, E)
+            plan, ws = (dout.new_empty((b,), dtype=torch.uint8) for b in (size, nbytes))
+            launch(dout, "tt_lookup_plan", ptr(ids), _lib.ids_dtype_code(ids), n, V, pad, ptr(plan), size)
+        launch(dout, "tt_lookup_bwd", dout.data_ptr(), _lib.ELEM_DTYPES[dout.dtype], ids.data_ptr(),
+               _lib.ids_dtype_code(ids), n, V, E, pad, scale, grad.data_ptr(), _lib.ELEM_DTYPES[dtype], ptr(plan), size,
+               ptr(ws), nbytes)
         return grad, None, None, None, None
 
 
@@ -590,33 +588,37 @@ def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0
     The gradient is dense: every row of the table, scale times the sum of its tokens' gradients in
     fp32 in a fixed order (bitwise reproducible), rounded once to the table's type; the row of
     ``padding_idx`` (negative: from the end, as in torch) gets zeros."""
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f"weight must be a non-empty (V, E) table, got shape {tuple(weight.shape)}")
+    shape, dtype = weight.shape, weight.dtype
+    if len(shape) != 2 or 0 in shape:
+        raise ValueError(f"weight must be a non-empty (V, E) table, got shape {tuple(shape)}")
     _lib.elem_dtype_code(weight, "weight")
     _lib.ids_dtype_code(ids)
-    V, E = weight.shape
-    if (weight.stride(1) != 1 and E > 1) or (weight.stride(0) < E and V > 1):
+    V, E = shape
+    s0, s1 = weight.stride()
+    if (s1 != 1 and E > 1) or (s0 < E and V > 1):
         raise ValueError(f"weight rows must be contiguous and must not overlap, got strides {weight.stride()}")
-    out_dtype = weight.dtype if out_dtype is None else out_dtype
-    if out_dtype != weight.dtype and not (weight.dtype == _FLOAT and out_dtype in _lib.ELEM_DTYPES):
-        raise TypeError(f"out_dtype {out_dtype} from a {weight.dtype} table is not supported")
+    if out_dtype is None:
+        out_dtype = dtype
+    elif out_dtype != dtype and not (dtype == _FLOAT and out_dtype in _lib.ELEM_DTYPES):
+        raise TypeError(f"out_dtype {out_dtype} from a {dtype} table is not supported")
     if ids.numel() >= 2 ** 31:
         raise ValueError(f"at most 2^31 - 1 ids per call, got {ids.numel()}")
-    scale = float(scale)
     pad = -1
     if padding_idx is not None:
         if not -V <= padding_idx < V:
             raise ValueError(f"padding_idx {padding_idx} outside a table of {V} rows")
         pad = padding_idx % V
     _lib.same_device(weight, ids)
+    want_grad = weight.requires_grad and torch.is_grad_enabled()
     col = getattr(weight, "_tt_column", None)
-    if col is not None and (col.stale or (torch.is_grad_enabled() and weight.requires_grad)):
+    if col is not None and (col.stale or want_grad):
         raise RuntimeError("embedding_lookup reads the whole table: this one is column-sharded; materialize() it and "
                            "call under no_grad, or use bag_mean_pool")
-    ids = ids.contiguous()
-    if weight.requires_grad and torch.is_grad_enabled():
-        return EmbeddingLookup.apply(weight, ids, scale, pad, out_dtype)
-    return _lookup_fwd(weight, ids, scale, out_dtype)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    if want_grad:
+        return EmbeddingLookup.apply(weight, ids, float(scale), pad, out_dtype)
+    return _lookup_fwd(weight, ids, float(scale), out_dtype)
 
 
 # --------------------------------------------------------------------------------------------
@@ -1170,24 +1172,24 @@ class MultiNegLossPacked(torch.autograd.Function):
 PREFERENCE_KINDS = {"sigmoid": 0, "squared": 1}
 
 
-def _pref_rows(t: torch.Tensor, name: str) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
 def _pref_args(q, p, n):
     """(q, p, n with a pair axis, element type) of a checked call."""
-    if q.dim() != 2 or p.shape != q.shape:
-        raise ValueError(f"q and p must both be (B, H), got {tuple(q.shape)} and {tuple(p.shape)}")
-    if n.dim() == 2:
+    sq, sn = q.shape, n.shape
+    if len(sq) != 2 or p.shape != sq:
+        raise ValueError(f"q and p must both be (B, H), got {tuple(sq)} and {tuple(p.shape)}")
+    if len(sn) == 2:
         n = n.unsqueeze(1)
-    if n.dim() != 3 or n.shape[0] != q.shape[0] or n.shape[2] != q.shape[1] or n.shape[1] < 1:
-        raise ValueError(f"n must be (B, H) or (B, K, H) with K >= 1 beside q {tuple(q.shape)}, got {tuple(n.shape)}")
-    if q.shape[1] < 1:
+        sn = n.shape
+    if len(sn) != 3 or sn[0] != sq[0] or sn[2] != sq[1] or sn[1] < 1:
+        raise ValueError(f"n must be (B, H) or (B, K, H) with K >= 1 beside q {tuple(sq)}, got {tuple(sn)}")
+    if sq[1] < 1:
         raise ValueError("H must be at least 1")
     dt = _lib.elem_dtype_code(q, "q")
     if p.dtype != q.dtype or n.dtype != q.dtype:
         raise TypeError(f"q, p and n must have one type, got {q.dtype}, {p.dtype}, {n.dtype}")
-    return _pref_rows(q, "q"), _pref_rows(p, "p"), _pref_rows(n, "n"), dt
+    if sq[1] > 1:  # (rows of contiguous elements, whatever their strides)
+        q, p, n = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, p, n))
+    return q, p, n, dt
 
 
 def _pref_pairs(t, name, dtype, B, K, device):
@@ -1214,20 +1216,20 @@ def _pref_fwd(q, p, n, dt, ref, mask, opts, margins=None, loss=None):
         side = q.new_empty((B * K + 1 + 2 * B,), dtype=_FLOAT)
         base = side.data_ptr()
         at = (base, base + 4 * B * K, base + 4 * (B * K + 1))
-    with _lib.on_device(q):
-        call("tt_preference_fwd", ptr(q), q.stride(0), ptr(p), p.stride(0), ptr(n), n.stride(0), n.stride(1), dt, B, K,
-             H, ptr(ref), ptr(mask), kind, beta, inv_tau, smooth, at[0], ptr(margins), ptr(loss), at[1], at[2], 8 * B,
-             stream_of(q))
+    sn = n.stride()
+    launch(q, "tt_preference_fwd", q.data_ptr(), q.stride(0), p.data_ptr(), p.stride(0), n.data_ptr(), sn[0], sn[1], dt, B,
+           K, H, ptr(ref), ptr(mask), kind, beta, inv_tau, smooth, at[0], ptr(margins), ptr(loss), at[1], at[2], 8 * B)
     return side
 
 
 def _pref_bwd(q, p, n, dt, mask, opts, side, g, dq, dp, dn):
     B, K, H = n.shape
-    g = g.to(_FLOAT).contiguous()
+    if g.dtype != _FLOAT:
+        g = g.to(_FLOAT)
     base = side.data_ptr()
-    with _lib.on_device(q):
-        call("tt_preference_bwd", ptr(q), q.stride(0), ptr(p), p.stride(0), ptr(n), n.stride(0), n.stride(1), dt, B, K,
-             H, ptr(mask), opts[2], base, base + 4 * B * K, ptr(g), ptr(dq), ptr(dp), ptr(dn), stream_of(q))
+    sn = n.stride()
+    launch(q, "tt_preference_bwd", q.data_ptr(), q.stride(0), p.data_ptr(), p.stride(0), n.data_ptr(), sn[0], sn[1], dt, B,
+           K, H, ptr(mask), opts[2], base, base + 4 * B * K, g.data_ptr(), dq.data_ptr(), dp.data_ptr(), dn.data_ptr())
 
 
 class PreferenceLoss(torch.autograd.Function):
@@ -1668,10 +1670,8 @@ def clip_grad_norm(grads, max_norm: float | None, norm_type: float = 2.0, out=No
     nbytes = _lib.lib().tt_clip_ws_size(n)
     ws = first.new_empty((nbytes,), dtype=torch.uint8)
     lists = [array.array("q", v) for v in (src_at, dst_at, sizes)]
-    with _lib.on_device(first):
-        call("tt_clip_grads", *[v.buffer_info()[0] for v in lists], bytes(types), bytes(otypes), n,
-             int(norm_type == float("inf")), float(max_norm) if scale else 0.0, int(scale), ptr(norm), ptr(ws), nbytes,
-             stream_of(first))
+    launch(first, "tt_clip_grads", *[v.buffer_info()[0] for v in lists], bytes(types), bytes(otypes), n,
+           int(norm_type == float("inf")), float(max_norm) if scale else 0.0, int(scale), ptr(norm), ptr(ws), nbytes)
     for o, t in copies:
         o.copy_(t)
     return norm
@@ -1872,9 +1872,7 @@ class Int4Rows:
         if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
             x = x.contiguous()
         r = cls._empty(x.shape[0], x.shape[1], group, x.device)
-        with _lib.on_device(x):
-            call("tt_int4_quantize", ptr(x), dt, r.n, r.H, max(x.stride(0), r.H), r.group, ptr(r.codes), ptr(r.scales),
-                 stream_of(x))
+        launch(x, "tt_int4_quantize", ptr(x), dt, r.n, r.H, max(x.stride(0), r.H), r.group, ptr(r.codes), ptr(r.scales))
         return r
 
     @classmethod
@@ -1888,16 +1886,13 @@ class Int4Rows:
         _lib.same_device(codes, scales)
         codes, scales = codes.contiguous(), scales.contiguous()
         r = cls._empty(n, H, group, codes.device)
-        with _lib.on_device(codes):
-            call("tt_int4_pack", ptr(codes), ptr(scales), n, H, r.group, ptr(r.codes), ptr(r.scales), stream_of(codes))
+        launch(codes, "tt_int4_pack", ptr(codes), ptr(scales), n, H, r.group, ptr(r.codes), ptr(r.scales))
         return r
 
     def dequantize(self) -> torch.Tensor:
         """The (n, H) float32 values the codes stand for."""
         out = torch.empty(self.n, self.H, dtype=_FLOAT, device=self.codes.device)
-        with _lib.on_device(self.codes):
-            call("tt_int4_unpack", ptr(self.codes), ptr(self.scales), self.n, self.H, self.group, ptr(out),
-                 stream_of(self.codes))
+        launch(self.codes, "tt_int4_unpack", ptr(self.codes), ptr(self.scales), self.n, self.H, self.group, ptr(out))
         return out
 
     def to(self, device) -> "Int4Rows":
@@ -1934,8 +1929,7 @@ def int4_scores(q: torch.Tensor, rows: Int4Rows) -> torch.Tensor:
     _lib.same_device(q, rows.codes)
     if q.stride(1) != 1 or q.stride(0) < rows.H:
         q = q.contiguous()
-    out = torch.empty(q.shape[0], rows.n, dtype=_FLOAT, device=q.device)
-    with _lib.on_device(q):
-        call("tt_int4_scores", ptr(q), dt, q.shape[0], max(q.stride(0), rows.H), ptr(rows.codes), ptr(rows.scales),
-             rows.n, rows.H, rows.group, ptr(out), stream_of(q))
+    out = q.new_empty((q.shape[0], rows.n), dtype=_FLOAT)
+    launch(q, "tt_int4_scores", q.data_ptr(), dt, q.shape[0], max(q.stride(0), rows.H), rows.codes.data_ptr(),
+           rows.scales.data_ptr(), rows.n, rows.H, rows.group, out.data_ptr())
     return out

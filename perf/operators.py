@@ -207,8 +207,9 @@ def _preference(s):
     if own:
         from twotower_amd import losses
 
+        smooth = c["smooth"] if c["kind"] == "sigmoid" else 0.0  # (the squared loss has none, and refuses it)
         loss = losses.preference_loss(s["q"], s["p"], s["n"], ref_margin=s["ref"], mask=s["mask"], beta=c["beta"],
-                                      temperature=c["temperature"], label_smoothing=c["smooth"], loss_type=c["kind"])
+                                      temperature=c["temperature"], label_smoothing=smooth, loss_type=c["kind"])
         return [loss, *torch.autograd.grad(loss, (s["q"], s["p"], s["n"]))]
     q, p, n = (s[k].detach().float() for k in ("q", "p", "n"))
     h = ((q * p).sum(-1, keepdim=True) - (q.unsqueeze(1) * n).sum(-1)) / c["temperature"]

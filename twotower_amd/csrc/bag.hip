@@ -1243,7 +1243,7 @@ struct BwdWs {
 // sum over long rows of ceil(len / piece_len) <= sum (len / kPieceT + 1) < 2 n / kPieceT
 int64_t max_pieces_for(int64_t n) { return 2 * ((n + kPieceT - 1) / kPieceT) + 1; }
 
-BwdWs carve(void* base, int64_t nseq, int L, int64_t V, int E, size_t sort_bytes, bool with_gs = true) {
+BwdWs carve(void* base, int64_t nseq, int L, int64_t V, int E, size_t sort_bytes, bool sort_only = false) {
   BwdWs w{};
   const size_t n = (size_t)nseq * L;
   size_t off = 0;
@@ -1254,12 +1254,13 @@ BwdWs carve(void* base, int64_t nseq, int L, int64_t V, int E, size_t sort_bytes
   };
   char* b = static_cast<char*>(base);
   const size_t o_ki = take(n * 4), o_ko = take(n * 4), o_vi = take(n * 4), o_vo = take(n * 4);
-  const size_t o_gs = take(with_gs ? (size_t)nseq * E * 4 : 0);
-  const size_t o_ss = take((size_t)(V + 1) * 4);
+  const size_t own = sort_only ? 0 : 1;  // (a token lookup's plan: nothing but the sort)
+  const size_t o_gs = take(own * nseq * E * 4);
+  const size_t o_ss = take(own * (V + 1) * 4);
   const size_t o_tmp = take(sort_bytes);
   const int64_t mp = max_pieces_for((int64_t)n);
-  const size_t o_nch = take((size_t)(V + 1) * 4), o_po = take((size_t)(V + 1) * 4);
-  const size_t o_pb = take((size_t)mp * 4), o_pe = take((size_t)mp * 4), o_pp = take((size_t)mp * E * 4);
+  const size_t o_nch = take(own * (V + 1) * 4), o_po = take(own * (V + 1) * 4);
+  const size_t o_pb = take(own * mp * 4), o_pe = take(own * mp * 4), o_pp = take(own * mp * E * 4);
   w.max_pieces = mp;
   if (b) {
     w.nch = reinterpret_cast<int32_t*>(b + o_nch);
@@ -1404,7 +1405,7 @@ int launch_piece_sum(const BwdWs& w, int64_t V, int E, hipStream_t s) {
 // pieces of long rows (bag_plan_starts_kernel, bag_plan_pieces_kernel).
 template <typename IdT>
 int plan_front(const IdT* ids, int64_t nseq, int L, int64_t ld, int64_t V, int64_t padding_idx, const BwdWs& w,
-               hipStream_t s, int part = -1, int64_t first = 1, bool pieces = true) {
+               hipStream_t s, int part = -1, int64_t first = 1, bool rows = true) {
   // part -1: the whole plan; 0: every sort pass but the last; 1: the last pass, the segment starts
   // and the pieces (tt_bag_plan_part: the two halves on one stream compute what one call does)
   const int64_t n = nseq * L;
@@ -1460,12 +1461,11 @@ int plan_front(const IdT* ids, int64_t nseq, int L, int64_t ld, int64_t V, int64
     src.keys = ko;
     src.vals = vo;
   }
-  if (part == 0) return TT_OK;
+  if (part == 0 || !rows) return TT_OK;
   const int64_t nst = (n + 1 + kStartsPT - 1) / kStartsPT;
   bag_plan_starts_kernel<<<dim3((unsigned)((nst + kBlock - 1) / kBlock)), block, 0, s>>>(w.keys_out, nvalid, V,
                                                                                        w.seg_start, w.piece_off + V);
   TT_LAUNCH_CHECK("bag_plan_starts");
-  if (!pieces) return TT_OK;
   bag_plan_pieces_kernel<<<dim3((unsigned)((V + 1 + kBlock - 1) / kBlock)), block, 0, s>>>(
       w.seg_start, V, w.nch, w.piece_off, w.piece_beg, w.piece_end);
   TT_LAUNCH_CHECK("bag_plan_pieces");
@@ -1516,10 +1516,10 @@ int check_common(int64_t V, int E, const void* ids, int ids_dtype, int64_t nseq,
 }  // namespace
 
 // The same sort for token lookups (lookup.hip): every id in [0, V) is a token, a sequence is one token,
-// so the sorted values are token indices; no scaled rows and no pieces to keep.
+// so the sorted values are token indices; the sort alone is kept (no scaled rows, row starts, pieces).
 static BwdWs token_plan_carve(void* ws, int64_t n, int64_t V) {
   void* base = ws ? reinterpret_cast<void*>(align_up(reinterpret_cast<size_t>(ws), 256)) : nullptr;
-  return carve(base, n, 1, V, 0, sort_tmp_bytes(n, V), false);
+  return carve(base, n, 1, V, 0, sort_tmp_bytes(n, V), true);
 }
 
 size_t token_plan_bytes(int64_t n, int64_t V) { return token_plan_carve(nullptr, n, V).total + 256; }
@@ -1528,7 +1528,7 @@ TokenPlan token_plan_view(void* plan, int64_t n, int64_t V) {
   const BwdWs w = token_plan_carve(plan, n, V);
   const SortShape sh = sort_shape(n, V);
   const int32_t* total = static_cast<const int32_t*>(w.sort_tmp) + ((size_t)1 << sh.D) * sh.ntiles;
-  return TokenPlan{w.seg_start, w.keys_out, w.vals_out, total + ((size_t)1 << sh.D)};
+  return TokenPlan{w.keys_out, w.vals_out, total + ((size_t)1 << sh.D)};
 }
 
 int token_plan_build(const void* ids, int ids_dtype, int64_t n, int64_t V, int64_t padding_idx, void* plan,

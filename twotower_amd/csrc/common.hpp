@@ -181,10 +181,9 @@ inline int vec_for(const int64_t* n, int nn, const void* const* p, const int* by
 }
 
 // The sort plan of a token lookup's gradient (built in bag.hip by the bags' counting sort, read by
-// lookup.hip): the kept tokens' rows `keys` in ascending order, their token indices `vals` (a row's in token
-// order), row r's at [seg_start[r], seg_start[r + 1]); *count tokens were kept.
+// lookup.hip): the kept tokens' rows `keys` in ascending order and their token indices `vals` (a row's in
+// token order); *count tokens were kept.
 struct TokenPlan {
-  const int32_t* seg_start;
   const uint32_t* keys;
   const int32_t* vals;
   const int32_t* count;

@@ -63,7 +63,10 @@ __global__ __launch_bounds__(kBlock) void lookup_fwd_kernel(const TW* __restrict
 // ---- gradient of a short call (n <= kDirectN): one launch, no workspace.  A workgroup owns R
 // consecutive rows; it reads all ids, keeps its own tokens in LDS in token order, and a wave per
 // row adds that row's tokens.  A row with more than kCoop tokens is shared by the workgroup's waves,
-// each adding the tokens of its part of the list, folded in wave order.
+// each adding the tokens of its part of the list, folded in wave order.  Its time grows with n V (every
+// workgroup reads all ids), the sorted form's hardly at all, and about kDirectN they meet (us, n = 1000 / 4000 /
+// 8000): 34 x 64 9 / 19 / 32 against 25 / 29 / 32; 2000 x 256 10 / 17 / 26 against 40 / 45 / 45; 50k x 128 21 / 40 /
+// 80 against 41 / 47 / 49; 200k x 256 47 / 80 / 150 against 71 / 79 / 80 (30 us of it the bytes of the gradient).
 constexpr int kDirectN = TT_LOOKUP_DIRECT_TOKENS;
 constexpr int kDirectThreads = 512;
 constexpr int kDirectWaves = kDirectThreads / kWave;
@@ -86,7 +89,7 @@ __device__ __forceinline__ void direct_add(const TO* __restrict__ dout, int E, i
         tok[u] = m ? (int64_t)(__builtin_amdgcn_readlane((int)v, __builtin_ctzll(m)) >> 8) : -1;
         m &= m - 1;  // (0 stays 0)
       }
-      float x[U][VEC];
+      float x[U][VEC];  // (filled before the first is used: loaded and added under one condition they ran one by one)
 #pragma unroll
       for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -293,9 +296,22 @@ __global__ __launch_bounds__(kBlock) void lookup_super_sum_kernel(TokenPlan p, c
   }
 }
 
+// the first position in [lo, hi) of the ascending keys with keys[i] >= r, hi if there is none
+__device__ __forceinline__ int first_at_least(const uint32_t* __restrict__ keys, int lo, int hi, uint32_t r) {
+  while (lo < hi) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if (keys[mid] < r) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
 // What the tiles left to do: the first `join_blocks` workgroups add up the rows that cross tiles (a group per
 // tile, for a row that leaves its first tile there; first, because the most frequent row is the longest
-// chain), the others write the rows without tokens.
+// chain), the others write the rows without tokens: a wave finds where kZeroRows rows would lie in the
+// sorted order and stores those that do not (a group of lanes per row at a time), the stores following
+// each other without a load between them.  (A table of the rows' starts, written from the keys, took one
+// thread through every gap between two of them: 135 us for 8192 tokens in 200k rows.)
 constexpr int kZeroRows = 32;
 template <typename TW, int VEC>
 __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, int64_t V, int E, float scale,
@@ -304,14 +320,14 @@ __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, in
                                                                  const float* __restrict__ tail,
                                                                  const float* __restrict__ sup) {
   const int c = threadIdx.x & ((1 << lg) - 1);
+  const int n = *p.count;
   if (blockIdx.x >= join_blocks) {
-    // a wave reads kZeroRows rows' bounds at once and stores the empty ones (a group of lanes per row at a
-    // time): the stores follow each other without a load between them
     const int64_t r0 = ((int64_t)(blockIdx.x - join_blocks) * kWavesPerBlock + (threadIdx.x >> 6)) * kZeroRows;
     const int lane = lane_id(), groups = kWave >> lg;
-    const int64_t mine = r0 + lane;
-    const bool none = lane < kZeroRows && mine < V && p.seg_start[mine] == p.seg_start[mine + 1];
-    const uint64_t empty = __ballot(none);
+    const int64_t r = r0 + (lane < kZeroRows ? lane : kZeroRows);
+    const int at = first_at_least(p.keys, 0, n, (uint32_t)(r < V ? r : V));
+    const int next = __shfl(at, lane < kZeroRows ? lane + 1 : kZeroRows);
+    const uint64_t empty = __ballot(lane < kZeroRows && r < V && next == at);
     const float zero[VEC] = {};
     for (int i = lane >> lg; i < kZeroRows; i += groups)
       if (empty >> i & 1)
@@ -319,10 +335,12 @@ __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, in
     return;
   }
   const int64_t t0 = ((int64_t)blockIdx.x * kBlock + threadIdx.x) >> lg;
-  if ((t0 + 1) * kTile >= *p.count) return;  // no tile after it
-  const uint32_t r = p.keys[(t0 + 1) * kTile];
-  const int beg = p.seg_start[r], end = p.seg_start[r + 1];
-  if (beg / kTile != t0 || beg == (t0 + 1) * kTile) return;  // no row crosses here, or it began before this tile
+  const int64_t next_tile = (t0 + 1) * kTile;
+  if (next_tile >= n) return;  // no tile after it
+  const uint32_t r = p.keys[next_tile];
+  if (p.keys[next_tile - 1] != r) return;                                  // no row crosses here,
+  if (t0 > 0 && p.keys[t0 * kTile - 1] == r) return;                       // or it began before this tile
+  const int end = first_at_least(p.keys, (int)next_tile, n, r + 1);
   const int64_t t1 = (end - 1) / kTile;
   // its heads t0 + 1 .. t1.  Super-tile j is the row's if the row began before it and holds its last token.
   const int64_t s0 = (t0 + kSuper) / kSuper, s1 = max((int64_t)end / (kSuper * kTile), s0);
@@ -374,7 +392,10 @@ int launch_bwd(const void* dout, const void* ids, int ids_dtype, int64_t n, int6
   const TO* d = static_cast<const TO*>(dout);
   TW* g = static_cast<TW*>(grad);
   if (n <= kDirectN) {
-    int64_t R = V / 1024;
+    // few rows each spread the frequent (low) ids over workgroups and give a wave one or two rows; at most
+    // kDirectRows, so that the ids are read V / 64 times at most (30k x 100, 1073 text-like tokens: 15 us, V / 1024
+    // rows each 30 us; 200k x 256, 4096 tokens: 38 and 39 us)
+    int64_t R = V / 4096;
     R = R < 1 ? 1 : R > kDirectRows ? kDirectRows : R;
     const dim3 grid((unsigned)((V + R - 1) / R)), block(kDirectThreads);
 #define TT_LD(VV) \

@@ -670,6 +670,20 @@ def test_int4_scores_against_plain(n, H, group, nq, dtype):
     assert torch.equal(ops.int4_scores(q, rows), got)
 
 
+@pytest.mark.parametrize("n, H, group, nq", [(70_001, 1024, 128, 9), (70_001, 1024, 32, 20), (33_000, 256, 64, 32),
+                                            (66_000, 256, 32, 64), (40_000, 36, 32, 3)])
+def test_int4_scores_of_a_long_index(n, H, group, nq):
+    """Enough rows for the larger workgroups, whose waves share the query operands."""
+    g = gen(47)
+    codes = torch.randint(-8, 8, (n, H), generator=g, device=DEV, dtype=torch.int8)
+    scales = (torch.rand(n, -(-H // group), generator=g, device=DEV) + 0.1).to(BF16)
+    rows = ops.Int4Rows.from_codes(codes, scales, group)
+    values = codes.double() * scales.double().repeat_interleave(group, 1)[:, :H]
+    assert torch.equal(rows.dequantize().double(), values)
+    q = torch.randn(nq, H, generator=g, device=DEV)
+    check_scores(ops.int4_scores(q, rows), q, values, scales, -(-H // 32))
+
+
 def test_int4_scores_strides_and_shapes():
     g = gen(42)
     x = torch.randn(100, 64, generator=g, device=DEV)

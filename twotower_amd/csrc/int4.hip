@@ -36,11 +36,10 @@ inline int64_t tiles_of(int64_t n) { return (n + kRows - 1) / kRows; }
 
 __device__ __forceinline__ float bf16_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
 
-// where row `row`'s dwords of column block b are: dword h at [h * 16 * dpl], dpl = dwords per lane of its quad
-__device__ __forceinline__ int64_t code_word(int64_t row, int b, int nblk, int& dpl) {
-  const int quad = b >> 2, d = b & 3;
-  dpl = nblk - 4 * quad < 4 ? nblk - 4 * quad : 4;
-  return (row / kRows) * nblk * 64 + quad * 256 + (row % kRows) * dpl + d;
+// where the codes of row `row`, column block b, columns 8 h .. 8 h + 7 of it are
+__device__ __forceinline__ int64_t code_word(int64_t row, int b, int h, int nblk) {
+  const int quad = b >> 2, dpl = nblk - 4 * quad < 4 ? nblk - 4 * quad : 4;  // dwords per lane of the quad
+  return (row / kRows) * nblk * 64 + quad * 256 + (h * kRows + row % kRows) * dpl + (b & 3);
 }
 __device__ __forceinline__ int64_t scale_at(int64_t row, int b, int nquad, int group) {
   const int spq = kQuad / group, quad = b >> 2;
@@ -53,13 +52,6 @@ __device__ __forceinline__ uint32_t pack8(const int* c) {
 #pragma unroll
   for (int s = 0; s < 4; ++s) u |= (uint32_t)c[2 * s] << (4 * s) | (uint32_t)c[2 * s + 1] << (4 * s + 16);
   return u;
-}
-
-__device__ __forceinline__ void write_codes(uint32_t* codes, int64_t row, int b, int nblk, const int* c) {
-  int dpl;
-  const int64_t at = code_word(row, b, nblk, dpl);
-#pragma unroll
-  for (int h = 0; h < 4; ++h) codes[at + (int64_t)h * kRows * dpl] = pack8(c + 8 * h);
 }
 
 // max / 7 rounded to bf16, to nearest even of the exact quotient: the fp32 quotient is on the right side
@@ -88,39 +80,65 @@ __device__ __forceinline__ int group_code(float x, float s) {
   return (int)fminf(fmaxf(r, -7.f), 7.f);
 }
 
-// One thread per (row, column block); the lanes of a group join their maxima.
+// elements k0 .. k0 + 7 of a row of H, zeros past H (wide: 4 at a time are aligned and H % 4 == 0)
+template <typename T>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int k0, int H, bool wide, float (&x)[8]) {
+#pragma unroll
+  for (int g = 0; g < 8; g += 4) {
+    float y[4] = {0.f, 0.f, 0.f, 0.f};
+    if (wide) {
+      if (k0 + g < H) load_elems<4>(row + k0 + g, y);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (k0 + g + e < H) y[e] = (float)row[k0 + g + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[g + e] = y[e];
+  }
+}
+
+// The layout kernels take a thread per (row, 8 columns), the threads of a row's columns side by side: the
+// rows are read and written in consecutive runs, and the threads of a group join their maxima.
+struct Place {
+  int64_t row;
+  int b, h;
+};
+__device__ __forceinline__ Place place_of(int64_t id, int nquad) {
+  const int64_t row = id / (16 * nquad);
+  const int w = (int)(id - row * (16 * nquad));
+  return Place{row, w >> 2, w & 3};
+}
+
 template <typename T>
 __global__ __launch_bounds__(kBlock) void int4_quantize_kernel(const T* __restrict__ x, int64_t n, int H, int64_t ld,
-                                                               int group, int nblk, int nquad,
+                                                               int group, int nblk, int nquad, bool wide,
                                                                uint32_t* __restrict__ codes,
                                                                uint16_t* __restrict__ scales) {
-  const int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  const int64_t row = id / (4 * nquad);
-  const int b = (int)(id - row * (4 * nquad));
-  if (row >= (n + kRows - 1) / kRows * kRows) return;  // (whole groups of lanes leave together)
-  float v[kBlk];
+  const Place p = place_of((int64_t)blockIdx.x * kBlock + threadIdx.x, nquad);
+  if (p.row >= (n + kRows - 1) / kRows * kRows) return;  // (whole groups of lanes leave together)
+  float v[8] = {};
+  if (p.row < n) load8(x + p.row * ld, p.b * kBlk + 8 * p.h, H, wide, v);
   float mx = 0.f;
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < kBlk; ++i) {
-    const int k = b * kBlk + i;
-    v[i] = row < n && k < H ? (float)x[row * ld + k] : 0.f;
+  for (int i = 0; i < 8; ++i) {
     bad = bad || !(fabsf(v[i]) <= 3.402823466e38f);
     mx = fmaxf(mx, fabsf(v[i]));
   }
-  for (int o = 1; o < group / kBlk; o <<= 1) {
+  for (int o = 1; o < group / 8; o <<= 1) {
     mx = fmaxf(mx, __shfl_xor(mx, o));
     bad = __shfl_xor((int)bad, o) || bad;
   }
   uint16_t sb = group_scale(mx);
   if (bad) sb = 0x7fc0u;
-  if ((b & (group / kBlk - 1)) == 0) scales[scale_at(row, b, nquad, group)] = sb;
-  if (b >= nblk) return;
+  if (p.h == 0 && (p.b & (group / kBlk - 1)) == 0) scales[scale_at(p.row, p.b, nquad, group)] = sb;
+  if (p.b >= nblk) return;
   const float s = bf16_value(sb);
-  int c[kBlk];
+  int c[8];
 #pragma unroll
-  for (int i = 0; i < kBlk; ++i) c[i] = 8 + ((bad || s == 0.f) ? 0 : group_code(v[i], s));
-  write_codes(codes, row, b, nblk, c);
+  for (int i = 0; i < 8; ++i) c[i] = 8 + ((bad || s == 0.f) ? 0 : group_code(v[i], s));
+  codes[code_word(p.row, p.b, p.h, nblk)] = pack8(c);
 }
 
 __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restrict__ src,
@@ -128,42 +146,44 @@ __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restr
                                                            int group, int nblk, int nquad,
                                                            uint32_t* __restrict__ codes,
                                                            uint16_t* __restrict__ scales) {
-  const int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  const int64_t row = id / (4 * nquad);
-  const int b = (int)(id - row * (4 * nquad));
-  if (row >= (n + kRows - 1) / kRows * kRows) return;
-  const int ng = (H + group - 1) / group, g = b * kBlk / group;
-  if ((b & (group / kBlk - 1)) == 0)
-    scales[scale_at(row, b, nquad, group)] = row < n && g < ng ? sc[row * ng + g] : (uint16_t)0;
-  if (b >= nblk) return;
-  int c[kBlk];
+  const Place p = place_of((int64_t)blockIdx.x * kBlock + threadIdx.x, nquad);
+  if (p.row >= (n + kRows - 1) / kRows * kRows) return;
+  const int ng = (H + group - 1) / group, g = p.b * kBlk / group;
+  if (p.h == 0 && (p.b & (group / kBlk - 1)) == 0)
+    scales[scale_at(p.row, p.b, nquad, group)] = p.row < n && g < ng ? sc[p.row * ng + g] : (uint16_t)0;
+  if (p.b >= nblk) return;
+  int c[8];
 #pragma unroll
-  for (int i = 0; i < kBlk; ++i) {
-    const int k = b * kBlk + i;
-    const int v = row < n && k < H ? (int)src[row * H + k] : 0;
+  for (int i = 0; i < 8; ++i) {
+    const int k = p.b * kBlk + 8 * p.h + i;
+    const int v = p.row < n && k < H ? (int)src[p.row * H + k] : 0;
     c[i] = 8 + (v < -8 ? -8 : v > 7 ? 7 : v);
   }
-  write_codes(codes, row, b, nblk, c);
+  codes[code_word(p.row, p.b, p.h, nblk)] = pack8(c);
 }
 
 __global__ __launch_bounds__(kBlock) void int4_unpack_kernel(const uint32_t* __restrict__ codes,
                                                              const uint16_t* __restrict__ scales, int64_t n, int H,
                                                              int group, int nblk, int nquad, float* __restrict__ out) {
-  const int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  const int64_t row = id / nblk;
-  const int b = (int)(id - row * nblk);
-  if (row >= n) return;
-  const float s = bf16_value(scales[scale_at(row, b, nquad, group)]);
-  int dpl;
-  const int64_t at = code_word(row, b, nblk, dpl);
-  for (int h = 0; h < 4; ++h) {
-    const uint32_t u = codes[at + (int64_t)h * kRows * dpl];
+  const Place p = place_of((int64_t)blockIdx.x * kBlock + threadIdx.x, nquad);
+  const int k0 = p.b * kBlk + 8 * p.h;
+  if (p.row >= n || k0 >= H) return;
+  const float s = bf16_value(scales[scale_at(p.row, p.b, nquad, group)]);
+  const uint32_t u = codes[code_word(p.row, p.b, p.h, nblk)];
+  float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int k = b * kBlk + 8 * h + i;
-      const int c = (int)(u >> (4 * (i >> 1) + 16 * (i & 1))) & 15;
-      if (k < H) out[row * H + k] = (float)(c - 8) * s;
+  for (int i = 0; i < 8; ++i) v[i] = (float)((int)(u >> (4 * (i >> 1) + 16 * (i & 1)) & 15) - 8) * s;
+  float* o = out + p.row * H + k0;
+  if (H % 4 == 0) {  // (H is then a multiple of every access: k0 + 4 <= H)
+#pragma unroll
+    for (int g = 0; g < 8; g += 4) {
+      const float y[4] = {v[g], v[g + 1], v[g + 2], v[g + 3]};
+      if (k0 + g < H) store_elems<4>(o + g, y);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k0 + i < H) o[i] = v[i];
   }
 }
 
@@ -194,26 +214,6 @@ __device__ __forceinline__ f16x8 widen(uint32_t u) {
 // 2^3 <= max |q| 2^e < 2^4: the fp16 terms then reach 2^-27 of the largest element or 33 bits below the element
 __device__ __forceinline__ int query_exponent(float mx) {
   return mx > 0.f && mx <= 3.402823466e38f ? 3 - ilogbf(mx) : 0;
-}
-
-// elements k0 .. k0 + 7 of query i, zeros past the queries and past H
-template <typename T>
-__device__ __forceinline__ void load_query(const T* __restrict__ q, int i, int nq, int64_t ldq, int H, int k0,
-                                           bool wide, float (&x)[8]) {
-  const T* p = q + i * ldq + k0;
-#pragma unroll
-  for (int g = 0; g < 8; g += 4) {
-    float y[4] = {0.f, 0.f, 0.f, 0.f};
-    if (i < nq && wide) {
-      if (k0 + g < H) load_elems<4>(p + g, y);
-    } else if (i < nq) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (k0 + g + e < H) y[e] = (float)p[g + e];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[g + e] = y[e];
-  }
 }
 
 // What a wave loads for one quad of its tiles.
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(BLOCK) void int4_scores_kernel(const T* __restrict_
   float x[8];
   for (int it = threadIdx.x; it < items; it += BLOCK) {
     const int i = (it >> 2) % Q::kQ, k0 = ((it >> 2) / Q::kQ) * kBlk + 8 * (it & 3);
-    load_query(q, i, nq, ldq, H, k0, wide, x);
+    load8(q + i * ldq, k0, i < nq ? H : 0, wide, x);
     uint32_t mx = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(fabsf(x[e])));
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(BLOCK) void int4_scores_kernel(const T* __restrict_
   __syncthreads();
   for (int it = threadIdx.x; it < items; it += BLOCK) {
     const int hh = it & 3, i = (it >> 2) % Q::kQ, b = (it >> 2) / Q::kQ;
-    if (items > BLOCK) load_query(q, i, nq, ldq, H, b * kBlk + 8 * hh, wide, x);
+    if (items > BLOCK) load8(q + i * ldq, b * kBlk + 8 * hh, i < nq ? H : 0, wide, x);
     f16x8 t0v, t1v, t2v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -389,12 +389,17 @@ int launch_scores_block(const T* q, int nq, int64_t ldq, const uint32_t* codes, 
   return TT_OK;
 }
 
-// Small workgroups spread a short index over the CUs; with more tiles than that, larger ones share one set
-// of query operands in LDS between more waves.
+// Sixteen waves a CU share the query operands in LDS: as many workgroups of 256 as it holds, or fewer, larger
+// ones where the operands are large (100k x 1024, 16 queries, 96 KB: 256 threads 47 us, 1024 threads 26 us).
+// An index too short to give each of those waves its tiles keeps to 256.
 template <typename T, int NQT, int SPQ>
 int launch_scores(const T* q, int nq, int64_t ldq, const uint32_t* codes, const uint16_t* scales, int64_t n, int H,
                   float* scores, int64_t ld_scores, hipStream_t s) {
-  if (NQT > 1 && tiles_of(n) > 256 * 4 * kTPW)
+  const size_t lds = (size_t)4 * quads_of(H) * QueryTiles<NQT>::kOps * kWave * 16;
+  const int64_t tiles = tiles_of(n);
+  if (lds > 78 * 1024 && tiles > 256 * 8 * kTPW)
+    return launch_scores_block<T, NQT, SPQ, 1024>(q, nq, ldq, codes, scales, n, H, scores, ld_scores, s);
+  if (lds > 39 * 1024 && tiles > 256 * 4 * kTPW)
     return launch_scores_block<T, NQT, SPQ, 512>(q, nq, ldq, codes, scales, n, H, scores, ld_scores, s);
   return launch_scores_block<T, NQT, SPQ, 256>(q, nq, ldq, codes, scales, n, H, scores, ld_scores, s);
 }
@@ -448,9 +453,9 @@ int check_int4(int64_t n, int H, int group, const void* codes, const void* scale
   return TT_OK;
 }
 
-// threads of the layout kernels: one per (row of a whole tile, column block of a whole quad)
+// workgroups of the layout kernels: a thread per (row of a whole tile, 8 columns of a whole quad)
 inline int64_t layout_blocks(int64_t n, int H) {
-  return (tiles_of(n) * kRows * 4 * quads_of(H) + kBlock - 1) / kBlock;
+  return (tiles_of(n) * kRows * 16 * quads_of(H) + kBlock - 1) / kBlock;
 }
 
 }  // namespace
@@ -474,9 +479,10 @@ extern "C" int tt_int4_quantize(const void* x, int dtype, int64_t n, int H, int6
   TT_REQUIRE(layout_blocks(n, H) < (int64_t(1) << 31), "int4: too many values");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)layout_blocks(n, H)), block(kBlock);
+  const bool wide = H % 4 == 0 && ld % 4 == 0 && reinterpret_cast<size_t>(x) % (4 * elem_bytes(dtype)) == 0;
 #define TT_QZ(T)                                                                                              \
   int4_quantize_kernel<T><<<grid, block, 0, s>>>(static_cast<const T*>(x), n, H, ld, group, blocks_of(H),     \
-                                                 quads_of(H), static_cast<uint32_t*>(codes),                  \
+                                                 quads_of(H), wide, static_cast<uint32_t*>(codes),                  \
                                                  static_cast<uint16_t*>(scales))
   if (dtype == TT_E_F32) TT_QZ(float);
   else if (dtype == TT_E_BF16) TT_QZ(__bf16);
@@ -503,8 +509,9 @@ extern "C" int tt_int4_unpack(const void* codes, const void* scales, int64_t n, 
                               tt_stream_t stream) {
   if (int rc = check_int4(n, H, group, codes, scales)) return rc;
   TT_REQUIRE(n == 0 || out, "null pointer");
+  TT_REQUIRE(reinterpret_cast<size_t>(out) % 16 == 0, "int4: out must be 16-byte aligned");
   if (n == 0) return TT_OK;
-  const int64_t blocks = (n * blocks_of(H) + kBlock - 1) / kBlock;
+  const int64_t blocks = layout_blocks(n, H);
   TT_REQUIRE(blocks < (int64_t(1) << 31), "int4: too many values");
   int4_unpack_kernel<<<dim3((unsigned)blocks), dim3(kBlock), 0, reinterpret_cast<hipStream_t>(stream)>>>(
       static_cast<const uint32_t*>(codes), static_cast<const uint16_t*>(scales), n, H, group, blocks_of(H),

@@ -155,6 +155,44 @@ def test_lookup_non_finite_rows_stay_in_their_places(n):
     assert grad.isfinite().all() and not grad[0].any()
 
 
+def test_lookup_odd_tables_and_ids():
+    w = torch.arange(4.0, device=DEV)
+    one = w.as_strided((1, 4), (1, 1)).detach().requires_grad_(True)  # one row: its stride says nothing
+    col = torch.arange(12.0, device=DEV).view(6, 2)[:, :1].detach().requires_grad_(True)  # rows of one element
+    for t in (one, col):
+        out = ops.embedding_lookup(t, torch.tensor(0, device=DEV), scale=2.0)  # a scalar id
+        assert torch.equal(out, 2.0 * t[0])
+        (g,) = torch.autograd.grad(out.sum(), t)
+        assert (g[0] == 2.0).all() and not g[1:].any()
+    plain = torch.randn(9, 4, device=DEV, requires_grad=True)
+    out = ops.embedding_lookup(plain * 3.0, torch.tensor([[1, 1]], device=DEV, dtype=torch.int32))  # not a leaf
+    (g,) = torch.autograd.grad(out.sum(), plain)
+    assert (g[1] == 6.0).all() and g.abs().sum() == 24.0
+    (g,) = torch.autograd.grad((ops.embedding_lookup(plain, torch.tensor([1], device=DEV)) ** 2).sum(), plain,
+                               create_graph=True)
+    with pytest.raises(RuntimeError):  # no second derivative, said rather than dropped
+        torch.autograd.grad(g.sum(), plain)
+
+
+def test_lookup_of_a_fused_table():
+    """The fused update takes pooled lookups: a step that also differentiates a plain one is refused, a step with
+    plain ones alone takes the dense gradient as any parameter does."""
+    emb = tt.embeddings.build("lookup", vocab_size=30, embedding_dim=64).to(DEV)
+    opt = optim.AdamW(emb.parameters(), fused_tables=True, tables=[emb])
+    ids = torch.randint(1, 30, (3, 5), generator=gen(11), device=DEV)
+    before = emb.weight.detach().clone()
+    emb(ids).sum().backward()
+    opt.step()
+    assert not torch.equal(emb.weight, before)
+    opt.zero_grad(set_to_none=True)
+    (emb(ids).sum() + emb.pool_mean(ids).sum()).backward()
+    with pytest.raises(RuntimeError, match="pooled lookups only"):
+        opt.step()
+    opt.zero_grad(set_to_none=True)
+    emb.pool_mean(ids).sum().backward()
+    opt.step()
+
+
 def test_lookup_backward_through_a_loss_matches_differences():
     w, ids, _ = lookup_case(9, 6, (4, 5), F32, torch.int64, None, 0, 0.0, 5)
     ids[0, :2] = 3  # the same id twice
@@ -835,6 +873,20 @@ def test_captured_fine_tuning_equals_eager():
         assert (a - b).norm() <= 1e-3 * b.norm()
 
 
+def test_captured_clipping_keeps_each_graphs_norm():
+    model = token_model(58).to(DEV)
+    opt = optim.AdamW(model.parameters(), lr=0.0, weight_decay=0.0, capturable=True)  # the parameters stay
+    step = tt.TrainStep(model, losses.build("preference", beta=0.5), opt, graph=True, eager_steps=1, max_grad_norm=0.1)
+    eager = tt.TrainStep(model, losses.build("preference", beta=0.5), opt, max_grad_norm=0.1)
+    small, large = triplets(8, 20, 61).to(DEV), triplets(24, 20, 62).to(DEV)
+    step(*small)
+    for b in (small, large, small, large, small):
+        step(*b)
+        got = step.grad_norm.item()
+        eager(*b)
+        assert abs(got - eager.grad_norm.item()) <= 1e-4 * got
+
+
 def test_clipping_beside_the_hand_written_tower_head():
     """The mean-pool tower's head may form its weight gradients on a side stream: the norm needs them all."""
     def build():
@@ -880,4 +932,6 @@ def test_search_with_a_4_bit_index(group, tmp_path):
     r = tt.search.TwoTowerSearch(model)
     r.load_index(str(tmp_path / "index.pt"))
     again, idx2 = r.search_ids(queries, top_k=5)
+    r.index_document_ids(docs[:50])  # its own kind of index replaces the loaded one
+    assert r.index is None and r.search_ids(queries, top_k=60)[0].shape == (9, 50)
     assert torch.equal(again, scores) and torch.equal(idx2, idx)

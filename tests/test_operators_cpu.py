@@ -101,6 +101,14 @@ def test_clip_refuses_the_same_memory_twice():
         ops.clip_grad_norm([t, t.view(2, 4)], 1.0)
 
 
+def test_clip_refuses_an_out_that_is_another_gradient():
+    a, b = torch.ones(8), torch.ones(8)
+    with pytest.raises(ValueError, match="memory of another gradient"):
+        ops.clip_grad_norm([a, b], 1.0, out=[b, a])
+    with pytest.raises(RuntimeError, match="no CPU fallback"):  # its own gradient's memory is fine
+        ops.clip_grad_norm([a, b], 1.0, out=[a, torch.ones(8)])
+
+
 def test_clip_of_nothing_and_of_a_fused_table():
     assert ops.clip_grad_norm([], 1.0).item() == 0.0
     assert optim.clip_grad_norm_([torch.nn.Parameter(torch.ones(2))], 1.0).item() == 0.0
@@ -164,6 +172,68 @@ def test_lookup_embedding_on_the_cpu_is_the_plain_gather():
     ids = torch.tensor([[1, 0, 8]])
     assert torch.equal(emb(ids), emb.embedding(ids) * 2.0)
     assert list(emb.state_dict()) == ["embedding.weight"]
+
+
+def _dp_clip_worker(rank, port, q):
+    import os
+
+    import torch.distributed as dist
+
+    from twotower_amd import train_step
+
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    try:
+        train_step.clip_grad_norm_ = torch.nn.utils.clip_grad_norm_  # (the kernels need a GPU; the order is what is tested)
+        model, step, batch = _dp_clip_step()
+        step(*(t[rank * 4:(rank + 1) * 4] for t in batch))
+        q.put((rank, [p.detach().numpy() for p in model.parameters()], float(step.grad_norm)))
+    finally:
+        dist.destroy_process_group()
+
+
+class _Linear(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.lin = torch.nn.Linear(6, 5)
+
+    def forward(self, q, p):
+        return self.lin(q), p
+
+
+def _dp_clip_step():
+    torch.manual_seed(3)
+    model = _Linear().double()
+    opt = torch.optim.SGD(model.parameters(), lr=1.0)
+    batch = torch.randn(8, 6, dtype=torch.float64), torch.randn(8, 5, dtype=torch.float64)
+    return model, tt.TrainStep(model, lambda a, b: ((a - b) ** 2).mean(), opt, max_grad_norm=0.1), batch
+
+
+def test_data_parallel_clipping_uses_the_global_gradient():
+    """Two ranks, half the batch each: the all-reduced gradient is clipped (by one norm on both ranks), so the
+    step equals the single-process step on the whole batch."""
+    import socket
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = torch.multiprocessing.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_dp_clip_worker, args=(r, port, q)) for r in range(2)]
+    [p.start() for p in procs]
+    got = dict((r, (ps, n)) for r, ps, n in (q.get(timeout=120) for _ in range(2)))
+    [p.join(60) for p in procs]
+    model, step, (x, y) = _dp_clip_step()
+    loss = ((model.lin(x) - y) ** 2).mean()
+    loss.backward()
+    norm = torch.nn.utils.clip_grad_norm_(model.parameters(), 0.1).item()
+    assert norm > 0.1
+    with torch.no_grad():
+        want = [p - p.grad for p in model.parameters()]
+    for ps, n in got.values():
+        assert abs(n - norm) < 1e-12
+        for a, b in zip(ps, want):
+            assert abs(torch.from_numpy(a) - b).max() < 1e-12
 
 
 # ---------------------------------------------------------------------------------------------

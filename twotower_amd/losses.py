@@ -79,7 +79,7 @@ def preference_loss(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg_embs: to
     q_emb, d_pos_emb (B, H); d_neg_embs (B, H) or (B, K, H); one of float32 / bfloat16 / float16, computed in
     fp32, gradients rounded once.  ref_margin: (B, K) floats ((B,) for K = 1), a constant.  mask: (B, K)
     bool, False for a missing pair, whose row is not read (it may hold anything), counts nothing and gets
-    a zero gradient; with no pair left the loss is 0."""
+    a zero gradient; with no pair left the loss is 0.  Data parallel: each rank's mean is over its own pairs."""
     packed = None
     if d_neg_embs.dim() in (2, 3) and q_emb.dim() == 2 and d_neg_embs.is_contiguous():
         B, K = q_emb.shape[0], 1 if d_neg_embs.dim() == 2 else d_neg_embs.shape[1]

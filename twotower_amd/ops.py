@@ -13,6 +13,7 @@ import operator
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, launch, ptr, require_gpu, stream_of
@@ -537,8 +538,8 @@ def _lookup_fwd(weight, ids, scale, out_dtype):
     out = weight.new_empty((*ids.shape, E), dtype=out_dtype)
     n = ids.numel()
     if n:
-        launch(weight, "tt_lookup_fwd", weight.data_ptr(), _lib.ELEM_DTYPES[weight.dtype], V, E, weight.stride(0),
-               ids.data_ptr(), _lib.ids_dtype_code(ids), n, scale, out.data_ptr(), _lib.ELEM_DTYPES[out_dtype])
+        launch(weight, "tt_lookup_fwd", weight.data_ptr(), _lib.ELEM_DTYPES[weight.dtype], V, E,
+               weight.stride(0) if V > 1 else E, ids.data_ptr(), _lib.ids_dtype_code(ids), n, scale, out.data_ptr(), _lib.ELEM_DTYPES[out_dtype])
     return out
 
 
@@ -553,9 +554,12 @@ class EmbeddingLookup(torch.autograd.Function):
         return _lookup_fwd(weight, ids, scale, out_dtype)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
         (V, E), dtype, scale, pad = ctx.meta
+        if getattr(ctx.weight_ref, "_tt_column", None) is not None:
+            raise RuntimeError("a column-sharded table takes its gradient from bag_mean_pool only")
         deferred = getattr(ctx.weight_ref, "_tt_deferred", None)
         if deferred is not None:
             deferred.added_dense()
@@ -611,9 +615,9 @@ def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0
     _lib.same_device(weight, ids)
     want_grad = weight.requires_grad and torch.is_grad_enabled()
     col = getattr(weight, "_tt_column", None)
-    if col is not None and (col.stale or want_grad):
-        raise RuntimeError("embedding_lookup reads the whole table: this one is column-sharded; materialize() it and "
-                           "call under no_grad, or use bag_mean_pool")
+    if col is not None and col.stale:
+        raise RuntimeError("embedding_lookup reads the whole table: this one is column-sharded and was updated since it was "
+                           "last gathered; materialize() it first, or use bag_mean_pool")
     if not ids.is_contiguous():
         ids = ids.contiguous()
     if want_grad:
@@ -1242,6 +1246,7 @@ class PreferenceLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         q, p, n, mask, side = ctx.saved_tensors
         # (empty_like: torch.empty with a device argument takes four times as long on autograd's thread)
@@ -1263,6 +1268,7 @@ class PreferenceLossPacked(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         qpn, mask, side = ctx.saved_tensors
         B, K, dt, opts = ctx.meta
@@ -1607,7 +1613,8 @@ def clip_grad_norm(grads, max_norm: float | None, norm_type: float = 2.0, out=No
     min(1, max_norm / (norm + 1e-6)), in place or into ``out`` (one tensor per gradient, of its type or
     float32, so half-precision accumulators can be clipped into the fp32 gradients an optimizer steps
     with).  max_norm None: the norm alone.  float32 / bfloat16 / float16 tensors, mixed at will; the norm is
-    formed in 64 bits in a fixed order, each product is rounded once; no host synchronisation.
+    formed in 64 bits in a fixed order, each product is rounded once; no host synchronisation.  Tensors must
+    not overlap (the same memory listed twice is refused), but out[i] may be grads[i].
     A non-finite norm spreads as in torch.nn.utils.clip_grad_norm_ (inf: zeros and NaN, NaN: NaN)."""
     grads = list(grads)
     if norm_type not in (2, 2.0, float("inf")):
@@ -1660,6 +1667,10 @@ def clip_grad_norm(grads, max_norm: float | None, norm_type: float = 2.0, out=No
         written = [a for a, n in zip(dst_at, sizes) if n]
         if len(set(written)) != len(written):
             raise ValueError("a gradient is written twice: the same memory is listed more than once")
+    if dst is not src and not set(src_at).isdisjoint(dst_at):
+        written = {d for s, d, n in zip(src_at, dst_at, sizes) if n and s != d}
+        if not written.isdisjoint(a for a, n in zip(src_at, sizes) if n):
+            raise ValueError("an out tensor is the memory of another gradient")
     devices = set(map(torch.Tensor.get_device, grads))
     if outs is not grads:
         devices.update(map(torch.Tensor.get_device, outs))

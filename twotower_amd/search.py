@@ -63,6 +63,7 @@ class TwoTowerSearch:
         self.index_document_ids(self._ids(documents), documents)
 
     def index_document_ids(self, ids: torch.Tensor, documents: list | None = None) -> None:
+        self.index = self.document_embeddings = None
         if self.index_dtype == "int4":
             if ids.shape[0] == 0:
                 raise ValueError("no documents to index")

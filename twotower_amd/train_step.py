@@ -166,7 +166,7 @@ class TrainStep:
                 self.graph = False
                 return self.eager(*inputs)
             self._graphs[key] = hit
-        graph, static_all, static_loss = hit
+        graph, static_all, static_loss, self.grad_norm = hit
         if all(t.shape[1:] == inputs[0].shape[1:] and t.dtype == inputs[0].dtype for t in inputs):
             if all(t.device == static_all.device and t.is_contiguous() for t in inputs) and len(inputs) <= 8:
                 ops.pack_blocks(inputs, static_all)  # one launch into the packed static buffer
@@ -221,7 +221,7 @@ class TrainStep:
         # as before.
         with torch.cuda.graph(graph, capture_error_mode="thread_local"):
             static_loss = self.eager(*static_in)
-        return graph, static_all, static_loss
+        return graph, static_all, static_loss, self.grad_norm  # (each graph writes its own norm)
 
 
 # messages of errors raised because a call is refused inside stream capture (HIP's and CUDA's

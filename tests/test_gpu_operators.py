@@ -168,10 +168,10 @@ def test_lookup_odd_tables_and_ids():
     out = ops.embedding_lookup(plain * 3.0, torch.tensor([[1, 1]], device=DEV, dtype=torch.int32))  # not a leaf
     (g,) = torch.autograd.grad(out.sum(), plain)
     assert (g[1] == 6.0).all() and g.abs().sum() == 24.0
-    (g,) = torch.autograd.grad((ops.embedding_lookup(plain, torch.tensor([1], device=DEV)) ** 2).sum(), plain,
-                               create_graph=True)
-    with pytest.raises(RuntimeError):  # no second derivative, said rather than dropped
-        torch.autograd.grad(g.sum(), plain)
+    for f in (lambda: ops.embedding_lookup(plain, torch.tensor([1], device=DEV)).square().sum(),
+              lambda: losses.preference_loss(plain, plain.flip(0), plain.roll(1, 0))):
+        with pytest.raises(RuntimeError, match="no second derivative"):  # said, not dropped
+            torch.autograd.grad(f(), plain, create_graph=True)
 
 
 def test_lookup_of_a_fused_table():

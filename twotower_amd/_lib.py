@@ -462,7 +462,13 @@ def launch(t: torch.Tensor, name: str, *args) -> None:
     """call(name, *args, stream) on t's GPU and its current stream, whichever GPU is current."""
     i = t.get_device()
     if i == _GET_DEVICE():
-        call(name, *args, _RAW_STREAM(i) if _RAW_STREAM is not None else stream_of(t))
+        stream = _RAW_STREAM(i) if _RAW_STREAM is not None else stream_of(t)
+        if _CALLS or TIMER.enabled or TIMER.stamping:
+            call(name, *args, stream)
+        else:
+            rc = getattr(lib(), name)(*args, stream)
+            if rc:
+                check(rc, name)
     else:
         with torch.cuda.device(i):
             call(name, *args, stream_of(t))

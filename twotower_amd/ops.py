@@ -13,7 +13,6 @@ import operator
 import os
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, launch, ptr, require_gpu, stream_of
@@ -533,6 +532,13 @@ def bag_mean_pool(weight: torch.Tensor, ids: torch.Tensor, padding_idx: int | No
 
 # --------------------------------------------------------------------------------------------
 # Token lookup with a scale   (twotower/embeddings.py:40, the (B, L, E) rows a tower may pool itself)
+def _no_second_derivative(what: str) -> None:
+    """In a backward: refuses create_graph=True (grad mode is on then), which would drop the second
+    derivative without a word.  (torch's once_differentiable says it later, and costs 5 us a call.)"""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no second derivative: backward with create_graph=True is not supported")
+
+
 def _lookup_fwd(weight, ids, scale, out_dtype):
     V, E = weight.shape
     out = weight.new_empty((*ids.shape, E), dtype=out_dtype)
@@ -554,8 +560,8 @@ class EmbeddingLookup(torch.autograd.Function):
         return _lookup_fwd(weight, ids, scale, out_dtype)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
+        _no_second_derivative("embedding_lookup")
         (ids,) = ctx.saved_tensors
         (V, E), dtype, scale, pad = ctx.meta
         if getattr(ctx.weight_ref, "_tt_column", None) is not None:
@@ -1191,8 +1197,8 @@ def _pref_args(q, p, n):
     dt = _lib.elem_dtype_code(q, "q")
     if p.dtype != q.dtype or n.dtype != q.dtype:
         raise TypeError(f"q, p and n must have one type, got {q.dtype}, {p.dtype}, {n.dtype}")
-    if sq[1] > 1:  # (rows of contiguous elements, whatever their strides)
-        q, p, n = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, p, n))
+    if sq[1] > 1 and not q.stride(1) == p.stride(1) == n.stride(2) == 1:
+        q, p, n = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, p, n))  # rows of contiguous elements
     return q, p, n, dt
 
 
@@ -1246,8 +1252,8 @@ class PreferenceLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _no_second_derivative("preference_loss")
         q, p, n, mask, side = ctx.saved_tensors
         # (empty_like: torch.empty with a device argument takes four times as long on autograd's thread)
         dq, dp, dn = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, p, n))
@@ -1268,8 +1274,8 @@ class PreferenceLossPacked(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _no_second_derivative("preference_loss")
         qpn, mask, side = ctx.saved_tensors
         B, K, dt, opts = ctx.meta
         grad = torch.empty_like(qpn)

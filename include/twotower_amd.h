@@ -6,7 +6,7 @@
  * PyTorch) reaches through ATen on its hot path.  The reference has no FFI of its own;
  * the Python host package `twotower_amd` binds these symbols with ctypes behind the
  * reference's plugin surface (BaseEmbedding / BaseTower / LOSS_REGISTRY).  Each
- * declaration cites the reference call site it replaces.
+ * declaration cites the reference call site it replaces or stands beside.
  *
  * Conventions
  *   - All pointers are DEVICE pointers owned by the caller (PyTorch's caching allocator).

@@ -8,7 +8,11 @@
 // launch takes up to TT_CLIP_MAX_TENSORS of them by value, so nothing is staged through memory and
 // a captured call keeps its own list.  Squares are added in 64 bits: the norm neither overflows
 // nor underflows before its own rounding to 32 bits, and the vector units have room for it beside
-// the loads.  All sums run in a fixed order (no atomics).
+// the loads (added in 32 bits the pass took 54 instead of 57 us).  All sums run in a fixed order (no atomics).
+//
+// 51.3M fp32 elements into another buffer: norm 38 us (205 MB, 5.4 TB/s), scaling 67 us (410 MB, 6.1 TB/s, its
+// reads partly cached; a 4 GiB copy runs at 4.8 TB/s).  16,384-element chunks on 1024 workgroups took 57 and
+// 70 us, and results kept in the caches 50 (the next norm's reads then wait for their write-back) and 72.
 #include "common.hpp"
 
 namespace tt {

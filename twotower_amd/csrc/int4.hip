@@ -9,6 +9,12 @@
 // (33 bits of it), so v_mfma_f32_16x16x32_f16 forms the sum of 32 exact products in fp32; the group's
 // scale multiplies that sum.  32 columns are the instruction's K and the smallest group.
 //
+// 1M x 256, group 32 (us for 1 / 16 / 64 queries): 33-39 / 49 / 121, for 148 MB of index and 4 MB of scores a
+// query (fp32 cosine scores of the same rows: 186 / 235 / 446); group 128: 31-33.  One query is bound by the index's
+// reads, 4.0-4.4 TB/s (1, 2 or 4 tiles a wave, half as many waves, loads past the caches: 36-40 us all).  Short
+// indexes are bound by the launch and the queries' layout: 200k x 128, 8 queries 10.4 us, 28,834 x 100, 33
+// queries 9.2.
+//
 // Layout (written once per index): tiles of 16 rows; a tile is a run of quads of 128 columns, a quad
 // of 64 lanes x 16 bytes in the order the kernel loads it: lane (row j = l % 16, h = l / 16), dword d
 // holds row j's columns 128 quad + 32 d + 8 h .. + 7.  A wave's load is 1 KB of consecutive bytes and

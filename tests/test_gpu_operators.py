@@ -96,6 +96,7 @@ LOOKUPS = [
     (129, 1030, (300,), BF16, torch.int32, None, 1, 0.3),
     (70_000, 8, (20_000,), BF16, torch.int64, None, 0, 0.1),
     (2048, 512, (9000,), F16, torch.int64, None, 0, 0.5),
+    (700, 256, (70_001,), F32, torch.int32, None, 0, 0.1),       # workgroups dealt to the XCDs in runs
 ]
 
 

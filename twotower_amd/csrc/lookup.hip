@@ -5,7 +5,7 @@
 //
 // Both move bytes and add: the forward reads each token's row (repeated rows from L2) and writes
 // n E elements, the backward reads n E elements once and writes V E.  8192 x 64 text-like tokens, half of them
-// padding, 200k x 256 fp32: forward 161 us (537 MB written, 128 MB read from memory; 86 us without the reads, 44
+// padding, 200k x 256 fp32: forward 152 us (537 MB written, 128 MB read from memory; 86 us without the reads, 44
 // without the writes, and 152-161 for 1 to 16 tokens in flight, stores past the caches or not), sort 40 us, tiles
 // 70 us (344 MB, 4.9 TB/s), joins and empty rows 42 us (148 MB); a 4 GiB copy runs at 4.8 TB/s.  The backward needs each
 // row's tokens together: a long call sorts them (the bags' stable counting sort, token_plan_build), a short one
@@ -29,13 +29,19 @@ inline int row_lanes_log2(int E, int vec) {
   return l;
 }
 
-// ---- forward: a group of 2^lg lanes per token, U tokens in flight per group.
+// ---- forward: a group of 2^lg lanes per token, U tokens in flight per group.  A long call deals its
+// workgroups to the XCDs (workgroup b runs on XCD b mod 8) in runs of kXcdRun consecutive ones, 1 MB of output
+// at 16 KB a workgroup: 152 us instead of 162 at 8192 x 64 rows of 1 KB (runs of 8: 155, an eighth of the
+// output to each: 157).
+constexpr int kXcdRun = 64;
 template <typename TW, typename TO, int VEC, int U>
 __global__ __launch_bounds__(kBlock) void lookup_fwd_kernel(const TW* __restrict__ table, int64_t V, int E, int64_t ld,
                                                             const void* __restrict__ ids, bool wide, int64_t n,
-                                                            float scale, TO* __restrict__ out, int lg) {
+                                                            float scale, TO* __restrict__ out, int lg, bool runs) {
   const int lane = lane_id(), groups = kWave >> lg, sub = lane >> lg, c = lane & ((1 << lg) - 1);
-  const int64_t wave = (int64_t)blockIdx.x * kWavesPerBlock + (threadIdx.x >> 6);
+  const unsigned in = blockIdx.x % (8 * kXcdRun);  // (runs: the grid is whole spans of 8 kXcdRun workgroups)
+  const unsigned block = runs ? blockIdx.x - in + (in & 7) * kXcdRun + (in >> 3) : blockIdx.x;
+  const int64_t wave = (int64_t)block * kWavesPerBlock + (threadIdx.x >> 6);
   const int64_t t0 = wave * groups * U + sub;
   int64_t id[U];
 #pragma unroll
@@ -373,11 +379,14 @@ int launch_fwd(const void* table, int64_t V, int E, int64_t ld, const void* ids,
   const int lg = row_lanes_log2(E, vec);
   constexpr int U = 4;
   const int64_t per_block = (int64_t)kWavesPerBlock * (kWave >> lg) * U;
-  const dim3 grid((unsigned)((n + per_block - 1) / per_block)), block(kBlock);
+  int64_t blocks = (n + per_block - 1) / per_block;
+  const bool runs = blocks >= 8 * 8 * kXcdRun;
+  if (runs) blocks = (blocks + 8 * kXcdRun - 1) / (8 * kXcdRun) * (8 * kXcdRun);
+  const dim3 grid((unsigned)blocks), block(kBlock);
   const TW* t = static_cast<const TW*>(table);
   TO* o = static_cast<TO*>(out);
 #define TT_LF(VV) \
-  case VV: lookup_fwd_kernel<TW, TO, VV, U><<<grid, block, 0, s>>>(t, V, E, ld, ids, wide, n, scale, o, lg); break;
+  case VV: lookup_fwd_kernel<TW, TO, VV, U><<<grid, block, 0, s>>>(t, V, E, ld, ids, wide, n, scale, o, lg, runs); break;
   switch (vec) { TT_LF(8) TT_LF(4) TT_LF(2) default: TT_LF(1) }
 #undef TT_LF
   TT_LAUNCH_CHECK("lookup_fwd");

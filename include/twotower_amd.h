@@ -203,6 +203,7 @@ int tt_bag_col_reduce_ex(const int32_t* seg_all, const int32_t* vals_all, int64_
  *   padding_idx, on the same stream or one that it waits for (it may run beside the forward).  The plan is
  *   only read by tt_lookup_bwd. */
 #define TT_LOOKUP_DIRECT_TOKENS 4096
+#define TT_LOOKUP_MAX 0x7fff0000LL /* tokens and rows stay below it */
 int tt_lookup_fwd(const void* table, int table_dtype, int64_t V, int E, int64_t ld_table, const void* ids,
                   int ids_dtype, int64_t n, float scale, void* out, int out_dtype, tt_stream_t stream);
 size_t tt_lookup_plan_size(int64_t n, int64_t V);
@@ -275,7 +276,8 @@ int tt_adamw_multi_ex(const tt_adamw_tensor* tensors, const tt_adamw_grad_parts*
  * rounded once to *norm; scale != 0: dst = src * min(1, max_norm / (norm + 1e-6)), formed in fp32 and
  * rounded once.  dst may be src (then an unclipped call writes nothing) or another tensor of src's type
  * or fp32; tensors must not overlap otherwise.  The five arrays (host memory) describe `count` tensors:
- * pointers, elements, tt_elem_dtype codes.  Any count: TT_CLIP_MAX_TENSORS per launch, passed by value.  ws: tt_clip_ws_size(count) bytes, 8-byte aligned. */
+ * pointers, elements, tt_elem_dtype codes.  Any count: TT_CLIP_MAX_TENSORS per launch, passed by value.
+ * ws: tt_clip_ws_size(count) bytes, 8-byte aligned. */
 #define TT_CLIP_MAX_TENSORS 128
 size_t tt_clip_ws_size(int count);
 int tt_clip_grads(const void* const* src, void* const* dst, const int64_t* n, const uint8_t* src_dtype,

@@ -169,10 +169,26 @@ def test_lookup_odd_tables_and_ids():
     out = ops.embedding_lookup(plain * 3.0, torch.tensor([[1, 1]], device=DEV, dtype=torch.int32))  # not a leaf
     (g,) = torch.autograd.grad(out.sum(), plain)
     assert (g[1] == 6.0).all() and g.abs().sum() == 24.0
-    for f in (lambda: ops.embedding_lookup(plain, torch.tensor([1], device=DEV)).square().sum(),
-              lambda: losses.preference_loss(plain, plain.flip(0), plain.roll(1, 0))):
-        with pytest.raises(RuntimeError, match="no second derivative"):  # said, not dropped
-            torch.autograd.grad(f(), plain, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):  # said, not dropped
+        torch.autograd.grad(losses.preference_loss(plain, plain.flip(0), plain.roll(1, 0)), plain, create_graph=True)
+
+
+@pytest.mark.parametrize("n", [30, 6000])
+@pytest.mark.parametrize("pad", [None, 2])
+def test_lookup_differentiated_twice(n, pad):
+    V, E = 12, 8  # small whole numbers: every sum is exact
+    g = gen(12)
+    w, c = (torch.randint(-3, 4, (V, E), generator=g, device=DEV).float() for _ in range(2))
+    ids = torch.randint(-1, V, (n,), generator=g, device=DEV)
+    x = torch.randint(-3, 4, (n, E), generator=g, device=DEV).float().requires_grad_(True)
+    w.requires_grad_(True)
+    out = ops.embedding_lookup(w, ids, scale=2.0, padding_idx=pad)
+    (dw,) = torch.autograd.grad((out * out * x).sum(), w, create_graph=True)  # 8 w sum of x, each row's
+    d2w, dx = torch.autograd.grad((dw * c).sum(), (w, x))
+    keep = (ids >= 0) & (ids != (-9 if pad is None else pad))
+    sums = torch.zeros(V, E, device=DEV).index_add_(0, ids[keep], x.detach()[keep])
+    assert torch.equal(dw.detach(), 8 * w.detach() * sums) and torch.equal(d2w, 8 * c * sums)
+    assert torch.equal(dx, torch.where(keep[:, None], 8 * (w.detach() * c)[ids], torch.zeros((), device=DEV)))
 
 
 def test_lookup_of_a_fused_table():
@@ -266,6 +282,42 @@ def test_lookup_offsets_beyond_32_bits():
     assert (grad[-1] == 2.0).all() and not grad[:-1].any()
 
 
+@pytest.mark.parametrize("V, n", [(140_000_001, 90), (300_000_001, 5000)])
+def test_lookup_gradient_of_a_very_long_table(V, n):
+    """More workgroups than one grid dimension takes (short and long calls)."""
+    w = torch.zeros(V, 1, dtype=F16, device=DEV, requires_grad=True)
+    ids = V - 1 - torch.arange(n, device=DEV) // 3
+    ids[:2] = torch.tensor([0, V // 2], device=DEV)
+    (grad,) = torch.autograd.grad(ops.embedding_lookup(w, ids, scale=0.5).sum(), w)
+    want = torch.zeros(V, 1, device=DEV).index_add_(0, ids, torch.full((n, 1), 0.5, device=DEV))
+    assert torch.equal(grad.float(), want)
+
+
+def test_rows_beyond_one_grid_dimension():
+    n = 33_600_005
+    ids = torch.arange(n, device=DEV, dtype=torch.int32) % 37
+    w = torch.randn(37, 65, generator=gen(14), device=DEV).to(F16)
+    out = ops.embedding_lookup(w, ids)
+    for lo in (0, n // 2, n - 100_000):
+        assert torch.equal(out[lo:lo + 100_000], w[ids[lo:lo + 100_000].long()])
+    del out
+    B = 8_400_003  # whole numbers: every sum and gradient is exact
+    q, p, nn = (torch.randint(-1, 2, (B, 65), generator=gen(15 + i), device=DEV).to(BF16).requires_grad_(True) for i in range(3))
+    assert torch.equal(losses.preference_margin(q, p, nn, 1.0), (q * (p - nn)).float().sum(1, keepdim=True))
+    loss = losses.preference_loss(q, p, nn, beta=0.5, temperature=1.0, loss_type="squared")
+    dq, _, dn = torch.autograd.grad(loss, (q, p, nn), torch.tensor(float(B), device=DEV))
+    with torch.no_grad():
+        c = 2 * ((q * (p - nn)).float().sum(1, keepdim=True) - 1)
+        for got, want in ((dq, c * (p - nn)), (dn, -c * q)):  # B (1 / B) is off by 2 U, then the rounding to bf16
+            assert ((got - want).abs() <= (2 ** -8 + 4 * U) * want.abs()).all()
+    del q, p, nn, dq, dn, c, got, want
+    rows = ops.Int4Rows.quantize(torch.randint(-7, 8, (n, 8), generator=gen(19), device=DEV, dtype=torch.int8).to(BF16))
+    x = rows.dequantize()
+    g = torch.randint(-7, 8, (n, 8), generator=gen(19), device=DEV, dtype=torch.int8).float()
+    full = g.abs().amax(1, keepdim=True) == 7  # scale 1: the codes are the values
+    assert torch.equal(torch.where(full, x, g), g)
+
+
 def test_lookup_embedding_module_uses_the_kernels():
     emb = tt.embeddings.build("lookup", vocab_size=50, embedding_dim=16, scale=4.0).to(DEV)
     ids = torch.randint(0, 50, (3, 7), generator=gen(10), device=DEV)
@@ -277,6 +329,34 @@ def test_lookup_embedding_module_uses_the_kernels():
     count = torch.zeros(50, device=DEV).index_add_(0, ids.flatten(), torch.ones(21, device=DEV))
     count[0] = 0  # the padding row
     assert torch.equal(emb.embedding.weight.grad, (4.0 * count).unsqueeze(1).expand(50, 16))
+
+
+def test_lookup_embedding_module_under_torchs_transforms():
+    """What follows torch's own calls (function transforms, tracing, dispatch modes, hooks) sees the plain gather."""
+    emb = tt.embeddings.build("lookup", vocab_size=50, embedding_dim=16, scale=4.0).to(DEV)
+    ids = torch.randint(0, 50, (3, 7), generator=gen(13), device=DEV)
+    w = emb.embedding.weight.detach()
+
+    def f(x):
+        return torch.func.functional_call(emb, {"embedding.weight": x}, (ids,)).square().sum()
+
+    x = w.clone().requires_grad_(True)
+    want = torch.autograd.grad(f(x), x)[0]  # the kernels: rows times a power of two, few terms a row
+    assert (torch.func.grad(f)(w) - want).abs().max() <= 32 * U * want.abs().max()  # (at most 21 terms a sum)
+    _, tangent = torch.func.jvp(f, (w,), (torch.ones_like(w),))
+    rows = emb.embedding(ids).detach()
+    assert abs(tangent.item() - 32 * rows.double().sum().item()) <= 32 * 336 * U * rows.abs().sum().item()
+    with torch.no_grad():
+        traced = torch.jit.trace(emb, (ids,))
+        with torch._subclasses.FakeTensorMode(allow_non_fake_inputs=True):
+            assert emb(torch.empty(2, 5, dtype=torch.int64, device=DEV)).shape == (2, 5, 16)
+        other = (ids + 1) % 50
+        assert torch.equal(traced(other), emb(other))
+    seen = []
+    hook = emb.embedding.register_forward_hook(lambda *a: seen.append(1))
+    emb(ids)
+    hook.remove()
+    assert seen == [1]
 
 
 # ---------------------------------------------------------------------------------------------
@@ -423,7 +503,7 @@ def test_preference_on_the_fused_tower_output(K):
     q, p, n = torch.split(y, [B, B, K * B])
     n3 = n if K == 1 else n.view(B, K, H)
     loss = losses.preference_loss(q, p, n3, beta=0.5)
-    assert "Packed" in type(loss.grad_fn).__name__
+    assert "Packed" in loss.grad_fn.name()
     (got,) = torch.autograd.grad(loss, base)
     a, b, c = (t.detach().clone().requires_grad_(True) for t in (q, p, n3))
     want = torch.autograd.grad(losses.preference_loss(a, b, c, beta=0.5), (a, b, c))

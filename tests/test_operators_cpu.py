@@ -133,15 +133,17 @@ def test_train_step_refuses_clipping_a_fused_table():
 
 
 def test_a_table_differentiated_both_ways_is_refused():
-    d = ops.DeferredTableGrad()
+    d, grad = ops.DeferredTableGrad(), torch.zeros(2, 2)
     d.added_dense()
-    assert not d.pending()  # a dense gradient alone is stepped as usual ...
+    assert not d.pending(grad)  # a dense gradient alone is stepped as usual ...
     d.parts.append(("part",))
-    assert d.pending()  # ... and says nothing about the next step
+    assert d.pending(grad)  # ... and says nothing about the next step
+    d.added_dense()
+    assert d.pending(None)  # dropped by zero_grad before the step
     d.added_dense()
     with pytest.raises(RuntimeError, match="pooled lookups only"):
-        d.pending()
-    assert not d.parts and not d.pending()
+        d.pending(grad)
+    assert not d.parts and not d.pending(grad)
 
 
 @pytest.mark.parametrize("make, err, msg", [

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib
 import os
 import re
 import threading
@@ -19,7 +20,7 @@ HEADER_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__fil
 
 TT_IDS_I32, TT_IDS_I64 = 0, 1
 ELEM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum tt_elem_dtype
-TT_LOOKUP_DIRECT_TOKENS, TT_INT4_MAX_H = 4096, 4096
+TT_LOOKUP_DIRECT_TOKENS, TT_INT4_MAX_H = 4096, 4096  # twotower_amd.h
 TT_INBATCH_TAIL_ROWS, TT_INBATCH_MAX_PARTS = 64, 512  # twotower_amd.h
 TT_F32, TT_BF16, TT_BF16_SPLIT = 0, 1, 2
 TT_SCATTER_SORTED, TT_SCATTER_ATOMIC = 0, 1
@@ -101,7 +102,7 @@ _SIGNATURES = {
     "tt_preference_bwd": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_int, _vp,
                                    _c_f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "tt_clip_ws_size": (_c_sz, [_c_int]),
-    "tt_clip_grads": (_c_int, [_vp, _vp, _vp, ctypes.c_char_p, ctypes.c_char_p, _c_int, _c_int, _c_f64, _c_int, _vp,
+    "tt_clip_grads": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_f64, _c_int, _vp,
                                _vp, _c_sz, _vp]),
     "tt_int4_codes_bytes": (_c_sz, [_c_i64, _c_int]),
     "tt_int4_scales_bytes": (_c_sz, [_c_i64, _c_int, _c_int]),
@@ -283,7 +284,6 @@ def _nullctx():
     return contextlib.nullcontext()
 
 
-
 def join_side_grads(params) -> None:
     """Make the current stream wait for every side-stream gradient of ``params``."""
     seen = set()
@@ -312,6 +312,29 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = cdll
     return _lib
+
+
+_nodes = None
+_NODE_SYMBOLS = ("tt_last_error", "tt_lookup_fwd", "tt_lookup_plan_size", "tt_lookup_plan", "tt_lookup_bwd_ws_size",
+                 "tt_lookup_bwd", "tt_preference_fwd", "tt_preference_bwd", "tt_clip_ws_size", "tt_clip_grads")
+
+
+def nodes():
+    """The module of the operators' eager calls (csrc/nodes.cpp), bound to this library.  Raises if it was not
+    built."""
+    global _nodes
+    if _nodes is None:
+        cdll = lib()
+        with _lock:
+            if _nodes is None:
+                try:
+                    mod = importlib.import_module("twotower_amd._nodes")
+                except ImportError as e:
+                    raise ImportError("twotower_amd: _nodes.so is missing or does not load; build it with "
+                                      "`make -C twotower_amd/csrc` (or __graft_entry__.build())") from e
+                mod.bind({n: ctypes.cast(getattr(cdll, n), _vp).value for n in _NODE_SYMBOLS}, _CALLS, TIMER, call)
+                _nodes = mod
+    return _nodes
 
 
 def last_error() -> str:

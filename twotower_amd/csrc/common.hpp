@@ -180,6 +180,14 @@ inline int vec_for(const int64_t* n, int nn, const void* const* p, const int* by
   return 1;
 }
 
+// The grid of `blocks` workgroups, and a workgroup's index in it: x holds fewer than 2^32 threads, so a larger
+// grid goes on in y (the indices past `blocks` have nothing to do).
+constexpr int64_t kGridX = int64_t(1) << 21;
+inline dim3 wide_grid(int64_t blocks) {
+  return blocks <= kGridX ? dim3((unsigned)blocks) : dim3((unsigned)kGridX, (unsigned)((blocks + kGridX - 1) / kGridX));
+}
+__device__ __forceinline__ int64_t block_index() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // The sort plan of a token lookup's gradient (built in bag.hip by the bags' counting sort, read by
 // lookup.hip): the kept tokens' rows `keys` in ascending order and their token indices `vals` (a row's in
 // token order); *count tokens were kept.

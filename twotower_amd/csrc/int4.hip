@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kBlock) void int4_quantize_kernel(const T* __restri
                                                                int group, int nblk, int nquad, bool wide,
                                                                uint32_t* __restrict__ codes,
                                                                uint16_t* __restrict__ scales) {
-  const Place p = place_of((int64_t)blockIdx.x * kBlock + threadIdx.x, nquad);
+  const Place p = place_of(block_index() * kBlock + threadIdx.x, nquad);
   if (p.row >= (n + kRows - 1) / kRows * kRows) return;  // (whole groups of lanes leave together)
   float v[8] = {};
   if (p.row < n) load8(x + p.row * ld, p.b * kBlk + 8 * p.h, H, wide, v);
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restr
                                                            int group, int nblk, int nquad,
                                                            uint32_t* __restrict__ codes,
                                                            uint16_t* __restrict__ scales) {
-  const Place p = place_of((int64_t)blockIdx.x * kBlock + threadIdx.x, nquad);
+  const Place p = place_of(block_index() * kBlock + threadIdx.x, nquad);
   if (p.row >= (n + kRows - 1) / kRows * kRows) return;
   const int ng = (H + group - 1) / group, g = p.b * kBlk / group;
   if (p.h == 0 && (p.b & (group / kBlk - 1)) == 0)
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restr
 __global__ __launch_bounds__(kBlock) void int4_unpack_kernel(const uint32_t* __restrict__ codes,
                                                              const uint16_t* __restrict__ scales, int64_t n, int H,
                                                              int group, int nblk, int nquad, float* __restrict__ out) {
-  const Place p = place_of((int64_t)blockIdx.x * kBlock + threadIdx.x, nquad);
+  const Place p = place_of(block_index() * kBlock + threadIdx.x, nquad);
   const int k0 = p.b * kBlk + 8 * p.h;
   if (p.row >= n || k0 >= H) return;
   const float s = bf16_value(scales[scale_at(p.row, p.b, nquad, group)]);
@@ -484,7 +484,7 @@ extern "C" int tt_int4_quantize(const void* x, int dtype, int64_t n, int H, int6
   if (n == 0) return TT_OK;
   TT_REQUIRE(layout_blocks(n, H) < (int64_t(1) << 31), "int4: too many values");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)layout_blocks(n, H)), block(kBlock);
+  const dim3 grid = wide_grid(layout_blocks(n, H)), block(kBlock);
   const bool wide = H % 4 == 0 && ld % 4 == 0 && reinterpret_cast<size_t>(x) % (4 * elem_bytes(dtype)) == 0;
 #define TT_QZ(T)                                                                                              \
   int4_quantize_kernel<T><<<grid, block, 0, s>>>(static_cast<const T*>(x), n, H, ld, group, blocks_of(H),     \
@@ -504,7 +504,7 @@ extern "C" int tt_int4_pack(const int8_t* c, const void* sc, int64_t n, int H, i
   TT_REQUIRE(n == 0 || (c && sc), "null pointer");
   if (n == 0) return TT_OK;
   TT_REQUIRE(layout_blocks(n, H) < (int64_t(1) << 31), "int4: too many values");
-  int4_pack_kernel<<<dim3((unsigned)layout_blocks(n, H)), dim3(kBlock), 0, reinterpret_cast<hipStream_t>(stream)>>>(
+  int4_pack_kernel<<<wide_grid(layout_blocks(n, H)), dim3(kBlock), 0, reinterpret_cast<hipStream_t>(stream)>>>(
       c, static_cast<const uint16_t*>(sc), n, H, group, blocks_of(H), quads_of(H), static_cast<uint32_t*>(codes),
       static_cast<uint16_t*>(scales));
   TT_LAUNCH_CHECK("int4_pack");
@@ -519,7 +519,7 @@ extern "C" int tt_int4_unpack(const void* codes, const void* scales, int64_t n, 
   if (n == 0) return TT_OK;
   const int64_t blocks = layout_blocks(n, H);
   TT_REQUIRE(blocks < (int64_t(1) << 31), "int4: too many values");
-  int4_unpack_kernel<<<dim3((unsigned)blocks), dim3(kBlock), 0, reinterpret_cast<hipStream_t>(stream)>>>(
+  int4_unpack_kernel<<<wide_grid(blocks), dim3(kBlock), 0, reinterpret_cast<hipStream_t>(stream)>>>(
       static_cast<const uint32_t*>(codes), static_cast<const uint16_t*>(scales), n, H, group, blocks_of(H),
       quads_of(H), out);
   TT_LAUNCH_CHECK("int4_unpack");

@@ -39,9 +39,12 @@ __global__ __launch_bounds__(kBlock) void lookup_fwd_kernel(const TW* __restrict
                                                             const void* __restrict__ ids, bool wide, int64_t n,
                                                             float scale, TO* __restrict__ out, int lg, bool runs) {
   const int lane = lane_id(), groups = kWave >> lg, sub = lane >> lg, c = lane & ((1 << lg) - 1);
-  const unsigned in = blockIdx.x % (8 * kXcdRun);  // (runs: the grid is whole spans of 8 kXcdRun workgroups)
-  const unsigned block = runs ? blockIdx.x - in + (in & 7) * kXcdRun + (in >> 3) : blockIdx.x;
-  const int64_t wave = (int64_t)block * kWavesPerBlock + (threadIdx.x >> 6);
+  int64_t block = block_index();
+  if (runs) {  // (the grid is whole spans of 8 kXcdRun workgroups)
+    const int in = (int)(block % (8 * kXcdRun));
+    block += (in & 7) * kXcdRun + (in >> 3) - in;
+  }
+  const int64_t wave = block * kWavesPerBlock + (threadIdx.x >> 6);
   const int64_t t0 = wave * groups * U + sub;
   int64_t id[U];
 #pragma unroll
@@ -124,7 +127,8 @@ __global__ __launch_bounds__(kDirectThreads) void lookup_grad_direct_kernel(
   __shared__ int wcnt[kDirectWaves];
   __shared__ float part[kDirectWaves][kWave * VEC];
   const int lane = lane_id(), w = threadIdx.x >> 6;
-  const int64_t r0 = (int64_t)blockIdx.x * R;
+  const int64_t r0 = block_index() * R;
+  if (r0 >= V) return;
   const int rows = (int)(V - r0 < R ? V - r0 : R);
   if (threadIdx.x < kDirectRows) cnt[threadIdx.x] = 0;
   int m = 0;  // tokens kept so far (the same in every thread)
@@ -330,8 +334,8 @@ __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, in
                                                                  const float* __restrict__ sup) {
   const int c = threadIdx.x & ((1 << lg) - 1);
   const int n = *p.count;
-  if (blockIdx.x >= join_blocks) {
-    const int64_t r0 = ((int64_t)(blockIdx.x - join_blocks) * kWavesPerBlock + (threadIdx.x >> 6)) * kZeroRows;
+  if (block_index() >= join_blocks) {
+    const int64_t r0 = ((block_index() - join_blocks) * kWavesPerBlock + (threadIdx.x >> 6)) * kZeroRows;
     const int lane = lane_id(), groups = kWave >> lg;
     const int64_t r = r0 + (lane < kZeroRows ? lane : kZeroRows);
     const int at = first_at_least(p.keys, 0, n, (uint32_t)(r < V ? r : V));
@@ -343,7 +347,7 @@ __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, in
         for (int e = c * VEC; e < E; e += VEC << lg) store_elems_nt<VEC>(grad + (r0 + i) * E + e, zero);
     return;
   }
-  const int64_t t0 = ((int64_t)blockIdx.x * kBlock + threadIdx.x) >> lg;
+  const int64_t t0 = (block_index() * kBlock + threadIdx.x) >> lg;
   const int64_t next_tile = (t0 + 1) * kTile;
   if (next_tile >= n) return;  // no tile after it
   const uint32_t r = p.keys[next_tile];
@@ -382,7 +386,7 @@ int launch_fwd(const void* table, int64_t V, int E, int64_t ld, const void* ids,
   int64_t blocks = (n + per_block - 1) / per_block;
   const bool runs = blocks >= 8 * 8 * kXcdRun;
   if (runs) blocks = (blocks + 8 * kXcdRun - 1) / (8 * kXcdRun) * (8 * kXcdRun);
-  const dim3 grid((unsigned)blocks), block(kBlock);
+  const dim3 grid = wide_grid(blocks), block(kBlock);
   const TW* t = static_cast<const TW*>(table);
   TO* o = static_cast<TO*>(out);
 #define TT_LF(VV) \
@@ -409,7 +413,7 @@ int launch_bwd(const void* dout, const void* ids, int ids_dtype, int64_t n, int6
     // rows each 30 us; 200k x 256, 4096 tokens: 38 and 39 us)
     int64_t R = V / 4096;
     R = R < 1 ? 1 : R > kDirectRows ? kDirectRows : R;
-    const dim3 grid((unsigned)((V + R - 1) / R)), block(kDirectThreads);
+    const dim3 grid = wide_grid((V + R - 1) / R), block(kDirectThreads);
 #define TT_LD(VV) \
   case VV: lookup_grad_direct_kernel<TO, TW, VV><<<grid, block, 0, s>>>(d, ids, ids_dtype == TT_IDS_I64, (int)n, V, E, (int)R, pad, scale, g); break;
     switch (vec) { TT_LD(8) TT_LD(4) TT_LD(2) default: TT_LD(1) }
@@ -423,7 +427,7 @@ int launch_bwd(const void* dout, const void* ids, int ids_dtype, int64_t n, int6
   float *head = ws, *tail = head + tiles * E, *sup = tail + tiles * E;
   auto grid = [&](int64_t groups) { return dim3((unsigned)((groups + per - 1) / per)); };
   const int64_t zero_rows = (int64_t)kWavesPerBlock * kZeroRows;
-  const dim3 block(kBlock), join((unsigned)(grid(tiles).x + (V + zero_rows - 1) / zero_rows));
+  const dim3 block(kBlock), join = wide_grid(grid(tiles).x + (V + zero_rows - 1) / zero_rows);
 #define TT_LS(VV)                                                                                                  \
   case VV:                                                                                                         \
     lookup_tile_sum_kernel<TO, TW, VV><<<grid(tiles), block, 0, s>>>(p, d, E, scale, g, lg, head, tail);           \
@@ -439,9 +443,9 @@ int launch_bwd(const void* dout, const void* ids, int ids_dtype, int64_t n, int6
 }
 
 int check_lookup(int64_t n, int64_t V, int E, const void* ids, int ids_dtype, int table_dtype, int out_dtype) {
-  TT_REQUIRE(V > 0 && V < (int64_t(1) << 31) - 1, "V=%lld out of range", (long long)V);
+  TT_REQUIRE(V > 0 && V < TT_LOOKUP_MAX, "V=%lld out of range", (long long)V);
   TT_REQUIRE(E > 0, "E=%d must be positive", E);
-  TT_REQUIRE(n >= 0 && n < (int64_t(1) << 31), "n=%lld tokens out of range", (long long)n);
+  TT_REQUIRE(n >= 0 && n < TT_LOOKUP_MAX, "n=%lld tokens out of range", (long long)n);
   TT_REQUIRE(ids_dtype == TT_IDS_I32 || ids_dtype == TT_IDS_I64, "ids_dtype=%d", ids_dtype);
   TT_REQUIRE(ids != nullptr || n == 0, "ids is NULL");
   TT_REQUIRE(elem_ok(table_dtype) && elem_ok(out_dtype) && (out_dtype == table_dtype || table_dtype == TT_E_F32),

@@ -135,7 +135,7 @@ __global__ __launch_bounds__(kBlock) void pref_fwd_kernel(PrefArgs a, const T* _
                                                           float* __restrict__ margins, float* __restrict__ rows,
                                                           int32_t* __restrict__ counts) {
   const int lane = lane_id(), sub = lane >> lg, c = lane & ((1 << lg) - 1);
-  const int64_t i = (((int64_t)blockIdx.x * kBlock + threadIdx.x) >> 6) * (kWave >> lg) + sub;
+  const int64_t i = ((block_index() * kBlock + threadIdx.x) >> 6) * (kWave >> lg) + sub;
   if (i >= a.B) return;
   float sum;
   int count;
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(kBlock) void pref_bwd_kernel(PrefArgs a, const T* _
                                                           const float* __restrict__ grad_loss, T* __restrict__ dq,
                                                           T* __restrict__ dp, T* __restrict__ dn) {
   const int lane = lane_id(), sub = lane >> lg, c = lane & ((1 << lg) - 1);
-  const int64_t i = (((int64_t)blockIdx.x * kBlock + threadIdx.x) >> 6) * (kWave >> lg) + sub;
+  const int64_t i = ((block_index() * kBlock + threadIdx.x) >> 6) * (kWave >> lg) + sub;
   if (i >= a.B) return;
   const float G = grad_loss[0] * (inv_pairs[0] * a.inv_tau);
   const T *qi = q + i * a.ldq, *pi = p + i * a.ldp, *ni = n + i * a.ldnb;
@@ -275,7 +275,7 @@ int launch_pref_fwd(const PrefArgs& a, const void* q, const void* p, const void*
   }
   const int64_t per = (kBlock / kWave) * (kWave >> lg);
   if (a.B > 0) {
-    const dim3 grid((unsigned)((a.B + per - 1) / per)), block(kBlock);
+    const dim3 grid = wide_grid((a.B + per - 1) / per), block(kBlock);
 #define TT_CALL(V) pref_fwd_kernel<T, V><<<grid, block, 0, s>>>(a, tq, tp, tn, lg, coef, margins, loss ? rows : nullptr, counts)
     TT_PREF_VEC(vec, TT_CALL)
 #undef TT_CALL
@@ -294,7 +294,7 @@ int launch_pref_bwd(const PrefArgs& a, const void* q, const void* p, const void*
   const void* ptrs[] = {q, p, n, dq, dp, dn};
   const int vec = pref_vec<T>(a, ptrs, 6), lg = lanes_log2(a.H, vec);
   const int64_t per = (kBlock / kWave) * (kWave >> lg);
-  const dim3 grid((unsigned)((a.B + per - 1) / per)), block(kBlock);
+  const dim3 grid = wide_grid((a.B + per - 1) / per), block(kBlock);
 #define TT_CALL(V)                                                                                              \
   pref_bwd_kernel<T, V><<<grid, block, 0, s>>>(a, static_cast<const T*>(q), static_cast<const T*>(p),           \
                                                static_cast<const T*>(n), lg, coef, inv_pairs, grad_loss,          \

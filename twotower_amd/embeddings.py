@@ -13,6 +13,7 @@ from abc import ABC
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 
@@ -34,8 +35,18 @@ class BaseEmbedding(nn.Module, ABC):
 
 def _plain_embedding(m: nn.Module) -> bool:
     """An nn.Embedding whose forward is nothing but the row gather of a type the HIP lookup has."""
+    w = m.weight
     return (type(m) is nn.Embedding and m.max_norm is None and not m.scale_grad_by_freq and not m.sparse
-            and m.weight.dtype in _lib.ELEM_DTYPES and not m._forward_hooks and not m._forward_pre_hooks)
+            and type(w) in (nn.Parameter, torch.Tensor) and w.dtype in _lib.ELEM_DTYPES and w.is_contiguous()
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks))
+
+
+def _observed() -> bool:
+    """Whether a tracer, function transform, forward-mode derivative or dispatch mode follows torch's own calls: it
+    would not see a kernel's."""
+    return (torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active()
+            or torch._C._len_torch_dispatch_stack() > 0 or torch.jit.is_tracing()
+            or forward_ad._current_level >= 0)
 
 
 class LookupEmbedding(BaseEmbedding):
@@ -62,7 +73,7 @@ class LookupEmbedding(BaseEmbedding):
         towers.  The towers of this package never call it (they use pool_mean).  On the GPU one HIP
         gather forward and, for the dense table gradient, a sum over sorted tokens (ops.embedding_lookup)."""
         inner = self.embedding
-        if input_ids.is_cuda and inner.weight.is_cuda and _plain_embedding(inner):
+        if input_ids.is_cuda and inner.weight.is_cuda and _plain_embedding(inner) and not _observed():
             return ops.embedding_lookup(inner.weight, input_ids, self.scale, inner.padding_idx)
         rows = inner(input_ids)
         return rows if self.scale == 1.0 else rows * self.scale

@@ -5,11 +5,9 @@ Reference call sites each op replaces are cited per function (paths inside k0r1g
 """
 from __future__ import annotations
 
-import array
 import contextlib
 import ctypes
 import functools
-import operator
 import os
 
 import torch
@@ -261,11 +259,12 @@ class DeferredTableGrad:
         self.queued = False
         self.dense = False  # an embedding_lookup of the table left a dense .grad this step
 
-    def pending(self) -> bool:
-        """Whether this step left parts for the fused update.  It takes no dense gradient beside them: a
-        step that differentiated the table both ways is refused, not updated with one of the two."""
+    def pending(self, grad: torch.Tensor | None) -> bool:
+        """Whether this step left parts for the fused update.  It takes no dense gradient (``grad``, the
+        table's .grad) beside them: a step that differentiated the table both ways is refused, not updated
+        with one of the two."""
         dense, self.dense = self.dense, False
-        if self.parts and dense:
+        if self.parts and dense and grad is not None:
             self.parts.clear()
             raise RuntimeError("the fused table update takes pooled lookups only, and this step also differentiated "
                                "an embedding_lookup of the table: build the optimizer with fused_tables=False")
@@ -532,60 +531,22 @@ def bag_mean_pool(weight: torch.Tensor, ids: torch.Tensor, padding_idx: int | No
 
 # --------------------------------------------------------------------------------------------
 # Token lookup with a scale   (twotower/embeddings.py:40, the (B, L, E) rows a tower may pool itself)
-def _no_second_derivative(what: str) -> None:
-    """In a backward: refuses create_graph=True (grad mode is on then), which would drop the second
-    derivative without a word.  (torch's once_differentiable says it later, and costs 5 us a call.)"""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{what} has no second derivative: backward with create_graph=True is not supported")
-
-
-def _lookup_fwd(weight, ids, scale, out_dtype):
-    V, E = weight.shape
-    out = weight.new_empty((*ids.shape, E), dtype=out_dtype)
-    n = ids.numel()
-    if n:
-        launch(weight, "tt_lookup_fwd", weight.data_ptr(), _lib.ELEM_DTYPES[weight.dtype], V, E,
-               weight.stride(0) if V > 1 else E, ids.data_ptr(), _lib.ids_dtype_code(ids), n, scale, out.data_ptr(), _lib.ELEM_DTYPES[out_dtype])
-    return out
-
-
-class EmbeddingLookup(torch.autograd.Function):
-    """out = scale * weight[ids], gradient by sorted tokens (see embedding_lookup)."""
+class _TableGate(torch.autograd.Function):
+    """A fused or column-sharded table on its way into a lookup that gives it a dense gradient."""
 
     @staticmethod
-    def forward(ctx, weight, ids, scale, padding_idx, out_dtype):
-        ctx.save_for_backward(ids)
-        ctx.meta = (weight.shape, weight.dtype, scale, padding_idx)
+    def forward(ctx, weight):
         ctx.weight_ref = weight
-        return _lookup_fwd(weight, ids, scale, out_dtype)
+        return weight.view_as(weight)
 
     @staticmethod
-    def backward(ctx, dout):
-        _no_second_derivative("embedding_lookup")
-        (ids,) = ctx.saved_tensors
-        (V, E), dtype, scale, pad = ctx.meta
+    def backward(ctx, grad):
         if getattr(ctx.weight_ref, "_tt_column", None) is not None:
             raise RuntimeError("a column-sharded table takes its gradient from bag_mean_pool only")
         deferred = getattr(ctx.weight_ref, "_tt_deferred", None)
         if deferred is not None:
             deferred.added_dense()
-        dout = dout.contiguous()
-        n = ids.numel()
-        grad = dout.new_empty((V, E), dtype=dtype)
-        plan = ws = None
-        size = nbytes = 0
-        if n > _lib.TT_LOOKUP_DIRECT_TOKENS:
-            # Sorted here, not beside the forward on a side stream: the gather fills the memory system and every CU,
-            # and the sort beside it ended no sooner (forward and backward back to back 352 against 344 us at
-            # 8192 x 64 tokens).  Buffers per call, not shared: two captured graphs, or streams, may run their
-            # backwards at once.
-            size, nbytes = _lib.lib().tt_lookup_plan_size(n, V), _lib.lib().tt_lookup_bwd_ws_size(n, E)
-            plan, ws = (dout.new_empty((b,), dtype=torch.uint8) for b in (size, nbytes))
-            launch(dout, "tt_lookup_plan", ptr(ids), _lib.ids_dtype_code(ids), n, V, pad, ptr(plan), size)
-        launch(dout, "tt_lookup_bwd", dout.data_ptr(), _lib.ELEM_DTYPES[dout.dtype], ids.data_ptr(),
-               _lib.ids_dtype_code(ids), n, V, E, pad, scale, grad.data_ptr(), _lib.ELEM_DTYPES[dtype], ptr(plan), size,
-               ptr(ws), nbytes)
-        return grad, None, None, None, None
+        return grad
 
 
 def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None,
@@ -597,38 +558,14 @@ def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0
 
     The gradient is dense: every row of the table, scale times the sum of its tokens' gradients in
     fp32 in a fixed order (bitwise reproducible), rounded once to the table's type; the row of
-    ``padding_idx`` (negative: from the end, as in torch) gets zeros."""
-    shape, dtype = weight.shape, weight.dtype
-    if len(shape) != 2 or 0 in shape:
-        raise ValueError(f"weight must be a non-empty (V, E) table, got shape {tuple(shape)}")
-    _lib.elem_dtype_code(weight, "weight")
-    _lib.ids_dtype_code(ids)
-    V, E = shape
-    s0, s1 = weight.stride()
-    if (s1 != 1 and E > 1) or (s0 < E and V > 1):
-        raise ValueError(f"weight rows must be contiguous and must not overlap, got strides {weight.stride()}")
-    if out_dtype is None:
-        out_dtype = dtype
-    elif out_dtype != dtype and not (dtype == _FLOAT and out_dtype in _lib.ELEM_DTYPES):
-        raise TypeError(f"out_dtype {out_dtype} from a {dtype} table is not supported")
-    if ids.numel() >= 2 ** 31:
-        raise ValueError(f"at most 2^31 - 1 ids per call, got {ids.numel()}")
-    pad = -1
-    if padding_idx is not None:
-        if not -V <= padding_idx < V:
-            raise ValueError(f"padding_idx {padding_idx} outside a table of {V} rows")
-        pad = padding_idx % V
-    _lib.same_device(weight, ids)
-    want_grad = weight.requires_grad and torch.is_grad_enabled()
+    ``padding_idx`` (negative: from the end, as in torch) gets zeros.  It can be differentiated again."""
     col = getattr(weight, "_tt_column", None)
     if col is not None and col.stale:
         raise RuntimeError("embedding_lookup reads the whole table: this one is column-sharded and was updated since it was "
                            "last gathered; materialize() it first, or use bag_mean_pool")
-    if not ids.is_contiguous():
-        ids = ids.contiguous()
-    if want_grad:
-        return EmbeddingLookup.apply(weight, ids, float(scale), pad, out_dtype)
-    return _lookup_fwd(weight, ids, float(scale), out_dtype)
+    if col is not None or getattr(weight, "_tt_deferred", None) is not None:
+        weight = _TableGate.apply(weight)
+    return _lib.nodes().embedding_lookup(weight, ids, float(scale), padding_idx, out_dtype)
 
 
 # --------------------------------------------------------------------------------------------
@@ -1182,108 +1119,6 @@ class MultiNegLossPacked(torch.autograd.Function):
 PREFERENCE_KINDS = {"sigmoid": 0, "squared": 1}
 
 
-def _pref_args(q, p, n):
-    """(q, p, n with a pair axis, element type) of a checked call."""
-    sq, sn = q.shape, n.shape
-    if len(sq) != 2 or p.shape != sq:
-        raise ValueError(f"q and p must both be (B, H), got {tuple(sq)} and {tuple(p.shape)}")
-    if len(sn) == 2:
-        n = n.unsqueeze(1)
-        sn = n.shape
-    if len(sn) != 3 or sn[0] != sq[0] or sn[2] != sq[1] or sn[1] < 1:
-        raise ValueError(f"n must be (B, H) or (B, K, H) with K >= 1 beside q {tuple(sq)}, got {tuple(sn)}")
-    if sq[1] < 1:
-        raise ValueError("H must be at least 1")
-    dt = _lib.elem_dtype_code(q, "q")
-    if p.dtype != q.dtype or n.dtype != q.dtype:
-        raise TypeError(f"q, p and n must have one type, got {q.dtype}, {p.dtype}, {n.dtype}")
-    if sq[1] > 1 and not q.stride(1) == p.stride(1) == n.stride(2) == 1:
-        q, p, n = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, p, n))  # rows of contiguous elements
-    return q, p, n, dt
-
-
-def _pref_pairs(t, name, dtype, B, K, device):
-    """A contiguous (B, K) side input (ref_margin, mask); (B,) is taken where K = 1."""
-    if t is None:
-        return None
-    if t.shape != (B, K) and not (K == 1 and t.shape == (B,)):
-        raise ValueError(f"{name} must be ({B}, {K}), got {tuple(t.shape)}")
-    if t.device != device:
-        raise RuntimeError(f"twotower_amd: {name} is on {t.device}, the embeddings on {device}")
-    if dtype == torch.bool:
-        if t.dtype != torch.bool:
-            raise TypeError(f"{name} must be bool, got {t.dtype}")
-    elif not t.dtype.is_floating_point:
-        raise TypeError(f"{name} must be a floating-point tensor, got {t.dtype}")
-    return t.detach().to(dtype).contiguous()
-
-
-def _pref_fwd(q, p, n, dt, ref, mask, opts, margins=None, loss=None):
-    """Fills margins, or loss and returns the side buffer: dl/dh (B K), 1 / pairs, then 2 B words of scratch."""
-    (B, K, H), (kind, beta, inv_tau, smooth) = n.shape, opts
-    side, at = None, (None, None, None)
-    if loss is not None:
-        side = q.new_empty((B * K + 1 + 2 * B,), dtype=_FLOAT)
-        base = side.data_ptr()
-        at = (base, base + 4 * B * K, base + 4 * (B * K + 1))
-    sn = n.stride()
-    launch(q, "tt_preference_fwd", q.data_ptr(), q.stride(0), p.data_ptr(), p.stride(0), n.data_ptr(), sn[0], sn[1], dt, B,
-           K, H, ptr(ref), ptr(mask), kind, beta, inv_tau, smooth, at[0], ptr(margins), ptr(loss), at[1], at[2], 8 * B)
-    return side
-
-
-def _pref_bwd(q, p, n, dt, mask, opts, side, g, dq, dp, dn):
-    B, K, H = n.shape
-    if g.dtype != _FLOAT:
-        g = g.to(_FLOAT)
-    base = side.data_ptr()
-    sn = n.stride()
-    launch(q, "tt_preference_bwd", q.data_ptr(), q.stride(0), p.data_ptr(), p.stride(0), n.data_ptr(), sn[0], sn[1], dt, B,
-           K, H, ptr(mask), opts[2], base, base + 4 * B * K, g.data_ptr(), dq.data_ptr(), dp.data_ptr(), dn.data_ptr())
-
-
-class PreferenceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, p, n, dt, ref, mask, opts):
-        loss = q.new_empty((), dtype=_FLOAT)
-        side = _pref_fwd(q, p, n, dt, ref, mask, opts, loss=loss)
-        ctx.save_for_backward(q, p, n, mask, side)
-        ctx.meta = (dt, opts)
-        return loss
-
-    @staticmethod
-    def backward(ctx, g):
-        _no_second_derivative("preference_loss")
-        q, p, n, mask, side = ctx.saved_tensors
-        # (empty_like: torch.empty with a device argument takes four times as long on autograd's thread)
-        dq, dp, dn = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, p, n))
-        _pref_bwd(q, p, n, ctx.meta[0], mask, ctx.meta[1], side, g, dq, dp, dn)
-        return dq, dp, dn, None, None, None, None
-
-
-class PreferenceLossPacked(torch.autograd.Function):
-    """The same loss on one ((2 + K) B, H) tensor [q; p; negatives] (TwoTower's fused output): the
-    three gradients are written into one tensor, so autograd runs no split backward."""
-
-    @staticmethod
-    def forward(ctx, qpn, B, K, dt, ref, mask, opts):
-        loss = qpn.new_empty((), dtype=_FLOAT)
-        side = _pref_fwd(qpn[:B], qpn[B:2 * B], qpn[2 * B:].view(B, K, -1), dt, ref, mask, opts, loss=loss)
-        ctx.save_for_backward(qpn, mask, side)
-        ctx.meta = (B, K, dt, opts)
-        return loss
-
-    @staticmethod
-    def backward(ctx, g):
-        _no_second_derivative("preference_loss")
-        qpn, mask, side = ctx.saved_tensors
-        B, K, dt, opts = ctx.meta
-        grad = torch.empty_like(qpn)
-        _pref_bwd(qpn[:B], qpn[B:2 * B], qpn[2 * B:].view(B, K, -1), dt, mask, opts, side, g, grad[:B], grad[B:2 * B],
-                  grad[2 * B:])
-        return grad, None, None, None, None, None, None
-
-
 def _pref_opts(beta, temperature, label_smoothing, loss_type):
     if loss_type not in PREFERENCE_KINDS:
         raise ValueError(f"loss_type must be one of {sorted(PREFERENCE_KINDS)}, got {loss_type!r}")
@@ -1303,25 +1138,13 @@ def preference_loss(q: torch.Tensor, p: torch.Tensor, n: torch.Tensor, ref_margi
                     packed: torch.Tensor | None = None) -> torch.Tensor:
     """losses.preference_loss on the HIP row kernels.  packed: the one tensor [q; p; n] that q, p and n are
     the consecutive row blocks of, which then receives the gradient."""
-    opts = _pref_opts(beta, temperature, label_smoothing, loss_type)
-    q, p, n, dt = _pref_args(q, p, n)
-    B, K, _ = n.shape
-    ref = _pref_pairs(ref_margin, "ref_margin", _FLOAT, B, K, q.device)
-    mask = _pref_pairs(mask, "mask", torch.bool, B, K, q.device)
-    _lib.same_device(q, p, n)
-    if packed is not None:
-        return PreferenceLossPacked.apply(packed, B, K, dt, ref, mask, opts)
-    return PreferenceLoss.apply(q, p, n, dt, ref, mask, opts)
+    return _lib.nodes().preference_loss(q, p, n, ref_margin, mask,
+                                        *_pref_opts(beta, temperature, label_smoothing, loss_type), packed)
 
 
 def preference_margin(q: torch.Tensor, p: torch.Tensor, n: torch.Tensor, temperature: float = 0.1) -> torch.Tensor:
     """losses.preference_margin: (B, K) float32 margins, no gradient."""
-    opts = _pref_opts(1.0, temperature, 0.0, "sigmoid")
-    q, p, n, dt = _pref_args(q.detach(), p.detach(), n.detach())
-    _lib.same_device(q, p, n)
-    margins = torch.empty(n.shape[:2], dtype=_FLOAT, device=q.device)
-    _pref_fwd(q, p, n, dt, None, None, opts, margins=margins)
-    return margins
+    return _lib.nodes().preference_margin(q, p, n, _pref_opts(1.0, temperature, 0.0, "sigmoid")[2])
 
 
 # --------------------------------------------------------------------------------------------
@@ -1605,15 +1428,6 @@ def in_batch_softmax_loss(q: torch.Tensor, d: torch.Tensor, temperature: float =
 
 # --------------------------------------------------------------------------------------------
 # global gradient norm and clipping (between twotower/train.py:138 and :139)
-_CLIP_TYPES = {(0, 0), (1, 1), (2, 2), (1, 0), (2, 0)}  # (gradient, out) type codes of tt_clip_grads
-_IS_SPARSE = operator.attrgetter("is_sparse")
-
-
-def _dense(t: torch.Tensor) -> bool:
-    """t's elements fill one block of memory, in any order (a norm and a product need no more)."""
-    return t.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(t)
-
-
 def clip_grad_norm(grads, max_norm: float | None, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """The global norm (norm_type 2 or inf) of all gradients as a 0-dim float32 tensor, and the gradients times
     min(1, max_norm / (norm + 1e-6)), in place or into ``out`` (one tensor per gradient, of its type or
@@ -1630,68 +1444,10 @@ def clip_grad_norm(grads, max_norm: float | None, norm_type: float = 2.0, out=No
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if not scale and out is not None:
         raise ValueError("out needs a max_norm")
-    outs = grads if out is None else list(out)
-    if len(outs) != len(grads):
-        raise ValueError(f"{len(outs)} out tensors for {len(grads)} gradients")
-    if not grads:
+    outs = None if out is None else list(out)
+    if not grads and not outs:
         return torch.zeros((), dtype=_FLOAT)
-    first = grads[0]
-    dev, codes = first.device, _lib.ELEM_DTYPES
-    # (a long list's call is bound by this loop-free Python: about 0.7 us a tensor)
-    types = [codes.get(g.dtype) for g in grads]
-    otypes = types if outs is grads else [codes.get(o.dtype) for o in outs]
-    if not _CLIP_TYPES.issuperset(zip(types, otypes)):
-        i = next(i for i, pair in enumerate(zip(types, otypes)) if pair not in _CLIP_TYPES)
-        raise TypeError(f"gradient {i} of {grads[i].dtype} into {outs[i].dtype}: float32, bfloat16 or float16, into its own "
-                        "type or float32")
-    if any(map(_IS_SPARSE, grads)):
-        raise RuntimeError("clip_grad_norm does not support sparse gradients")
-    copies = []
-    src = dst = grads
-    if outs is grads:
-        if not all(map(torch.Tensor.is_contiguous, grads)):
-            src = dst = [g if _dense(g) else g.contiguous() for g in grads]
-            if scale:
-                copies = [(g, t) for g, t in zip(grads, src) if t is not g]
-                for g, _ in copies:
-                    if torch._debug_has_internal_overlap(g) == 1:
-                        raise ValueError(f"a gradient of shape {tuple(g.shape)} has elements that share memory (an expanded "
-                                         "tensor): clip a copy")
-    else:
-        if [g.shape for g in grads] != [o.shape for o in outs]:
-            i = next(i for i, (g, o) in enumerate(zip(grads, outs)) if g.shape != o.shape)
-            raise ValueError(f"out {i} has shape {tuple(outs[i].shape)}, the gradient {tuple(grads[i].shape)}")
-        dst = outs
-        if not (all(map(torch.Tensor.is_contiguous, grads)) and all(map(torch.Tensor.is_contiguous, outs))):
-            src = [g.contiguous() for g in grads]
-            dst = [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in outs]
-            copies = [(o, t) for o, t in zip(outs, dst) if t is not o]
-    sizes = list(map(torch.Tensor.numel, grads))
-    src_at = list(map(torch.Tensor.data_ptr, src))
-    dst_at = src_at if dst is src else list(map(torch.Tensor.data_ptr, dst))
-    if scale and len(set(dst_at)) != len(dst_at):
-        written = [a for a, n in zip(dst_at, sizes) if n]
-        if len(set(written)) != len(written):
-            raise ValueError("a gradient is written twice: the same memory is listed more than once")
-    if dst is not src and not set(src_at).isdisjoint(dst_at):
-        written = {d for s, d, n in zip(src_at, dst_at, sizes) if n and s != d}
-        if not written.isdisjoint(a for a, n in zip(src_at, sizes) if n):
-            raise ValueError("an out tensor is the memory of another gradient")
-    devices = set(map(torch.Tensor.get_device, grads))
-    if outs is not grads:
-        devices.update(map(torch.Tensor.get_device, outs))
-    if len(devices) > 1 or -1 in devices:
-        _lib.same_device(first, *grads, *outs)  # (says which)
-    n = len(grads)
-    norm = first.new_empty((), dtype=_FLOAT)
-    nbytes = _lib.lib().tt_clip_ws_size(n)
-    ws = first.new_empty((nbytes,), dtype=torch.uint8)
-    lists = [array.array("q", v) for v in (src_at, dst_at, sizes)]
-    launch(first, "tt_clip_grads", *[v.buffer_info()[0] for v in lists], bytes(types), bytes(otypes), n,
-           int(norm_type == float("inf")), float(max_norm) if scale else 0.0, int(scale), ptr(norm), ptr(ws), nbytes)
-    for o, t in copies:
-        o.copy_(t)
-    return norm
+    return _lib.nodes().clip_grad_norm(grads, float(max_norm) if scale else None, norm_type == float("inf"), outs)
 
 
 # --------------------------------------------------------------------------------------------

@@ -218,7 +218,7 @@ class AdamW(torch.optim.Optimizer):
         self._side_grads.join()
         for p in group["params"]:
             deferred = getattr(p, "_tt_deferred", None)
-            if deferred is not None and deferred.pending():
+            if deferred is not None and deferred.pending(p.grad):
                 st = self._state(p, False)
                 st["step"] += 1
                 col = self._columns.get(id(p))
@@ -257,7 +257,7 @@ class AdamW(torch.optim.Optimizer):
         slots, dense, fused, shards, dense_ids, columns = [], [], [], [], [], []
         for p in group["params"]:
             deferred = getattr(p, "_tt_deferred", None)
-            if deferred is not None and deferred.pending():
+            if deferred is not None and deferred.pending(p.grad):
                 st = self._state(p, True)
                 a = self._adam_args(p)
                 slots.append((st["step"], a))
@@ -500,7 +500,7 @@ class BackwardTableUpdate:
     def __call__(self) -> None:
         w = self.weight
         deferred = w._tt_deferred
-        if not deferred.pending():
+        if not deferred.pending(w.grad):
             return
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("table_update 'backward' runs eagerly (host step counter); use TrainStep with "

@@ -197,19 +197,20 @@ int tt_bag_col_reduce_ex(const int32_t* seg_all, const int32_t* vals_all, int64_
  * tt_lookup_bwd: grad[r, :] = scale * sum of dout[t, :] over the tokens with ids[t] = r (none for r =
  *   padding_idx, -1: no padding id), every one of the V rows written.  Sums are fp32 in a fixed order
  *   (bitwise reproducible), rounded once to grad's type; dout has out's type, grad the table's.
- *   ws: tt_lookup_bwd_ws_size bytes, 16-byte aligned (0 for short calls, of up to TT_LOOKUP_DIRECT_TOKENS).
+ *   ws: tt_lookup_bwd_ws_size bytes, 16-byte aligned (0 for short calls, of up to
+ *   TT_LOOKUP_DIRECT_TOKENS, fewer of wide rows).
  * tt_lookup_plan: the half of the backward that needs the ids alone, their sort (tt_lookup_plan_size bytes;
- *   0 for short calls, which need none), to be called before tt_lookup_bwd with the same ids, n, V and
+ *   0 for short calls: nothing to do), to be called before tt_lookup_bwd with the same ids, n, V and
  *   padding_idx, on the same stream or one that it waits for (it may run beside the forward).  The plan is
  *   only read by tt_lookup_bwd. */
-#define TT_LOOKUP_DIRECT_TOKENS 4096
+#define TT_LOOKUP_DIRECT_TOKENS 8192
 #define TT_LOOKUP_MAX 0x7fff0000LL /* tokens and rows stay below it */
 int tt_lookup_fwd(const void* table, int table_dtype, int64_t V, int E, int64_t ld_table, const void* ids,
                   int ids_dtype, int64_t n, float scale, void* out, int out_dtype, tt_stream_t stream);
-size_t tt_lookup_plan_size(int64_t n, int64_t V);
+size_t tt_lookup_plan_size(int64_t n, int64_t V, int E, int dout_dtype);
 int tt_lookup_plan(const void* ids, int ids_dtype, int64_t n, int64_t V, int64_t padding_idx, void* plan,
                    size_t plan_bytes, tt_stream_t stream);
-size_t tt_lookup_bwd_ws_size(int64_t n, int E);
+size_t tt_lookup_bwd_ws_size(int64_t n, int E, int dout_dtype);
 int tt_lookup_bwd(const void* dout, int dout_dtype, const void* ids, int ids_dtype, int64_t n, int64_t V, int E,
                   int64_t padding_idx, float scale, void* grad, int grad_dtype, const void* plan, size_t plan_bytes,
                   void* ws, size_t ws_bytes, tt_stream_t stream);

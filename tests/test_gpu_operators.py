@@ -96,6 +96,13 @@ LOOKUPS = [
     (129, 1030, (300,), BF16, torch.int32, None, 1, 0.3),
     (70_000, 8, (20_000,), BF16, torch.int64, None, 0, 0.1),
     (2048, 512, (9000,), F16, torch.int64, None, 0, 0.5),
+    (129, 513, (9000,), F32, torch.int32, None, 1, 0.3),
+    (50, 65, (8192,), BF16, torch.int64, None, 0, 0.2),          # the longest call without a sort, and one more
+    (50, 64, (8193,), BF16, torch.int64, None, 0, 0.2),
+    (30, 600, (2000,), F32, torch.int32, None, None, 0.4),       # frequent rows of 3, 9 and 1 column chunks
+    (40, 1030, (700,), F32, torch.int64, None, None, 0.5),
+    (20, 1, (3000,), F32, torch.int64, None, None, 0.6),
+    (20, 7, (257,), BF16, torch.int32, None, None, 1.0),         # one id alone
     (700, 256, (70_001,), F32, torch.int32, None, 0, 0.1),       # workgroups dealt to the XCDs in runs
 ]
 
@@ -119,7 +126,7 @@ def test_lookup_against_plain(V, E, shape, dtype, ids_dtype, out_dtype, pad, hot
         assert torch.equal(ops.embedding_lookup(w, ids, scale=scale, out_dtype=out_dtype), out)
 
 
-@pytest.mark.parametrize("n", [0, 600, 5000])
+@pytest.mark.parametrize("n", [0, 600, 5000, 9000])
 def test_lookup_ids_outside_the_table(n):
     V, E = 40, 24
     w, ids, dout = lookup_case(V, E, (n,), F32, torch.int64, None, None, 0.0, 2)
@@ -173,7 +180,7 @@ def test_lookup_odd_tables_and_ids():
         torch.autograd.grad(losses.preference_loss(plain, plain.flip(0), plain.roll(1, 0)), plain, create_graph=True)
 
 
-@pytest.mark.parametrize("n", [30, 6000])
+@pytest.mark.parametrize("n", [30, 6000, 9000])
 @pytest.mark.parametrize("pad", [None, 2])
 def test_lookup_differentiated_twice(n, pad):
     V, E = 12, 8  # small whole numbers: every sum is exact
@@ -282,7 +289,7 @@ def test_lookup_offsets_beyond_32_bits():
     assert (grad[-1] == 2.0).all() and not grad[:-1].any()
 
 
-@pytest.mark.parametrize("V, n", [(140_000_001, 90), (300_000_001, 5000)])
+@pytest.mark.parametrize("V, n", [(140_000_001, 90), (300_000_001, 9000)])
 def test_lookup_gradient_of_a_very_long_table(V, n):
     """More workgroups than one grid dimension takes (short and long calls)."""
     w = torch.zeros(V, 1, dtype=F16, device=DEV, requires_grad=True)

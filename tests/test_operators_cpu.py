@@ -257,10 +257,10 @@ def _clip(src=P, dst=P, n=3, st=0, dt=0, max_norm=1.0, ws=1 << 20):
     ("tt_lookup_fwd", (P, 0, 5, 4, 4, P, 0, 2 ** 31, 1.0, P, 0, None), "out of range"),
     ("tt_lookup_fwd", (None, 0, 5, 4, 4, P, 0, 1, 1.0, P, 0, None), "null pointer"),
     ("tt_lookup_bwd", (None, 0, P, 0, 1, 5, 4, -1, 1.0, P, 0, None, 0, None, 0, None), "null pointer"),
-    ("tt_lookup_bwd", (P, 0, P, 0, 5000, 5, 4, -1, 1.0, P, 0, None, 0, P, 1 << 30, None), "plan too small"),
-    ("tt_lookup_bwd", (P, 0, P, 0, 5000, 5, 4, -1, 1.0, P, 0, P, 1 << 30, P, 8, None), "workspace too small"),
-    ("tt_lookup_plan", (P, 0, 5000, 5, -1, P, 100, None), "workspace too small"),
-    ("tt_lookup_plan", (None, 0, 5000, 5, -1, P, 1 << 30, None), "ids is NULL"),
+    ("tt_lookup_bwd", (P, 0, P, 0, 9000, 5, 4, -1, 1.0, P, 0, None, 0, P, 1 << 30, None), "plan too small"),
+    ("tt_lookup_bwd", (P, 0, P, 0, 9000, 5, 4, -1, 1.0, P, 0, P, 1 << 30, P, 8, None), "workspace too small"),
+    ("tt_lookup_plan", (P, 0, 9000, 5, -1, P, 100, None), "workspace too small"),
+    ("tt_lookup_plan", (None, 0, 9000, 5, -1, P, 1 << 30, None), "ids is NULL"),
     ("tt_preference_fwd", (P, 4, P, 4, P, 4, 4, 3, 2, 1, 4, None, None, 0, 1.0, 1.0, 0.0, P, None, P, P, P, 16, None),
      "element type 3"),
     ("tt_preference_fwd", (P, 4, P, 4, P, 4, 4, 0, 2, 0, 4, None, None, 0, 1.0, 1.0, 0.0, P, None, P, P, P, 16, None),
@@ -300,10 +300,12 @@ def test_c_abi_refusals(name, args, msg):
 def test_c_abi_sizes():
     lib = _lib.lib()
     for n, short in ((_lib.TT_LOOKUP_DIRECT_TOKENS, True), (_lib.TT_LOOKUP_DIRECT_TOKENS + 1, False)):
-        assert (lib.tt_lookup_plan_size(n, 50) == 0) is short and (lib.tt_lookup_bwd_ws_size(n, 8) == 0) is short
-    assert lib.tt_lookup_bwd_ws_size(100, 8) == lib.tt_lookup_plan_size(100, 50) == 0  # short calls take none
-    assert lib.tt_lookup_bwd_ws_size(100_000, 8) == (2 * 3125 + 97) * 8 * 4  # heads, tails, super-tiles
-    assert lib.tt_lookup_plan_size(100_000, 50) > 4 * 4 * 100_000
+        for rows, E, dtype in ((n, 256, 0), (n, 512, 1), (n // 2 + (n & 1), 260, 0), (n // 4 + (n & 1), 2048, 2),
+                               (n // 2 + (n & 1), 339, 1)):
+            sizes = lib.tt_lookup_plan_size(rows, 50, E, dtype), lib.tt_lookup_bwd_ws_size(rows, E, dtype)
+            assert [s == 0 for s in sizes] == [short, short]  # short calls take neither
+    assert lib.tt_lookup_bwd_ws_size(100_000, 8, 0) == (2 * 3125 + 97) * 8 * 4  # heads, tails, super-tiles
+    assert lib.tt_lookup_plan_size(100_000, 50, 8, 0) > 4 * 4 * 100_000
     assert lib.tt_int4_codes_bytes(17, 33) == 2 * 2 * 256  # two tiles of 16 rows, two 32-column blocks
     assert lib.tt_int4_scales_bytes(17, 33, 32) == 2 * 1 * 16 * 4 * 2
     assert lib.tt_clip_ws_size(1) == lib.tt_clip_ws_size(1000) == 2048 * 8

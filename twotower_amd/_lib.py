@@ -20,7 +20,7 @@ HEADER_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__fil
 
 TT_IDS_I32, TT_IDS_I64 = 0, 1
 ELEM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum tt_elem_dtype
-TT_LOOKUP_DIRECT_TOKENS, TT_INT4_MAX_H = 4096, 4096  # twotower_amd.h
+TT_LOOKUP_DIRECT_TOKENS, TT_INT4_MAX_H = 8192, 4096  # twotower_amd.h
 TT_INBATCH_TAIL_ROWS, TT_INBATCH_MAX_PARTS = 64, 512  # twotower_amd.h
 TT_F32, TT_BF16, TT_BF16_SPLIT = 0, 1, 2
 TT_SCATTER_SORTED, TT_SCATTER_ATOMIC = 0, 1
@@ -92,9 +92,9 @@ _SIGNATURES = {
                                    ctypes.POINTER(AdamSlot), _c_int, _c_f64, _c_f64, _c_f64, _c_f64, _c_f64, _vp,
                                    _vp]),
     "tt_lookup_fwd": (_c_int, [_vp, _c_int, _c_i64, _c_int, _c_i64, _vp, _c_int, _c_i64, _c_f32, _vp, _c_int, _vp]),
-    "tt_lookup_plan_size": (_c_sz, [_c_i64, _c_i64]),
+    "tt_lookup_plan_size": (_c_sz, [_c_i64, _c_i64, _c_int, _c_int]),
     "tt_lookup_plan": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_sz, _vp]),
-    "tt_lookup_bwd_ws_size": (_c_sz, [_c_i64, _c_int]),
+    "tt_lookup_bwd_ws_size": (_c_sz, [_c_i64, _c_int, _c_int]),
     "tt_lookup_bwd": (_c_int, [_vp, _c_int, _vp, _c_int, _c_i64, _c_i64, _c_int, _c_i64, _c_f32, _vp, _c_int, _vp,
                                _c_sz, _vp, _c_sz, _vp]),
     "tt_preference_fwd": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_int, _vp,

@@ -9,8 +9,10 @@
 // without the writes, and 152-161 for 1 to 16 tokens in flight, stores past the caches or not), sort 40 us, tiles
 // 70 us (344 MB, 4.9 TB/s), joins and empty rows 42 us (148 MB); a 4 GiB copy runs at 4.8 TB/s.  The backward needs each
 // row's tokens together: a long call sorts them (the bags' stable counting sort, token_plan_build), a short one
-// lets every workgroup pick the tokens of its own rows from the ids.
+// finds them among the ids in LDS.
 #include "common.hpp"
+
+#include <algorithm>
 
 namespace tt {
 namespace {
@@ -72,119 +74,224 @@ __global__ __launch_bounds__(kBlock) void lookup_fwd_kernel(const TW* __restrict
   }
 }
 
-// ---- gradient of a short call (n <= kDirectN): one launch, no workspace.  A workgroup owns R
-// consecutive rows; it reads all ids, keeps its own tokens in LDS in token order, and a wave per
-// row adds that row's tokens.  A row with more than kCoop tokens is shared by the workgroup's waves,
-// each adding the tokens of its part of the list, folded in wave order.  Its time grows with n V (every
-// workgroup reads all ids), the sorted form's hardly at all, and about kDirectN they meet (us, n = 1000 / 4000 /
-// 8000): 34 x 64 9 / 19 / 32 against 25 / 29 / 32; 2000 x 256 10 / 17 / 26 against 40 / 45 / 45; 50k x 128 21 / 40 /
-// 80 against 41 / 47 / 49; 200k x 256 47 / 80 / 150 against 71 / 79 / 80 (30 us of it the bytes of the gradient).
+// ---- gradient of a short call, in one launch: some workgroups write the rows without tokens, in the others a wave
+// per token writes the row of its id if it is the first of them.  A token workgroup holds the n ids in LDS; a wave
+// walks them in order, leaves at an earlier token of its id, and lists the later ones.  A short list is
+// added up by the wave, a long one by the whole workgroup (a wide row in chunks of columns, one after the other), the
+// parts folded in a fixed order.  Bound by the fill of the table where that is large (200k x 256, 1000 tokens: 29 us for
+// 205 MB), else by a chain of latencies: ids, walk, rows.
+// (Every workgroup owning rows, and reading all ids to find their tokens: 38 us there; at 4000 tokens 34 x 64 18, 30k x
+// 100 fp16 39, 200k x 256 79 us instead of the 15, 14 and 33 below.)
+//
+// Short is up to kDirectN tokens, fewer of rows wider than 1 KB or 192 accesses, whose long lists take as many
+// chunks: about there the sort is as fast (us, text-like ids, n = 4000 / 8000 / 12000; then sorted, 8000 / 12000):
+// 34 x 64 15 / 25 / 34, 31 / 34; 30k x 100 fp16 14 / 29 / 48, 48 / 49; 50k x 128 16 / 31 / 51, 48 / 49; 200k x 256 33 /
+// 50 / 70, 80 / 80; half the ids one row, 2000 x 256: 29 / 59 / 85, 51 / 53; 500 x 512 48 / 96, 51; 116 x 339 fp16 95 / 214, 78.
 constexpr int kDirectN = TT_LOOKUP_DIRECT_TOKENS;
+bool short_call(int64_t n, int E, int row_dtype) {
+  const int bytes = elem_bytes(row_dtype);
+  int vec = 16 / bytes;
+  while (E % vec) vec >>= 1;
+  return n * std::max(((int64_t)E * bytes + 1023) / 1024, ((int64_t)E / vec + 191) / 192) <= kDirectN;
+}
 constexpr int kDirectThreads = 512;
 constexpr int kDirectWaves = kDirectThreads / kWave;
-constexpr int kDirectRows = 64;
-constexpr int kCoop = 64;
+constexpr int kStrip = 4 * kWave;  // tokens that a wave looks at together
+constexpr int kZeroSpan = 1 << 16;  // rows of a workgroup that writes empty ones, at most
+constexpr int kLight = 32;  // tokens that a wave lists for itself
+static_assert(kDirectN <= 1 << 16, "a list names its tokens in 16 bits");
 
-// acc += the rows of dout named by list[beg, end) whose local row is r, in list order
-template <typename TO, int VEC>
-__device__ __forceinline__ void direct_add(const TO* __restrict__ dout, int E, int e, bool on,
-                                           const uint32_t* list, int beg, int end, int r, float (&acc)[VEC]) {
-  constexpr int U = 8;
-  const int lane = lane_id();
-  for (int b = beg; b < end; b += kWave) {
-    const uint32_t v = b + lane < end ? list[b + lane] : 0xffffffffu;
-    uint64_t m = __ballot((int)(v & 255u) == r);
-    while (m) {
-      int64_t tok[U];
+// acc += the rows of dout named by list[first], list[first + step], ... below `count`, column e on: U in
+// flight, past the end the last one again (loads under a condition of their own ran one by one)
+template <int U, typename TO, int VEC>
+__device__ __forceinline__ void list_add(const TO* __restrict__ dout, int E, int e, const uint16_t* list, int first,
+                                         int step, int count, float (&acc)[VEC]) {
+  for (int j = first; j < count; j += U * step) {
+    Elems<TO, VEC> x[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        tok[u] = m ? (int64_t)(__builtin_amdgcn_readlane((int)v, __builtin_ctzll(m)) >> 8) : -1;
-        m &= m - 1;  // (0 stays 0)
-      }
-      float x[U][VEC];  // (filled before the first is used: loaded and added under one condition they ran one by one)
+    for (int u = 0; u < U; ++u)
+      x[u] = *reinterpret_cast<const Elems<TO, VEC>*>(dout + (int64_t)list[min(j + u * step, count - 1)] * E + e);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) x[u][i] = 0.f;
-        if (on && tok[u] >= 0) load_elems<VEC>(dout + tok[u] * E + e, x[u]);
-      }
+      for (int i = 0; i < VEC; ++i) acc[i] += j + u * step < count ? (float)x[u].v[i] : 0.f;
+  }
+}
+
+// Which of 256 tokens (from `row` on, 4 a lane) have id r: any, and per lane the number of them before the
+// lane's own and a bit per own token.
+struct Matches {
+  uint32_t own;
+  int before, all;
+  __device__ __forceinline__ Matches(const int32_t* row, int r, int lane) {
+    const int4 v = *reinterpret_cast<const int4*>(row + 4 * lane);
+    own = (v.x == r) | (v.y == r) << 1 | (v.z == r) << 2 | (v.w == r) << 3;
+    before = all = 0;
+    if (!__ballot(own != 0)) return;
+    const uint64_t below = (uint64_t(1) << lane) - 1;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (tok[u] >= 0) {
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t m = __ballot(own >> j & 1);
+      before += __popcll(m & below);
+      all += __popcll(m);
+    }
+  }
+};
+
+// the sums of a wave's groups of 2^lg lanes, in every group
+template <int VEC>
+__device__ __forceinline__ void fold_groups(float (&acc)[VEC], int lg) {
+  for (int o = 1 << lg; o < kWave; o <<= 1) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) acc[i] += x[u][i];
-        }
+    for (int i = 0; i < VEC; ++i) acc[i] += __shfl_xor(acc[i], o);
+  }
+}
+
+// f(i, ids[i]) for every i < limit (-1 for i >= n), eight loads in flight
+template <typename F>
+__device__ __forceinline__ void each_id(const void* ids, bool wide, int n, int limit, F f) {
+  for (int i0 = threadIdx.x; i0 < limit; i0 += 8 * kDirectThreads) {
+    int64_t id[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) id[u] = i0 + u * kDirectThreads < n ? id_at(ids, wide, i0 + u * kDirectThreads) : -1;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i0 + u * kDirectThreads < limit) f(i0 + u * kDirectThreads, id[u]);
+  }
+}
+
+// Zeros in those of a workgroup's rows [lo, hi) that no token has (a bit per row in `mark`): EPU elements
+// of consecutive memory at a time, one by one where rows with and without tokens meet.
+template <int EPU, typename TW>
+__device__ __forceinline__ void zero_rows(const void* ids, bool wide, int n, int64_t lo, int64_t hi, int E, int64_t pad,
+                                          uint32_t* mark, TW* __restrict__ grad) {
+  const int rows = (int)(hi - lo);
+  for (int i = threadIdx.x; i < (rows + 31) / 32; i += kDirectThreads) mark[i] = 0;
+  __syncthreads();
+  each_id(ids, wide, n, n, [&](int, int64_t id) {
+    if (id >= lo && id < hi && id != pad) atomicOr(&mark[(id - lo) >> 5], 1u << ((id - lo) & 31));
+  });
+  __syncthreads();
+  auto marked = [&](int r) { return (mark[r >> 5] >> (r & 31) & 1) != 0; };
+  TW* base = grad + lo * E;
+  const int64_t total = (int64_t)rows * E, at0 = (int64_t)threadIdx.x * EPU;
+  const int rows_on = kDirectThreads * EPU / E, cols_on = kDirectThreads * EPU % E;
+  int r = (int)(at0 / E), c = (int)(at0 % E);
+  for (int64_t at = at0; at < total; at += kDirectThreads * EPU) {
+    const int over = c + EPU - E;  // elements of the next row (E >= EPU, or EPU = 1)
+    const bool m0 = marked(r), m1 = over > 0 && r + 1 < rows ? marked(r + 1) : m0;
+    if (!m0 && !m1 && at + EPU <= total) {
+      const float zero[EPU] = {};
+      store_elems<EPU>(base + at, zero);
+    } else if (!m0 || !m1) {
+#pragma unroll
+      for (int j = 0; j < EPU; ++j)
+        if (at + j < total && !(c + j < E ? m0 : m1)) base[at + j] = (TW)0.f;
+    }
+    r += rows_on;
+    c += cols_on;
+    if (c >= E) {
+      c -= E;
+      ++r;
     }
   }
 }
 
+// workgroups [0, token_blocks): the tokens; the others: the rows without any, zero_span rows each
 template <typename TO, typename TW, int VEC>
 __global__ __launch_bounds__(kDirectThreads) void lookup_grad_direct_kernel(
-    const TO* __restrict__ dout, const void* __restrict__ ids, bool wide, int n, int64_t V, int E, int R, int64_t pad,
-    float scale, TW* __restrict__ grad) {
-  __shared__ uint32_t list[kDirectN];  // token << 8 | local row
-  __shared__ int cnt[kDirectRows];
-  __shared__ int wcnt[kDirectWaves];
-  __shared__ float part[kDirectWaves][kWave * VEC];
-  const int lane = lane_id(), w = threadIdx.x >> 6;
-  const int64_t r0 = block_index() * R;
-  if (r0 >= V) return;
-  const int rows = (int)(V - r0 < R ? V - r0 : R);
-  if (threadIdx.x < kDirectRows) cnt[threadIdx.x] = 0;
-  int m = 0;  // tokens kept so far (the same in every thread)
-  __syncthreads();
-  for (int base = 0; base < n; base += kDirectThreads) {
-    const int i = base + threadIdx.x;
-    const int64_t id = i < n ? id_at(ids, wide, i) : -1;
-    const bool mine = id >= r0 && id < r0 + rows && id != pad;
-    const uint64_t b = __ballot(mine);
-    if (lane == 0) wcnt[w] = __popcll(b);
-    __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int k = 0; k < kDirectWaves; ++k) {
-      before += k < w ? wcnt[k] : 0;
-      all += wcnt[k];
-    }
-    if (mine) {
-      const int local = (int)(id - r0);
-      list[m + before + __popcll(b & ((uint64_t(1) << lane) - 1))] = (uint32_t)i << 8 | (uint32_t)local;
-      atomicAdd(&cnt[local], 1);
-    }
-    m += all;
-    __syncthreads();
+    const TO* __restrict__ dout, const void* __restrict__ ids, bool wide, int n, int64_t V, int E, int lg, int64_t pad,
+    float scale, TW* __restrict__ grad, int token_blocks, int zero_span) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  if ((int)blockIdx.x >= token_blocks) {
+    constexpr int kEpu = 16 / sizeof(TW);
+    const int64_t lo = (int64_t)((int)blockIdx.x - token_blocks) * zero_span, hi = min(lo + zero_span, V);
+    uint32_t* mark = reinterpret_cast<uint32_t*>(smem);
+    if (E >= kEpu && (reinterpret_cast<size_t>(grad) & 15) == 0) zero_rows<kEpu>(ids, wide, n, lo, hi, E, pad, mark, grad);
+    else zero_rows<1>(ids, wide, n, lo, hi, E, pad, mark, grad);
+    return;
   }
-  for (int r = w; r < rows; r += kDirectWaves) {
-    const int c = cnt[r];
-    if (c > kCoop) continue;
-    for (int e0 = 0; e0 < E; e0 += kWave * VEC) {
-      const int e = e0 + lane * VEC;
+  __shared__ uint16_t own[kDirectWaves][kLight];
+  __shared__ int heavy[kDirectWaves], wcnt[kDirectWaves];
+  const int np = (n + kStrip - 1) / kStrip * kStrip, strips = np / kStrip;
+  float(*part)[kWave * VEC] = reinterpret_cast<float(*)[kWave * VEC]>(smem);          // [kDirectWaves - 1]
+  int32_t* row = reinterpret_cast<int32_t*>(smem + (kDirectWaves - 1) * kWave * VEC * 4);  // [np], -1: no token
+  uint16_t* list = reinterpret_cast<uint16_t*>(row + np);                              // [np]
+  const int lane = lane_id(), w = threadIdx.x >> 6, c = lane & ((1 << lg) - 1), g = lane >> lg, groups = kWave >> lg;
+  const int chunk = VEC << lg, chunks = (E + chunk - 1) / chunk;
+  each_id(ids, wide, n, np, [&](int i, int64_t id) { row[i] = id >= 0 && id < V && id != pad ? (int32_t)id : -1; });
+  __syncthreads();
+  // consecutive tokens go to different workgroups: the frequent ids' first ones, all near the start, do too
+  const int t = w * token_blocks + (int)blockIdx.x;
+  const int r = t < n ? __builtin_amdgcn_readfirstlane(row[t]) : -1;
+  int count = 0;
+  if (r >= 0)
+    for (int b = 0; b < np; b += kStrip) {
+      const Matches m(row + b, r, lane);
+      if (!m.all) continue;
+      int at = count + m.before;
+      for (uint32_t o = m.own; o; o &= o - 1, ++at)
+        if (at < kLight) own[w][at] = (uint16_t)(b + 4 * lane + __builtin_ctz(o));
+      if (count == 0 && __ballot(m.before == 0 && m.own && b + 4 * lane + __builtin_ctz(m.own) < t)) break;
+      count += m.all;
+    }
+  const bool light = count <= kLight && count * chunks <= 2 * kLight;
+  if (lane == 0) heavy[w] = light ? -1 : r;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (own[w] is the wave's alone)
+  if (count > 0 && light)
+    for (int e = c * VEC; e < chunks * chunk; e += chunk) {
       float acc[VEC] = {};
-      if (c) direct_add<TO, VEC>(dout, E, e, e < E, list, 0, m, r, acc);
+      if (e < E) list_add<4>(dout, E, e, own[w], g, groups, count, acc);
+      fold_groups<VEC>(acc, lg);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) acc[i] *= scale;
-      if (e < E) store_elems<VEC>(grad + (r0 + r) * E + e, acc);
+      if (g == 0 && e < E) store_elems<VEC>(grad + (int64_t)r * E + e, acc);
     }
-  }
-  const int share = (m + kDirectWaves - 1) / kDirectWaves;
-  for (int r = 0; r < rows; ++r) {
-    if (cnt[r] <= kCoop) continue;
-    for (int e0 = 0; e0 < E; e0 += kWave * VEC) {
-      const int e = e0 + lane * VEC;
+  __syncthreads();
+  // the workgroup's long lists: `parts` waves to a column chunk
+  const int parts = chunks >= kDirectWaves ? 1 : kDirectWaves / chunks, step = kDirectWaves / parts;
+  const int per = (strips + kDirectWaves - 1) / kDirectWaves;
+  const int b0 = w * per, b1 = min(b0 + per, strips);
+  for (int k = 0; k < kDirectWaves; ++k) {
+    const int hr = heavy[k];
+    if (hr < 0) continue;
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) mine += Matches(row + b * kStrip, hr, lane).all;
+    if (lane == 0) wcnt[w] = mine;
+    __syncthreads();
+    int at = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kDirectWaves; ++i) {
+      at += i < w ? wcnt[i] : 0;
+      all += wcnt[i];
+    }
+    for (int b = b0; b < b1; ++b) {
+      const Matches m(row + b * kStrip, hr, lane);
+      int to = at + m.before;
+      for (uint32_t o = m.own; o; o &= o - 1, ++to) list[to] = (uint16_t)(b * kStrip + 4 * lane + __builtin_ctz(o));
+      at += m.all;
+    }
+    __syncthreads();
+    const int p = w % parts;
+    for (int k0 = 0; k0 < chunks; k0 += step) {
+      const int e = (k0 + w / parts) * chunk + c * VEC;
+      const bool on = w < parts * step && e < E;
       float acc[VEC] = {};
-      direct_add<TO, VEC>(dout, E, e, e < E, list, min(w * share, m), min((w + 1) * share, m), r, acc);
+      if (on) list_add<8>(dout, E, e, list, p * groups + g, parts * groups, all, acc);
+      fold_groups<VEC>(acc, lg);
+      if (on && p > 0) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) part[w][lane * VEC + i] = acc[i];
+        for (int i = 0; i < VEC; ++i) part[w - 1][lane * VEC + i] = acc[i];
+      }
       __syncthreads();
-      if (w == 0) {
+      if (on && p == 0 && g == 0) {
+        for (int q = 1; q < parts; ++q) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          float a = part[0][lane * VEC + i];
-#pragma unroll
-          for (int k = 1; k < kDirectWaves; ++k) a += part[k][lane * VEC + i];
-          acc[i] = a * scale;
+          for (int i = 0; i < VEC; ++i) acc[i] += part[w + q - 1][lane * VEC + i];
         }
-        if (e < E) store_elems<VEC>(grad + (r0 + r) * E + e, acc);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] *= scale;
+        store_elems<VEC>(grad + (int64_t)hr * E + e, acc);
       }
       __syncthreads();
     }
@@ -407,22 +514,32 @@ int launch_bwd(const void* dout, const void* ids, int ids_dtype, int64_t n, int6
   if (sizeof(TW) == 4 && sizeof(TO) == 4 && vec > 4) vec = 4;
   const TO* d = static_cast<const TO*>(dout);
   TW* g = static_cast<TW*>(grad);
-  if (n <= kDirectN) {
-    // few rows each spread the frequent (low) ids over workgroups and give a wave one or two rows; at most
-    // kDirectRows, so that the ids are read V / 64 times at most (30k x 100, 1073 text-like tokens: 15 us, V / 1024
-    // rows each 30 us; 200k x 256, 4096 tokens: 38 and 39 us)
-    int64_t R = V / 4096;
-    R = R < 1 ? 1 : R > kDirectRows ? kDirectRows : R;
-    const dim3 grid = wide_grid((V + R - 1) / R), block(kDirectThreads);
-#define TT_LD(VV) \
-  case VV: lookup_grad_direct_kernel<TO, TW, VV><<<grid, block, 0, s>>>(d, ids, ids_dtype == TT_IDS_I64, (int)n, V, E, (int)R, pad, scale, g); break;
+  const int lg = row_lanes_log2(E, vec);
+  if (plan == nullptr) {
+    const int64_t np = (n + kStrip - 1) / kStrip * kStrip, bytes = V * E * (int64_t)sizeof(TW);
+    const size_t need = (size_t)(kDirectWaves - 1) * kWave * vec * 4 + (size_t)np * 6;
+    const size_t lds = std::max<size_t>(need, kZeroSpan / 8);
+    // the empty rows' workgroups: 64 KB each or more (up to two to a CU), and a bit a row in LDS
+    int64_t zero = std::min<int64_t>((bytes + (1 << 16) - 1) >> 16, 2048);
+    const int64_t span = std::min<int64_t>(((V + zero - 1) / zero + 7) & ~7, kZeroSpan);  // (whole 16 bytes)
+    zero = (V + span - 1) / span;
+    const int tokens = (int)((n + kDirectWaves - 1) / kDirectWaves);
+    const dim3 grid((unsigned)(tokens + zero)), block(kDirectThreads);
+#define TT_LD(VV)                                                                                                     \
+  case VV: {                                                                                                          \
+    auto kernel = lookup_grad_direct_kernel<TO, TW, VV>;                                                              \
+    if (lds > 60 * 1024)                                                                                              \
+      TT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,    \
+                                 (int)lds), "lookup_grad_direct LDS");                                                \
+    kernel<<<grid, block, lds, s>>>(d, ids, ids_dtype == TT_IDS_I64, (int)n, V, E, lg, pad, scale, g, tokens, (int)span); \
+    break;                                                                                                            \
+  }
     switch (vec) { TT_LD(8) TT_LD(4) TT_LD(2) default: TT_LD(1) }
 #undef TT_LD
     TT_LAUNCH_CHECK("lookup_grad_direct");
     return TT_OK;
   }
   const TokenPlan p = token_plan_view(const_cast<void*>(plan), n, V);
-  const int lg = row_lanes_log2(E, vec);
   const int64_t tiles = (n + kTile - 1) / kTile, supers = tiles / kSuper, per = kBlock >> lg;
   float *head = ws, *tail = head + tiles * E, *sup = tail + tiles * E;
   auto grid = [&](int64_t groups) { return dim3((unsigned)((groups + per - 1) / per)); };
@@ -480,19 +597,19 @@ extern "C" int tt_lookup_fwd(const void* table, int table_dtype, int64_t V, int 
 #undef TT_CALL
 }
 
-extern "C" size_t tt_lookup_plan_size(int64_t n, int64_t V) {
-  return n <= kDirectN || V <= 0 ? 0 : token_plan_bytes(n, V);
+extern "C" size_t tt_lookup_plan_size(int64_t n, int64_t V, int E, int dout_dtype) {
+  return n < 0 || V <= 0 || short_call(n, E, dout_dtype) ? 0 : token_plan_bytes(n, V);
 }
 
 extern "C" int tt_lookup_plan(const void* ids, int ids_dtype, int64_t n, int64_t V, int64_t padding_idx, void* plan,
                               size_t plan_bytes, tt_stream_t stream) {
   if (int rc = check_lookup(n, V, 1, ids, ids_dtype, TT_E_F32, TT_E_F32)) return rc;
-  if (n <= kDirectN) return TT_OK;
+  if (plan_bytes == 0) return TT_OK;  // a short call's
   return token_plan_build(ids, ids_dtype, n, V, padding_idx, plan, plan_bytes, reinterpret_cast<hipStream_t>(stream));
 }
 
-extern "C" size_t tt_lookup_bwd_ws_size(int64_t n, int E) {
-  if (n <= kDirectN || E <= 0) return 0;
+extern "C" size_t tt_lookup_bwd_ws_size(int64_t n, int E, int dout_dtype) {
+  if (n < 0 || E <= 0 || short_call(n, E, dout_dtype)) return 0;
   const size_t tiles = (size_t)(n + kTile - 1) / kTile;
   return (2 * tiles + tiles / kSuper) * (size_t)E * sizeof(float);
 }
@@ -502,15 +619,17 @@ extern "C" int tt_lookup_bwd(const void* dout, int dout_dtype, const void* ids, 
                              size_t plan_bytes, void* ws, size_t ws_bytes, tt_stream_t stream) {
   if (int rc = check_lookup(n, V, E, ids, ids_dtype, grad_dtype, dout_dtype)) return rc;
   TT_REQUIRE(grad && (dout || n == 0), "null pointer");
-  if (n > kDirectN) {
+  const bool direct = short_call(n, E, dout_dtype);
+  if (!direct) {
     TT_REQUIRE(plan && plan_bytes >= token_plan_bytes(n, V), "plan too small: need %zu have %zu",
                token_plan_bytes(n, V), plan_bytes);
-    TT_REQUIRE(ws && ws_bytes >= tt_lookup_bwd_ws_size(n, E) && reinterpret_cast<size_t>(ws) % 16 == 0,
-               "workspace too small: need %zu have %zu", tt_lookup_bwd_ws_size(n, E), ws_bytes);
+    TT_REQUIRE(ws && ws_bytes >= tt_lookup_bwd_ws_size(n, E, dout_dtype) && reinterpret_cast<size_t>(ws) % 16 == 0,
+               "workspace too small: need %zu have %zu", tt_lookup_bwd_ws_size(n, E, dout_dtype), ws_bytes);
   }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define TT_CALL(TW, TO) \
-  (launch_bwd<TW, TO>(dout, ids, ids_dtype, n, V, E, padding_idx, scale, grad, plan, static_cast<float*>(ws), s))
+  (launch_bwd<TW, TO>(dout, ids, ids_dtype, n, V, E, padding_idx, scale, grad, direct ? nullptr : plan,              \
+                      static_cast<float*>(ws), s))
   TT_LOOKUP_TYPES(grad_dtype, dout_dtype, TT_CALL);
 #undef TT_CALL
 }

@@ -163,14 +163,13 @@ Tensor lookup_grad(const Tensor& grad_rows, const Tensor& ids, const LookupArgs&
   const int64_t n = ids.numel();
   const Tensor grad = at::empty({a.V, a.E}, dout.options().dtype(a.table));
   Tensor plan, ws;
-  size_t plan_bytes = 0, ws_bytes = 0;
-  if (n > TT_LOOKUP_DIRECT_TOKENS) {
+  const size_t plan_bytes = abi.lookup_plan_size(n, a.V, (int)a.E, elem_code(dout));
+  const size_t ws_bytes = abi.lookup_bwd_ws_size(n, (int)a.E, elem_code(dout));
+  if (plan_bytes) {  // (a short call takes neither)
     // Sorted here, not beside the forward on a side stream: the gather fills the memory system and every CU,
     // and the sort beside it ended no sooner (forward and backward back to back 352 against 344 us at
     // 8192 x 64 tokens).  Buffers per call, not shared: two captured graphs, or streams, may run their
     // backwards at once.
-    plan_bytes = abi.lookup_plan_size(n, a.V);
-    ws_bytes = abi.lookup_bwd_ws_size(n, (int)a.E);
     plan = bytes_like(dout, plan_bytes);
     ws = bytes_like(dout, ws_bytes);
     launch(dout, "tt_lookup_plan", abi.lookup_plan, as<const void>(ids), ids_code(ids), n, a.V, a.pad, as<void>(plan),

@@ -307,6 +307,9 @@ __global__ __launch_bounds__(kDirectThreads) void lookup_grad_direct_kernel(
 // 1.7 TB/s, 132 us with the frequent rows' tiles at 8192 x 64 text-like tokens, 200k rows of 256 floats.)
 constexpr int kTile = 32;
 constexpr int kSuper = 32;
+// a group's columns of a row: the grid's z chunks of them run side by side (1051 x 306 bf16, 38,318 tokens: tiles and
+// joins 12 and 10 us, chunk after chunk in one group 19 and 22)
+#define TT_COLUMNS(e) for (int64_t e = (((int64_t)blockIdx.z << lg) + c) * VEC; e < E; e += (int64_t)(VEC << lg) * gridDim.z)
 
 template <typename TO, typename TW, int VEC>
 __global__ __launch_bounds__(kBlock) void lookup_tile_sum_kernel(TokenPlan p, const TO* __restrict__ dout, int E,
@@ -320,7 +323,7 @@ __global__ __launch_bounds__(kBlock) void lookup_tile_sum_kernel(TokenPlan p, co
   const int lo = (int)(tile * kTile), hi = min(lo + kTile, n);
   const uint32_t first = p.keys[lo], last = p.keys[hi - 1];
   const bool before = lo > 0 && p.keys[lo - 1] == first, after = hi < n && p.keys[hi] == last;
-  for (int e = c * VEC; e < E; e += VEC << lg) {
+  TT_COLUMNS(e) {
     float acc[VEC] = {};
     uint32_t cur = first;
     auto flush = [&](bool end) {
@@ -374,7 +377,7 @@ __global__ __launch_bounds__(kBlock) void lookup_tile_sum_kernel(TokenPlan p, co
 
 // sum of rows [beg, end) of part: U sums (row k to sum k % U), folded in order
 template <int VEC>
-__device__ __forceinline__ void part_add(const float* __restrict__ part, int E, int e, int64_t beg, int64_t end,
+__device__ __forceinline__ void part_add(const float* __restrict__ part, int E, int64_t e, int64_t beg, int64_t end,
                                          float (&acc)[VEC]) {
   constexpr int U = 4;
   float s[U][VEC];
@@ -409,7 +412,7 @@ __global__ __launch_bounds__(kBlock) void lookup_super_sum_kernel(TokenPlan p, c
   const int c = threadIdx.x & ((1 << lg) - 1);
   const int64_t lo = j * kSuper * kTile, hi = lo + kSuper * kTile;
   if (lo == 0 || hi > *p.count || p.keys[lo - 1] != p.keys[hi - 1]) return;
-  for (int e = c * VEC; e < E; e += VEC << lg) {
+  TT_COLUMNS(e) {
     float acc[VEC] = {};
     part_add<VEC>(head, E, e, j * kSuper, (j + 1) * kSuper, acc);
     store_elems<VEC>(sup + j * E + e, acc);
@@ -451,7 +454,7 @@ __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, in
     const float zero[VEC] = {};
     for (int i = lane >> lg; i < kZeroRows; i += groups)
       if (empty >> i & 1)
-        for (int e = c * VEC; e < E; e += VEC << lg) store_elems_nt<VEC>(grad + (r0 + i) * E + e, zero);
+        TT_COLUMNS(e) store_elems_nt<VEC>(grad + (r0 + i) * E + e, zero);
     return;
   }
   const int64_t t0 = (block_index() * kBlock + threadIdx.x) >> lg;
@@ -465,7 +468,7 @@ __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, in
   // its heads t0 + 1 .. t1.  Super-tile j is the row's if the row began before it and holds its last token.
   const int64_t s0 = (t0 + kSuper) / kSuper, s1 = max((int64_t)end / (kSuper * kTile), s0);
   const bool whole = s1 > s0;
-  for (int e = c * VEC; e < E; e += VEC << lg) {
+  TT_COLUMNS(e) {
     float acc[VEC];
     load_elems<VEC>(tail + t0 * E + e, acc);
     for (int k = 0; k < 3; ++k) {  // heads, super-tiles, heads
@@ -478,6 +481,8 @@ __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, in
     store_elems_nt<VEC>(grad + (int64_t)r * E + e, acc);
   }
 }
+
+#undef TT_COLUMNS
 
 template <typename TW, typename TO>
 int launch_fwd(const void* table, int64_t V, int E, int64_t ld, const void* ids, bool wide, int64_t n, float scale,
@@ -542,9 +547,12 @@ int launch_bwd(const void* dout, const void* ids, int ids_dtype, int64_t n, int6
   const TokenPlan p = token_plan_view(const_cast<void*>(plan), n, V);
   const int64_t tiles = (n + kTile - 1) / kTile, supers = tiles / kSuper, per = kBlock >> lg;
   float *head = ws, *tail = head + tiles * E, *sup = tail + tiles * E;
-  auto grid = [&](int64_t groups) { return dim3((unsigned)((groups + per - 1) / per)); };
+  const unsigned chunks = (unsigned)std::min<int64_t>(((int64_t)E + (vec << lg) - 1) / (vec << lg), 65535);
+  auto grid = [&](int64_t groups) { return dim3((unsigned)((groups + per - 1) / per), 1, chunks); };
   const int64_t zero_rows = (int64_t)kWavesPerBlock * kZeroRows;
-  const dim3 block(kBlock), join = wide_grid(grid(tiles).x + (V + zero_rows - 1) / zero_rows);
+  const dim3 block(kBlock);
+  dim3 join = wide_grid(grid(tiles).x + (V + zero_rows - 1) / zero_rows);
+  join.z = chunks;
 #define TT_LS(VV)                                                                                                  \
   case VV:                                                                                                         \
     lookup_tile_sum_kernel<TO, TW, VV><<<grid(tiles), block, 0, s>>>(p, d, E, scale, g, lg, head, tail);           \

@@ -11,11 +11,11 @@
 //   dq_i = G sum_k c_ik (p_i - n_ik),   dp_i = G (sum_k c_ik) q_i,   dn_ik = -G c_ik q_i.
 // A masked pair is not read, counts nothing and gets a zero gradient; no valid pair: loss 0.
 // Row passes, bound by their bytes (forward: q, p, n once; backward: again, and the gradients): 8192 x 256 fp32,
-// one negative: forward 9.8 us + 4.1 for the mean (25 MB), backward 9.2 (50 MB, 5.5 TB/s); bf16, four
-// negatives: 9.0 + 4.1 and 9.4 us.  A group of lanes takes a query and up to kKT of its pairs at once: q and p are
+// one negative: forward 9.0 us + 3.0 for the mean (25 MB), backward 9.0 (50 MB, 5.6 TB/s); bf16, four
+// negatives: 8.8 + 3.0 and 9.4 us.  A group of lanes takes a query and up to kKT of its pairs at once: q and p are
 // then read once however many pairs there are up to that, and a row's loads are all in flight together.
 // The differences p - n are formed before the products, so two close documents lose nothing to
-// cancellation.  One workgroup does all of a small batch, the mean included (64 x 128: 5.9 us, one launch).
+// cancellation.  One workgroup does all of a small batch, the mean included (64 x 128: 5.6 us, one launch).
 #include "common.hpp"
 
 namespace tt {
@@ -110,21 +110,25 @@ __device__ __forceinline__ void pref_row(const PrefArgs& a, const T* __restrict_
 
 // loss = sum / max(count, 1) and 1 / max(count, 1), the sums folded in a fixed order.
 __device__ __forceinline__ void pref_finish(double sum, double count, float* loss, float* inv_pairs) {
-  __shared__ double ss[kFinish], sc[kFinish];
+  __shared__ double ss[kFinish / kWave], sc[kFinish / kWave];
   const int t = threadIdx.x;
-  ss[t] = sum;
-  sc[t] = count;
-  __syncthreads();
-  for (int w = kFinish / 2; w > 0; w >>= 1) {
-    if (t < w) {
-      ss[t] += ss[t + w];
-      sc[t] += sc[t + w];
-    }
-    __syncthreads();
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    sum += __shfl_xor(sum, o);
+    count += __shfl_xor(count, o);
   }
+  if (lane_id() == 0) {
+    ss[t >> 6] = sum;
+    sc[t >> 6] = count;
+  }
+  __syncthreads();
   if (t == 0) {
-    const double inv = 1.0 / (sc[0] > 1.0 ? sc[0] : 1.0);
-    *loss = (float)(ss[0] * inv);
+    for (int w = 1; w < kFinish / kWave; ++w) {
+      sum += ss[w];
+      count += sc[w];
+    }
+    const double inv = 1.0 / (count > 1.0 ? count : 1.0);
+    *loss = (float)(sum * inv);
     *inv_pairs = (float)inv;
   }
 }
@@ -171,9 +175,21 @@ __global__ __launch_bounds__(kFinish) void pref_mean_kernel(const float* __restr
                                                             const int32_t* __restrict__ counts, int64_t B,
                                                             float* __restrict__ loss, float* __restrict__ inv_pairs) {
   double s = 0.0, c = 0.0;
-  for (int64_t i = threadIdx.x; i < B; i += kFinish) {
-    s += (double)rows[i];
-    c += (double)counts[i];
+  constexpr int U = 8;  // loads in flight (one at a time: 4.1 us instead of 3.0 for 8192 rows)
+  for (int64_t i = threadIdx.x; i < B; i += U * kFinish) {
+    float x[U];
+    int32_t n[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = min(i + u * kFinish, B - 1);
+      x[u] = rows[k];
+      n[u] = counts[k];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      s += i + u * kFinish < B ? (double)x[u] : 0.0;
+      c += i + u * kFinish < B ? (double)n[u] : 0.0;
+    }
   }
   pref_finish(s, c, loss, inv_pairs);
 }

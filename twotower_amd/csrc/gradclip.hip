@@ -10,16 +10,17 @@
 // nor underflows before its own rounding to 32 bits, and the vector units have room for it beside
 // the loads (added in 32 bits the pass took 54 instead of 57 us).  All sums run in a fixed order (no atomics).
 //
-// 51.3M fp32 elements into another buffer: norm 38 us (205 MB, 5.4 TB/s), scaling 67 us (410 MB, 6.1 TB/s, its
+// 51.3M fp32 elements into another buffer: norm 38 us (205 MB, 5.4 TB/s), scaling 65 us (410 MB, 6.3 TB/s, its
 // reads partly cached; a 4 GiB copy runs at 4.8 TB/s).  16,384-element chunks on 1024 workgroups took 57 and
-// 70 us, and results kept in the caches 50 (the next norm's reads then wait for their write-back) and 72.
+// 70 us, and results kept in the caches 50 (the next norm's reads then wait for their write-back) and 72.  Few
+// elements: 131,584 in 4 tensors 4.0 + 4.5 us (chunks of 8192 4.7 + 4.9), 1.7M of three types 4.5 + 7.8 (5.3 + 12.6).
 #include "common.hpp"
 
 namespace tt {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kChunk = 8192;        // elements per chunk
+constexpr int kChunk = 8192, kMinChunk = 2048;  // elements per chunk
 constexpr int kMaxParts = 2048;     // partial norms of all launches together
 constexpr int kNormBlocks = 2048;   // workgroups (= partials) of one norm launch
 constexpr int kScaleBlocks = 2048;
@@ -30,7 +31,7 @@ struct ClipList {
   int64_t n[TT_CLIP_MAX_TENSORS];
   int32_t first[TT_CLIP_MAX_TENSORS + 1];  // first chunk of each tensor
   uint8_t type[TT_CLIP_MAX_TENSORS];       // src type | dst type << 2
-  int count;
+  int count, chunk;                        // tensors; elements per chunk
 };
 
 __device__ __forceinline__ int tensor_of(const ClipList& l, int chunk) {
@@ -113,9 +114,9 @@ __global__ __launch_bounds__(kBlock) void clip_norm_kernel(ClipList l, double* _
   const int chunks = l.first[l.count];
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
     const int t = tensor_of(l, c);
-    const int64_t at = (int64_t)(c - l.first[t]) * kChunk;
+    const int64_t at = (int64_t)(c - l.first[t]) * l.chunk;
     const int64_t left = l.n[t] - at;
-    const int n = (int)(left < kChunk ? left : kChunk);
+    const int n = (int)(left < l.chunk ? left : l.chunk);
     const int ty = l.type[t] & 3;
     double a;
     if (ty == TT_E_F32) a = norm_chunk<float, INF>(static_cast<const float*>(l.src[t]) + at, n);
@@ -129,8 +130,15 @@ __global__ __launch_bounds__(kBlock) void clip_norm_kernel(ClipList l, double* _
 
 template <bool INF>
 __device__ __forceinline__ double joined_norm(const double* __restrict__ parts, int np) {
+  constexpr int U = kMaxParts / kBlock;  // loads in flight: all of them, where kMaxParts is not exceeded
   double a = 0.0;
-  for (int i = threadIdx.x; i < np; i += kBlock) a = norm_join<INF>(a, parts[i]);
+  for (int i = threadIdx.x; i < np; i += U * kBlock) {
+    double x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = parts[min(i + u * kBlock, np - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) a = i + u * kBlock < np ? norm_join<INF>(a, x[u]) : a;
+  }
   a = block_join<INF>(a);
   return INF ? a : __builtin_sqrt(a);
 }
@@ -195,9 +203,9 @@ __global__ __launch_bounds__(kBlock) void clip_scale_kernel(ClipList l, const do
   const int chunks = l.first[l.count];
   for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
     const int t = tensor_of(l, c);
-    const int64_t at = (int64_t)(c - l.first[t]) * kChunk;
+    const int64_t at = (int64_t)(c - l.first[t]) * l.chunk;
     const int64_t left = l.n[t] - at;
-    const int n = (int)(left < kChunk ? left : kChunk);
+    const int n = (int)(left < l.chunk ? left : l.chunk);
     const int ty = l.type[t];
     if (coef.a == 1.f && coef.b == 1.f && l.src[t] == l.dst[t]) continue;  // in place and not clipped: nothing changes
 #define TT_SC(TS, TD) scale_chunk<TS, TD>(static_cast<const TS*>(l.src[t]) + at, static_cast<TD*>(l.dst[t]) + at, n, coef)
@@ -223,14 +231,18 @@ struct ClipCall {
 // tensors [at, at + TT_CLIP_MAX_TENSORS) of the call as one launch's list
 void fill_list(ClipList& l, const ClipCall& t, int at) {
   const int m = t.count - at < TT_CLIP_MAX_TENSORS ? t.count - at : TT_CLIP_MAX_TENSORS;
-  int64_t chunk = 0;
+  // smaller chunks where there are few: a workgroup's time is then its latencies
+  int64_t total = 0, chunk = 0;
+  for (int i = 0; i < m; ++i) total += t.n[at + i];
+  l.chunk = kChunk;
+  while (l.chunk > kMinChunk && total < (int64_t)l.chunk * 1024) l.chunk >>= 1;
   for (int i = 0; i < m; ++i) {
     l.src[i] = t.src[at + i];
     l.dst[i] = t.dst[at + i];
     l.n[i] = t.n[at + i];
     l.type[i] = (uint8_t)(t.src_dtype[at + i] | t.dst_dtype[at + i] << 2);
     l.first[i] = (int32_t)chunk;
-    chunk += (t.n[at + i] + kChunk - 1) / kChunk;
+    chunk += (t.n[at + i] + l.chunk - 1) / l.chunk;
   }
   l.first[m] = (int32_t)chunk;
   l.count = m;

@@ -1,4 +1,5 @@
-"""ctypes binding of libtwotower_amd.so (the C ABI declared in include/twotower_amd.h).
+"""ctypes binding of libtwotower_amd.so (the C ABI declared in include/twotower_amd.h), and the module of the
+operators' eager calls (csrc/nodes.cpp).
 
 The product path has no fallback: if the shared library is missing, or a tensor is not on a
 GPU, the call raises.  Torch only supplies device memory and the current HIP stream.

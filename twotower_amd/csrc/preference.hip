@@ -11,11 +11,11 @@
 //   dq_i = G sum_k c_ik (p_i - n_ik),   dp_i = G (sum_k c_ik) q_i,   dn_ik = -G c_ik q_i.
 // A masked pair is not read, counts nothing and gets a zero gradient; no valid pair: loss 0.
 // Row passes, bound by their bytes (forward: q, p, n once; backward: again, and the gradients): 8192 x 256 fp32,
-// one negative: forward 9.0 us + 3.0 for the mean (25 MB), backward 9.0 (50 MB, 5.6 TB/s); bf16, four
-// negatives: 8.8 + 3.0 and 9.4 us.  A group of lanes takes a query and up to kKT of its pairs at once: q and p are
+// one negative: forward 7.9 us + 3.0 for the mean (25 MB), backward 9.0 (50 MB, 5.6 TB/s); bf16, four
+// negatives: 7.5 + 3.0 and 9.3 us.  A group of lanes takes a query and up to kKT of its pairs at once: q and p are
 // then read once however many pairs there are up to that, and a row's loads are all in flight together.
 // The differences p - n are formed before the products, so two close documents lose nothing to
-// cancellation.  One workgroup does all of a small batch, the mean included (64 x 128: 5.6 us, one launch).
+// cancellation.  One workgroup does all of a small batch, the mean included (64 x 128: 5.0 us, one launch).
 #include "common.hpp"
 
 namespace tt {
@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kFinish = 1024;  // the one workgroup that joins the rows
-constexpr int kKT = 4;         // pairs of a query in flight
+constexpr int kKT = 4;         // pairs of a query in flight (a query with one has a form of its own)
 
 enum { kSigmoid = 0, kSquared = 1 };
 
@@ -56,55 +56,76 @@ __device__ __forceinline__ void pair_loss(const PrefArgs& a, float h, float& los
 }
 
 // One group of 2^lg lanes: query i's pairs.  Returns (in every lane) the row's loss sum and count.
-template <typename T, int VEC>
+template <typename T, int VEC, int KT>
 __device__ __forceinline__ void pref_row(const PrefArgs& a, const T* __restrict__ q, const T* __restrict__ p,
                                          const T* __restrict__ n, int64_t i, int c, int lg, float* __restrict__ coef,
                                          float* __restrict__ margins, float& sum, int& count) {
   sum = 0.f;
   count = 0;
   const T *qi = q + i * a.ldq, *pi = p + i * a.ldp, *ni = n + i * a.ldnb;
-  for (int k0 = 0; k0 < a.K; k0 += kKT) {
-    bool on[kKT], any = false;
+  for (int k0 = 0; k0 < a.K; k0 += KT) {
+    bool on[KT], any = false;
 #pragma unroll
-    for (int k = 0; k < kKT; ++k) {
+    for (int k = 0; k < KT; ++k) {
       on[k] = k0 + k < a.K && pair_valid(a, i, k0 + k);
       any = any || on[k];
     }
-    float dot[kKT] = {};
+    float dot[KT] = {};
     if (any) {
       for (int e = c * VEC; e < a.H; e += VEC << lg) {
-        float x[VEC], y[VEC], z[kKT][VEC];
+        float x[VEC], y[VEC], z[KT][VEC];
         load_elems<VEC>(qi + e, x);
         load_elems<VEC>(pi + e, y);
 #pragma unroll
-        for (int k = 0; k < kKT; ++k)
+        for (int k = 0; k < KT; ++k)
           if (on[k]) load_elems<VEC>(ni + (k0 + k) * a.ldnk + e, z[k]);
 #pragma unroll
-        for (int k = 0; k < kKT; ++k)
+        for (int k = 0; k < KT; ++k)
           if (on[k]) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) dot[k] = __builtin_fmaf(x[j], y[j] - z[k][j], dot[k]);
           }
       }
     }
+    for (int o = 1; o < 1 << lg; o <<= 1) {
 #pragma unroll
-    for (int k = 0; k < kKT; ++k) {
-      if (k0 + k >= a.K) break;
-      float s = dot[k];
-      for (int o = 1; o < 1 << lg; o <<= 1) s += __shfl_xor(s, o);
-      const int64_t at = i * a.K + k0 + k;
+      for (int k = 0; k < KT; ++k) dot[k] += __shfl_xor(dot[k], o);
+    }
+    // every lane has the products: lanes c, c + 4, ... take pair c's loss, or each lane all of them where a group
+    // has fewer lanes (one after the other in every lane, 16 x 256 with 8 pairs took 11 us instead of 7)
+    float part = 0.f;
+    auto pair = [&](int m, float s, bool valid, bool writes) {
+      const int64_t at = i * a.K + k0 + m;
       float h = 0.f, loss = 0.f, dl = 0.f;
-      if (on[k]) {
+      if (valid) {
         h = s * a.inv_tau - (a.ref ? a.ref[at] : 0.f);
         pair_loss(a, h, loss, dl);
-        sum += loss;
-        ++count;
       }
-      if (c == 0) {
+      part += loss;
+      if (writes && k0 + m < a.K) {
         if (coef) coef[at] = dl;
         if (margins) margins[at] = h;
       }
+    };
+    if (KT == 4 && lg >= 2) {
+      const int m = c & 3;
+      float s = dot[0];
+      bool valid = on[0];
+#pragma unroll
+      for (int k = 1; k < KT; ++k) {
+        s = m == k ? dot[k] : s;
+        valid = m == k ? on[k] : valid;
+      }
+      pair(m, s, valid, c < 4);
+      part += __shfl_xor(part, 1);
+      part += __shfl_xor(part, 2);
+    } else {
+#pragma unroll
+      for (int k = 0; k < KT; ++k) pair(k, dot[k], on[k], c == 0);
     }
+    sum += part;
+#pragma unroll
+    for (int k = 0; k < KT; ++k) count += on[k];
   }
 }
 
@@ -133,7 +154,7 @@ __device__ __forceinline__ void pref_finish(double sum, double count, float* los
   }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, int KT>
 __global__ __launch_bounds__(kBlock) void pref_fwd_kernel(PrefArgs a, const T* __restrict__ q, const T* __restrict__ p,
                                                           const T* __restrict__ n, int lg, float* __restrict__ coef,
                                                           float* __restrict__ margins, float* __restrict__ rows,
@@ -143,7 +164,7 @@ __global__ __launch_bounds__(kBlock) void pref_fwd_kernel(PrefArgs a, const T* _
   if (i >= a.B) return;
   float sum;
   int count;
-  pref_row<T, VEC>(a, q, p, n, i, c, lg, coef, margins, sum, count);
+  pref_row<T, VEC, KT>(a, q, p, n, i, c, lg, coef, margins, sum, count);
   if (c == 0 && rows) {
     rows[i] = sum;
     counts[i] = count;
@@ -151,7 +172,7 @@ __global__ __launch_bounds__(kBlock) void pref_fwd_kernel(PrefArgs a, const T* _
 }
 
 // the same and the mean in one launch, for a batch that one workgroup passes in a few rounds
-template <typename T, int VEC>
+template <typename T, int VEC, int KT>
 __global__ __launch_bounds__(kFinish) void pref_fwd_small_kernel(PrefArgs a, const T* __restrict__ q,
                                                                  const T* __restrict__ p, const T* __restrict__ n,
                                                                  int lg, float* __restrict__ coef,
@@ -162,7 +183,7 @@ __global__ __launch_bounds__(kFinish) void pref_fwd_small_kernel(PrefArgs a, con
   for (int64_t i = (int64_t)(threadIdx.x >> 6) * (kWave >> lg) + sub; i < a.B; i += kFinish >> lg) {
     float sum;
     int count;
-    pref_row<T, VEC>(a, q, p, n, i, c, lg, coef, margins, sum, count);
+    pref_row<T, VEC, KT>(a, q, p, n, i, c, lg, coef, margins, sum, count);
     if (c == 0) {
       ds += (double)sum;
       dc += (double)count;
@@ -282,8 +303,11 @@ int launch_pref_fwd(const PrefArgs& a, const void* q, const void* p, const void*
   const void* ptrs[] = {q, p, n};
   const int vec = pref_vec<T>(a, ptrs, 3), lg = lanes_log2(a.H, vec);
   const T *tq = static_cast<const T*>(q), *tp = static_cast<const T*>(p), *tn = static_cast<const T*>(n);
-  if (loss && (a.B << lg) <= 4 * kFinish) {
-#define TT_CALL(V) pref_fwd_small_kernel<T, V><<<dim3(1), dim3(kFinish), 0, s>>>(a, tq, tp, tn, lg, coef, margins, loss, inv_pairs)
+  // one workgroup, and no launch for the mean, while it has its rows, pairs and columns in two steps (us, it and the
+  // two launches: one step, 16 x 256 4.0 and 5.4; two, 64 x 128 5.2 and 5.3; four, 64 x 256 8.0 and 5.4)
+  const int64_t rounds = ((a.B << lg) + kFinish - 1) / kFinish, chunks = (a.H + (vec << lg) - 1) / (vec << lg);
+  if (loss && rounds * chunks * ((a.K + kKT - 1) / kKT) <= 2) {
+#define TT_CALL(V) (a.K == 1 ? pref_fwd_small_kernel<T, V, 1> : pref_fwd_small_kernel<T, V, kKT>)<<<dim3(1), dim3(kFinish), 0, s>>>(a, tq, tp, tn, lg, coef, margins, loss, inv_pairs)
     TT_PREF_VEC(vec, TT_CALL)
 #undef TT_CALL
     TT_LAUNCH_CHECK("preference_fwd_small");
@@ -292,7 +316,7 @@ int launch_pref_fwd(const PrefArgs& a, const void* q, const void* p, const void*
   const int64_t per = (kBlock / kWave) * (kWave >> lg);
   if (a.B > 0) {
     const dim3 grid = wide_grid((a.B + per - 1) / per), block(kBlock);
-#define TT_CALL(V) pref_fwd_kernel<T, V><<<grid, block, 0, s>>>(a, tq, tp, tn, lg, coef, margins, loss ? rows : nullptr, counts)
+#define TT_CALL(V) (a.K == 1 ? pref_fwd_kernel<T, V, 1> : pref_fwd_kernel<T, V, kKT>)<<<grid, block, 0, s>>>(a, tq, tp, tn, lg, coef, margins, loss ? rows : nullptr, counts)
     TT_PREF_VEC(vec, TT_CALL)
 #undef TT_CALL
     TT_LAUNCH_CHECK("preference_fwd");

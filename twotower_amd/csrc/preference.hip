@@ -18,12 +18,16 @@
 // cancellation.  One workgroup does all of a small batch, the mean included (64 x 128: 5.0 us, one launch).
 #include "common.hpp"
 
+#include <algorithm>
+
 namespace tt {
 namespace {
 
 constexpr int kBlock = 256;
 constexpr int kFinish = 1024;  // the one workgroup that joins the rows
 constexpr int kKT = 4;         // pairs of a query in flight (a query with one has a form of its own)
+
+constexpr int64_t kFewWaves = 4096;  // what the card runs at half its residence
 
 enum { kSigmoid = 0, kSquared = 1 };
 
@@ -228,15 +232,28 @@ __global__ __launch_bounds__(kBlock) void pref_bwd_kernel(PrefArgs a, const T* _
   const float G = grad_loss[0] * (inv_pairs[0] * a.inv_tau);
   const T *qi = q + i * a.ldq, *pi = p + i * a.ldp, *ni = n + i * a.ldnb;
   const float* ci = coef + i * a.K;
-  float csum = 0.f;
-  bool any = false;
-  for (int k = 0; k < a.K; ++k)
-    if (pair_valid(a, i, k)) {
+  float csum = 0.f;  // (a masked pair's coefficient is 0)
+  int any = 0;
+  if (a.K <= kKT) {
+#pragma unroll
+    for (int k = 0; k < kKT; ++k)
+      if (k < a.K) {
+        csum += ci[k];
+        any |= pair_valid(a, i, k);
+      }
+  } else {
+    for (int k = c; k < a.K; k += 1 << lg) {
       csum += ci[k];
-      any = true;
+      any |= pair_valid(a, i, k);
     }
+    for (int o = 1; o < 1 << lg; o <<= 1) {
+      csum += __shfl_xor(csum, o);
+      any |= __shfl_xor(any, o);
+    }
+  }
   csum *= G;
-  for (int e = c * VEC; e < a.H; e += VEC << lg) {
+  // (the grid's z chunks of a row's columns run side by side)
+  for (int64_t e = (((int64_t)blockIdx.z << lg) + c) * VEC; e < a.H; e += (int64_t)(VEC << lg) * gridDim.z) {
     float x[VEC] = {}, y[VEC] = {}, gq[VEC] = {}, gp[VEC] = {};
     if (any) {
       load_elems<VEC>(qi + e, x);
@@ -334,7 +351,12 @@ int launch_pref_bwd(const PrefArgs& a, const void* q, const void* p, const void*
   const void* ptrs[] = {q, p, n, dq, dp, dn};
   const int vec = pref_vec<T>(a, ptrs, 6), lg = lanes_log2(a.H, vec);
   const int64_t per = (kBlock / kWave) * (kWave >> lg);
-  const dim3 grid = wide_grid((a.B + per - 1) / per), block(kBlock);
+  const dim3 block(kBlock);
+  dim3 grid = wide_grid((a.B + per - 1) / per);
+  // a wide row's column chunks side by side where there are few rows (33 x 382 fp16, 8 pairs: 11 us one after the
+  // other, 6 side by side; 5236 x 181 bf16, 3 pairs: 10 and 12)
+  const int64_t chunks = (a.H + (vec << lg) - 1) / (vec << lg), waves = (a.B << lg) / kWave + 1;
+  grid.z = (unsigned)std::min(chunks, (kFewWaves + waves - 1) / waves);
 #define TT_CALL(V)                                                                                              \
   pref_bwd_kernel<T, V><<<grid, block, 0, s>>>(a, static_cast<const T*>(q), static_cast<const T*>(p),           \
                                                static_cast<const T*>(n), lg, coef, inv_pairs, grad_loss,          \

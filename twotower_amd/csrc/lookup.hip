@@ -307,8 +307,10 @@ __global__ __launch_bounds__(kDirectThreads) void lookup_grad_direct_kernel(
 // 1.7 TB/s, 132 us with the frequent rows' tiles at 8192 x 64 text-like tokens, 200k rows of 256 floats.)
 constexpr int kTile = 32;
 constexpr int kSuper = 32;
-// a group's columns of a row: the grid's z chunks of them run side by side (1051 x 306 bf16, 38,318 tokens: tiles and
-// joins 12 and 10 us, chunk after chunk in one group 19 and 22)
+// a group's columns of a row: the grid's z chunks of them run side by side.  The tiles' and the joins' do where there are
+// few (kFewWaves): 1051 x 306 bf16, 38,318 tokens: tiles and joins 10 and 10 us, chunk after chunk 18 and 21;
+// 200k x 306, 524,288 tokens: 153 and 73, 142 and 51, as every chunk reads the tokens' names again.
+constexpr int64_t kFewWaves = 4096;
 #define TT_COLUMNS(e) for (int64_t e = (((int64_t)blockIdx.z << lg) + c) * VEC; e < E; e += (int64_t)(VEC << lg) * gridDim.z)
 
 template <typename TO, typename TW, int VEC>
@@ -445,6 +447,7 @@ __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, in
   const int c = threadIdx.x & ((1 << lg) - 1);
   const int n = *p.count;
   if (block_index() >= join_blocks) {
+    if (blockIdx.z > 0) return;
     const int64_t r0 = ((block_index() - join_blocks) * kWavesPerBlock + (threadIdx.x >> 6)) * kZeroRows;
     const int lane = lane_id(), groups = kWave >> lg;
     const int64_t r = r0 + (lane < kZeroRows ? lane : kZeroRows);
@@ -454,7 +457,7 @@ __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, in
     const float zero[VEC] = {};
     for (int i = lane >> lg; i < kZeroRows; i += groups)
       if (empty >> i & 1)
-        TT_COLUMNS(e) store_elems_nt<VEC>(grad + (r0 + i) * E + e, zero);
+        for (int64_t e = c * VEC; e < E; e += VEC << lg) store_elems_nt<VEC>(grad + (r0 + i) * E + e, zero);
     return;
   }
   const int64_t t0 = (block_index() * kBlock + threadIdx.x) >> lg;
@@ -549,13 +552,16 @@ int launch_bwd(const void* dout, const void* ids, int ids_dtype, int64_t n, int6
   float *head = ws, *tail = head + tiles * E, *sup = tail + tiles * E;
   const unsigned chunks = (unsigned)std::min<int64_t>(((int64_t)E + (vec << lg) - 1) / (vec << lg), 65535);
   auto grid = [&](int64_t groups) { return dim3((unsigned)((groups + per - 1) / per), 1, chunks); };
+  dim3 tile_grid = grid(tiles);
+  const int64_t waves = (tiles << lg) / kWave + 1;
+  tile_grid.z = (unsigned)std::min<int64_t>(chunks, (kFewWaves + waves - 1) / waves);
   const int64_t zero_rows = (int64_t)kWavesPerBlock * kZeroRows;
   const dim3 block(kBlock);
   dim3 join = wide_grid(grid(tiles).x + (V + zero_rows - 1) / zero_rows);
-  join.z = chunks;
+  join.z = tile_grid.z;
 #define TT_LS(VV)                                                                                                  \
   case VV:                                                                                                         \
-    lookup_tile_sum_kernel<TO, TW, VV><<<grid(tiles), block, 0, s>>>(p, d, E, scale, g, lg, head, tail);           \
+    lookup_tile_sum_kernel<TO, TW, VV><<<tile_grid, block, 0, s>>>(p, d, E, scale, g, lg, head, tail);             \
     TT_LAUNCH_CHECK("lookup_tile_sum");                                                                            \
     if (supers > 0) lookup_super_sum_kernel<VV><<<grid(supers), block, 0, s>>>(p, head, E, lg, sup);               \
     TT_LAUNCH_CHECK("lookup_super_sum");                                                                           \

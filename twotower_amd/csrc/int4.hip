@@ -9,11 +9,11 @@
 // (33 bits of it), so v_mfma_f32_16x16x32_f16 forms the sum of 32 exact products in fp32; the group's
 // scale multiplies that sum.  32 columns are the instruction's K and the smallest group.
 //
-// 1M x 256, group 32 (us for 1 / 16 / 64 queries): 33-39 / 49 / 121, for 148 MB of index and 4 MB of scores a
-// query (fp32 cosine scores of the same rows: 186 / 235 / 446); group 128: 31-33.  One query is bound by the index's
-// reads, 4.0-4.4 TB/s (1, 2 or 4 tiles a wave, half as many waves, loads past the caches: 36-40 us all).  Short
-// indexes are bound by the launch and the queries' layout: 200k x 128, 8 queries 10.4 us, 28,834 x 100, 33
-// queries 9.2.
+// 1M x 256, group 32 (us for 1 / 16 / 64 queries): 30-36 / 47 / 118, for 148 MB of index and 4 MB of scores a
+// query (fp32 cosine scores of the same rows: 188 / 234 / 437); group 128: 30 / 45 / 117.  One query is bound by the
+// index's reads, 4.2-5.0 TB/s (workgroups of 256: 32-38; with these 1, 2 or 4 tiles a wave, half as many waves, loads
+// past the caches: no faster).  Short indexes are bound by the launch and the queries' layout: 200k x 128, 8 queries
+// 10.3 us, 28,834 x 100, 33 queries 8.7.
 //
 // Layout (written once per index): tiles of 16 rows; a tile is a run of quads of 128 columns, a quad
 // of 64 lanes x 16 bytes in the order the kernel loads it: lane (row j = l % 16, h = l / 16), dword d
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(kBlock) void int4_quantize_kernel(const T* __restri
 
 __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restrict__ src,
                                                            const uint16_t* __restrict__ sc, int64_t n, int H,
-                                                           int group, int nblk, int nquad,
+                                                           int group, int nblk, int nquad, bool wide,
                                                            uint32_t* __restrict__ codes,
                                                            uint16_t* __restrict__ scales) {
   const Place p = place_of(block_index() * kBlock + threadIdx.x, nquad);
@@ -158,13 +158,19 @@ __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restr
   if (p.h == 0 && (p.b & (group / kBlk - 1)) == 0)
     scales[scale_at(p.row, p.b, nquad, group)] = p.row < n && g < ng ? sc[p.row * ng + g] : (uint16_t)0;
   if (p.b >= nblk) return;
+  const int k0 = p.b * kBlk + 8 * p.h;
+  const int8_t* at = src + p.row * H + k0;
+  Elems<int8_t, 8> v = {};
+  if (wide) {  // (8 at a time are aligned and H % 8 == 0)
+    if (p.row < n && k0 < H) v = *reinterpret_cast<const Elems<int8_t, 8>*>(at);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (p.row < n && k0 + i < H) v.v[i] = at[i];
+  }
   int c[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int k = p.b * kBlk + 8 * p.h + i;
-    const int v = p.row < n && k < H ? (int)src[p.row * H + k] : 0;
-    c[i] = 8 + (v < -8 ? -8 : v > 7 ? 7 : v);
-  }
+  for (int i = 0; i < 8; ++i) c[i] = 8 + (v.v[i] < -8 ? -8 : v.v[i] > 7 ? 7 : (int)v.v[i]);
   codes[code_word(p.row, p.b, p.h, nblk)] = pack8(c);
 }
 
@@ -267,48 +273,63 @@ __global__ __launch_bounds__(BLOCK) void int4_scores_kernel(const T* __restrict_
   QuadLoad<SPQ> cur;  // the first documents are on their way while the queries are laid out
   if (t0 < ntile) load_quad<SPQ>(cur, codes, scales, t0, ntile, 0, nblk, nquad, lane);
 
-  // A thread takes 8 elements of one query (several runs of 8 where there are more): their maximum joins the
-  // query's (an integer maximum of the bits, whatever the order), then their terms go to the operands.
+  // A thread takes runs of 8 elements of a query, kRuns of them in flight: their maxima join the query's (an
+  // integer maximum of the bits, whatever the order), then their terms go to the operands.  (us, 1 and 4 runs in
+  // flight: 3994 x 327, 31 queries 12.9 and 11.3; 1M x 256, one query, which has one run a thread, 30.0 and 32.9.)
+  constexpr int kRuns = NQT >= 2 ? 4 : 1;
   if (threadIdx.x < Q::kQ) qe[threadIdx.x] = 0;
   __syncthreads();
   const int items = nblk * Q::kQ * 4;
-  float x[8];
-  for (int it = threadIdx.x; it < items; it += BLOCK) {
-    const int i = (it >> 2) % Q::kQ, k0 = ((it >> 2) / Q::kQ) * kBlk + 8 * (it & 3);
-    load8(q + i * ldq, k0, i < nq ? H : 0, wide, x);
-    uint32_t mx = 0;
+  float x[kRuns][8];
+  auto load_runs = [&](int it0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(fabsf(x[e])));
-    if (mx) atomicMax(reinterpret_cast<uint32_t*>(&qe[i]), mx);
+    for (int u = 0; u < kRuns; ++u) {
+      const int it = it0 + u * BLOCK, i = (it >> 2) % Q::kQ;
+      load8(q + i * ldq, ((it >> 2) / Q::kQ) * kBlk + 8 * (it & 3), it < items && i < nq ? H : 0, wide, x[u]);
+    }
+  };
+  for (int it0 = threadIdx.x; it0 < items; it0 += kRuns * BLOCK) {
+    load_runs(it0);
+#pragma unroll
+    for (int u = 0; u < kRuns; ++u) {
+      uint32_t mx = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(fabsf(x[u][e])));
+      if (mx) atomicMax(reinterpret_cast<uint32_t*>(&qe[((it0 + u * BLOCK) >> 2) % Q::kQ]), mx);
+    }
   }
   __syncthreads();
   int own_e = threadIdx.x < Q::kQ ? query_exponent(__int_as_float(qe[threadIdx.x])) : 0;
   __syncthreads();
   if (threadIdx.x < Q::kQ) qe[threadIdx.x] = own_e;
   __syncthreads();
-  for (int it = threadIdx.x; it < items; it += BLOCK) {
-    const int hh = it & 3, i = (it >> 2) % Q::kQ, b = (it >> 2) / Q::kQ;
-    if (items > BLOCK) load8(q + i * ldq, b * kBlk + 8 * hh, i < nq ? H : 0, wide, x);
-    f16x8 t0v, t1v, t2v;
+  for (int it0 = threadIdx.x; it0 < items; it0 += kRuns * BLOCK) {
+    if (items > kRuns * BLOCK) load_runs(it0);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float y = ldexpf(x[e], qe[i]);
-      t0v[e] = (_Float16)y;
-      const float r1 = y - (float)t0v[e];
-      t1v[e] = (_Float16)r1;
-      t2v[e] = (_Float16)(r1 - (float)t1v[e]);
-    }
-    if constexpr (NQT == 0) {
-      f16x8* at = A + b * kWave + hh * 16 + 4 * i;
-      at[0] = t0v;
-      at[1] = t1v;
-      at[2] = t2v;
-      at[3] = f16x8{};
-    } else {
-      f16x8* at = A + ((size_t)b * Q::kOps + 3 * (i >> 4)) * kWave + hh * 16 + (i & 15);
-      at[0] = t0v;
-      at[kWave] = t1v;
-      at[2 * kWave] = t2v;
+    for (int u = 0; u < kRuns; ++u) {
+      const int it = it0 + u * BLOCK, hh = it & 3, i = (it >> 2) % Q::kQ, b = (it >> 2) / Q::kQ;
+      if (it >= items) break;
+      f16x8 t0v, t1v, t2v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = ldexpf(x[u][e], qe[i]);
+        t0v[e] = (_Float16)y;
+        const float r1 = y - (float)t0v[e];
+        t1v[e] = (_Float16)r1;
+        t2v[e] = (_Float16)(r1 - (float)t1v[e]);
+      }
+      if constexpr (NQT == 0) {
+        f16x8* at = A + b * kWave + hh * 16 + 4 * i;
+        at[0] = t0v;
+        at[1] = t1v;
+        at[2] = t2v;
+        at[3] = f16x8{};
+      } else {
+        f16x8* at = A + ((size_t)b * Q::kOps + 3 * (i >> 4)) * kWave + hh * 16 + (i & 15);
+        at[0] = t0v;
+        at[kWave] = t1v;
+        at[2 * kWave] = t2v;
+      }
     }
   }
   __syncthreads();
@@ -395,19 +416,16 @@ int launch_scores_block(const T* q, int nq, int64_t ldq, const uint32_t* codes, 
   return TT_OK;
 }
 
-// Sixteen waves a CU share the query operands in LDS: as many workgroups of 256 as it holds, or fewer, larger
-// ones where the operands are large (100k x 1024, 16 queries, 96 KB: 256 threads 47 us, 1024 threads 26 us).
-// An index too short to give each of those waves its tiles keeps to 256.
+// The workgroups of a CU share its LDS, each with the query operands: workgroups of 512, or of 1024 where the
+// operands are large and the index gives each of their waves its tiles (us, 256 / 512 / 1024 threads: 1M x 256, one query
+// 32.0 / 30.1 / 30.0; 200k x 256, 42 queries 47 / 33 / 28; 9729 x 384, 32 queries 11.3 / 10.1 / 12.9).
 template <typename T, int NQT, int SPQ>
 int launch_scores(const T* q, int nq, int64_t ldq, const uint32_t* codes, const uint16_t* scales, int64_t n, int H,
                   float* scores, int64_t ld_scores, hipStream_t s) {
   const size_t lds = (size_t)4 * quads_of(H) * QueryTiles<NQT>::kOps * kWave * 16;
-  const int64_t tiles = tiles_of(n);
-  if (lds > 78 * 1024 && tiles > 256 * 8 * kTPW)
+  if (lds > 78 * 1024 && tiles_of(n) > 256 * 8 * kTPW)
     return launch_scores_block<T, NQT, SPQ, 1024>(q, nq, ldq, codes, scales, n, H, scores, ld_scores, s);
-  if (lds > 39 * 1024 && tiles > 256 * 4 * kTPW)
-    return launch_scores_block<T, NQT, SPQ, 512>(q, nq, ldq, codes, scales, n, H, scores, ld_scores, s);
-  return launch_scores_block<T, NQT, SPQ, 256>(q, nq, ldq, codes, scales, n, H, scores, ld_scores, s);
+  return launch_scores_block<T, NQT, SPQ, 512>(q, nq, ldq, codes, scales, n, H, scores, ld_scores, s);
 }
 
 template <typename T, int SPQ>
@@ -505,8 +523,8 @@ extern "C" int tt_int4_pack(const int8_t* c, const void* sc, int64_t n, int H, i
   if (n == 0) return TT_OK;
   TT_REQUIRE(layout_blocks(n, H) < (int64_t(1) << 31), "int4: too many values");
   int4_pack_kernel<<<wide_grid(layout_blocks(n, H)), dim3(kBlock), 0, reinterpret_cast<hipStream_t>(stream)>>>(
-      c, static_cast<const uint16_t*>(sc), n, H, group, blocks_of(H), quads_of(H), static_cast<uint32_t*>(codes),
-      static_cast<uint16_t*>(scales));
+      c, static_cast<const uint16_t*>(sc), n, H, group, blocks_of(H), quads_of(H),
+      H % 8 == 0 && reinterpret_cast<size_t>(c) % 8 == 0, static_cast<uint32_t*>(codes), static_cast<uint16_t*>(scales));
   TT_LAUNCH_CHECK("int4_pack");
   return TT_OK;
 }

@@ -338,6 +338,49 @@ def test_lookup_embedding_module_uses_the_kernels():
     assert torch.equal(emb.embedding.weight.grad, (4.0 * count).unsqueeze(1).expand(50, 16))
 
 
+def test_calls_are_timed_and_recorded_on_autograds_thread():
+    w = torch.randn(50, 16, device=DEV, requires_grad=True)
+    q, p, n = (torch.randn(4, 16, device=DEV, requires_grad=True) for _ in range(3))
+    _lib.TIMER.reset()
+    _lib.TIMER.enabled = True
+    try:
+        ops.embedding_lookup(w, torch.arange(9, device=DEV)).sum().backward()
+        losses.preference_loss(q, p, n).backward()
+        optim.clip_grad_norm_([w, q, p, n], 1.0)
+    finally:
+        _lib.TIMER.enabled = False
+    got = _lib.TIMER.summary()
+    _lib.TIMER.reset()
+    names = {"tt_lookup_fwd", "tt_lookup_bwd", "tt_preference_fwd", "tt_preference_bwd", "tt_clip_grads"}
+    assert names <= set(got) and all(got[k]["calls"] == 1 and got[k]["total_ms"] > 0 for k in names)
+
+
+def test_lookups_of_two_threads_at_once():
+    import threading
+
+    cases = [lookup_case(3000, 64, (n,), F32, torch.int64, None, 0, 0.1, 15 + n) for n in (700, 20_000)]
+    for w, _, _ in cases:
+        w.requires_grad_(True)
+
+    def grad(w, ids, dout):
+        return torch.autograd.grad(ops.embedding_lookup(w, ids, 2.0, 0), w, dout)[0]
+
+    want = [grad(*c) for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            got[i] = [grad(*cases[i]) for _ in range(20)]
+        side.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert all(len(g) == 20 and all(torch.equal(x, want[i]) for x in g) for i, g in enumerate(got))
+
+
 def test_lookup_embedding_module_under_torchs_transforms():
     """What follows torch's own calls (function transforms, tracing, dispatch modes, hooks) sees the plain gather."""
     emb = tt.embeddings.build("lookup", vocab_size=50, embedding_dim=16, scale=4.0).to(DEV)
@@ -427,6 +470,12 @@ PREFS = [
     (33, 1030, 9, F32, True, 0.8, 0.5, 0.1, 0.0, "squared"),
     (129, 2048, 1, BF16, False, 0.0, 1.0, 0.05, 0.0, "sigmoid"),
     (5000, 20, 3, F16, True, 0.9, 1.0, 0.1, 0.0, "squared"),
+    (33, 382, 8, F16, True, 0.0, 0.1, 0.05, 0.0, "squared"),       # columns side by side in the backward
+    (2, 5001, 5, F32, False, 0.0, 0.5, 0.1, 0.1, "sigmoid"),
+    (40, 1, 9, BF16, True, 0.4, 0.5, 0.1, 0.0, "sigmoid"),         # one lane a query, several rounds of pairs
+    (40, 2, 6, F32, True, 0.4, 0.5, 0.1, 0.2, "sigmoid"),
+    (16, 256, 4, F32, False, 0.2, 1.0, 0.1, 0.0, "sigmoid"),       # one workgroup, four pairs together
+    (128, 128, 8, BF16, True, 0.2, 1.0, 0.1, 0.0, "squared"),
 ]
 
 

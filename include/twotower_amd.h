@@ -279,7 +279,7 @@ int tt_adamw_multi_ex(const tt_adamw_tensor* tensors, const tt_adamw_grad_parts*
  * or fp32; tensors must not overlap otherwise.  The five arrays (host memory) describe `count` tensors:
  * pointers, elements, tt_elem_dtype codes.  Any count: TT_CLIP_MAX_TENSORS per launch, passed by value.
  * ws: tt_clip_ws_size(count) bytes, 8-byte aligned. */
-#define TT_CLIP_MAX_TENSORS 128
+#define TT_CLIP_MAX_TENSORS 168
 size_t tt_clip_ws_size(int count);
 int tt_clip_grads(const void* const* src, void* const* dst, const int64_t* n, const uint8_t* src_dtype,
                   const uint8_t* dst_dtype, int count, int inf_norm, double max_norm, int scale, float* norm, void* ws,

@@ -644,7 +644,8 @@ CLIPS = [
     ([5, 0, 70001, 3], [F16, F32, BF16, F32], 1.0, 2.0),
     ([5, 0, 70001, 3], [F16, F32, BF16, F32], 0.3, math.inf),
     ([100_003], [F32], 1e6, 2.0),   # not clipped
-    ([1000] * 128, [F32] * 128, 1.0, 2.0),
+    ([1000] * 168, [F32] * 168, 1.0, 2.0),   # one launch, and one tensor more
+    ([1000, 3] * 84 + [2049], [F32] * 169, 1.0, 2.0),
     ([97] * 129 + [30_000] * 150, [F32, BF16, F16] * 93, 1.0, 2.0),  # several launches
 ]
 
@@ -740,7 +741,7 @@ def test_clip_offsets_beyond_32_bits():
 
 
 def test_clip_captured_and_replayed():
-    sizes, types = [70_000, 33, 5000] * 50, [F32, BF16, F32] * 50  # two launches' lists
+    sizes, types = [70_000, 33, 5000] * 60, [F32, BF16, F32] * 60  # two launches' lists
     grads = clip_case(sizes, types, 33)
     outs = [torch.empty(s, device=DEV) for s in sizes]
     ops.clip_grad_norm(grads, 1.0, out=outs)

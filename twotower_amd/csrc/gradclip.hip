@@ -28,8 +28,8 @@ constexpr int kScaleBlocks = 2048;
 struct ClipList {
   const void* src[TT_CLIP_MAX_TENSORS];
   void* dst[TT_CLIP_MAX_TENSORS];
-  int64_t n[TT_CLIP_MAX_TENSORS];
   int32_t first[TT_CLIP_MAX_TENSORS + 1];  // first chunk of each tensor
+  uint16_t last[TT_CLIP_MAX_TENSORS];      // elements of its last chunk
   uint8_t type[TT_CLIP_MAX_TENSORS];       // src type | dst type << 2
   int count, chunk;                        // tensors; elements per chunk
 };
@@ -115,8 +115,7 @@ __global__ __launch_bounds__(kBlock) void clip_norm_kernel(ClipList l, double* _
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
     const int t = tensor_of(l, c);
     const int64_t at = (int64_t)(c - l.first[t]) * l.chunk;
-    const int64_t left = l.n[t] - at;
-    const int n = (int)(left < l.chunk ? left : l.chunk);
+    const int n = c + 1 < l.first[t + 1] ? l.chunk : l.last[t];
     const int ty = l.type[t] & 3;
     double a;
     if (ty == TT_E_F32) a = norm_chunk<float, INF>(static_cast<const float*>(l.src[t]) + at, n);
@@ -204,8 +203,7 @@ __global__ __launch_bounds__(kBlock) void clip_scale_kernel(ClipList l, const do
   for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
     const int t = tensor_of(l, c);
     const int64_t at = (int64_t)(c - l.first[t]) * l.chunk;
-    const int64_t left = l.n[t] - at;
-    const int n = (int)(left < l.chunk ? left : l.chunk);
+    const int n = c + 1 < l.first[t + 1] ? l.chunk : l.last[t];
     const int ty = l.type[t];
     if (coef.a == 1.f && coef.b == 1.f && l.src[t] == l.dst[t]) continue;  // in place and not clipped: nothing changes
 #define TT_SC(TS, TD) scale_chunk<TS, TD>(static_cast<const TS*>(l.src[t]) + at, static_cast<TD*>(l.dst[t]) + at, n, coef)
@@ -239,10 +237,11 @@ void fill_list(ClipList& l, const ClipCall& t, int at) {
   for (int i = 0; i < m; ++i) {
     l.src[i] = t.src[at + i];
     l.dst[i] = t.dst[at + i];
-    l.n[i] = t.n[at + i];
     l.type[i] = (uint8_t)(t.src_dtype[at + i] | t.dst_dtype[at + i] << 2);
     l.first[i] = (int32_t)chunk;
-    chunk += (t.n[at + i] + l.chunk - 1) / l.chunk;
+    const int64_t chunks = (t.n[at + i] + l.chunk - 1) / l.chunk;
+    l.last[i] = (uint16_t)(t.n[at + i] - (chunks - 1) * l.chunk);
+    chunk += chunks;
   }
   l.first[m] = (int32_t)chunk;
   l.count = m;
@@ -254,7 +253,7 @@ int run_clip(const ClipCall& t, bool scale, double max_norm, float* norm, double
   const int count = t.count, launches = (count + TT_CLIP_MAX_TENSORS - 1) / TT_CLIP_MAX_TENSORS;
   int cap = launches > 0 ? kMaxParts / launches : 1;
   cap = cap < 1 ? 1 : cap > kNormBlocks ? kNormBlocks : cap;
-  static_assert(sizeof(ClipList) <= 3840, "kernel arguments");
+  static_assert(sizeof(ClipList) <= 4096 - 64, "kernel arguments");  // (4 KB, with the others)
   ClipList l;
   int np = 0;
   for (int at = 0; at < count; at += TT_CLIP_MAX_TENSORS) {

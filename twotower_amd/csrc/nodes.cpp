@@ -5,7 +5,7 @@
 // own, where a node written in Python costs twice what it does on the caller's, and a list of gradients is
 // walked tensor by tensor.  Calls in Python and here (us): lookup of 37 x 29 tokens of 100 with its gradient 78 and
 // 43 (a node that does nothing 39; GPU 11), preference loss of 64 x 128 with its gradients 103 and 50-67 (GPU 9),
-// clipping of 150 tensors 120 and 42 (GPU 43).
+// clipping of 150 tensors 120 and 42 (GPU 43; 30 since a launch takes them all).
 //
 // The C ABI comes as addresses from the loaded library (bind), so the module has no second copy of it.  Calls are
 // made directly unless someone times or records them (_lib.TIMER, record_calls); then through _lib.call.

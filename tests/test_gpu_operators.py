@@ -236,7 +236,7 @@ def test_lookup_backward_through_a_loss_matches_differences():
             assert abs(grad[r, e].item() - want) <= 30 * U * abs(want) + 1e-9
 
 
-@pytest.mark.parametrize("n", [700, 30_000])
+@pytest.mark.parametrize("n", [700, 8000, 30_000])
 def test_lookup_captured_and_replayed(n):
     V, E = 400, 64
     w, ids, dout = lookup_case(V, E, (n,), F32, torch.int64, None, 0, 0.2, 6)

@@ -10,10 +10,12 @@
 // nor underflows before its own rounding to 32 bits, and the vector units have room for it beside
 // the loads (added in 32 bits the pass took 54 instead of 57 us).  All sums run in a fixed order (no atomics).
 //
-// 51.3M fp32 elements into another buffer: norm 38 us (205 MB, 5.4 TB/s), scaling 65 us (410 MB, 6.3 TB/s, its
+// 51.3M fp32 elements into another buffer: norm 36 us (205 MB, 5.7 TB/s), scaling 64 us (410 MB, 6.4 TB/s, its
 // reads partly cached; a 4 GiB copy runs at 4.8 TB/s).  16,384-element chunks on 1024 workgroups took 57 and
 // 70 us, and results kept in the caches 50 (the next norm's reads then wait for their write-back) and 72.  Few
-// elements: 131,584 in 4 tensors 4.0 + 4.5 us (chunks of 8192 4.7 + 4.9), 1.7M of three types 4.5 + 7.8 (5.3 + 12.6).
+// elements: 131,584 in 4 tensors 3.9 + 4.2 us (chunks of 8192 4.7 + 4.9), 1.7M of three types 4.5 + 7.8 (5.3 + 12.6).
+// Loads that a condition guards wait for each other in some of these loops and not in others (measured one by one:
+// the norm's aligned one 36 us without and 40 with, the scaling's unaligned one, 12M elements, 16.6 and 19.8).
 #include "common.hpp"
 
 namespace tt {
@@ -29,10 +31,14 @@ struct ClipList {
   const void* src[TT_CLIP_MAX_TENSORS];
   void* dst[TT_CLIP_MAX_TENSORS];
   int32_t first[TT_CLIP_MAX_TENSORS + 1];  // first chunk of each tensor
-  uint16_t last[TT_CLIP_MAX_TENSORS];      // elements of its last chunk
-  uint8_t type[TT_CLIP_MAX_TENSORS];       // src type | dst type << 2
+  // elements of its last chunk, src type | dst type << 2: 16 and 8 bits each, read as words (kernel arguments come
+  // by scalar loads, which have no narrower ones)
+  uint32_t last2[TT_CLIP_MAX_TENSORS / 2], type4[TT_CLIP_MAX_TENSORS / 4];
   int count, chunk;                        // tensors; elements per chunk
 };
+
+__device__ __forceinline__ int last_of(const ClipList& l, int t) { return l.last2[t >> 1] >> (t & 1) * 16 & 0xffff; }
+__device__ __forceinline__ int type_of(const ClipList& l, int t) { return l.type4[t >> 2] >> (t & 3) * 8 & 0xff; }
 
 __device__ __forceinline__ int tensor_of(const ClipList& l, int chunk) {
   int lo = 0, hi = l.count - 1;  // the last tensor with first[] <= chunk
@@ -69,17 +75,16 @@ __device__ __forceinline__ double norm_chunk(const T* __restrict__ p, int n) {
   if (aligned16(p)) {
     const int nv = n / VEC;
     for (int i = threadIdx.x; i < nv; i += U * kBlock) {
-      float x[U][VEC];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) x[u][j] = 0.f;
-        if (i + u * kBlock < nv) load_elems<VEC>(p + (size_t)(i + u * kBlock) * VEC, x[u]);
-      }
+      Elems<T, VEC> x[U];  // (past the end the last one again: no load waits for a condition)
 #pragma unroll
       for (int u = 0; u < U; ++u)
+        x[u] = *reinterpret_cast<const Elems<T, VEC>*>(p + (size_t)min(i + u * kBlock, nv - 1) * VEC);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) norm_add<INF>(acc[u], x[u][j]);
+      for (int u = 0; u < U; ++u)
+        if (i + u * kBlock < nv) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) norm_add<INF>(acc[u], (float)x[u].v[j]);
+        }
     }
     for (int i = nv * VEC + threadIdx.x; i < n; i += kBlock) norm_add<INF>(acc[0], (float)p[i]);
   } else {
@@ -115,8 +120,8 @@ __global__ __launch_bounds__(kBlock) void clip_norm_kernel(ClipList l, double* _
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
     const int t = tensor_of(l, c);
     const int64_t at = (int64_t)(c - l.first[t]) * l.chunk;
-    const int n = c + 1 < l.first[t + 1] ? l.chunk : l.last[t];
-    const int ty = l.type[t] & 3;
+    const int n = c + 1 < l.first[t + 1] ? l.chunk : last_of(l, t);
+    const int ty = type_of(l, t) & 3;
     double a;
     if (ty == TT_E_F32) a = norm_chunk<float, INF>(static_cast<const float*>(l.src[t]) + at, n);
     else if (ty == TT_E_BF16) a = norm_chunk<__bf16, INF>(static_cast<const __bf16*>(l.src[t]) + at, n);
@@ -184,7 +189,7 @@ __device__ __forceinline__ void scale_chunk(const TS* src, TD* dst, int n, Coef 
     for (int i = threadIdx.x; i < n; i += 4 * U * kBlock) {
       float x[4 * U];
 #pragma unroll
-      for (int u = 0; u < 4 * U; ++u) x[u] = i + u * kBlock < n ? (float)src[i + u * kBlock] : 0.f;
+      for (int u = 0; u < 4 * U; ++u) x[u] = (float)src[min(i + u * kBlock, n - 1)];
 #pragma unroll
       for (int u = 0; u < 4 * U; ++u)
         if (i + u * kBlock < n) dst[i + u * kBlock] = (TD)coef(x[u]);
@@ -203,8 +208,8 @@ __global__ __launch_bounds__(kBlock) void clip_scale_kernel(ClipList l, const do
   for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
     const int t = tensor_of(l, c);
     const int64_t at = (int64_t)(c - l.first[t]) * l.chunk;
-    const int n = c + 1 < l.first[t + 1] ? l.chunk : l.last[t];
-    const int ty = l.type[t];
+    const int n = c + 1 < l.first[t + 1] ? l.chunk : last_of(l, t);
+    const int ty = type_of(l, t);
     if (coef.a == 1.f && coef.b == 1.f && l.src[t] == l.dst[t]) continue;  // in place and not clipped: nothing changes
 #define TT_SC(TS, TD) scale_chunk<TS, TD>(static_cast<const TS*>(l.src[t]) + at, static_cast<TD*>(l.dst[t]) + at, n, coef)
     if (ty == (TT_E_F32 | TT_E_F32 << 2)) TT_SC(float, float);
@@ -237,10 +242,12 @@ void fill_list(ClipList& l, const ClipCall& t, int at) {
   for (int i = 0; i < m; ++i) {
     l.src[i] = t.src[at + i];
     l.dst[i] = t.dst[at + i];
-    l.type[i] = (uint8_t)(t.src_dtype[at + i] | t.dst_dtype[at + i] << 2);
+    if (i % 2 == 0) l.last2[i / 2] = 0;
+    if (i % 4 == 0) l.type4[i / 4] = 0;
+    l.type4[i / 4] |= (uint32_t)(t.src_dtype[at + i] | t.dst_dtype[at + i] << 2) << i % 4 * 8;
     l.first[i] = (int32_t)chunk;
     const int64_t chunks = (t.n[at + i] + l.chunk - 1) / l.chunk;
-    l.last[i] = (uint16_t)(t.n[at + i] - (chunks - 1) * l.chunk);
+    l.last2[i / 2] |= (uint32_t)(t.n[at + i] - (chunks - 1) * l.chunk) << i % 2 * 16;
     chunk += chunks;
   }
   l.first[m] = (int32_t)chunk;

@@ -5,7 +5,7 @@
 //
 // Both move bytes and add: the forward reads each token's row (repeated rows from L2) and writes
 // n E elements, the backward reads n E elements once and writes V E.  8192 x 64 text-like tokens, half of them
-// padding, 200k x 256 fp32: forward 152 us (537 MB written, 128 MB read from memory; 86 us without the reads, 44
+// padding, 200k x 256 fp32: forward 151 us (537 MB written, 128 MB read from memory; 86 us without the reads, 44
 // without the writes, and 152-161 for 1 to 16 tokens in flight, stores past the caches or not), sort 40 us, tiles
 // 70 us (344 MB, 4.9 TB/s), joins and empty rows 42 us (148 MB); a 4 GiB copy runs at 4.8 TB/s.  The backward needs each
 // row's tokens together: a long call sorts them (the bags' stable counting sort, token_plan_build), a short one
@@ -55,20 +55,18 @@ __global__ __launch_bounds__(kBlock) void lookup_fwd_kernel(const TW* __restrict
     id[u] = t < n ? id_at(ids, wide, t) : -1;
   }
   for (int e = c * VEC; e < E; e += VEC << lg) {
-    float x[U][VEC];
+    Elems<TW, VEC> x[U];  // (row 0 for an id outside: no load waits for a condition)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) x[u][i] = 0.f;
-      if (id[u] >= 0 && id[u] < V) load_elems<VEC>(table + id[u] * ld + e, x[u]);
-    }
+    for (int u = 0; u < U; ++u)
+      x[u] = *reinterpret_cast<const Elems<TW, VEC>*>(table + (id[u] >= 0 && id[u] < V ? id[u] : 0) * ld + e);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t t = t0 + (int64_t)u * groups;
       if (t < n) {
+        float y[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) x[u][i] = (id[u] >= 0 && id[u] < V) ? scale * x[u][i] : 0.f;
-        store_elems_nt<VEC>(out + t * E + e, x[u]);
+        for (int i = 0; i < VEC; ++i) y[i] = (id[u] >= 0 && id[u] < V) ? scale * (float)x[u].v[i] : 0.f;
+        store_elems_nt<VEC>(out + t * E + e, y);
       }
     }
   }

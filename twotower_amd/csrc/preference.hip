@@ -11,9 +11,10 @@
 //   dq_i = G sum_k c_ik (p_i - n_ik),   dp_i = G (sum_k c_ik) q_i,   dn_ik = -G c_ik q_i.
 // A masked pair is not read, counts nothing and gets a zero gradient; no valid pair: loss 0.
 // Row passes, bound by their bytes (forward: q, p, n once; backward: again, and the gradients): 8192 x 256 fp32,
-// one negative: forward 7.9 us + 3.0 for the mean (25 MB), backward 9.0 (50 MB, 5.6 TB/s); bf16, four
-// negatives: 7.5 + 3.0 and 9.3 us.  A group of lanes takes a query and up to kKT of its pairs at once: q and p are
-// then read once however many pairs there are up to that, and a row's loads are all in flight together.
+// one negative: forward 7.9 us + 3.0 for the mean (25 MB), backward 8.8 (50 MB, 5.7 TB/s); bf16, four
+// negatives: 7.5 + 3.0 and 8.9 us.  A group of lanes takes a query and up to kKT of its pairs at once: q and p are
+// then read once however many pairs there are up to that, and a row's loads are all in flight together (a masked
+// pair's from p again: behind a condition the backward's waited, 9.3 instead of 8.9 us).
 // The differences p - n are formed before the products, so two close documents lose nothing to
 // cancellation.  One workgroup does all of a small batch, the mean included (64 x 128: 5.0 us, one launch).
 #include "common.hpp"
@@ -82,7 +83,7 @@ __device__ __forceinline__ void pref_row(const PrefArgs& a, const T* __restrict_
         load_elems<VEC>(pi + e, y);
 #pragma unroll
         for (int k = 0; k < KT; ++k)
-          if (on[k]) load_elems<VEC>(ni + (k0 + k) * a.ldnk + e, z[k]);
+          load_elems<VEC>((on[k] ? ni + (k0 + k) * a.ldnk : pi) + e, z[k]);
 #pragma unroll
         for (int k = 0; k < KT; ++k)
           if (on[k]) {
@@ -265,7 +266,7 @@ __global__ __launch_bounds__(kBlock) void pref_bwd_kernel(PrefArgs a, const T* _
 #pragma unroll
       for (int k = 0; k < kKT; ++k) {
         on[k] = k0 + k < a.K && pair_valid(a, i, k0 + k);
-        if (on[k]) load_elems<VEC>(ni + (k0 + k) * a.ldnk + e, z[k]);
+        load_elems<VEC>((on[k] ? ni + (k0 + k) * a.ldnk : pi) + e, z[k]);
       }
 #pragma unroll
       for (int k = 0; k < kKT; ++k) {

@@ -5,11 +5,10 @@
 //
 // Both move bytes and add: the forward reads each token's row (repeated rows from L2) and writes
 // n E elements, the backward reads n E elements once and writes V E.  8192 x 64 text-like tokens, half of them
-// padding, 200k x 256 fp32: forward 151 us (537 MB written, 128 MB read from memory; 86 us without the reads, 44
-// without the writes, and 152-161 for 1 to 16 tokens in flight, stores past the caches or not), sort 40 us, tiles
-// 70 us (344 MB, 4.9 TB/s), joins and empty rows 42 us (148 MB); a 4 GiB copy runs at 4.8 TB/s.  The backward needs each
-// row's tokens together: a long call sorts them (the bags' stable counting sort, token_plan_build), a short one
-// finds them among the ids in LDS.
+// padding, 200k x 256 fp32: forward 150 us (537 MB written, 128 MB read from memory; 86 us without the reads, 44
+// without the writes; eight tokens in flight instead of four 164), sort 40 us, tiles 70 us (344 MB, 4.9 TB/s), joins and
+// empty rows 42 us (148 MB); a 4 GiB copy runs at 4.8 TB/s.  The backward needs each row's tokens together: a long
+// call sorts them (the bags' stable counting sort, token_plan_build), a short one finds them among the ids in LDS.
 #include "common.hpp"
 
 #include <algorithm>

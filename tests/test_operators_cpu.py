@@ -238,6 +238,26 @@ def test_data_parallel_clipping_uses_the_global_gradient():
             assert abs(torch.from_numpy(a) - b).max() < 1e-12
 
 
+def test_a_capture_waits_for_the_watchdogs_of_gpu_groups(monkeypatch):
+    """Only groups whose watchdog queries events are waited for (gloo has none), and none without a group."""
+    from twotower_amd import distributed
+
+    waited = []
+
+    class Group:
+        def __init__(self, kind):
+            self.kind = kind
+
+        def _wait_for_pending_works(self):
+            waited.append(self.kind)
+
+    distributed.settle_watchdogs()  # no process group
+    monkeypatch.setattr(distributed, "_backend_kind", lambda g: g.kind)
+    distributed.settle_watchdogs([Group("gloo"), Group("nccl"), Group("other"), Group("nccl")])
+    assert waited == ["nccl", "nccl"]
+    assert hasattr(torch.distributed.ProcessGroup, "_wait_for_pending_works")
+
+
 # ---------------------------------------------------------------------------------------------
 # C ABI
 

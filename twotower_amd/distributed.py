@@ -78,6 +78,21 @@ def capture_blocker(group=None) -> str | None:
     return None
 
 
+def settle_watchdogs(groups=None) -> None:
+    """Before a graph capture, once the device is idle: wait until no process group's watchdog has a finished
+    collective left to look at (it passes every 100 ms).  The collective's end event was recorded on the
+    group's own stream; while that stream takes part in a capture the event counts as one "last recorded in a
+    capturing stream", and the watchdog's query of it fails and ends the process.  Collectives recorded during
+    the capture are not in its list.  groups: the process groups (default: all of this process)."""
+    if groups is None:
+        if not (dist.is_available() and dist.is_initialized()):
+            return
+        groups = list(dist.distributed_c10d._world.pg_map)
+    for g in groups:
+        if _backend_kind(g) == "nccl":
+            g._wait_for_pending_works()
+
+
 def is_active(group=None) -> bool:
     """Data-parallel exchanges on: more than one rank, or TT_DIST_FORCE=1 with any initialised
     group (a one-rank rehearsal of every collective of the N-rank step, e.g. RCCL under HIP-graph

@@ -18,7 +18,7 @@ import os
 import torch
 
 from . import ops
-from .distributed import GradSync, capture_blocker, is_active
+from .distributed import GradSync, capture_blocker, is_active, settle_watchdogs
 from .losses import scorer_prep_dtype
 from .optim import clip_grad_norm_
 
@@ -213,6 +213,7 @@ class TrainStep:
             dst.copy_(src)
         graph = torch.cuda.CUDAGraph()
         torch.cuda.synchronize()
+        settle_watchdogs()
         # thread-local capture mode: a process group's watchdog thread polls the events of the
         # collectives issued before the capture (hipEventQuery); under the default global mode
         # that query is refused while this thread captures and the watchdog aborts the process

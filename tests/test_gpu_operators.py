@@ -1073,3 +1073,20 @@ def test_search_with_a_4_bit_index(group, tmp_path):
     r.index_document_ids(docs[:50])  # its own kind of index replaces the loaded one
     assert r.index is None and r.search_ids(queries, top_k=60)[0].shape == (9, 50)
     assert torch.equal(again, scores) and torch.equal(idx2, idx)
+
+
+def test_empty_calls():
+    """No token, pair, element, query or row: empty results, a loss and a norm of 0."""
+    w = torch.randn(5, 8, device=DEV, requires_grad=True)
+    out = ops.embedding_lookup(w, torch.empty(0, 3, dtype=torch.int64, device=DEV))
+    assert out.shape == (0, 3, 8) and not torch.autograd.grad(out.sum(), w)[0].any()
+    q, p, n = (torch.empty(s, device=DEV, requires_grad=True) for s in ((0, 8), (0, 8), (0, 2, 8)))
+    loss = losses.preference_loss(q, p, n)
+    assert loss.item() == 0.0 and [g.shape for g in torch.autograd.grad(loss, (q, p, n))] == [q.shape, p.shape, n.shape]
+    assert losses.preference_margin(q, p, n).shape == (0, 2)
+    empty = torch.empty(0, device=DEV)
+    assert ops.clip_grad_norm([empty, empty.clone()], 1.0).item() == 0.0 == ops.clip_grad_norm([empty], None).item()
+    rows = ops.Int4Rows.quantize(torch.empty(0, 40, device=DEV))
+    assert ops.int4_scores(torch.randn(3, 40, device=DEV), rows).shape == (3, 0) and rows.dequantize().shape == (0, 40)
+    rows = ops.Int4Rows.quantize(torch.randn(4, 40, device=DEV))
+    assert ops.int4_scores(torch.empty(0, 40, device=DEV), rows).shape == (0, 4)

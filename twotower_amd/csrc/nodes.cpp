@@ -13,7 +13,6 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
-#include <cmath>
 #include <optional>
 #include <unordered_set>
 

@@ -581,6 +581,73 @@ def test_preference_on_views_that_are_their_own_leaves():
     assert not g[:20].any() and torch.equal(g[20:40], got[1]) and torch.equal(g[40:], got[2])
 
 
+class _Halved(torch.autograd.Function):
+    """A view whose gradient is scaled (gradient scaling or reversal layers have this form)."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, g):
+        return g * 0.5
+
+
+@pytest.mark.parametrize("split", [torch.split, ops.split_rows])
+@pytest.mark.parametrize("K", [1, 3])
+def test_preference_sees_what_autograd_has_on_the_blocks(K, split):
+    """Blocks of one tensor: a function between a block and the loss, hooks, retained gradients, and gradients with
+    respect to the blocks, against the same loss of separate tensors."""
+    B, H = 37, 48
+    x = torch.randn((2 + K) * B, H, generator=gen(29), device=DEV)
+
+    def blocks():
+        leaf = x.clone().requires_grad_(True)
+        return leaf, list(split(leaf * 1.0, [B, B, K * B]))
+
+    def loss(q, p, n):
+        return losses.preference_loss(q, p, n if K == 1 else n.view(B, K, H), beta=0.5)
+
+    alone = [t.clone().requires_grad_(True) for t in x.split([B, B, K * B])]
+    want = torch.autograd.grad(loss(*alone), alone)
+    leaf, parts = blocks()
+    (got,) = torch.autograd.grad(loss(*parts), leaf)
+    assert torch.equal(got, torch.cat(want))
+    leaf, parts = blocks()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss(*parts), parts), want))
+    for i in range(3):
+        leaf, parts = blocks()
+        out = loss(*[_Halved.apply(t) if j == i else t for j, t in enumerate(parts)])
+        (got,) = torch.autograd.grad(out, leaf)
+        assert torch.equal(got, torch.cat([w * (0.5 if j == i else 1.0) for j, w in enumerate(want)]))
+        leaf, parts = blocks()
+        seen = []
+        parts[i].register_hook(lambda g: seen.append(g.clone()))
+        parts[i].register_hook(lambda g: g * 4.0)
+        parts[(i + 1) % 3].retain_grad()
+        loss(*parts).backward()
+        assert torch.equal(seen[0], want[i]) and torch.equal(parts[(i + 1) % 3].grad, want[(i + 1) % 3])
+        assert torch.equal(leaf.grad, torch.cat([w * (4.0 if j == i else 1.0) for j, w in enumerate(want)]))
+
+
+def test_preference_gradient_of_the_tower_output_is_not_copied():
+    torch.manual_seed(30)
+    emb = tt.embeddings.build("lookup", vocab_size=60, embedding_dim=64)
+    model = tt.build_two_tower("mean", emb, hidden_dim=128, tied_weights=True).to(DEV)
+    ids = torch.randint(1, 60, (3, 20, 8), generator=gen(30), device=DEV)
+    q, p, n = model(*ids)
+    base = q._base
+    base.retain_grad()
+    seen = []
+    q.register_hook(lambda g: seen.append(g.data_ptr()))
+    whole = []
+    base.register_hook(lambda g: whole.append(g.data_ptr()))
+    losses.preference_loss(q, p, n, beta=0.5).backward()
+    assert seen == whole  # the loss's own buffer
+    alone = [t.detach().requires_grad_(True) for t in (q, p, n)]
+    assert torch.equal(base.grad, torch.cat(torch.autograd.grad(losses.preference_loss(*alone, beta=0.5), alone)))
+
+
 def test_preference_margin_is_the_reference_term():
     q, p, n, _, _ = pref_case(77, 48, 2, BF16, False, 0.0, 25)
     r = losses.preference_margin(q.requires_grad_(True), p, n, temperature=0.1)

@@ -258,6 +258,95 @@ def test_a_capture_waits_for_the_watchdogs_of_gpu_groups(monkeypatch):
     assert hasattr(torch.distributed.ProcessGroup, "_wait_for_pending_works")
 
 
+class _Halved(torch.autograd.Function):
+    """A view whose gradient is scaled (gradient scaling or reversal layers have this form)."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, g):
+        return g * 0.5
+
+
+def _buffer_node(seen=None):
+    """A loss of consecutive blocks whose gradients are blocks of one buffer (as preference_loss's are)."""
+
+    class Node(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, *blocks):
+            ctx.save_for_backward(*blocks)
+            return sum((b ** 2).sum() for b in blocks)
+
+        @staticmethod
+        def backward(ctx, g):
+            whole = 2 * g * torch.cat([b.reshape(-1, b.shape[-1]) for b in ctx.saved_tensors])
+            if seen is not None:
+                seen.append(whole)
+            out, at = [], 0
+            for b in ctx.saved_tensors:
+                rows = b.numel() // b.shape[-1]
+                out.append(whole[at:at + rows].view(b.shape))
+                at += rows
+            return tuple(out)
+
+    return Node.apply
+
+
+def _split_case(sizes=(3, 3, 6)):
+    x = torch.randn(sum(sizes), 4, dtype=torch.float64, requires_grad=True)
+    y = x * 1.0
+    return x, y, _lib.nodes().split_rows(y, list(sizes))
+
+
+def test_split_rows_is_torch_split():
+    x, y, blocks = _split_case((3, 0, 6))
+    assert [b.shape[0] for b in blocks] == [3, 0, 6] and all(b._base is y for b in blocks)
+    assert all(torch.equal(a, b) for a, b in zip(blocks, torch.split(y, [3, 0, 6])))
+    with pytest.raises(RuntimeError, match="inplace"):  # as torch.split's outputs
+        blocks[0].mul_(2)
+    (g,) = torch.autograd.grad((blocks[2] ** 3).sum(), x, create_graph=True)  # blocks without a gradient count zeros
+    assert torch.equal(g, torch.cat([torch.zeros(3, 4), 3 * x[3:] ** 2]))
+    (h,) = torch.autograd.grad(g.sum(), x)
+    assert torch.equal(h, torch.cat([torch.zeros(3, 4), 6 * x[3:]]))
+    for sizes in ([3, 4], [], [-1, 10], [10]):
+        with pytest.raises(ValueError, match="split_rows"):
+            _lib.nodes().split_rows(y, sizes)
+    assert torch.autograd.gradcheck(lambda t: _lib.nodes().split_rows(t, [2, 1]), torch.randn(3, 2, dtype=torch.float64,
+                                                                                             requires_grad=True))
+
+
+def test_split_rows_hands_one_buffer_on_without_a_copy():
+    seen = []
+    x, y, (a, b, c) = _split_case()
+    got = []
+    y.register_hook(lambda g: got.append((g.data_ptr(), torch.equal(g, 2 * y))))
+    _buffer_node(seen)(a, b, c.view(3, 2, 4)).backward()
+    assert got == [(seen[0].data_ptr(), True)]
+    x, y, (a, b, c) = _split_case()  # another order is joined
+    (g,) = torch.autograd.grad(_buffer_node()(b, a, c), y)
+    assert torch.equal(g, 2 * y)
+
+
+def test_split_rows_blocks_keep_what_autograd_has_on_them():
+    """Functions, hooks, retained gradients and other uses of a block, and gradients with respect to the blocks."""
+    node = _buffer_node()
+    x, y, (a, b, c) = _split_case()
+    (g,) = torch.autograd.grad(node(_Halved.apply(a), b, c), x)
+    assert torch.equal(g, torch.cat([x[:3], 2 * x[3:]]))
+    x, y, (a, b, c) = _split_case()
+    b.register_hook(lambda g: g * 3)
+    a.retain_grad()
+    node(a, b, c).backward()
+    assert torch.equal(x.grad, torch.cat([2 * x[:3], 6 * x[3:6], 2 * x[6:]])) and torch.equal(a.grad, 2 * a)
+    x, y, blocks = _split_case()
+    assert all(torch.equal(g, 2 * t) for g, t in zip(torch.autograd.grad(node(*blocks), blocks), blocks))
+    x, y, (a, b, c) = _split_case()
+    (g,) = torch.autograd.grad(node(a, b, c) + (5 * b).sum(), x)
+    assert torch.equal(g, torch.cat([2 * x[:3], 2 * x[3:6] + 5, 2 * x[6:]]))
+
+
 # ---------------------------------------------------------------------------------------------
 # C ABI
 

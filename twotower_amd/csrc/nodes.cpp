@@ -270,50 +270,112 @@ void pref_grad(const Tensor& q, const Tensor& p, const Tensor& n, const Tensor& 
          (float)inv_tau, s, s + B * K, as<const float>(g), as<void>(dq), as<void>(dp), as<void>(dn));
 }
 
+// t[0], t[1], ... are contiguous and follow each other in one storage
+bool consecutive(at::ArrayRef<Tensor> t) {
+  for (size_t i = 0; i < t.size(); ++i) {
+    if (!t[i].is_contiguous()) return false;
+    if (i && (t[i].scalar_type() != t[0].scalar_type() || !t[i].is_alias_of(t[0]) ||
+              t[i].storage_offset() != t[i - 1].storage_offset() + t[i - 1].numel()))
+      return false;
+  }
+  return true;
+}
+
+Tensor pref_forward(AutogradContext* ctx, const Tensor& q, const Tensor& p, const Tensor& n, const PrefArgs& a) {
+  const Tensor loss = at::empty({}, q.options().dtype(at::kFloat));
+  ctx->save_for_backward({q, p, n, a.mask, pref_loss(q, p, n, a, loss)});
+  ctx->saved_data["inv_tau"] = a.inv_tau;
+  return loss;
+}
+
+variable_list pref_backward(AutogradContext* ctx, const variable_list& g, bool one_buffer) {
+  no_second_derivative("preference_loss");
+  const auto s = ctx->get_saved_variables();
+  const Tensor &q = s[0], &p = s[1], &n = s[2];
+  Tensor dq, dp, dn;
+  if (one_buffer) {
+    const int64_t B = q.size(0);
+    const Tensor all = at::empty({B * (2 + n.size(1)), q.size(1)}, q.options());
+    dq = all.narrow(0, 0, B);
+    dp = all.narrow(0, B, B);
+    dn = all.narrow(0, 2 * B, B * n.size(1)).view(n.sizes());
+  } else {
+    auto like = [](const Tensor& t) { return at::empty_like(t, {}, at::MemoryFormat::Contiguous); };
+    dq = like(q);
+    dp = like(p);
+    dn = like(n);
+  }
+  pref_grad(q, p, n, s[3], ctx->saved_data["inv_tau"].toDouble(), s[4], g[0], dq, dp, dn);
+  return {dq, dp, dn, Tensor()};
+}
+
 struct PreferenceLoss : Function<PreferenceLoss> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& p, const Tensor& n,
-                        const PrefArgs& a) {
-    const Tensor loss = at::empty({}, q.options().dtype(at::kFloat));
-    ctx->save_for_backward({q, p, n, a.mask, pref_loss(q, p, n, a, loss)});
-    ctx->saved_data["inv_tau"] = a.inv_tau;
-    return loss;
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& p, const Tensor& n, const PrefArgs& a) {
+    return pref_forward(ctx, q, p, n, a);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) { return pref_backward(ctx, g, false); }
+};
+
+// The same loss of consecutive row blocks of one tensor (TwoTower's fused output): the three gradients are
+// written as consecutive blocks too, which SplitRows hands on whole.
+struct PreferenceLossPacked : Function<PreferenceLossPacked> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& p, const Tensor& n, const PrefArgs& a) {
+    return pref_forward(ctx, q, p, n, a);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) { return pref_backward(ctx, g, true); }
+};
+
+// x cut into consecutive row blocks, as torch.split does, but gradients that are consecutive blocks of one buffer
+// again (PreferenceLossPacked's) are that buffer: no launch and no copy (torch.split joins them by a cat: 25 MB read
+// and written for 3 x 8192 x 256 floats).  Whatever autograd has between the blocks and the loss -- a hook, a retained
+// gradient, a function of the caller's -- sees its own block's gradient.
+struct SplitRows : Function<SplitRows> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, std::vector<int64_t> sizes) {
+    ctx->set_materialize_grads(false);
+    variable_list blocks;
+    int64_t at = 0;
+    for (const int64_t n : sizes) {
+      blocks.push_back(x.narrow(0, at, n));
+      at += n;
+    }
+    ctx->saved_data["sizes"] = sizes;
+    auto shape = x.sizes().vec();
+    shape[0] = 0;
+    ctx->saved_data["like"] = at::empty(shape, x.options());  // (type and width, for a block without a gradient)
+    return blocks;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    no_second_derivative("preference_loss");
-    const auto s = ctx->get_saved_variables();
-    auto like = [](const Tensor& t) { return at::empty_like(t, {}, at::MemoryFormat::Contiguous); };
-    const Tensor dq = like(s[0]), dp = like(s[1]), dn = like(s[2]);
-    pref_grad(s[0], s[1], s[2], s[3], ctx->saved_data["inv_tau"].toDouble(), s[4], g[0], dq, dp, dn);
-    return {dq, dp, dn, Tensor()};
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    const Tensor like = ctx->saved_data["like"].toTensor();
+    int64_t rows = 0;
+    bool all = true;
+    for (size_t i = 0; i < g.size(); ++i) {
+      rows += sizes[i];
+      all = all && g[i].defined();
+    }
+    auto shape = like.sizes().vec();
+    shape[0] = rows;
+    if (all && !at::GradMode::is_enabled() && consecutive(g))
+      return {g[0].as_strided(shape, at::detail::defaultStrides(shape), g[0].storage_offset()), Tensor()};
+    for (size_t i = 0; i < g.size(); ++i)
+      if (!g[i].defined()) {
+        shape[0] = sizes[i];
+        g[i] = at::zeros(shape, like.options());
+      }
+    return {at::cat(g, 0), Tensor()};
   }
 };
 
-// The same loss on one ((2 + K) B, H) tensor [q; p; negatives] (TwoTower's fused output): the
-// three gradients are written into one tensor, so autograd runs no split backward.
-struct PreferenceLossPacked : Function<PreferenceLossPacked> {
-  static std::array<Tensor, 3> blocks(const Tensor& t, int64_t B, int64_t K) {
-    return {t.narrow(0, 0, B), t.narrow(0, B, B), t.narrow(0, 2 * B, B * K).view({B, K, t.size(1)})};
+variable_list split_rows(const Tensor& x, std::vector<int64_t> sizes) {
+  int64_t rows = 0;
+  for (const int64_t n : sizes) {
+    TORCH_CHECK_VALUE(n >= 0, "split_rows: a block of ", n, " rows");
+    rows += n;
   }
-  static Tensor forward(AutogradContext* ctx, const Tensor& qpn, int64_t B, int64_t K, const PrefArgs& a) {
-    const Tensor loss = at::empty({}, qpn.options().dtype(at::kFloat));
-    const auto [q, p, n] = blocks(qpn, B, K);
-    ctx->save_for_backward({qpn, a.mask, pref_loss(q, p, n, a, loss)});
-    ctx->saved_data["inv_tau"] = a.inv_tau;
-    ctx->saved_data["B"] = B;
-    ctx->saved_data["K"] = K;
-    return loss;
-  }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
-    no_second_derivative("preference_loss");
-    const auto s = ctx->get_saved_variables();
-    const int64_t B = ctx->saved_data["B"].toInt(), K = ctx->saved_data["K"].toInt();
-    const Tensor grad = at::empty_like(s[0], {}, at::MemoryFormat::Contiguous);
-    const auto [q, p, n] = blocks(s[0], B, K);
-    const auto [dq, dp, dn] = blocks(grad, B, K);
-    pref_grad(q, p, n, s[1], ctx->saved_data["inv_tau"].toDouble(), s[2], g[0], dq, dp, dn);
-    return {grad, Tensor(), Tensor(), Tensor()};
-  }
-};
+  TORCH_CHECK_VALUE(x.dim() >= 1 && !sizes.empty() && rows == x.size(0), "split_rows: blocks of ", rows,
+                    " rows for shape ", x.sizes());
+  return SplitRows::apply(x, std::move(sizes));
+}
 
 // (q, p, n with a pair axis) of a checked call, rows of contiguous elements
 std::array<Tensor, 3> pref_args(const Tensor& q, const Tensor& p, const Tensor& n) {
@@ -347,14 +409,15 @@ Tensor pref_pairs(const std::optional<Tensor>& t, const char* name, ScalarType t
 }
 
 Tensor preference_loss(const Tensor& q_, const Tensor& p_, const Tensor& n_, const std::optional<Tensor>& ref_margin,
-                       const std::optional<Tensor>& mask_, int64_t kind, double beta, double inv_tau, double smooth,
-                       const std::optional<Tensor>& packed) {
+                       const std::optional<Tensor>& mask_, int64_t kind, double beta, double inv_tau, double smooth) {
   const auto [q, p, n] = pref_args(q_, p_, n_);
   const Tensor ref = pref_pairs(ref_margin, "ref_margin", ScalarType::Float, n);
   const Tensor mask = pref_pairs(mask_, "mask", ScalarType::Bool, n);
   check_gpu(q, {&p, &n});
   const PrefArgs a{ref, mask, kind, beta, inv_tau, smooth};
-  return packed ? PreferenceLossPacked::apply(*packed, n.size(0), n.size(1), a) : PreferenceLoss::apply(q, p, n, a);
+  // (leaves keep gradients of their own memory)
+  const bool packed = !q.is_leaf() && !p.is_leaf() && !n.is_leaf() && consecutive({q, p, n});
+  return packed ? PreferenceLossPacked::apply(q, p, n, a) : PreferenceLoss::apply(q, p, n, a);
 }
 
 Tensor preference_margin(const Tensor& q_, const Tensor& p_, const Tensor& n_, double inv_tau) {
@@ -448,5 +511,6 @@ PYBIND11_MODULE(_nodes, m) {
   m.def("embedding_lookup", &embedding_lookup, unlocked);
   m.def("preference_loss", &preference_loss, unlocked);
   m.def("preference_margin", &preference_margin, unlocked);
+  m.def("split_rows", &split_rows, unlocked);
   m.def("clip_grad_norm", &clip_grad_norm, unlocked);
 }

@@ -214,11 +214,11 @@ class TwoTower(nn.Module):
                 prep = ops.scorer_prep(nq, self.scorer_prep) if self.scorer_prep else contextlib.nullcontext()
                 with prep, _sole_head(self.query_tower, pooled):
                     # one head over all rows: its normalise pass may also prep the in-batch scorer
-                    return list(torch.split(self.query_tower.encode_pooled(pooled), sizes, dim=0))
+                    return list(ops.split_rows(self.query_tower.encode_pooled(pooled), sizes))
         pooled = pool_mean(self.query_tower.embedding, all_ids)
         q = self.query_tower.encode_pooled(pooled[:nq])
         docs = self.document_tower.encode_pooled(pooled[nq:])
-        return [q] + list(torch.split(docs, sizes[1:], dim=0))
+        return [q] + list(ops.split_rows(docs, sizes[1:]))
 
     def encode_query(self, query_input):
         return self.query_tower(query_input)

@@ -81,23 +81,7 @@ def preference_loss(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg_embs: to
     bool, False for a missing pair, whose row is not read (it may hold anything), counts nothing and gets
     a zero gradient; with no pair left the loss is 0.  Data parallel: each rank's mean is over its own pairs."""
     return ops.preference_loss(q_emb, d_pos_emb, d_neg_embs, ref_margin=ref_margin, mask=mask, beta=beta,
-                               temperature=temperature, label_smoothing=label_smoothing, loss_type=loss_type,
-                               packed=_packed_pairs(q_emb, d_pos_emb, d_neg_embs) if q_emb._base is not None else None)
-
-
-def _packed_pairs(q: torch.Tensor, p: torch.Tensor, n: torch.Tensor) -> torch.Tensor | None:
-    """The tensor whose consecutive row blocks are q, p and n (TwoTower's fused output), where one gradient of
-    it stands for theirs: not for leaves that are views of a plain tensor, nor for views taken under
-    no_grad, where autograd would not bring it there."""
-    if q.dim() != 2 or p.shape != q.shape or n.dim() not in (2, 3) or not n.is_contiguous():
-        return None
-    B, K = q.shape[0], 1 if n.dim() == 2 else n.shape[1]
-    if not B or not K or n.numel() != B * K * q.shape[1]:
-        return None
-    base = _packed(q, p, n.view(B * K, -1))
-    if base is None or any(v.is_leaf == base.requires_grad or v.requires_grad != base.requires_grad for v in (q, p, n)):
-        return None
-    return base
+                               temperature=temperature, label_smoothing=label_smoothing, loss_type=loss_type)
 
 
 def preference_margin(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg_embs: torch.Tensor,

@@ -1134,12 +1134,18 @@ def _pref_opts(beta, temperature, label_smoothing, loss_type):
 
 def preference_loss(q: torch.Tensor, p: torch.Tensor, n: torch.Tensor, ref_margin: torch.Tensor | None = None,
                     mask: torch.Tensor | None = None, beta: float = 0.1, temperature: float = 0.1,
-                    label_smoothing: float = 0.0, loss_type: str = "sigmoid",
-                    packed: torch.Tensor | None = None) -> torch.Tensor:
-    """losses.preference_loss on the HIP row kernels.  packed: the one tensor [q; p; n] that q, p and n are
-    the consecutive row blocks of, which then receives the gradient."""
+                    label_smoothing: float = 0.0, loss_type: str = "sigmoid") -> torch.Tensor:
+    """losses.preference_loss on the HIP row kernels."""
     return _lib.nodes().preference_loss(q, p, n, ref_margin, mask,
-                                        *_pref_opts(beta, temperature, label_smoothing, loss_type), packed)
+                                        *_pref_opts(beta, temperature, label_smoothing, loss_type))
+
+
+def split_rows(x: torch.Tensor, sizes) -> tuple[torch.Tensor, ...]:
+    """torch.split(x, sizes, dim=0), whose backward does not copy gradients that already lie in one buffer
+    (preference_loss writes its three so)."""
+    if not (x.is_cuda and x.requires_grad and torch.is_grad_enabled()):
+        return torch.split(x, list(sizes), dim=0)
+    return tuple(_lib.nodes().split_rows(x, list(sizes)))
 
 
 def preference_margin(q: torch.Tensor, p: torch.Tensor, n: torch.Tensor, temperature: float = 0.1) -> torch.Tensor:

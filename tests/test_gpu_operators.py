@@ -630,6 +630,38 @@ def test_preference_sees_what_autograd_has_on_the_blocks(K, split):
         assert torch.equal(leaf.grad, torch.cat([w * (4.0 if j == i else 1.0) for j, w in enumerate(want)]))
 
 
+@pytest.mark.parametrize("name", ["triplet", "multiple_negatives", "in_batch"])
+def test_contrastive_losses_see_what_autograd_has_on_the_blocks(name):
+    B, H = 32, 64
+    x = torch.randn(3 * B, H, generator=gen(31), device=DEV)
+    fn = losses.build(name)
+
+    def blocks():
+        leaf = x.clone().requires_grad_(True)
+        return leaf, list(torch.split(leaf * 1.0, B))
+
+    alone = [t.clone().requires_grad_(True) for t in x.split(B)]
+    want = torch.autograd.grad(fn(*alone), alone)
+
+    def same(got, scale):  # (the two forms of a loss may differ by roundings)
+        for j, w in enumerate(want):
+            assert (got[j * B:(j + 1) * B] - scale[j] * w).norm() <= 1e-5 * w.norm()
+
+    leaf, parts = blocks()
+    same(torch.autograd.grad(fn(*parts), leaf)[0], (1, 1, 1))
+    for i in range(3):
+        scale = [0.5 if j == i else 1.0 for j in range(3)]
+        leaf, parts = blocks()
+        same(torch.autograd.grad(fn(*[_Halved.apply(t) if j == i else t for j, t in enumerate(parts)]), leaf)[0], scale)
+        leaf, parts = blocks()
+        parts[i].register_hook(lambda g: g * 0.5)
+        same(torch.autograd.grad(fn(*parts), leaf)[0], scale)
+        leaf, parts = blocks()
+        parts[i].retain_grad()
+        fn(*parts).backward()
+        assert (parts[i].grad - want[i]).norm() <= 1e-5 * want[i].norm()
+
+
 def test_preference_gradient_of_the_tower_output_is_not_copied():
     torch.manual_seed(30)
     emb = tt.embeddings.build("lookup", vocab_size=60, embedding_dim=64)

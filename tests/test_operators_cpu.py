@@ -347,6 +347,48 @@ def test_split_rows_blocks_keep_what_autograd_has_on_them():
     assert torch.equal(g, torch.cat([2 * x[:3], 2 * x[3:6] + 5, 2 * x[6:]]))
 
 
+def _base_and_blocks(split=torch.split):
+    y = torch.randn(12, 4, requires_grad=True) * 1.0
+    return y, list(split(y, [3, 3, 6]))
+
+
+@pytest.mark.parametrize("split", [torch.split, _lib.nodes().split_rows, lambda y, s: (y[:3], y.narrow(0, 3, 3), y[6:])])
+def test_losses_take_the_base_only_where_it_stands_for_its_views(split):
+    """The losses that differentiate the common tensor of q, p and n: whatever autograd has on a view must not be
+    passed by."""
+    y, (q, p, n) = _base_and_blocks(split)
+    assert losses._packed(q, p, n) is y and losses._packed(q, p, n.view(3, 2, 4).view(6, 4)) is y
+    assert losses._candidates(p, n)._base is y
+    assert losses._packed(_Halved.apply(q), p, n) is None
+    assert losses._packed(q, p, _Halved.apply(n)) is None
+    assert losses._candidates(_Halved.apply(p), n)._base is None
+    p.register_hook(lambda g: g * 2)
+    assert losses._packed(q, p, n) is None and losses._candidates(p, n)._base is None
+    y, (q, p, n) = _base_and_blocks(split)
+    n.retain_grad()
+    assert losses._packed(q, p, n) is None and losses._candidates(p, n)._base is None
+    y, (q, p, n) = _base_and_blocks(split)
+    m = n.view(3, 2, 4)
+    m.register_hook(lambda g: None)
+    assert losses._packed(q, p, m.view(6, 4)) is None
+    with torch.no_grad():
+        assert losses._packed(y[:3], p, n) is None and losses._candidates(y[3:6], n)._base is None
+        assert losses._packed(*(t.detach() for t in (q, p, n))) is None  # (the base still needs its gradient)
+    x = torch.randn(12, 4)
+    q, p, n = split(x, [3, 3, 6])
+    assert losses._packed(q, p, n) is x  # no gradient anywhere
+    assert losses._packed(q.requires_grad_(True), p, n) is None
+
+
+def test_candidates_keep_what_autograd_has_on_them():
+    y, (q, p, n) = _base_and_blocks()
+    out = losses._candidates(p, n)
+    (want,) = torch.autograd.grad((out * torch.arange(9.0)[:, None]).sum(), y, retain_graph=True)
+    out = losses._candidates(_Halved.apply(p), n)
+    (got,) = torch.autograd.grad((out * torch.arange(9.0)[:, None]).sum(), y)
+    assert torch.equal(got[3:6], 0.5 * want[3:6]) and torch.equal(got[6:], want[6:])
+
+
 # ---------------------------------------------------------------------------------------------
 # C ABI
 

@@ -14,6 +14,7 @@
 #include <torch/extension.h>
 
 #include <optional>
+#include <string>
 #include <unordered_set>
 
 #include "twotower_amd.h"
@@ -377,6 +378,33 @@ variable_list split_rows(const Tensor& x, std::vector<int64_t> sizes) {
   return SplitRows::apply(x, std::move(sizes));
 }
 
+// Whether all of autograd between base and each view are torch's own slices and reshapes (or split_rows): a gradient
+// of base then stands for the views'.  Not with a hook or a retained gradient on the way, nor a function of the
+// caller's that returns a view, nor for a view that is a leaf of its own or was taken under no_grad.
+bool direct_views(const Tensor& base, const std::vector<Tensor>& views) {
+  static const std::unordered_set<std::string> slices = {
+      "SplitBackward0", "SplitWithSizesBackward0", "UnsafeSplitBackward0", "UnsafeSplitWithSizesBackward0",
+      "SliceBackward0", "ViewBackward0", "UnsafeViewBackward0", "ReshapeAliasBackward0", "AliasBackward0",
+      "UnsqueezeBackward0"};
+  using torch::autograd::Node;
+  for (const Tensor& v : views)
+    if (v.requires_grad() != base.requires_grad()) return false;
+  if (!base.requires_grad()) return true;
+  const auto to = torch::autograd::impl::gradient_edge(base);
+  for (const Tensor& v : views) {
+    auto at = torch::autograd::impl::gradient_edge(v);
+    while (!(at == to)) {
+      Node* const node = at.function.get();
+      if (!node || node->num_outputs() != 1 || !node->tensor_pre_hooks().empty() || !node->pre_hooks().empty() ||
+          !node->post_hooks().empty() || !node->retains_grad_hooks().empty() ||
+          !(slices.count(node->name()) || dynamic_cast<torch::autograd::CppNode<SplitRows>*>(node)))
+        return false;
+      at = node->next_edge(0);
+    }
+  }
+  return true;
+}
+
 // (q, p, n with a pair axis) of a checked call, rows of contiguous elements
 std::array<Tensor, 3> pref_args(const Tensor& q, const Tensor& p, const Tensor& n) {
   TORCH_CHECK_VALUE(q.dim() == 2 && p.sizes() == q.sizes(), "q and p must both be (B, H), got ", q.sizes(), " and ",
@@ -512,5 +540,6 @@ PYBIND11_MODULE(_nodes, m) {
   m.def("preference_loss", &preference_loss, unlocked);
   m.def("preference_margin", &preference_margin, unlocked);
   m.def("split_rows", &split_rows, unlocked);
+  m.def("direct_views", &direct_views);
   m.def("clip_grad_norm", &clip_grad_norm, unlocked);
 }

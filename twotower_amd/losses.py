@@ -17,14 +17,15 @@ from typing import Callable
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 logger = logging.getLogger("twotower_amd.losses")
 
 
 def _packed(*views: torch.Tensor) -> torch.Tensor | None:
     """The common base when the views are consecutive, equally wide row blocks of one contiguous
-    2-D tensor in order (TwoTower's fused output split into q, p, n); else None."""
+    2-D tensor in order (TwoTower's fused output split into q, p, n) and autograd would bring their
+    gradients to it unchanged (_direct); else None."""
     base = views[0]._base
     if base is None or base.dim() != 2 or not base.is_contiguous():
         return None
@@ -38,7 +39,15 @@ def _packed(*views: torch.Tensor) -> torch.Tensor | None:
         at += v.shape[0] * row
     if at != base.data_ptr() + base.shape[0] * row:
         return None
-    return base
+    return base if _direct(base, *views) else None
+
+
+def _direct(base: torch.Tensor, *views: torch.Tensor) -> bool:
+    """Whether the base may be differentiated in place of its views: no function, hook or retained gradient
+    of the caller's is between them."""
+    if not base.requires_grad and not any(v.requires_grad for v in views):
+        return True
+    return _lib.nodes().direct_views(base, views)
 
 
 def contrastive_triplet_loss(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg_emb: torch.Tensor,
@@ -99,7 +108,8 @@ def _candidates(p: torch.Tensor, n: torch.Tensor) -> torch.Tensor:
             and p.is_contiguous() and n.is_contiguous() and p.shape[1] == base.shape[1] == n.shape[1]):
         row = base.shape[1] * base.element_size()
         start = (p.data_ptr() - base.data_ptr()) // row
-        if (p.data_ptr() - base.data_ptr()) % row == 0 and n.data_ptr() == p.data_ptr() + p.shape[0] * row:
+        if ((p.data_ptr() - base.data_ptr()) % row == 0 and n.data_ptr() == p.data_ptr() + p.shape[0] * row
+                and _direct(base, p, n)):
             return base.narrow(0, start, p.shape[0] + n.shape[0])
     return torch.cat([p, n], dim=0)
 

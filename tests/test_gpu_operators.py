@@ -198,6 +198,30 @@ def test_lookup_differentiated_twice(n, pad):
     assert torch.equal(dx, torch.where(keep[:, None], 8 * (w.detach() * c)[ids], torch.zeros((), device=DEV)))
 
 
+@pytest.mark.parametrize("dtype, out_dtype", [(F32, None), (F32, BF16), (F16, None)])
+@pytest.mark.parametrize("leaf", [False, True])
+def test_lookup_of_a_dual_table(leaf, dtype, out_dtype):
+    """Forward mode: the rows' tangents are the tangent's rows, whether or not the table needs a gradient too."""
+    from torch.autograd import forward_ad
+
+    w, ids, _ = lookup_case(40, 24, (5, 9), dtype, torch.int64, out_dtype, 0, 0.0, 14)
+    ids[0, 0] = 40  # outside
+    t = torch.randn(24, 40, generator=gen(14), device=DEV).to(dtype).t()  # its own layout
+    w.requires_grad_(leaf)
+    with forward_ad.dual_level():
+        plain = ops.embedding_lookup(w, ids, 4.0, 0, out_dtype)  # no tangent
+        assert forward_ad.unpack_dual(plain).tangent is None
+        out = ops.embedding_lookup(forward_ad.make_dual(w, t), ids, 4.0, 0, out_dtype)
+        rows, tangent = forward_ad.unpack_dual(out)
+        assert torch.equal(rows, plain) and rows.requires_grad == leaf
+        assert torch.equal(tangent, ops.embedding_lookup(t.contiguous(), ids, 4.0, None, out_dtype))
+        if leaf:
+            d = torch.randn(rows.shape, generator=gen(15), device=DEV).to(rows.dtype)
+            assert torch.equal(*(torch.autograd.grad(x, w, d)[0] for x in (rows, plain)))
+    with pytest.raises(RuntimeError):  # a function transform's tensors have no memory of their own
+        torch.func.jvp(lambda x: ops.embedding_lookup(x, ids, 4.0, 0, out_dtype), (w.detach(),), (t.contiguous(),))
+
+
 def test_lookup_of_a_fused_table():
     """The fused update takes pooled lookups: a step that also differentiates a plain one is refused, a step with
     plain ones alone takes the dense gradient as any parameter does."""

@@ -11,6 +11,7 @@ import functools
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import call, launch, ptr, require_gpu, stream_of
@@ -558,11 +559,17 @@ def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0
 
     The gradient is dense: every row of the table, scale times the sum of its tokens' gradients in
     fp32 in a fixed order (bitwise reproducible), rounded once to the table's type; the row of
-    ``padding_idx`` (negative: from the end, as in torch) gets zeros.  It can be differentiated again."""
+    ``padding_idx`` (negative: from the end, as in torch) gets zeros.  It can be differentiated again, and
+    a forward-mode tangent of the table (torch.autograd.forward_ad) is looked up beside it."""
     col = getattr(weight, "_tt_column", None)
     if col is not None and col.stale:
         raise RuntimeError("embedding_lookup reads the whole table: this one is column-sharded and was updated since it was "
                            "last gathered; materialize() it first, or use bag_mean_pool")
+    if forward_ad._current_level >= 0:  # (the node knows no tangents, and a plain call would drop them)
+        primal, tangent = forward_ad.unpack_dual(weight)
+        if tangent is not None:
+            rows = embedding_lookup(primal, ids, scale, padding_idx, out_dtype)
+            return forward_ad.make_dual(rows, embedding_lookup(tangent.contiguous(), ids, scale, None, out_dtype))
     if col is not None or getattr(weight, "_tt_deferred", None) is not None:
         weight = _TableGate.apply(weight)
     return _lib.nodes().embedding_lookup(weight, ids, float(scale), padding_idx, out_dtype)

@@ -1025,6 +1025,31 @@ def test_int4_scores_query_scales_and_non_finite():
         assert not got[3, fine].any()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("nq", [1, 4, 12, 40])
+@pytest.mark.parametrize("ratio", [300.0, 3e4, 1e6])
+def test_int4_scores_beside_a_dominant_element(ratio, nq, dtype):
+    """One query element far above the others, at a column whose codes are zero: nothing of the others is lost but
+    what lies below 2^-39 of it."""
+    g = gen(48)
+    n, H = 300, 96
+    codes = torch.randint(-8, 8, (n, H), generator=g, device=DEV, dtype=torch.int8)
+    codes[:, 37] = 0
+    codes[0] = 0
+    codes[0, 70] = 7  # one product alone: exact but for the terms' sum and two roundings
+    scales = (torch.rand(n, 3, generator=g, device=DEV) + 0.1).to(BF16)
+    values = codes.double() * scales.double().repeat_interleave(32, 1)
+    q = (torch.randn(nq, H, generator=g, device=DEV) / ratio).to(dtype)
+    q[:, 37] = 1.0
+    got = ops.int4_scores(q, ops.Int4Rows.from_codes(codes, scales, 32))
+    q = q.double()
+    want, mass = q @ values.t(), q.abs() @ values.abs().t()
+    lost = 2.0 ** -39 * values.abs().sum(1)
+    # (2 (3 x 32 + 3) + 3 + 4) u as in check_scores, what the terms leave out beside it
+    check(got, want, 205 * U * mass + lost, "scores")
+    check(got[:, 0], want[:, 0], 10 * U * want[:, 0].abs() + lost[0], "one product")
+
+
 def test_int4_scores_offsets_beyond_32_bits():
     n, H = 34_000_000, 256  # 4.35 GB of codes
     codes = torch.zeros(n, H, dtype=torch.int8, device=DEV)

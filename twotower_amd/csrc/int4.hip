@@ -6,7 +6,7 @@
 // One or a few queries are bound by the index bytes (n (H / 2 + 2 H / group)); 256 codes a row leave no
 // time to widen each code to a float in vector instructions, so the inner sums run on the
 // matrix cores: codes are small integers, exact in fp16, and q is cut into three fp16 terms
-// (33 bits of it), so v_mfma_f32_16x16x32_f16 forms the sum of 32 exact products in fp32; the group's
+// (query_exponent says what they hold), so v_mfma_f32_16x16x32_f16 forms the sum of 32 exact products in fp32; the group's
 // scale multiplies that sum.  32 columns are the instruction's K and the smallest group.
 //
 // 1M x 256, group 32 (us for 1 / 16 / 64 queries): 30-36 / 47 / 118, for 148 MB of index and 4 MB of scores a
@@ -223,9 +223,14 @@ __device__ __forceinline__ f16x8 widen(uint32_t u) {
   return r.v;
 }
 
-// 2^3 <= max |q| 2^e < 2^4: the fp16 terms then reach 2^-27 of the largest element or 33 bits below the element
+// 2^14 <= max |q| 2^e < 2^15, as far up as fp16 goes.  The three terms take 11 bits each of a scaled element, but none
+// below fp16's least step 2^-24: fp32's 24 bits are whole from 2^-1 up, that is down to 2^-15 of the query's largest
+// element, and a smaller one is off by at most 2^-25, 2^-39 of the largest.  (Under 2^4 that was 2^-28: with zero codes at
+// a dominant column and the other elements 2^-15 of it scores were off by 1.7e-5 of their mass, in fp32 by 5e-8.
+// Terms with factors of their own, 1, 2^-11 and 2^-22, reach further, but the codes under each factor take vector
+// instructions: 64 queries, 1M x 256, 172 us instead of 118.)
 __device__ __forceinline__ int query_exponent(float mx) {
-  return mx > 0.f && mx <= 3.402823466e38f ? 3 - ilogbf(mx) : 0;
+  return mx > 0.f && mx <= 3.402823466e38f ? 14 - ilogbf(mx) : 0;
 }
 
 // What a wave loads for one quad of its tiles.

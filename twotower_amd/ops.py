@@ -1705,8 +1705,8 @@ def _int4_shape(n, H, group) -> tuple[int, int]:
 
 def int4_scores(q: torch.Tensor, rows: Int4Rows) -> torch.Tensor:
     """(nq, n) float32 products q_i . row_j of (nq, H) or (H,) float32 / bfloat16 / float16 queries with 4-bit
-    rows, in fp32 accuracy (the codes are exact, each query element keeps 33 bits or more than fp32 beside
-    the largest).  A query with a non-finite value scores NaN everywhere."""
+    rows, in fp32 (the codes are exact; a query's elements keep all their bits down to 2^-15 of its largest, smaller
+    ones are taken to within 2^-39 of that).  A query with a non-finite value scores NaN everywhere."""
     if q.dim() == 1:
         q = q.unsqueeze(0)
     if q.dim() != 2 or q.shape[1] != rows.H:

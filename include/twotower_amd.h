@@ -503,8 +503,8 @@ int tt_topk_rows_ex(const float* scores, int64_t nrows, int64_t ncols, int k, vo
  * tt_int4_scores: scores[i n + j] = sum_k q[i, k] value[j, k] for nq fp32 / bf16 / fp16 queries (row
  *   stride ldq): products of the codes with q (as three fp16 terms: every bit of an element down to 2^-15 of its
  *   query's largest, smaller ones to within 2^-39 of that) on the matrix cores, accumulated in fp32 per 32
- *   columns, scaled and added in fp32.  A query with a non-finite
- *   value scores NaN. */
+ *   columns, scaled and added in fp32.  Infinities and NaN in q act as in a product of floats (an infinity
+ *   times a zero code: NaN). */
 #define TT_INT4_MAX_H 4096
 size_t tt_int4_codes_bytes(int64_t n, int H);
 size_t tt_int4_scales_bytes(int64_t n, int H, int group);

@@ -1050,6 +1050,33 @@ def test_int4_scores_beside_a_dominant_element(ratio, nq, dtype):
     check(got[:, 0], want[:, 0], 10 * U * want[:, 0].abs() + lost[0], "one product")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("nq", [4, 12, 40])
+def test_int4_scores_of_infinite_queries(nq, dtype):
+    """Infinities as in a product of floats: signed by their codes, NaN at a zero code or against another one; the other
+    queries of the batch and finite elements beside them, however large, change nothing."""
+    g = gen(49)
+    n, H = 200, 80
+    codes = torch.randint(-8, 8, (n, H), generator=g, device=DEV, dtype=torch.int8)
+    codes[:20, 7] = 0
+    scales = (torch.rand(n, 2, generator=g, device=DEV) + 0.1).to(BF16)
+    scales[30, 0] = 0.0
+    values = codes.double() * scales.double().repeat_interleave(64, 1)[:, :H]
+    rows = ops.Int4Rows.from_codes(codes, scales, 64)
+    q = torch.randn(nq, H, generator=g, device=DEV).to(dtype)
+    plain = ops.int4_scores(q, rows)
+    q[0, 7] = math.inf
+    q[0, 70] = torch.finfo(dtype).max
+    q[1, [7, 60]] = torch.tensor([math.inf, -math.inf], device=DEV, dtype=dtype)
+    q[2, 7] = math.nan
+    q[3] = -math.inf
+    got = ops.int4_scores(q, rows)
+    want = (q.double().cpu() @ values.cpu().t()).to(DEV)
+    assert torch.equal(got[:4].isnan(), want[:4].isnan())
+    check(got[:4], want[:4], 0.0, "infinite")  # nothing is finite there
+    assert got[0].isinf().sum() > 150 and got[1].isinf().any() and torch.equal(got[4:], plain[4:])
+
+
 def test_int4_scores_offsets_beyond_32_bits():
     n, H = 34_000_000, 256  # 4.35 GB of codes
     codes = torch.zeros(n, H, dtype=torch.int8, device=DEV)

@@ -223,14 +223,14 @@ __device__ __forceinline__ f16x8 widen(uint32_t u) {
   return r.v;
 }
 
-// 2^14 <= max |q| 2^e < 2^15, as far up as fp16 goes.  The three terms take 11 bits each of a scaled element, but none
-// below fp16's least step 2^-24: fp32's 24 bits are whole from 2^-1 up, that is down to 2^-15 of the query's largest
-// element, and a smaller one is off by at most 2^-25, 2^-39 of the largest.  (Under 2^4 that was 2^-28: with zero codes at
+// 2^14 <= max |q| 2^e < 2^15 over a query's finite elements, as far up as fp16 goes.  The three terms take 11 bits each
+// of a scaled element, but none below fp16's least step 2^-24: fp32's 24 bits are whole from 2^-1 up, that is down to
+// 2^-15 of the query's largest element, and a smaller one is off by at most 2^-25, 2^-39 of the largest.  (Under 2^4 that was 2^-28: with zero codes at
 // a dominant column and the other elements 2^-15 of it scores were off by 1.7e-5 of their mass, in fp32 by 5e-8.
 // Terms with factors of their own, 1, 2^-11 and 2^-22, reach further, but the codes under each factor take vector
 // instructions: 64 queries, 1M x 256, 172 us instead of 118.)
 __device__ __forceinline__ int query_exponent(float mx) {
-  return mx > 0.f && mx <= 3.402823466e38f ? 14 - ilogbf(mx) : 0;
+  return mx > 0.f ? 14 - ilogbf(mx) : 0;
 }
 
 // What a wave loads for one quad of its tiles.
@@ -257,6 +257,19 @@ __device__ __forceinline__ void load_quad(QuadLoad<SPQ>& x, const uint32_t* __re
       for (int d = 0; d < 4; ++d) x.c[u][d] = d < dpl ? p[d] : kZeroCodes;
     }
     x.s[u] = *reinterpret_cast<const Elems<uint16_t, SPQ>*>(scales + ((t * nquad + b) * kRows + (lane & 15)) * SPQ);
+  }
+}
+
+constexpr uint32_t kInf = 0x7f800000u;
+
+// f(query, column block, column in it, value) for a workgroup's queries, element by element
+template <typename T, typename F>
+__device__ __forceinline__ void each_element(const T* __restrict__ q, int nq, int64_t ldq, int H, int items, int nrow,
+                                             int nthread, F f) {
+#pragma unroll 1
+  for (int it = threadIdx.x; it < 8 * items; it += nthread) {
+    const int k = it % kBlk, i = it / kBlk % nrow, b = it / kBlk / nrow;
+    if (i < nq && b * kBlk + k < H) f(i, b, k, (float)q[i * ldq + b * kBlk + k]);
   }
 }
 
@@ -304,9 +317,24 @@ __global__ __launch_bounds__(BLOCK) void int4_scores_kernel(const T* __restrict_
     }
   }
   __syncthreads();
-  int own_e = threadIdx.x < Q::kQ ? query_exponent(__int_as_float(qe[threadIdx.x])) : 0;
+  uint32_t own = (uint32_t)qe[lane % Q::kQ];
+  // an infinity or a NaN among the queries: their exponents from the finite elements, and an infinity's terms mended
+  // below, apart from the loop that does them all: within it that took a register too many (1M x 256, one query: 32.3
+  // instead of 31.5 us).
+  const bool wild = __any(own >= kInf);  // (every wave reads every query's)
   __syncthreads();
-  if (threadIdx.x < Q::kQ) qe[threadIdx.x] = own_e;
+  if (wild) {
+    if (threadIdx.x < Q::kQ) qe[threadIdx.x] = 0;
+    __syncthreads();
+    each_element(q, nq, ldq, H, items, Q::kQ, BLOCK, [&](int i, int, int, float v) {
+      const uint32_t a = __float_as_uint(fabsf(v));
+      if (a < kInf) atomicMax(reinterpret_cast<uint32_t*>(&qe[i]), a);
+    });
+    __syncthreads();
+    own = (uint32_t)qe[lane % Q::kQ];
+    __syncthreads();
+  }
+  if (threadIdx.x < Q::kQ) qe[threadIdx.x] = query_exponent(__uint_as_float(own));
   __syncthreads();
   for (int it0 = threadIdx.x; it0 < items; it0 += kRuns * BLOCK) {
     if (items > kRuns * BLOCK) load_runs(it0);
@@ -338,6 +366,16 @@ __global__ __launch_bounds__(BLOCK) void int4_scores_kernel(const T* __restrict_
     }
   }
   __syncthreads();
+  if (wild) {  // an infinity less its first term is NaN: it is that term alone
+    each_element(q, nq, ldq, H, items, Q::kQ, BLOCK, [&](int i, int b, int k, float v) {
+      if (!__builtin_isinf(v)) return;
+      const int hh = k >> 3, step = NQT == 0 ? 1 : kWave;
+      f16x8* at = NQT == 0 ? A + b * kWave + hh * 16 + 4 * i
+                           : A + ((size_t)b * Q::kOps + 3 * (i >> 4)) * kWave + hh * 16 + (i & 15);
+      for (int t = 1; t < 3; ++t) reinterpret_cast<_Float16*>(at + t * step)[k & 7] = (_Float16)0.f;
+    });
+    __syncthreads();
+  }
 
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   for (; t0 < ntile; t0 += step) {

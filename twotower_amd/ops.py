@@ -1706,7 +1706,7 @@ def _int4_shape(n, H, group) -> tuple[int, int]:
 def int4_scores(q: torch.Tensor, rows: Int4Rows) -> torch.Tensor:
     """(nq, n) float32 products q_i . row_j of (nq, H) or (H,) float32 / bfloat16 / float16 queries with 4-bit
     rows, in fp32 (the codes are exact; a query's elements keep all their bits down to 2^-15 of its largest, smaller
-    ones are taken to within 2^-39 of that).  A query with a non-finite value scores NaN everywhere."""
+    ones are taken to within 2^-39 of that).  Infinities and NaN act as in a product of floats."""
     if q.dim() == 1:
         q = q.unsqueeze(0)
     if q.dim() != 2 or q.shape[1] != rows.H:

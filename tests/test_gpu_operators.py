@@ -1077,6 +1077,16 @@ def test_int4_scores_of_infinite_queries(nq, dtype):
     assert got[0].isinf().sum() > 150 and got[1].isinf().any() and torch.equal(got[4:], plain[4:])
 
 
+def test_int4_scores_of_queries_that_need_a_gradient():
+    rows = ops.Int4Rows.quantize(torch.randn(100, 48, generator=gen(50), device=DEV))
+    q = torch.randn(3, 48, generator=gen(51), device=DEV, requires_grad=True)
+    scores = ops.int4_scores(q, rows)
+    assert torch.equal(scores, ops.int4_scores(q.detach(), rows))
+    assert torch.equal(ops.topk_rows(scores, 4)[0], scores.topk(4, dim=1).values)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        (scores.sum() + q.sum()).backward()
+
+
 def test_int4_scores_offsets_beyond_32_bits():
     n, H = 34_000_000, 256  # 4.35 GB of codes
     codes = torch.zeros(n, H, dtype=torch.int8, device=DEV)

@@ -164,6 +164,25 @@ def test_int4_refusals(make, err, msg):
         make()
 
 
+def test_scores_without_a_gradient_are_not_differentiated_silently(monkeypatch):
+    """The scores of queries that need a gradient are computed, and refused where they are differentiated."""
+    from torch.autograd import forward_ad
+
+    monkeypatch.setattr(ops, "_int4_scores", lambda q, rows: q.detach() @ rows.t())
+    q, rows = torch.randn(3, 8, requires_grad=True), torch.randn(5, 8)
+    scores = ops.int4_scores(q, rows)
+    assert torch.equal(scores, q @ rows.t())
+    with pytest.raises(RuntimeError, match="int4_scores has no gradient"):
+        scores.sum().backward()
+    with torch.no_grad():
+        assert not ops.int4_scores(q, rows).requires_grad
+    assert not ops.int4_scores(q.detach(), rows).requires_grad
+    with forward_ad.dual_level():
+        assert torch.equal(ops.int4_scores(q.detach(), rows), scores)
+        with pytest.raises(RuntimeError, match="int4_scores has no derivative"):
+            ops.int4_scores(forward_ad.make_dual(q.detach(), torch.ones(3, 8)), rows)
+
+
 def test_search_refuses_an_unknown_index_type():
     with pytest.raises(ValueError, match="index_dtype"):
         tt.search.TwoTowerSearch(torch.nn.Identity(), device="cpu", index_dtype="int8")

@@ -1703,10 +1703,34 @@ def _int4_shape(n, H, group) -> tuple[int, int]:
     return int(n), int(H)
 
 
+class _NoGradient(torch.autograd.Function):
+    """fn(q, *args) for queries that need a gradient, which there is none of: differentiating the result raises."""
+
+    @staticmethod
+    def forward(ctx, what, fn, q, *args):
+        ctx.what = what
+        return fn(q, *args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what} has no gradient: detach its queries, or score under torch.no_grad()")
+
+    @staticmethod
+    def jvp(ctx, *tangents):
+        raise RuntimeError(f"{ctx.what} has no derivative: detach its queries")
+
+
 def int4_scores(q: torch.Tensor, rows: Int4Rows) -> torch.Tensor:
     """(nq, n) float32 products q_i . row_j of (nq, H) or (H,) float32 / bfloat16 / float16 queries with 4-bit
     rows, in fp32 (the codes are exact; a query's elements keep all their bits down to 2^-15 of its largest, smaller
-    ones are taken to within 2^-39 of that).  Infinities and NaN act as in a product of floats."""
+    ones are taken to within 2^-39 of that).  Infinities and NaN act as in a product of floats.  The scores of
+    queries that need a gradient are refused when they are differentiated."""
+    if (q.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
+        return _NoGradient.apply("int4_scores", _int4_scores, q, rows)
+    return _int4_scores(q, rows)
+
+
+def _int4_scores(q: torch.Tensor, rows: Int4Rows) -> torch.Tensor:
     if q.dim() == 1:
         q = q.unsqueeze(0)
     if q.dim() != 2 or q.shape[1] != rows.H:

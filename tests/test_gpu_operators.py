@@ -853,6 +853,35 @@ def test_clip_grad_norm_of_parameters():
     check_clip(before, [p.grad for p in ps[:2]], norm, 1.0, 2.0)
 
 
+def test_clip_counts_as_an_in_place_change():
+    """A backward that saved a gradient must not run with its clipped values, as with torch's own in-place calls."""
+    flat = torch.randn(600, generator=gen(36), device=DEV)
+    a, b = torch.randn(600, generator=gen(37), device=DEV), flat[100:].view(20, 25)
+    x = torch.ones(600, device=DEV, requires_grad=True)
+    for fn in (lambda: ops.clip_grad_norm([a], 0.5), lambda: ops.clip_grad_norm([b.clone()], 0.5, out=[a[:500].view(20, 25)]),
+               lambda: ops.clip_grad_norm([a, b.t()[:, ::2]], 0.5)):
+        y = (x * a).sum()
+        fn()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    y = (x * flat).sum()
+    ops.clip_grad_norm([b], 0.5)  # a view's change is its base's
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    y = (x * a).sum()
+    ops.clip_grad_norm([a], None)  # the norm alone changes nothing
+    ops.clip_grad_norm([a], 0.5, out=[torch.empty_like(a)])
+    y.backward()
+    with torch.inference_mode():
+        t = torch.ones(40, device=DEV)
+        ops.clip_grad_norm([t], 1.0)
+    p = torch.nn.Parameter(torch.zeros(40, device=DEV))
+    p.grad = torch.ones(40, device=DEV)
+    before = p.grad._version
+    optim.clip_grad_norm_([p], 1.0)
+    assert p.grad._version > before
+
+
 def test_clip_offsets_beyond_32_bits():
     n = 2 ** 31 + 5
     t = torch.zeros(n, dtype=BF16, device=DEV)

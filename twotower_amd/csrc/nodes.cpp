@@ -527,6 +527,9 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, std::optional<double> ma
   launch(first, "tt_clip_grads", abi.clip_grads, (const void* const*)src.data(), (void* const*)dst.data(),
          (const int64_t*)n.data(), (const uint8_t*)type.data(), (const uint8_t*)otype.data(), (int)count, (int)inf_norm,
          max_norm.value_or(0.0), (int)scale, as<float>(norm), as<void>(ws), ws_bytes);
+  if (scale)  // written past autograd's eyes: what was saved of them is not what they hold
+    for (const Tensor& o : outs)
+      if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
   for (const auto& [o, t] : copies) o.copy_(t);
   return norm;
 }

@@ -119,6 +119,23 @@ def test_clip_of_nothing_and_of_a_fused_table():
         optim.clip_grad_norm_([w], 1.0)
 
 
+def test_clip_refuses_parameters_that_are_stepped_inside_backward():
+    """Nothing of their gradients is left to clip, and the norm would leave them out."""
+    emb = tt.embeddings.build("lookup", vocab_size=20, embedding_dim=8)
+    model = tt.build_two_tower("mean", emb, hidden_dim=16, tied_weights=True)
+    opt = torch.optim.AdamW(model.parameters())
+    assert optim.clip_grad_norm_(model.parameters(), 1.0).item() == 0.0
+    (table,) = optim.fuse_table_update(opt, model)
+    with pytest.raises(RuntimeError, match="stepped inside backward"):
+        optim.clip_grad_norm_(model.parameters(), 1.0)
+    table.release()
+    dense = optim.fuse_dense_update(opt, model)
+    with pytest.raises(RuntimeError, match="stepped inside backward"):
+        optim.clip_grad_norm_(model.parameters(), 1.0)
+    dense.release()
+    assert optim.clip_grad_norm_(model.parameters(), 1.0).item() == 0.0
+
+
 def test_train_step_refuses_clipping_a_fused_table():
     emb = tt.embeddings.build("lookup", vocab_size=20, embedding_dim=8)
     model = tt.build_two_tower("mean", emb, hidden_dim=16, tied_weights=True)

@@ -428,14 +428,19 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
     """torch.nn.utils.clip_grad_norm_ on the HIP kernels (ops.clip_grad_norm): scales every parameter's .grad in
     place by min(1, max_norm / (norm + 1e-6)) and returns the global norm as a device tensor, without a
     host synchronisation (error_if_nonfinite reads it and raises).  A parameter listed twice counts
-    once.  A table whose gradient a fused optimizer holds in factored form has no .grad to take part: such
-    a call is refused rather than clipped without it."""
+    once.  A table whose gradient a fused optimizer holds in factored form has no .grad to take part, nor has a
+    parameter that was stepped inside backward (fuse_table_update, fuse_dense_update): such a call is
+    refused rather than clipped without it."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     params = list({id(p): p for p in parameters}.values())
     if any(getattr(p, "_tt_deferred", None) is not None and p._tt_deferred.parts for p in params):
         raise RuntimeError("clip_grad_norm_: a fused table's gradient is kept in factored form and has no norm here; "
                            "build the optimizer with fused_tables=False to clip it")
+    if any(p.grad is None and (getattr(p, "_tt_dense_update", None) is not None or getattr(
+            getattr(p, "_tt_deferred", None), "on_backward", None) is not None) for p in params):
+        raise RuntimeError("clip_grad_norm_: a parameter is stepped inside backward(), before its gradient can be clipped: "
+                           "release() its update to clip it")
     for p in params:
         if getattr(p, "_tt_side_grads", None) is not None:
             p._tt_side_grads.join()  # gradients still being formed on a side stream
@@ -558,6 +563,8 @@ class BackwardDenseUpdate:
         self._ids = {id(p) for p in self.params}
         self._queued = False
         self._handles = [p.register_post_accumulate_grad_hook(self._on_grad) for p in self.params]
+        for p in self.params:
+            p._tt_dense_update = self
 
     def _on_grad(self, _p) -> None:
         if not self._queued:
@@ -594,6 +601,9 @@ class BackwardDenseUpdate:
         for h in self._handles:
             h.remove()
         self._handles = []
+        for p in self.params:
+            if getattr(p, "_tt_dense_update", None) is self:
+                del p._tt_dense_update
 
 
 def fuse_dense_update(optimizer: torch.optim.Optimizer, model: torch.nn.Module) -> BackwardDenseUpdate:

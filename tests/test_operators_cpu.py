@@ -109,6 +109,32 @@ def test_clip_refuses_an_out_that_is_another_gradient():
         ops.clip_grad_norm([a, b], 1.0, out=[a, torch.ones(8)])
 
 
+def test_clip_refuses_tensors_that_overlap_in_part():
+    t, h = torch.ones(40), torch.ones(40, dtype=torch.bfloat16)
+    other = torch.ones(40)
+
+    def refused(match, *args, **kw):
+        with pytest.raises(ValueError, match=match):
+            ops.clip_grad_norm(*args, 1.0, **kw)
+
+    def taken(*args, **kw):  # (as far as the check for GPU tensors, after the others)
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            ops.clip_grad_norm(*args, 1.0, **kw)
+
+    refused("written twice", [t[:20], t[19:]])
+    refused("written twice", [t[30:], other, t[5:31]])
+    refused("written twice", [t, t[7:9]])
+    refused("written twice", [other, other.clone()], out=[t[:40], t.view(2, 20).view(40)])
+    refused("memory of another gradient", [t[:20], other[:20]], out=[other[20:], t[10:30]])
+    refused("memory of another gradient", [t[:20]], out=[t[1:21]])
+    refused("memory of another gradient", [h[:20]], out=[h.view(torch.float32)])
+    taken([t[20:], t[:20], other])
+    taken([t[:20], h], out=[t[20:], other])
+    taken([t[:20], t[20:]], out=[other[20:], other[:20]])
+    taken([t[:20], t[20:]], out=[t[:20], t[20:]])
+    taken([t[20:], t[:0], other[:0], t[:20]], out=[t[20:], t[:0], t[:0], t[:20]])  # nothing to write
+
+
 def test_clip_of_nothing_and_of_a_fused_table():
     assert ops.clip_grad_norm([], 1.0).item() == 0.0
     assert optim.clip_grad_norm_([torch.nn.Parameter(torch.ones(2))], 1.0).item() == 0.0

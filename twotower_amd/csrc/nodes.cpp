@@ -13,6 +13,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <unordered_set>
@@ -509,15 +510,28 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, std::optional<double> ma
     if (!s.is_same(g)) kept.push_back(s);
     if (!d.is_same(o)) copies.emplace_back(o, d);
   }
-  if (scale) {
-    std::unordered_set<const void*> written(2 * count);
+  if (scale) {  // what is written lies apart, and apart from what is read elsewhere
+    auto bytes = [](int code) { return code == TT_E_F32 ? 4 : 2; };
+    std::vector<std::pair<const char*, const char*>> written;
+    written.reserve(count);
     for (size_t i = 0; i < count; ++i)
-      TORCH_CHECK_VALUE(!n[i] || written.insert(dst[i]).second,
+      if (n[i]) {
+        const char* at = static_cast<const char*>(dst[i]);
+        written.emplace_back(at, at + n[i] * bytes(otype[i]));
+      }
+    std::sort(written.begin(), written.end());
+    for (size_t k = 1; k < written.size(); ++k)
+      TORCH_CHECK_VALUE(written[k - 1].second <= written[k].first,
                         "a gradient is written twice: the same memory is listed more than once");
     if (out)
-      for (size_t i = 0; i < count; ++i)
-        TORCH_CHECK_VALUE(!n[i] || src[i] == dst[i] || !written.count(src[i]),
-                          "an out tensor is the memory of another gradient");
+      for (size_t i = 0; i < count; ++i) {
+        if (!n[i] || (src[i] == dst[i] && type[i] == otype[i])) continue;
+        const char* at = static_cast<const char*>(src[i]);
+        const auto next = std::upper_bound(written.begin(), written.end(), at,
+                                           [](const char* x, const auto& r) { return x < r.second; });
+        TORCH_CHECK_VALUE(next == written.end() || next->first >= at + n[i] * bytes(type[i]),
+                          "an out tensor is the memory of another gradient, or of its own in another type or place");
+      }
   }
   const Tensor& first = grads[0];
   for (size_t i = 0; i < count; ++i) check_gpu(first, {&grads[i], &outs[i]});

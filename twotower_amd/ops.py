@@ -1447,7 +1447,8 @@ def clip_grad_norm(grads, max_norm: float | None, norm_type: float = 2.0, out=No
     float32, so half-precision accumulators can be clipped into the fp32 gradients an optimizer steps
     with).  max_norm None: the norm alone.  float32 / bfloat16 / float16 tensors, mixed at will; the norm is
     formed in 64 bits in a fixed order, each product is rounded once; no host synchronisation.  Tensors must
-    not overlap (the same memory listed twice is refused), but out[i] may be grads[i].
+    not overlap (memory that is written twice, or written as one tensor and read as another, is refused), but
+    out[i] may be grads[i].
     A non-finite norm spreads as in torch.nn.utils.clip_grad_norm_ (inf: zeros and NaN, NaN: NaN)."""
     grads = list(grads)
     if norm_type not in (2, 2.0, float("inf")):

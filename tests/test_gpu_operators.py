@@ -433,6 +433,17 @@ def test_lookup_embedding_module_under_torchs_transforms():
     assert seen == [1]
 
 
+@pytest.mark.parametrize("how", [torch.fx.symbolic_trace, torch.jit.script, lambda m: torch.compile(m, backend="eager", fullgraph=True)],
+                         ids=["fx", "script", "compile"])
+def test_lookup_embedding_module_traced_and_compiled(how):
+    emb = tt.embeddings.build("lookup", vocab_size=50, embedding_dim=16, scale=4.0).to(DEV)
+    ids = torch.randint(0, 50, (3, 7), generator=gen(17), device=DEV)
+    got, want = how(emb)(ids), emb(ids)
+    assert torch.equal(got, want)
+    a, b = (torch.autograd.grad(x.square().sum(), emb.weight)[0] for x in (got, want))
+    assert (a - b).abs().max() <= 32 * U * b.abs().max()  # (at most 21 terms a sum)
+
+
 # ---------------------------------------------------------------------------------------------
 # preference loss
 def pref_case(B, H, K, dtype, ref, mask, seed):

@@ -238,6 +238,31 @@ def test_lookup_embedding_on_the_cpu_is_the_plain_gather():
     assert list(emb.state_dict()) == ["embedding.weight"]
 
 
+class _Pooler(torch.nn.Module):
+    def __init__(self, embedding):
+        super().__init__()
+        self.embedding = embedding
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        return self.embedding(ids).sum(1)
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0])
+@pytest.mark.parametrize("how", [torch.fx.symbolic_trace, torch.jit.script,
+                                 lambda m: torch.jit.trace(m, torch.tensor([[1, 2]])),
+                                 lambda m: torch.compile(m, backend="eager", fullgraph=True),
+                                 lambda m: torch.export.export(m, (torch.tensor([[1, 0, 8]]),)).module()],
+                         ids=["fx", "script", "trace", "compile", "export"])
+def test_lookup_embedding_can_be_traced_and_compiled(how, scale):
+    emb = tt.embeddings.build("lookup", vocab_size=9, embedding_dim=6, scale=scale)
+    ids = torch.tensor([[1, 0, 8]])
+    for module in (emb, _Pooler(emb)):
+        got = how(module)(ids)
+        assert torch.equal(got, module(ids))
+        want = torch.autograd.grad(module(ids).square().sum(), emb.weight)[0]
+        assert torch.equal(torch.autograd.grad(got.square().sum(), emb.weight)[0], want)
+
+
 def _dp_clip_worker(rank, port, q):
     import os
 

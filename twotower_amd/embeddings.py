@@ -33,7 +33,7 @@ class BaseEmbedding(nn.Module, ABC):
         logger.info(f"Embedding parameters: {self.vocab_size * self.embedding_dim:,}")
 
 
-def _plain_embedding(m: nn.Module) -> bool:
+def _plain_embedding(m) -> bool:
     """An nn.Embedding whose forward is nothing but the row gather of a type the HIP lookup has."""
     w = m.weight
     return (type(m) is nn.Embedding and m.max_norm is None and not m.scale_grad_by_freq and not m.sparse
@@ -72,8 +72,15 @@ class LookupEmbedding(BaseEmbedding):
         """(B, L) ids -> (B, L, E) rows times ``scale``: the reference's unfused contract, for foreign
         towers.  The towers of this package never call it (they use pool_mean).  On the GPU one HIP
         gather forward and, for the dense table gradient, a sum over sorted tokens (ops.embedding_lookup)."""
+        if torch.jit.is_scripting():
+            return self.embedding(input_ids) * self.scale
+        return self._rows(input_ids)
+
+    @torch.jit.unused
+    def _rows(self, input_ids: torch.Tensor) -> torch.Tensor:
         inner = self.embedding
-        if input_ids.is_cuda and inner.weight.is_cuda and _plain_embedding(inner) and not _observed():
+        if (isinstance(input_ids, torch.Tensor) and input_ids.is_cuda and inner.weight.is_cuda  # (fx: a Proxy is none)
+                and not _observed() and _plain_embedding(inner)):
             return ops.embedding_lookup(inner.weight, input_ids, self.scale, inner.padding_idx)
         rows = inner(input_ids)
         return rows if self.scale == 1.0 else rows * self.scale

@@ -263,6 +263,16 @@ def test_lookup_embedding_can_be_traced_and_compiled(how, scale):
         assert torch.equal(torch.autograd.grad(got.square().sum(), emb.weight)[0], want)
 
 
+def test_lookup_embedding_pickled_without_a_scale():
+    import copy
+
+    emb = tt.embeddings.build("lookup", vocab_size=9, embedding_dim=6)
+    old = copy.deepcopy(emb)
+    del old.__dict__["scale"]
+    ids = torch.tensor([[1, 0, 8]])
+    assert torch.equal(old(ids), emb(ids))
+
+
 def _dp_clip_worker(rank, port, q):
     import os
 

@@ -52,6 +52,8 @@ def _observed() -> bool:
 class LookupEmbedding(BaseEmbedding):
     """Trainable lookup table (twotower/embeddings.py:24-40) with a fused pooled lookup."""
 
+    scale = 1.0  # (of modules that were pickled without one)
+
     def __init__(self, vocab_size: int, embedding_dim: int, padding_idx: int = 0,
                  scatter_mode: str = "sorted", scale: float = 1.0):
         """scale: factor of the token rows that forward() returns (e.g. embedding_dim ** 0.5); the pooled

@@ -444,6 +444,38 @@ def test_lookup_embedding_module_traced_and_compiled(how):
     assert (a - b).abs().max() <= 32 * U * b.abs().max()  # (at most 21 terms a sum)
 
 
+def test_lookup_embedding_module_runs_what_is_around_the_inner_one():
+    """Global hooks, a forward of the instance's own and function modes see torch's gather; a default device does not
+    turn the kernels off."""
+    emb = tt.embeddings.build("lookup", vocab_size=50, embedding_dim=16, scale=4.0).to(DEV)
+    ids = torch.randint(0, 50, (3, 7), generator=gen(16), device=DEV)
+    want = emb(ids)
+    seen = []
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, a, out: seen.append(type(m)))
+    try:
+        assert torch.equal(emb(ids), want)
+    finally:
+        handle.remove()
+    assert torch.nn.Embedding in seen
+    plain = emb.embedding.forward
+    emb.embedding.forward = lambda x: plain(x) + 1.0
+    assert torch.equal(emb(ids), (emb.weight[ids] + 1.0) * 4.0)
+    del emb.embedding.forward
+    names = []
+
+    class Mode(torch.overrides.TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            names.append(getattr(func, "__name__", ""))
+            return func(*args, **(kwargs or {}))
+
+    with Mode():
+        assert torch.equal(emb(ids), want)
+    assert "embedding" in names
+    with torch.device("cpu"), _lib.record_calls() as calls:
+        assert torch.equal(emb(ids), want)
+    assert "tt_lookup_fwd" in calls
+
+
 # ---------------------------------------------------------------------------------------------
 # preference loss
 def pref_case(B, H, K, dtype, ref, mask, seed):

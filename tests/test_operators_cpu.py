@@ -273,6 +273,46 @@ def test_lookup_embedding_pickled_without_a_scale():
     assert torch.equal(old(ids), emb(ids))
 
 
+def test_only_an_embedding_as_torch_made_it_is_plain(monkeypatch):
+    """What a user puts around the inner embedding's forward must run: its own hooks, global ones, another forward."""
+    from twotower_amd import embeddings
+
+    def fresh():
+        return torch.nn.Embedding(5, 4, padding_idx=0)
+
+    assert embeddings._plain_embedding(fresh())
+    m = fresh()
+    m.forward = lambda ids: torch.zeros(1)
+    assert not embeddings._plain_embedding(m)
+    handles = [lambda: torch.nn.modules.module.register_module_forward_hook(lambda *a: None),
+               lambda: torch.nn.modules.module.register_module_forward_pre_hook(lambda *a: None),
+               lambda: torch.nn.modules.module.register_module_full_backward_hook(lambda *a: None),
+               lambda: torch.nn.modules.module.register_module_full_backward_pre_hook(lambda *a: None)]
+    for register in handles:
+        handle = register()
+        try:
+            assert not embeddings._plain_embedding(fresh())
+        finally:
+            handle.remove()
+    assert embeddings._plain_embedding(fresh())
+    monkeypatch.setattr(torch.nn.Embedding, "forward", lambda self, ids: None)
+    assert not embeddings._plain_embedding(fresh())
+
+
+def test_function_modes_observe_the_lookup():
+    from twotower_amd import embeddings
+
+    class Mode(torch.overrides.TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    assert not embeddings._observed()
+    with Mode():
+        assert embeddings._observed()
+    with torch.device("cpu"):  # factories' default: nothing that follows a lookup
+        assert not embeddings._observed()
+
+
 def _dp_clip_worker(rank, port, q):
     import os
 

@@ -14,6 +14,8 @@ from abc import ABC
 import torch
 import torch.nn as nn
 from torch.autograd import forward_ad
+from torch.overrides import _get_current_function_mode_stack
+from torch.utils._device import DeviceContext
 
 from . import _lib, ops
 
@@ -33,20 +35,27 @@ class BaseEmbedding(nn.Module, ABC):
         logger.info(f"Embedding parameters: {self.vocab_size * self.embedding_dim:,}")
 
 
+_EMBEDDING_FORWARD = nn.Embedding.forward
+
+
 def _plain_embedding(m) -> bool:
     """An nn.Embedding whose forward is nothing but the row gather of a type the HIP lookup has."""
     w = m.weight
     return (type(m) is nn.Embedding and m.max_norm is None and not m.scale_grad_by_freq and not m.sparse
             and type(w) in (nn.Parameter, torch.Tensor) and w.dtype in _lib.ELEM_DTYPES and w.is_contiguous()
-            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks))
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+            and "forward" not in m.__dict__ and nn.Embedding.forward is _EMBEDDING_FORWARD
+            and not nn.modules.module._has_any_global_hook())
 
 
 def _observed() -> bool:
-    """Whether a tracer, function transform, forward-mode derivative or dispatch mode follows torch's own calls: it
-    would not see a kernel's."""
+    """Whether a tracer, function transform, forward-mode derivative, dispatch or function mode follows torch's own
+    calls: it would not see a kernel's.  (torch.set_default_device is such a mode, and looks at factories alone.)"""
     return (torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active()
             or torch._C._len_torch_dispatch_stack() > 0 or torch.jit.is_tracing()
-            or forward_ad._current_level >= 0)
+            or forward_ad._current_level >= 0
+            or (torch._C._len_torch_function_stack() > 0
+                and any(type(m) is not DeviceContext for m in _get_current_function_mode_stack())))
 
 
 class LookupEmbedding(BaseEmbedding):

@@ -192,7 +192,7 @@ int tt_bag_col_reduce_ex(const int32_t* seg_all, const int32_t* vals_all, int64_
 
 /* ---- token lookup with a scale (LookupEmbedding.forward's (B, L, E) rows, twotower/embeddings.py:40) ----
  * tt_lookup_fwd: out[t, :] = scale * table[ids[t], :] for n tokens, formed in fp32 and rounded once; an
- *   id outside [0, V) yields a zero row.  table: V rows of E elements, row stride ld_table; out: n x E.
+ *   id outside [0, V) yields a zero row, or with TT_LOOKUP_NAN_OUTSIDE added to ids_dtype a row of NaN.  table: V rows of E elements, row stride ld_table; out: n x E.
  *   Types (tt_elem_dtype): out = table's, or bf16 / fp16 rows of an fp32 table.
  * tt_lookup_bwd: grad[r, :] = scale * sum of dout[t, :] over the tokens with ids[t] = r (none for r =
  *   padding_idx, -1: no padding id), every one of the V rows written.  Sums are fp32 in a fixed order
@@ -204,6 +204,7 @@ int tt_bag_col_reduce_ex(const int32_t* seg_all, const int32_t* vals_all, int64_
  *   padding_idx, on the same stream or one that it waits for (it may run beside the forward).  The plan is
  *   only read by tt_lookup_bwd. */
 #define TT_LOOKUP_DIRECT_TOKENS 8192
+#define TT_LOOKUP_NAN_OUTSIDE 4
 #define TT_LOOKUP_MAX 0x7fff0000LL /* tokens and rows stay below it */
 int tt_lookup_fwd(const void* table, int table_dtype, int64_t V, int E, int64_t ld_table, const void* ids,
                   int ids_dtype, int64_t n, float scale, void* out, int out_dtype, tt_stream_t stream);

@@ -444,6 +444,36 @@ def test_lookup_embedding_module_traced_and_compiled(how):
     assert (a - b).abs().max() <= 32 * U * b.abs().max()  # (at most 21 terms a sum)
 
 
+@pytest.mark.parametrize("dtype, out_dtype", [(F32, None), (BF16, None), (F16, None), (F32, F16)])
+@pytest.mark.parametrize("n", [5, 900, 70_000])
+def test_strict_lookup_of_ids_outside_the_table(n, dtype, out_dtype):
+    w, ids, dout = lookup_case(700, 64, (n,), dtype, torch.int64, out_dtype, 0, 0.0, 18)
+    ids[::5] = torch.tensor([700, -1, 2 ** 40, -2 ** 63], device=DEV).repeat(n)[:len(ids[::5])]
+    out = (ids < 0) | (ids >= 700)
+    w.requires_grad_(True)
+    got = ops.embedding_lookup(w, ids, 3.0, 0, out_dtype, strict=True)
+    loose = ops.embedding_lookup(w, ids, 3.0, 0, out_dtype)
+    assert got[out].isnan().all() and torch.equal(got[~out], loose[~out]) and not loose[out].any()
+    assert torch.equal(*(torch.autograd.grad(x, w, dout)[0] for x in (got, loose)))
+
+
+def test_a_wrong_vocabulary_does_not_train_silently():
+    emb = tt.embeddings.build("lookup", vocab_size=50, embedding_dim=16, scale=4.0).to(DEV)
+    ids = torch.randint(0, 50, (3, 7), generator=gen(19), device=DEV)
+    fine = emb(ids)
+    assert fine.isfinite().all()
+    ids[1, 2] = 50
+    rows = emb(ids)
+    assert rows[1, 2].isnan().all() and rows.isnan().sum() == 16
+    assert rows.square().mean().isnan()
+    rows.logsumexp((0, 1, 2)).backward()  # (a loss that joins its tokens; the squares' other terms stay finite)
+    assert emb.weight.grad.isnan().any() and optim.clip_grad_norm_(emb.parameters(), 1.0).isnan()
+    with torch.autograd.forward_ad.dual_level():
+        t = torch.autograd.forward_ad.make_dual(emb.weight.detach(), torch.ones_like(emb.weight))
+        rows = torch.autograd.forward_ad.unpack_dual(ops.embedding_lookup(t, ids, strict=True))
+        assert rows.primal[1, 2].isnan().all() and not rows.tangent[1, 2].any()
+
+
 def test_lookup_embedding_module_runs_what_is_around_the_inner_one():
     """Global hooks, a forward of the instance's own and function modes see torch's gather; a default device does not
     turn the kernels off."""

@@ -542,6 +542,8 @@ def _clip(src=P, dst=P, n=3, st=0, dt=0, max_norm=1.0, ws=1 << 20):
     ("tt_lookup_fwd", (P, 0, 5, 4, 4, None, 0, 1, 1.0, P, 0, None), "ids is NULL"),
     ("tt_lookup_fwd", (P, 0, 5, 4, 4, P, 2, 1, 1.0, P, 0, None), "ids_dtype=2"),
     ("tt_lookup_fwd", (P, 1, 5, 4, 4, P, 0, 1, 1.0, P, 0, None), "rows of type 0"),
+    ("tt_lookup_fwd", (P, 0, 5, 4, 4, P, 6, 1, 1.0, P, 0, None), "ids_dtype=2"),
+    ("tt_lookup_bwd", (P, 0, P, 4, 1, 5, 4, -1, 1.0, P, 0, None, 0, None, 0, None), "ids_dtype=4"),
     ("tt_lookup_fwd", (P, 0, 5, 4, 4, P, 0, 2 ** 31, 1.0, P, 0, None), "out of range"),
     ("tt_lookup_fwd", (None, 0, 5, 4, 4, P, 0, 1, 1.0, P, 0, None), "null pointer"),
     ("tt_lookup_bwd", (None, 0, P, 0, 1, 5, 4, -1, 1.0, P, 0, None, 0, None, 0, None), "null pointer"),

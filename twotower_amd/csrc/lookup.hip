@@ -1,6 +1,6 @@
 // Token lookup with a scale, and its gradient by sorted tokens.
 //
-//   out[t, :]  = s W[id_t, :]                                  (ids outside [0, V): a zero row)
+//   out[t, :]  = s W[id_t, :]                                  (ids outside [0, V): a zero row, or NaN)
 //   dW[r, :]   = s sum_{t : id_t = r, r != padding_idx} dout[t, :]     (every row written)
 //
 // Both move bytes and add: the forward reads each token's row (repeated rows from L2) and writes
@@ -38,7 +38,8 @@ constexpr int kXcdRun = 64;
 template <typename TW, typename TO, int VEC, int U>
 __global__ __launch_bounds__(kBlock) void lookup_fwd_kernel(const TW* __restrict__ table, int64_t V, int E, int64_t ld,
                                                             const void* __restrict__ ids, bool wide, int64_t n,
-                                                            float scale, TO* __restrict__ out, int lg, bool runs) {
+                                                            float scale, float outside, TO* __restrict__ out, int lg,
+                                                            bool runs) {
   const int lane = lane_id(), groups = kWave >> lg, sub = lane >> lg, c = lane & ((1 << lg) - 1);
   int64_t block = block_index();
   if (runs) {  // (the grid is whole spans of 8 kXcdRun workgroups)
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(kBlock) void lookup_fwd_kernel(const TW* __restrict
       if (t < n) {
         float y[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) y[i] = (id[u] >= 0 && id[u] < V) ? scale * (float)x[u].v[i] : 0.f;
+        for (int i = 0; i < VEC; ++i) y[i] = (id[u] >= 0 && id[u] < V) ? scale * (float)x[u].v[i] : outside;
         store_elems_nt<VEC>(out + t * E + e, y);
       }
     }
@@ -486,7 +487,7 @@ __global__ __launch_bounds__(kBlock) void lookup_row_join_kernel(TokenPlan p, in
 
 template <typename TW, typename TO>
 int launch_fwd(const void* table, int64_t V, int E, int64_t ld, const void* ids, bool wide, int64_t n, float scale,
-               void* out, hipStream_t s) {
+               float outside, void* out, hipStream_t s) {
   const int64_t counts[] = {E, ld};
   const void* ptrs[] = {table, out};
   const int bytes[] = {(int)sizeof(TW), (int)sizeof(TO)};
@@ -502,7 +503,7 @@ int launch_fwd(const void* table, int64_t V, int E, int64_t ld, const void* ids,
   const TW* t = static_cast<const TW*>(table);
   TO* o = static_cast<TO*>(out);
 #define TT_LF(VV) \
-  case VV: lookup_fwd_kernel<TW, TO, VV, U><<<grid, block, 0, s>>>(t, V, E, ld, ids, wide, n, scale, o, lg, runs); break;
+  case VV: lookup_fwd_kernel<TW, TO, VV, U><<<grid, block, 0, s>>>(t, V, E, ld, ids, wide, n, scale, outside, o, lg, runs); break;
   switch (vec) { TT_LF(8) TT_LF(4) TT_LF(2) default: TT_LF(1) }
 #undef TT_LF
   TT_LAUNCH_CHECK("lookup_fwd");
@@ -598,12 +599,14 @@ using namespace tt;
 
 extern "C" int tt_lookup_fwd(const void* table, int table_dtype, int64_t V, int E, int64_t ld_table, const void* ids,
                              int ids_dtype, int64_t n, float scale, void* out, int out_dtype, tt_stream_t stream) {
+  const float outside = ids_dtype & TT_LOOKUP_NAN_OUTSIDE ? __builtin_nanf("") : 0.f;
+  ids_dtype &= ~TT_LOOKUP_NAN_OUTSIDE;
   if (int rc = check_lookup(n, V, E, ids, ids_dtype, table_dtype, out_dtype)) return rc;
   TT_REQUIRE(ld_table >= E, "ld_table=%lld < E=%d", (long long)ld_table, E);
   if (n == 0) return TT_OK;
   TT_REQUIRE(table && out, "null pointer");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define TT_CALL(TW, TO) (launch_fwd<TW, TO>(table, V, E, ld_table, ids, ids_dtype == TT_IDS_I64, n, scale, out, s))
+#define TT_CALL(TW, TO) (launch_fwd<TW, TO>(table, V, E, ld_table, ids, ids_dtype == TT_IDS_I64, n, scale, outside, out, s))
   TT_LOOKUP_TYPES(table_dtype, out_dtype, TT_CALL);
 #undef TT_CALL
 }

@@ -138,6 +138,7 @@ struct LookupArgs {
   int64_t V, E, pad;
   double scale;
   ScalarType table, rows;
+  bool strict = false;  // of the call's own rows alone: NaN for an id outside the table
   void save(AutogradContext* ctx) const {
     ctx->saved_data["lookup"] = std::make_tuple(V, E, pad, scale, (int64_t)table, (int64_t)rows);
   }
@@ -154,8 +155,8 @@ Tensor lookup_rows(const Tensor& weight, const Tensor& ids, const LookupArgs& a)
   const Tensor out = at::empty(shape, weight.options().dtype(a.rows));
   if (ids.numel())
     launch(weight, "tt_lookup_fwd", abi.lookup_fwd, as<const void>(weight), elem_code(weight), a.V, (int)a.E,
-           a.V > 1 ? weight.stride(0) : a.E, as<const void>(ids), ids_code(ids), ids.numel(), (float)a.scale,
-           as<void>(out), elem_code(out));
+           a.V > 1 ? weight.stride(0) : a.E, as<const void>(ids),
+           ids_code(ids) | (a.strict ? TT_LOOKUP_NAN_OUTSIDE : 0), ids.numel(), (float)a.scale, as<void>(out), elem_code(out));
   return out;
 }
 
@@ -216,7 +217,7 @@ variable_list Lookup::backward(AutogradContext* ctx, variable_list g) {
 }
 
 Tensor embedding_lookup(const Tensor& weight, const Tensor& ids, double scale, std::optional<int64_t> padding_idx,
-                        std::optional<ScalarType> out_dtype) {
+                        std::optional<ScalarType> out_dtype, bool strict) {
   TORCH_CHECK_VALUE(weight.dim() == 2 && weight.numel() > 0, "weight must be a non-empty (V, E) table, got shape ",
                     weight.sizes());
   check_elem(weight, "weight");
@@ -238,7 +239,7 @@ Tensor embedding_lookup(const Tensor& weight, const Tensor& ids, double scale, s
     pad += pad < 0 ? V : 0;
   }
   check_gpu(weight, {&ids});
-  const LookupArgs a{V, E, pad, scale, table, rows};
+  const LookupArgs a{V, E, pad, scale, table, rows, strict};
   const Tensor i = ids.contiguous();
   return weight.requires_grad() && at::GradMode::is_enabled() ? Lookup::apply(weight, i, a) : lookup_rows(weight, i, a);
 }

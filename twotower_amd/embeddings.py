@@ -82,7 +82,8 @@ class LookupEmbedding(BaseEmbedding):
     def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
         """(B, L) ids -> (B, L, E) rows times ``scale``: the reference's unfused contract, for foreign
         towers.  The towers of this package never call it (they use pool_mean).  On the GPU one HIP
-        gather forward and, for the dense table gradient, a sum over sorted tokens (ops.embedding_lookup)."""
+        gather forward and, for the dense table gradient, a sum over sorted tokens (ops.embedding_lookup).  An
+        id outside the table, which torch's gather stops at, yields a row of NaN there."""
         if torch.jit.is_scripting():
             return self.embedding(input_ids) * self.scale
         return self._rows(input_ids)
@@ -92,7 +93,7 @@ class LookupEmbedding(BaseEmbedding):
         inner = self.embedding
         if (isinstance(input_ids, torch.Tensor) and input_ids.is_cuda and inner.weight.is_cuda  # (fx: a Proxy is none)
                 and not _observed() and _plain_embedding(inner)):
-            return ops.embedding_lookup(inner.weight, input_ids, self.scale, inner.padding_idx)
+            return ops.embedding_lookup(inner.weight, input_ids, self.scale, inner.padding_idx, strict=True)
         rows = inner(input_ids)
         return rows if self.scale == 1.0 else rows * self.scale
 

@@ -551,11 +551,12 @@ class _TableGate(torch.autograd.Function):
 
 
 def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None,
-                     out_dtype: torch.dtype | None = None) -> torch.Tensor:
+                     out_dtype: torch.dtype | None = None, strict: bool = False) -> torch.Tensor:
     """scale * weight[ids]: the rows (ids.shape + (E,)) of a (V, E) float32 / bfloat16 / float16 table for
     int32 / int64 ids of any shape, formed in fp32 and rounded once to ``out_dtype`` (the table's type, or
     bfloat16 / float16 rows of a float32 table).  An id outside [0, V) yields a zero row and no
-    gradient (torch.nn.functional.embedding aborts the process on the GPU).
+    gradient (torch.nn.functional.embedding aborts the process on the GPU); with ``strict`` its row is NaN, so
+    that a wrong vocabulary shows in the loss of the same step.
 
     The gradient is dense: every row of the table, scale times the sum of its tokens' gradients in
     fp32 in a fixed order (bitwise reproducible), rounded once to the table's type; the row of
@@ -568,11 +569,11 @@ def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0
     if forward_ad._current_level >= 0:  # (the node knows no tangents, and a plain call would drop them)
         primal, tangent = forward_ad.unpack_dual(weight)
         if tangent is not None:
-            rows = embedding_lookup(primal, ids, scale, padding_idx, out_dtype)
+            rows = embedding_lookup(primal, ids, scale, padding_idx, out_dtype, strict)
             return forward_ad.make_dual(rows, embedding_lookup(tangent.contiguous(), ids, scale, None, out_dtype))
     if col is not None or getattr(weight, "_tt_deferred", None) is not None:
         weight = _TableGate.apply(weight)
-    return _lib.nodes().embedding_lookup(weight, ids, float(scale), padding_idx, out_dtype)
+    return _lib.nodes().embedding_lookup(weight, ids, float(scale), padding_idx, out_dtype, bool(strict))
 
 
 # --------------------------------------------------------------------------------------------

@@ -1298,6 +1298,22 @@ def test_captured_fine_tuning_equals_eager():
         assert (a - b).norm() <= 1e-3 * b.norm()
 
 
+def test_no_capture_beside_a_live_graph_of_the_parameters():
+    model = token_model(66).to(DEV)
+    opt = optim.AdamW(model.parameters(), lr=0.0, weight_decay=0.0, capturable=True)
+    loss_fn = losses.build("preference", beta=0.5)
+    step = tt.TrainStep(model, loss_fn, opt, graph=True, eager_steps=1)
+    ids = triplets(12, 20, 67).to(DEV)
+    first = step(*ids).item()
+    held = loss_fn(*model(*ids))
+    with pytest.raises(RuntimeError, match="still alive"):
+        step(*ids)
+    held = held.item()
+    assert abs(step(*ids).item() - first) <= 1e-5 and abs(step(*ids).item() - held) <= 1e-5
+    held = loss_fn(*model(*ids))  # a recorded step needs no more
+    assert abs(step(*ids).item() - first) <= 1e-5
+
+
 def test_captured_clipping_keeps_each_graphs_norm():
     model = token_model(58).to(DEV)
     opt = optim.AdamW(model.parameters(), lr=0.0, weight_decay=0.0, capturable=True)  # the parameters stay

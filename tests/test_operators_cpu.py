@@ -175,6 +175,17 @@ def test_train_step_refuses_clipping_a_fused_table():
         tt.TrainStep(model, loss, opt, max_grad_norm=-1.0)
 
 
+def test_a_live_graph_of_a_parameter_is_found():
+    a, b = torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(3))
+    assert _lib.nodes().live_leaf([a, b]) == -1
+    loss = (b * 2).sum()
+    assert _lib.nodes().live_leaf([a, b]) == 1
+    loss.backward()
+    assert _lib.nodes().live_leaf([a, b]) == 1  # (its tensors are freed, its nodes are not)
+    loss = loss.detach()
+    assert _lib.nodes().live_leaf([a, b]) == -1
+
+
 def test_a_table_differentiated_both_ways_is_refused():
     d, grad = ops.DeferredTableGrad(), torch.zeros(2, 2)
     d.added_dense()

@@ -369,6 +369,13 @@ struct SplitRows : Function<SplitRows> {
   }
 };
 
+// The first of some leaves that an autograd graph lives of (-1: none does).
+int64_t live_leaf(const std::vector<Tensor>& leaves) {
+  for (size_t i = 0; i < leaves.size(); ++i)
+    if (torch::autograd::impl::try_get_grad_accumulator(leaves[i])) return (int64_t)i;
+  return -1;
+}
+
 variable_list split_rows(const Tensor& x, std::vector<int64_t> sizes) {
   int64_t rows = 0;
   for (const int64_t n : sizes) {
@@ -559,5 +566,6 @@ PYBIND11_MODULE(_nodes, m) {
   m.def("preference_margin", &preference_margin, unlocked);
   m.def("split_rows", &split_rows, unlocked);
   m.def("direct_views", &direct_views);
+  m.def("live_leaf", &live_leaf);
   m.def("clip_grad_norm", &clip_grad_norm, unlocked);
 }

@@ -17,7 +17,7 @@ import os
 
 import torch
 
-from . import ops
+from . import _lib, ops
 from .distributed import GradSync, capture_blocker, is_active, settle_watchdogs
 from .losses import scorer_prep_dtype
 from .optim import clip_grad_norm_
@@ -204,7 +204,22 @@ class TrainStep:
             side.reset()
         self.optimizer.zero_grad(set_to_none=True)
 
+    def _check_no_graph_lives(self) -> None:
+        """A parameter's gradient node belongs to the stream of the first graph that has it.  While an eager graph
+        lives, a captured backward would add to its gradients there, outside the capture: the process ends."""
+        params = [p for p in self.model.parameters() if p.requires_grad]
+        if _lib.nodes().live_leaf(params) >= 0:
+            import gc
+
+            gc.collect()  # (a graph that only a reference cycle holds)
+        i = _lib.nodes().live_leaf(params)
+        if i >= 0:
+            name = next(n for n, p in self.model.named_parameters() if p is params[i])
+            raise RuntimeError(f"TrainStep: an autograd graph of {name} is still alive (a loss or an output of the model "
+                               "that is held without detach()): drop it before the step of a new shape is recorded")
+
     def _capture(self, inputs):
+        self._check_no_graph_lives()
         # the static inputs are consecutive row blocks of one buffer, so the fused TwoTower
         # forward uses them in place (no concatenation inside the step)
         static_all = _packed_like(inputs)

@@ -1298,6 +1298,36 @@ def test_captured_fine_tuning_equals_eager():
         assert (a - b).norm() <= 1e-3 * b.norm()
 
 
+@pytest.mark.parametrize("graph", [False, True])
+def test_each_batch_trains_against_its_own_reference(graph):
+    """Margins and masks of the batch, passed to the step: eager and captured steps against the loss of that batch, in
+    any order of shapes, with and without them, from tensors of other layouts and types."""
+    model = token_model(63).to(DEV)
+    opt = optim.AdamW(model.parameters(), lr=0.0, weight_decay=0.0, capturable=True)  # the parameters stay
+    loss_fn = losses.build("preference", beta=0.5)
+    step = tt.TrainStep(model, loss_fn, opt, graph=graph, eager_steps=1, max_grad_norm=1e9)
+    g = gen(64)
+    batches = []
+    for k, B in enumerate((12, 12, 20, 12, 20, 12)):
+        ids = triplets(B, 20, 65 + k).to(DEV)
+        kw = {"ref_margin": torch.randn(B, 2, generator=g, device=DEV)[:, 1],
+              "mask": (torch.rand(1, B, generator=g, device=DEV) > 0.3).t()}
+        batches.append((ids, kw if k != 3 else {"mask": kw["mask"], "ref_margin": None}))
+    batches += [(ids, {"ref_margin": kw["ref_margin"]}) for ids, kw in batches[:2]] + [(batches[0][0], {})]
+    batches += [(ids, dict(reversed(kw.items()))) for ids, kw in batches[:2]]  # the names' order means nothing
+
+    def plain(ids, kw):  # (numbers alone: no graph of the parameters may live while a step is captured)
+        want = loss_fn(*model(*ids), **kw)
+        grads = torch.autograd.grad(want, list(model.parameters()))
+        return want.item(), torch.cat([x.flatten() for x in grads]).norm().item()
+
+    for ids, kw in batches * 2:
+        loss = step(*ids, **kw).item()
+        want, norm = plain(ids, kw)
+        assert abs(loss - want) <= 1e-5 * max(1.0, want)
+        assert abs(step.grad_norm.item() - norm) <= 1e-4 * norm
+
+
 def test_no_capture_beside_a_live_graph_of_the_parameters():
     model = token_model(66).to(DEV)
     opt = optim.AdamW(model.parameters(), lr=0.0, weight_decay=0.0, capturable=True)

@@ -175,6 +175,26 @@ def test_train_step_refuses_clipping_a_fused_table():
         tt.TrainStep(model, loss, opt, max_grad_norm=-1.0)
 
 
+def test_train_step_hands_each_batch_its_own_loss_inputs():
+    torch.manual_seed(4)
+    model = _Linear()
+    seen = []
+
+    def loss_fn(a, b, target=None, mask=None):
+        seen.append((target, mask))
+        return ((a - b) * (1.0 if target is None else target)).square().mean()
+
+    step = tt.TrainStep(model, loss_fn, torch.optim.SGD(model.parameters(), lr=0.1))
+    x, y, t1, t2 = torch.randn(4, 6), torch.randn(4, 5), torch.rand(4, 5), torch.rand(4, 5)
+    step(x, y, target=t1)
+    step(x, y, target=t2, mask=None)
+    step(x, y)
+    assert seen[0][0] is t1 and seen[1][0] is t2
+    assert seen[2] == (None, None) and seen[1][1] is None
+    with pytest.raises(TypeError, match="loss input target must be a tensor"):
+        step(x, y, target=0.5)
+
+
 def test_a_live_graph_of_a_parameter_is_found():
     a, b = torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(3))
     assert _lib.nodes().live_leaf([a, b]) == -1

@@ -9,6 +9,11 @@ the step's ~40 kernel launches then cost one graph launch, and the GPU no longer
 Python issues short kernels.  Each call is still exactly one training step on its own batch
 (the batch is copied into the graph's static input buffers first).  Needs a capturable
 optimizer (optim.AdamW(capturable=True)); a new input shape is captured anew.
+
+What a loss needs beside the embeddings of each batch (preference_loss's ref_margin and mask) is passed to the
+call by name, ``step(q, p, n, ref_margin=ref)``, and takes part as the ids do: copied into the graph's own
+buffers before a replay.  A tensor bound to the loss once (losses.build(..., ref_margin=ref)) stays the same
+tensor for every batch.
 """
 from __future__ import annotations
 
@@ -71,9 +76,9 @@ class TrainStep:
         self._seed: dict[torch.device, torch.Tensor] = {}  # d(loss) seed of backward, kept on device
 
     def eager(self, queries: torch.Tensor, positive_docs: torch.Tensor,
-              negative_docs: torch.Tensor | None = None) -> torch.Tensor:
+              negative_docs: torch.Tensor | None = None, **loss_inputs: torch.Tensor | None) -> torch.Tensor:
         """One step.  negative_docs None: a (query, positive) pair step -- model(q, p), loss_fn(q, p)
-        (e.g. the in-batch loss over the positives alone)."""
+        (e.g. the in-batch loss over the positives alone).  loss_inputs: this batch's tensors for loss_fn, by name."""
         # forward, backward and step back to back: the optimizer may take gradients computed on
         # a side stream and join them itself (_lib.SideGrads)
         side = getattr(self.optimizer, "_side_grads", None)
@@ -85,7 +90,7 @@ class TrainStep:
             defer = ops.deferred_loss_mean() if self._defer_mean else contextlib.nullcontext()
             with defer, self._scorer_prep_open():  # the loss is read after the backward below
                 ins = (queries, positive_docs) if negative_docs is None else (queries, positive_docs, negative_docs)
-                loss = self.loss_fn(*self.model(*ins))
+                loss = self.loss_fn(*self.model(*ins), **loss_inputs)
             self.optimizer.zero_grad(set_to_none=True)
             # backward seeded with the (1/world pre-scaled) unit gradient from a resident tensor:
             # no fill / scale kernels per step
@@ -124,21 +129,28 @@ class TrainStep:
             self.model.scorer_prep = prev
 
     def __call__(self, queries: torch.Tensor, positive_docs: torch.Tensor,
-                 negative_docs: torch.Tensor | None = None) -> torch.Tensor:
+                 negative_docs: torch.Tensor | None = None, **loss_inputs: torch.Tensor | None) -> torch.Tensor:
+        for name, t in loss_inputs.items():  # (a number would be the first batch's in every replay)
+            if t is not None and not isinstance(t, torch.Tensor):
+                raise TypeError(f"TrainStep: loss input {name} must be a tensor or None, got {type(t).__name__}: bind "
+                                "what does not change to the loss (losses.build)")
         if not self.graph:
-            return self.eager(queries, positive_docs, negative_docs)
+            return self.eager(queries, positive_docs, negative_docs, **loss_inputs)
         inputs = (queries, positive_docs) if negative_docs is None else (queries, positive_docs, negative_docs)
+        extra = {k: loss_inputs[k] for k in sorted(loss_inputs)}
         key = tuple((tuple(t.shape), t.dtype, t.device) for t in inputs)
+        if extra:
+            key += tuple((k, None if t is None else (tuple(t.shape), t.dtype, t.device)) for k, t in extra.items())
         hit = self._graphs.get(key)
         if hit is None:
             if self._eager_left > 0:
                 self._eager_left -= 1
-                return self.eager(*inputs)
+                return self.eager(*inputs, **extra)
             why = capture_blocker(self.group) if is_active(self.group) else None
             err = fatal = None
             if why is None:
                 try:
-                    hit = self._capture(inputs)
+                    hit = self._capture(inputs, extra)
                 except RuntimeError as e:  # e.g. a collective this backend cannot capture
                     if _is_capture_error(e):
                         err = e
@@ -164,9 +176,9 @@ class TrainStep:
                                  else "another rank's HIP graph capture failed")
                 warnings.warn(f"TrainStep: {reason}; running the step eagerly")
                 self.graph = False
-                return self.eager(*inputs)
+                return self.eager(*inputs, **extra)
             self._graphs[key] = hit
-        graph, static_all, static_loss, self.grad_norm = hit
+        graph, static_all, static_extra, static_loss, self.grad_norm = hit
         if all(t.shape[1:] == inputs[0].shape[1:] and t.dtype == inputs[0].dtype for t in inputs):
             if all(t.device == static_all.device and t.is_contiguous() for t in inputs) and len(inputs) <= 8:
                 ops.pack_blocks(inputs, static_all)  # one launch into the packed static buffer
@@ -175,6 +187,9 @@ class TrainStep:
         else:
             for dst, src in zip(_views(static_all, inputs), inputs):
                 dst.copy_(src)
+        for name, t in extra.items():
+            if t is not None:
+                static_extra[name].copy_(t)
         graph.replay()
         return static_loss
 
@@ -218,7 +233,7 @@ class TrainStep:
             raise RuntimeError(f"TrainStep: an autograd graph of {name} is still alive (a loss or an output of the model "
                                "that is held without detach()): drop it before the step of a new shape is recorded")
 
-    def _capture(self, inputs):
+    def _capture(self, inputs, extra):
         self._check_no_graph_lives()
         # the static inputs are consecutive row blocks of one buffer, so the fused TwoTower
         # forward uses them in place (no concatenation inside the step)
@@ -226,6 +241,8 @@ class TrainStep:
         static_in = tuple(_views(static_all, inputs))
         for dst, src in zip(static_in, inputs):
             dst.copy_(src)
+        static_extra = {k: None if t is None else t.detach().clone(memory_format=torch.contiguous_format)
+                        for k, t in extra.items()}
         graph = torch.cuda.CUDAGraph()
         torch.cuda.synchronize()
         settle_watchdogs()
@@ -236,8 +253,8 @@ class TrainStep:
         # capturing" from the ProcessGroupNCCL watchdog).  Calls made by this thread are checked
         # as before.
         with torch.cuda.graph(graph, capture_error_mode="thread_local"):
-            static_loss = self.eager(*static_in)
-        return graph, static_all, static_loss, self.grad_norm  # (each graph writes its own norm)
+            static_loss = self.eager(*static_in, **static_extra)
+        return graph, static_all, static_extra, static_loss, self.grad_norm  # (each graph writes its own norm)
 
 
 # messages of errors raised because a call is refused inside stream capture (HIP's and CUDA's

@@ -557,6 +557,21 @@ def test_candidates_keep_what_autograd_has_on_them():
     assert torch.equal(got[3:6], 0.5 * want[3:6]) and torch.equal(got[6:], want[6:])
 
 
+def _make(*args):
+    import os
+    import subprocess
+
+    where = os.path.join(os.path.dirname(os.path.abspath(tt.__file__)), "csrc")
+    return subprocess.run(["make", "-C", where, *args], check=True, capture_output=True, text=True).stdout
+
+
+def test_the_library_builds_without_torch():
+    assert "nodes.cpp" in _make("-n", "-B")
+    for how in (["TORCH="], ["PYINC=/nowhere"], ["TORCH=/nowhere"], ["PYTHON=/nowhere/python"], ["lib"]):
+        plan = _make("-n", "-B", *how)
+        assert "lookup.hip" in plan and "nodes.cpp" not in plan
+
+
 # ---------------------------------------------------------------------------------------------
 # C ABI
 

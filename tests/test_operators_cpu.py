@@ -572,6 +572,27 @@ def test_the_library_builds_without_torch():
         assert "lookup.hip" in plan and "nodes.cpp" not in plan
 
 
+def test_the_module_is_built_anew_for_another_torch(tmp_path):
+    """A compiler that only notes its runs: a second make does nothing, one with another torch compiles."""
+    import sys
+
+    stub, log = tmp_path / "cxx.py", tmp_path / "log"
+    stub.write_text(f"import sys; open(sys.argv[sys.argv.index('-o') + 1], 'w'); open({str(log)!r}, 'a').write('x')")
+    torches = []
+    for version in ("1", "2"):
+        root = tmp_path / version
+        (root / "include" / "torch").mkdir(parents=True)
+        (root / "include" / "torch" / "extension.h").touch()
+        (root / "version.py").write_text(f"__version__ = '{version}'")
+        torches.append(root)
+    (tmp_path / "Python.h").touch()
+    for root, runs in ((torches[0], 1), (torches[0], 1), (torches[1], 2), (torches[1], 2), (torches[0], 3)):
+        out = tmp_path / "_nodes.so"
+        _make(str(out), f"NODES={out}", f"BUILD={tmp_path}/build", f"CXX={sys.executable} {stub}", f"TORCH={root}",
+              f"PYINC={tmp_path}")
+        assert len(log.read_text()) == runs
+
+
 # ---------------------------------------------------------------------------------------------
 # C ABI
 

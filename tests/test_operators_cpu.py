@@ -497,6 +497,16 @@ def test_split_rows_hands_one_buffer_on_without_a_copy():
     assert torch.equal(g, 2 * y)
 
 
+@pytest.mark.parametrize("sizes", [(1, 1, 2), (1, 0, 3), (0, 2, 1), (1,), (2, 1)])
+def test_split_rows_of_short_blocks(sizes):
+    x, y, blocks = _split_case(sizes)
+    (g,) = torch.autograd.grad(_buffer_node()(*blocks), y)
+    assert torch.equal(g, 2 * y) and g.shape == y.shape
+    whole = torch.randn(sum(sizes), 4, dtype=torch.float64)  # one row's stride means nothing
+    parts = [w.as_strided(w.shape, (77, 1), w.storage_offset()) if len(w) == 1 else w for w in whole.split(list(sizes))]
+    assert torch.equal(torch.autograd.grad(_lib.nodes().split_rows(x * 1.0, list(sizes)), x, parts)[0], whole)
+
+
 def test_split_rows_blocks_keep_what_autograd_has_on_them():
     """Functions, hooks, retained gradients and other uses of a block, and gradients with respect to the blocks."""
     node = _buffer_node()

@@ -16,6 +16,8 @@
 #include <algorithm>
 #include <optional>
 #include <string>
+#include <typeindex>
+#include <unordered_map>
 #include <unordered_set>
 
 #include "twotower_amd.h"
@@ -342,28 +344,29 @@ struct SplitRows : Function<SplitRows> {
       at += n;
     }
     ctx->saved_data["sizes"] = sizes;
-    auto shape = x.sizes().vec();
-    shape[0] = 0;
-    ctx->saved_data["like"] = at::empty(shape, x.options());  // (type and width, for a block without a gradient)
     return blocks;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
-    const Tensor like = ctx->saved_data["like"].toTensor();
     int64_t rows = 0;
-    bool all = true;
+    size_t defined = 0, one = 0;
     for (size_t i = 0; i < g.size(); ++i) {
       rows += sizes[i];
-      all = all && g[i].defined();
+      if (g[i].defined()) {
+        ++defined;
+        one = i;
+      }
     }
-    auto shape = like.sizes().vec();
-    shape[0] = rows;
-    if (all && !at::GradMode::is_enabled() && consecutive(g))
+    if (!defined) return {Tensor(), Tensor()};
+    auto shape = g[one].sizes().vec();
+    if (defined == g.size() && !at::GradMode::is_enabled() && consecutive(g)) {
+      shape[0] = rows;
       return {g[0].as_strided(shape, at::detail::defaultStrides(shape), g[0].storage_offset()), Tensor()};
+    }
     for (size_t i = 0; i < g.size(); ++i)
       if (!g[i].defined()) {
         shape[0] = sizes[i];
-        g[i] = at::zeros(shape, like.options());
+        g[i] = at::zeros(shape, g[one].options());
       }
     return {at::cat(g, 0), Tensor()};
   }
@@ -390,11 +393,19 @@ variable_list split_rows(const Tensor& x, std::vector<int64_t> sizes) {
 // Whether all of autograd between base and each view are torch's own slices and reshapes (or split_rows): a gradient
 // of base then stands for the views'.  Not with a hook or a retained gradient on the way, nor a function of the
 // caller's that returns a view, nor for a view that is a leaf of its own or was taken under no_grad.
-bool direct_views(const Tensor& base, const std::vector<Tensor>& views) {
-  static const std::unordered_set<std::string> slices = {
+bool is_slice(torch::autograd::Node& node) {  // (under the GIL)
+  static const std::unordered_set<std::string> names = {
       "SplitBackward0", "SplitWithSizesBackward0", "UnsafeSplitBackward0", "UnsafeSplitWithSizesBackward0",
       "SliceBackward0", "ViewBackward0", "UnsafeViewBackward0", "ReshapeAliasBackward0", "AliasBackward0",
       "UnsqueezeBackward0"};
+  static std::unordered_map<std::type_index, bool> known;
+  const auto [at, is_new] = known.try_emplace(typeid(node), false);
+  if (is_new)
+    at->second = names.count(node.name()) || dynamic_cast<torch::autograd::CppNode<SplitRows>*>(&node);
+  return at->second;
+}
+
+bool direct_views(const Tensor& base, const std::vector<Tensor>& views) {
   using torch::autograd::Node;
   for (const Tensor& v : views)
     if (v.requires_grad() != base.requires_grad()) return false;
@@ -406,7 +417,7 @@ bool direct_views(const Tensor& base, const std::vector<Tensor>& views) {
       Node* const node = at.function.get();
       if (!node || node->num_outputs() != 1 || !node->tensor_pre_hooks().empty() || !node->pre_hooks().empty() ||
           !node->post_hooks().empty() || !node->retains_grad_hooks().empty() ||
-          !(slices.count(node->name()) || dynamic_cast<torch::autograd::CppNode<SplitRows>*>(node)))
+          !is_slice(*node))
         return false;
       at = node->next_edge(0);
     }

@@ -746,6 +746,14 @@ def test_contrastive_losses_see_what_autograd_has_on_the_blocks(name):
 
     leaf, parts = blocks()
     same(torch.autograd.grad(fn(*parts), leaf)[0], (1, 1, 1))
+    for split in (torch.split, lambda y, n: ops.split_rows(y, [n] * 3)):  # with respect to the blocks, and late hooks
+        y = x.clone().requires_grad_(True) * 1.0
+        parts = split(y, B)
+        loss = fn(*parts)
+        assert "Packed" in loss.grad_fn.name()
+        same(torch.cat(torch.autograd.grad(loss, parts, retain_graph=True)), (1, 1, 1))
+        parts[1].register_hook(lambda g: g * 2)
+        same(torch.autograd.grad(loss, y)[0], (1, 2, 1))
     for i in range(3):
         scale = [0.5 if j == i else 1.0 for j in range(3)]
         leaf, parts = blocks()

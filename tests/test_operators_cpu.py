@@ -525,16 +525,21 @@ def test_split_rows_blocks_keep_what_autograd_has_on_them():
     assert torch.equal(g, torch.cat([2 * x[:3], 2 * x[3:6] + 5, 2 * x[6:]]))
 
 
+def _split_rows(y, sizes):
+    return _lib.nodes().split_rows(y, sizes)
+
+
 def _base_and_blocks(split=torch.split):
     y = torch.randn(12, 4, requires_grad=True) * 1.0
     return y, list(split(y, [3, 3, 6]))
 
 
-@pytest.mark.parametrize("split", [torch.split, _lib.nodes().split_rows, lambda y, s: (y[:3], y.narrow(0, 3, 3), y[6:])])
+@pytest.mark.parametrize("split", [torch.split, _split_rows, lambda y, s: (y[:3], y.narrow(0, 3, 3), y[6:])])
 def test_losses_take_the_base_only_where_it_stands_for_its_views(split):
     """The losses that differentiate the common tensor of q, p and n: whatever autograd has on a view must not be
     passed by."""
     y, (q, p, n) = _base_and_blocks(split)
+    assert losses._direct(y, q, p, n.view(3, 2, 4), rows=True) == (split is _split_rows)
     assert losses._packed(q, p, n) is y and losses._packed(q, p, n.view(3, 2, 4).view(6, 4)) is y
     assert losses._candidates(p, n)._base is y
     assert losses._packed(_Halved.apply(q), p, n) is None

@@ -390,9 +390,6 @@ variable_list split_rows(const Tensor& x, std::vector<int64_t> sizes) {
   return SplitRows::apply(x, std::move(sizes));
 }
 
-// Whether all of autograd between base and each view are torch's own slices and reshapes (or split_rows): a gradient
-// of base then stands for the views'.  Not with a hook or a retained gradient on the way, nor a function of the
-// caller's that returns a view, nor for a view that is a leaf of its own or was taken under no_grad.
 bool is_slice(torch::autograd::Node& node) {  // (under the GIL)
   static const std::unordered_set<std::string> names = {
       "SplitBackward0", "SplitWithSizesBackward0", "UnsafeSplitBackward0", "UnsafeSplitWithSizesBackward0",
@@ -405,24 +402,54 @@ bool is_slice(torch::autograd::Node& node) {  // (under the GIL)
   return at->second;
 }
 
-bool direct_views(const Tensor& base, const std::vector<Tensor>& views) {
+// Whether all of autograd between base and each view are torch's own slices and reshapes (or split_rows): a gradient
+// of base then stands for the views'.  Not with a hook or a retained gradient on the way, nor a function of the
+// caller's that returns a view, nor for a view that is a leaf of its own or was taken under no_grad.  kRows: and the
+// last of them is split_rows for all, so that gradients in one buffer reach the base as that buffer.
+enum Views { kOther = 0, kDirect = 1, kRows = 2 };
+Views views_of(const Tensor& base, const std::vector<Tensor>& views) {
   using torch::autograd::Node;
   for (const Tensor& v : views)
-    if (v.requires_grad() != base.requires_grad()) return false;
-  if (!base.requires_grad()) return true;
+    if (v.requires_grad() != base.requires_grad()) return kOther;
+  if (!base.requires_grad()) return kRows;
   const auto to = torch::autograd::impl::gradient_edge(base);
+  Views kind = kRows;
   for (const Tensor& v : views) {
     auto at = torch::autograd::impl::gradient_edge(v);
     while (!(at == to)) {
       Node* const node = at.function.get();
       if (!node || node->num_outputs() != 1 || !node->tensor_pre_hooks().empty() || !node->pre_hooks().empty() ||
-          !node->post_hooks().empty() || !node->retains_grad_hooks().empty() ||
-          !is_slice(*node))
-        return false;
+          !node->post_hooks().empty() || !node->retains_grad_hooks().empty() || !is_slice(*node))
+        return kOther;
       at = node->next_edge(0);
+      if (at == to && !dynamic_cast<torch::autograd::CppNode<SplitRows>*>(node)) kind = kDirect;
     }
   }
-  return true;
+  return kind;
+}
+bool direct_views(const Tensor& base, const std::vector<Tensor>& views, bool rows) {
+  return views_of(base, views) >= (rows ? kRows : kDirect);
+}
+
+// The contiguous matrix whose consecutive row blocks, all of them and in order, are the views, where it stands for
+// them (views_of); and whether the blocks are split_rows'.
+std::pair<std::optional<Tensor>, bool> packed_base(const std::vector<Tensor>& views) {
+  const std::pair<std::optional<Tensor>, bool> none{std::nullopt, false};
+  if (!views[0].is_view()) return none;
+  const Tensor base(views[0]._base());
+  if (base.dim() != 2 || !base.is_contiguous()) return none;
+  int64_t at = base.storage_offset();
+  for (const Tensor& v : views) {
+    if (!v.is_view() || v._base().unsafeGetTensorImpl() != base.unsafeGetTensorImpl() || v.dim() != 2 ||
+        !v.is_contiguous() || v.size(1) != base.size(1) || v.scalar_type() != base.scalar_type() ||
+        v.storage_offset() != at)
+      return none;
+    at += v.numel();
+  }
+  if (at != base.storage_offset() + base.numel()) return none;
+  const Views kind = views_of(base, views);
+  if (kind == kOther) return none;
+  return {base, kind == kRows};
 }
 
 // (q, p, n with a pair axis) of a checked call, rows of contiguous elements
@@ -577,6 +604,7 @@ PYBIND11_MODULE(_nodes, m) {
   m.def("preference_margin", &preference_margin, unlocked);
   m.def("split_rows", &split_rows, unlocked);
   m.def("direct_views", &direct_views);
+  m.def("packed_base", &packed_base);
   m.def("live_leaf", &live_leaf);
   m.def("clip_grad_norm", &clip_grad_norm, unlocked);
 }

@@ -26,28 +26,14 @@ def _packed(*views: torch.Tensor) -> torch.Tensor | None:
     """The common base when the views are consecutive, equally wide row blocks of one contiguous
     2-D tensor in order (TwoTower's fused output split into q, p, n) and autograd would bring their
     gradients to it unchanged (_direct); else None."""
-    base = views[0]._base
-    if base is None or base.dim() != 2 or not base.is_contiguous():
-        return None
-    row = base.shape[1] * base.element_size()
-    at = base.data_ptr()
-    for v in views:
-        if v._base is not base or v.dim() != 2 or not v.is_contiguous() or v.shape[1] != base.shape[1]:
-            return None
-        if v.data_ptr() != at:
-            return None
-        at += v.shape[0] * row
-    if at != base.data_ptr() + base.shape[0] * row:
-        return None
-    return base if _direct(base, *views) else None
+    return _lib.nodes().packed_base(views)[0]
 
 
-def _direct(base: torch.Tensor, *views: torch.Tensor) -> bool:
+def _direct(base: torch.Tensor, *views: torch.Tensor, rows: bool = False) -> bool:
     """Whether the base may be differentiated in place of its views: no function, hook or retained gradient
-    of the caller's is between them."""
-    if not base.requires_grad and not any(v.requires_grad for v in views):
-        return True
-    return _lib.nodes().direct_views(base, views)
+    of the caller's is between them.  rows: and ops.split_rows made them, so that gradients in one buffer reach
+    the base as that buffer."""
+    return _lib.nodes().direct_views(base, views, rows)
 
 
 def contrastive_triplet_loss(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg_emb: torch.Tensor,
@@ -55,7 +41,7 @@ def contrastive_triplet_loss(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg
     """mean(relu(margin - cos(q, d+) + cos(q, d-))) (losses.py:9-44)."""
     base = _packed(q_emb, d_pos_emb, d_neg_emb)
     if base is not None and q_emb.shape[0] == d_pos_emb.shape[0] == d_neg_emb.shape[0]:
-        return ops.TripletLossPacked.apply(base, margin)
+        return ops.TripletLossPacked.apply(q_emb, d_pos_emb, d_neg_emb, margin)
     return ops.TripletLoss.apply(q_emb, d_pos_emb, d_neg_emb, margin)
 
 
@@ -66,9 +52,10 @@ def multiple_negatives_loss(q_emb: torch.Tensor, d_pos_emb: torch.Tensor, d_neg_
         d_neg_embs = d_neg_embs.unsqueeze(1)
     B, K = d_neg_embs.shape[0], d_neg_embs.shape[1]
     if d_neg_embs.is_contiguous() and d_pos_emb.shape[0] == q_emb.shape[0] == B:
-        base = _packed(q_emb, d_pos_emb, d_neg_embs.view(B * K, -1))
+        base, rows = _lib.nodes().packed_base((q_emb, d_pos_emb, d_neg_embs.view(B * K, -1)))
         if base is not None:  # [q; p; negatives] in one tensor (TwoTower's fused output): one gradient tensor
-            return ops.MultiNegLossPacked.apply(base, B, K, 1.0 / float(temperature))
+            return ops.MultiNegLossPacked.apply((base if rows else None,), q_emb, d_pos_emb, d_neg_embs,
+                                                1.0 / float(temperature))
     return ops.MultiNegLoss.apply(q_emb, d_pos_emb, d_neg_embs, 1.0 / float(temperature))
 
 
@@ -126,19 +113,18 @@ def in_batch_sampled_softmax_loss(q_emb: torch.Tensor, d_emb: torch.Tensor, *arg
         if isinstance(args[0], torch.Tensor):
             if len(args) > 1:
                 temperature = args[1]
-            base = None if cross_device_negatives else _packed(q_emb, d_emb, args[0])
-            if base is not None:  # [q; p; n] in one tensor: zero-copy candidates and gradient
-                return ops.InBatchSoftmaxLossPacked.apply(base, q_emb.shape[0], 1.0 / float(temperature),
-                                                          compute_dtype, None)
+            if not cross_device_negatives:
+                loss = _in_batch_packed(temperature, compute_dtype, q_emb, d_emb, args[0])
+                if loss is not None:  # [q; p; n] in one tensor: zero-copy candidates and gradient
+                    return loss
             d_emb = _candidates(d_emb, args[0])
         else:
             temperature = args[0]
     if not cross_device_negatives and (not args or not isinstance(args[0], torch.Tensor)):
-        base = _packed(q_emb, d_emb)
-        if base is not None:  # (query, positive) pairs as [q; d] in one tensor (TwoTower(q, d)): the
+        loss = _in_batch_packed(temperature, compute_dtype, q_emb, d_emb)
+        if loss is not None:  # (query, positive) pairs as [q; d] in one tensor (TwoTower(q, d)): the
             # same packed path, so the head's operand prep and fused L2 backward apply to M = B too
-            return ops.InBatchSoftmaxLossPacked.apply(base, q_emb.shape[0], 1.0 / float(temperature),
-                                                      compute_dtype, None)
+            return loss
     label_off = 0
     if cross_device_negatives:
         from . import distributed
@@ -149,6 +135,13 @@ def in_batch_sampled_softmax_loss(q_emb: torch.Tensor, d_emb: torch.Tensor, *arg
                                                      group)
         d_emb, label_off = distributed.gather_candidates(d_emb, group=group)
     return ops.in_batch_softmax_loss(q_emb, d_emb, temperature, label_off=label_off, compute_dtype=compute_dtype)
+
+
+def _in_batch_packed(temperature: float, compute_dtype: str, *blocks: torch.Tensor) -> torch.Tensor | None:
+    base, rows = _lib.nodes().packed_base(blocks)
+    if base is None:
+        return None
+    return ops.InBatchSoftmaxLossPacked.apply((base,), rows, 1.0 / float(temperature), compute_dtype, None, *blocks)
 
 
 def scorer_prep_dtype(loss_fn) -> str | None:

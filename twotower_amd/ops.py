@@ -1033,24 +1033,25 @@ class TripletLoss(torch.autograd.Function):
 
 
 class TripletLossPacked(torch.autograd.Function):
-    """Same loss on one (3B, H) tensor holding [q; p; n] (TwoTower's fused output): the gradient
-    is written as one tensor, so autograd never runs the split backward (zeros + cat)."""
+    """Same loss of three consecutive row blocks of one tensor (TwoTower's fused output): the gradients
+    are written into one buffer, which split_rows hands on whole (no zeros + cat)."""
 
     @staticmethod
-    def forward(ctx, qpn, margin):
-        require_gpu(qpn)
-        qpn = _contig_f32(qpn, "qpn")
-        q, p, n = torch.chunk(qpn, 3)
-        ctx.save_for_backward(qpn)
+    def forward(ctx, q, p, n, margin):
+        require_gpu(q)
+        q, p, n = (_contig_f32(t, nm) for t, nm in ((q, "q"), (p, "p"), (n, "n")))
+        ctx.save_for_backward(q, p, n)
         ctx.margin = float(margin)
         return _triplet_fwd(q, p, n, margin)
 
     @staticmethod
     def backward(ctx, g):
-        (qpn,) = ctx.saved_tensors
-        grad = torch.empty_like(qpn)
-        _triplet_bwd(*torch.chunk(qpn, 3), ctx.margin, g, *torch.chunk(grad, 3))
-        return grad, None
+        q, p, n = ctx.saved_tensors
+        B = q.shape[0]
+        grad = q.new_empty(3 * B, q.shape[1])
+        dq, dp, dn = grad[:B], grad[B:2 * B], grad[2 * B:]
+        _triplet_bwd(q, p, n, ctx.margin, g, dq, dp, dn)
+        return dq, dp, dn, None
 
 
 # --------------------------------------------------------------------------------------------
@@ -1083,43 +1084,39 @@ class MultiNegLoss(torch.autograd.Function):
 
 
 class MultiNegLossPacked(torch.autograd.Function):
-    """The same loss on one ((2 + K) B, H) tensor [q; p; negatives (B K rows, query-major)]
-    (TwoTower's fused output): the three gradients are written into one tensor, so autograd
-    runs no split backward (a cat of the three, 50 MB at C5, on the step's critical path)."""
+    """The same loss of consecutive row blocks [q; p; negatives (B K rows, query-major)] of one tensor
+    (TwoTower's fused output, ``whole``: a tuple of it): the three gradients are written into one buffer, which
+    split_rows hands on whole (a cat of the three is 50 MB at C5, on the step's critical path)."""
 
     @staticmethod
-    def forward(ctx, qpn, B, K, inv_tau):
-        require_gpu(qpn)
-        qpn = _contig_f32(qpn, "qpn")
-        H = qpn.shape[1]
-        if qpn.shape[0] != (2 + K) * B:
-            raise ValueError(f"packed multiple-negatives input must have (2 + K) B = {(2 + K) * B} rows")
-        rows = torch.empty(B, dtype=_FLOAT, device=qpn.device)
-        loss = torch.empty((), dtype=_FLOAT, device=qpn.device)
-        q, p, n = qpn[:B], qpn[B:2 * B], qpn[2 * B:]
-        call("tt_multi_neg_fwd", ptr(q), ptr(p), ptr(n), B, K, H, float(inv_tau), ptr(rows), ptr(loss), stream_of(qpn))
-        ctx.save_for_backward(qpn)
-        ctx.meta = (B, K, float(inv_tau))
-        tok = getattr(qpn, "_tt_l2_token", None)  # the tower head's output itself, whole
-        ctx.l2_token = tok if tok is not None and tok.norms.shape[0] == qpn.shape[0] and H == 256 and K <= 15 else None
+    def forward(ctx, whole, q, p, n, inv_tau):
+        require_gpu(q)
+        q, p, n = (_contig_f32(t, nm) for t, nm in ((q, "q"), (p, "p"), (n, "negs")))
+        B, K, H = n.shape
+        rows = torch.empty(B, dtype=_FLOAT, device=q.device)
+        loss = torch.empty((), dtype=_FLOAT, device=q.device)
+        call("tt_multi_neg_fwd", ptr(q), ptr(p), ptr(n), B, K, H, float(inv_tau), ptr(rows), ptr(loss), stream_of(q))
+        ctx.save_for_backward(q, p, n)
+        ctx.inv_tau = float(inv_tau)
+        tok = getattr(whole[0], "_tt_l2_token", None)  # the tower head's output itself, whole
+        ctx.l2_token = tok if tok is not None and tok.norms.shape[0] == (2 + K) * B and H == 256 and K <= 15 else None
         return loss
 
     @staticmethod
     def backward(ctx, g):
-        (qpn,) = ctx.saved_tensors
-        B, K, inv_tau = ctx.meta
-        H = qpn.shape[1]
+        q, p, n = ctx.saved_tensors
+        B, K, H = n.shape
         g = g.to(_FLOAT).contiguous().reshape(1)
-        grad = torch.empty_like(qpn)
+        grad = q.new_empty((2 + K) * B, H)
+        dq, dp, dn = grad[:B], grad[B:2 * B], grad[2 * B:].view(B, K, H)
         tok, ctx.l2_token = ctx.l2_token, None
         if tok is not None and _FUSED_HEAD_BWD[0] > 0:  # the head's F.normalize backward in the same pass
-            call("tt_multi_neg_bwd_l2", ptr(qpn), B, K, ptr(tok.norms), inv_tau, ptr(g), ptr(grad), stream_of(qpn))
+            call("tt_multi_neg_bwd_l2", ptr(q), B, K, ptr(tok.norms), ctx.inv_tau, ptr(g), ptr(grad), stream_of(q))
             tok.dy = grad
-            return grad, None, None, None
-        q, p, n = qpn[:B], qpn[B:2 * B], qpn[2 * B:]
-        call("tt_multi_neg_bwd", ptr(q), ptr(p), ptr(n), B, K, H, inv_tau, ptr(g), ptr(grad[:B]), ptr(grad[B:2 * B]),
-             ptr(grad[2 * B:]), stream_of(qpn))
-        return grad, None, None, None
+        else:
+            call("tt_multi_neg_bwd", ptr(q), ptr(p), ptr(n), B, K, H, ctx.inv_tau, ptr(g), ptr(dq), ptr(dp), ptr(dn),
+                 stream_of(q))
+        return None, dq, dp, dn, None
 
 
 # --------------------------------------------------------------------------------------------
@@ -1233,47 +1230,48 @@ class InBatchSoftmaxLoss(torch.autograd.Function):
 
 
 class InBatchSoftmaxLossPacked(torch.autograd.Function):
-    """In-batch loss on one (B + M, H) tensor [q; candidates] (TwoTower's fused output): dq and
-    dd are written into one gradient tensor (no split backward)."""
+    """In-batch loss of consecutive row blocks [q; candidates (one block or more)] of one tensor (TwoTower's fused
+    output, ``whole``: a tuple of it): their gradients are written into one buffer, which split_rows hands
+    on whole.  fuse: the head's F.normalize backward may be part of it (the blocks are split_rows' own)."""
 
     @staticmethod
-    def forward(ctx, qd, nq, inv_tau, compute_dtype, grad_scale):
+    def forward(ctx, whole, fuse, inv_tau, compute_dtype, grad_scale, q, *cands):
+        (qd,) = whole
         require_gpu(qd)
         prep = qd.__dict__.pop("_tt_inbatch_prep", None)  # taken once (TowerHead under scorer_prep)
         qd = _contig_f32(qd, "qd")
-        q, d = qd[:nq], qd[nq:]
-        want_grad = bool(ctx.needs_input_grad[0])
-        ctx.l2_token = prep[4] if prep is not None else None
+        nq = q.shape[0]
+        want_grad = any(ctx.needs_input_grad[5:])
+        ctx.l2_token = prep[4] if prep is not None and fuse else None
         # inside TrainStep (deferred_loss_mean) the loss is read only after the step: its mean is
         # formed by the backward's combine launch (tt_inbatch_bwd_l2, or tt_inbatch_bwd when the head's L2
         # backward is not fused) instead of a launch of its own
         # between the forward combine and the backward engine
         defer = want_grad and _DEFER_MEAN[0] > 0 and os.environ.get("TT_DEFER_MEAN", "1") != "0"
-        loss, lse, dqu, ws = _inbatch_fwd(ctx, q, d, inv_tau, 0, compute_dtype, grad_scale, want_grad,
+        loss, lse, dqu, ws = _inbatch_fwd(ctx, qd[:nq], qd[nq:], inv_tau, 0, compute_dtype, grad_scale, want_grad,
                                           prep[:4] if prep is not None else None, defer_mean=defer)
         if want_grad:
-            ctx.save_for_backward(qd, lse, dqu, ws)
-        ctx.nq = nq
+            ctx.save_for_backward(lse, dqu, ws, q, *cands)
         return loss
 
     @staticmethod
     def backward(ctx, g):
-        qd, lse, dqu, ws = ctx.saved_tensors
-        grad = torch.empty_like(qd)
-        nq = ctx.nq
+        lse, dqu, ws, *blocks = ctx.saved_tensors
+        q, d = blocks[0], blocks[1]  # (the other candidates lie behind the first)
         tok, ctx.l2_token = ctx.l2_token, None
         B, M, H, dt, inv_tau, label_off, grad_scale = ctx.meta
+        grad = q.new_empty(B + M, H)
         dm, ctx.deferred_mean = ctx.deferred_mean, None
         if tok is not None and _FUSED_HEAD_BWD[0] > 0 and _l2_fusable(H, dt):
             # the head's F.normalize backward in the combine: grad is the head's dy (see _L2Token)
             gs = g.to(_FLOAT).contiguous().reshape(1)
-            call("tt_inbatch_bwd_l2", ptr(qd), B, M, H, dt, inv_tau, label_off, ptr(lse), ptr(dqu), ptr(gs),
+            call("tt_inbatch_bwd_l2", ptr(q), B, M, H, dt, inv_tau, label_off, ptr(lse), ptr(dqu), ptr(gs),
                  grad_scale, ptr(tok.norms), ptr(grad), ptr(dm[0]) if dm else None, ptr(dm[1]) if dm else None,
-                 ptr(ws), ws.numel(), stream_of(qd))
+                 ptr(ws), ws.numel(), stream_of(q))
             tok.dy = grad
-            return grad, None, None, None, None
-        _inbatch_bwd(ctx.meta, qd[:nq], qd[nq:], lse, dqu, ws, g, grad[:nq], grad[nq:], mean=dm)
-        return grad, None, None, None, None
+        else:
+            _inbatch_bwd(ctx.meta, q, d, lse, dqu, ws, g, grad[:B], grad[B:], mean=dm)
+        return (None,) * 5 + torch.split(grad, [t.shape[0] for t in blocks])
 
 
 def _l2_fusable(H: int, dt: int) -> bool:

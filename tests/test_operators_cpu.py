@@ -585,6 +585,7 @@ def test_the_library_builds_without_torch():
     for how in (["TORCH="], ["PYINC=/nowhere"], ["TORCH=/nowhere"], ["PYTHON=/nowhere/python"], ["lib"]):
         plan = _make("-n", "-B", *how)
         assert "lookup.hip" in plan and "nodes.cpp" not in plan
+        assert ("needs _nodes.so" in plan) == (how != ["lib"])
 
 
 def test_the_module_is_built_anew_for_another_torch(tmp_path):
